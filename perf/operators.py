@@ -229,7 +229,7 @@ def calls(s):
     """the calls of one pass with their arguments, and what they leave: a serving program keeps these structures"""
     W = library()
     lib, c, op = W.lib(), s["case"], s["case"]["op"]
-    types = {torch.float32: W.F32, torch.bfloat16: W.BF16, torch.float16: W.F16}
+    types = {torch.float32: W.TYPE_F32, torch.bfloat16: W.TYPE_BF16, torch.float16: W.TYPE_F16}
     st = torch.cuda.current_stream().cuda_stream or None
 
     def mat(codes, scales, fmt):
@@ -252,7 +252,7 @@ def calls(s):
             todo = [(lib.wzy_mx_quantize, (at(x), t, ld, rows, cols, C.byref(q), st))]
             if c["fmt"] == "e2m1":
                 out = dict(values=s["values"], scales=e8m0(s["scales"]))
-                todo.append((lib.wzy_mx_dequantize, (C.byref(q), rows, cols, at(s["values"]), W.BF16, cols, st)))
+                todo.append((lib.wzy_mx_dequantize, (C.byref(q), rows, cols, at(s["values"]), W.TYPE_BF16, cols, st)))
         return todo, out, q
     a, w, y = mat(*s["a"], c["fmt"]), mat(*s["w"], "e2m1"), s["y"]
     if op == "gemm":
