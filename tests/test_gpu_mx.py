@@ -1,0 +1,513 @@
+"""Microscaled (MX) operators on the GPU against plain 64-bit formulations (tests/mx_ref.py)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import mx_ref as R
+import wzy_amd
+from mx_ref import BF16, E2M1, E4M3, F16, F32
+
+pytestmark = pytest.mark.gpu
+DA = wzy_amd.DeviceArray
+FILL = 0xA5
+
+
+class Mat:
+    """An MX matrix on the device, its rows with gaps that must keep their bytes"""
+
+    def __init__(self, rows, cols, fmt, gap=0, sgap=0, codes=None, scales=None):
+        self.rows, self.cols, self.fmt = rows, cols, fmt
+        self.nb = cols // 2 if fmt == E2M1 else cols
+        c = np.full((rows, self.nb + gap), FILL, np.uint8)
+        s = np.full((rows, cols // 32 + sgap), FILL, np.uint8)
+        if codes is not None:
+            c[:, :self.nb], s[:, :cols // 32] = R.pack(codes, fmt), scales
+        self.c, self.s = DA.from_numpy(c), DA.from_numpy(s)
+        self.m = wzy_amd.MxMat(self.c.ptr, self.s.ptr, self.nb + gap, cols // 32 + sgap, fmt)
+
+    def ref(self):
+        return C.byref(self.m)
+
+    def read(self):
+        c, s = self.c.numpy(), self.s.numpy()
+        assert (c[:, self.nb:] == FILL).all() and (s[:, self.cols // 32:] == FILL).all()
+        return R.unpack(c[:, :self.nb], self.fmt), s[:, :self.cols // 32]
+
+
+def wide(bits, gap):
+    """rows with `gap` more elements each, filled with a bit pattern"""
+    a = np.zeros((bits.shape[0], bits.shape[1] + gap), bits.dtype)
+    a.view(np.uint8)[:] = FILL
+    a[:, :bits.shape[1]] = bits
+    return a
+
+
+def out_rows(rows, cols, t, gap=0):
+    return DA.from_numpy(wide(np.zeros((rows, cols), np.float32 if t == F32 else np.uint16), gap))
+
+
+def read_rows(d, cols, t):
+    a = d.numpy()
+    assert (np.ascontiguousarray(a[:, cols:]).view(np.uint8) == FILL).all()
+    return R.values(np.ascontiguousarray(a[:, :cols]), t)
+
+
+def activations(rng, rows, cols):
+    x = rng.standard_normal((rows, cols)).astype(np.float32)
+    x[:, rng.integers(0, cols, max(1, cols // 128))] *= 10
+    return x * np.exp(rng.standard_normal((rows, 1)) * 0.5).astype(np.float32)
+
+
+def borders(fmt):
+    """values on and next to every rounding border of a block whose scale is 1, ties among them, and its limits"""
+    t = R.element_values(fmt)[:8 if fmt == E2M1 else 127]
+    mid = (t[1:] + t[:-1]) / 2
+    v = np.concatenate([t, mid, mid * (1 - 2.0 ** -20), mid * (1 + 2.0 ** -20), [R.MOST[fmt] * 1.1]])
+    return np.concatenate([v, -v])
+
+
+def special_rows(fmt, cols):
+    """32-value blocks: borders under scale 1 (led by the block's largest), zeros, denormals, the type's ends, NaN, inf"""
+    b = borders(fmt)
+    lead = 2.0 ** R.EMAX[fmt] * 1.25
+    blocks = [np.concatenate([[lead], b[i:i + 31], np.zeros(31)])[:32] for i in range(0, len(b), 31)]
+    z = np.zeros(32)
+
+    def one(*at):
+        a = z.copy()
+        for i, v in at:
+            a[i] = v
+        return a
+    blocks += [z, -z, one((3, 1e-40)), one((3, -1e-38), (9, 2e-45)), one((0, 2.0 ** -126)), one((5, 3.4e38), (6, -1e30)),
+               one((31, np.nan)), one((0, np.inf), (1, 1.0)), one((7, -np.inf)), np.full(32, 1.0), np.full(32, 0.75),
+               np.full(32, 7.999), np.arange(32) / 31 * 6.5 - 3]
+    while len(blocks) % (cols // 32):
+        blocks.append(z)
+    return np.array(blocks, np.float64).reshape(-1, cols)
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,cols,gap", [(1, 32, 0), (1, 2048, 8), (3, 96, 40), (77, 320, 0), (513, 2560, 16)])
+def test_quantize_bit_exact(wz, gpu, fmt, t, rows, cols, gap):
+    rng = np.random.default_rng(rows * 7 + cols + t)
+    bits, x = R.typed(activations(rng, rows, cols) * 2.0 ** rng.integers(-9, 9, (rows, 1)), t)
+    d = DA.from_numpy(wide(bits, gap))
+    q = Mat(rows, cols, fmt, gap=16 if gap else 0, sgap=3 if gap else 0)
+    wz.wzy_mx_quantize(d.ptr, t, cols + gap, rows, cols, q.ref(), None)
+    codes, scales = q.read()
+    wc, ws = R.quantize(x, fmt)
+    np.testing.assert_array_equal(scales, ws)
+    np.testing.assert_array_equal(codes, wc)
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_quantize_borders_and_specials(wz, gpu, fmt, t):
+    bits, x = R.typed(special_rows(fmt, 96), t)
+    rows = x.shape[0]
+    d = DA.from_numpy(bits)
+    q = Mat(rows, 96, fmt)
+    wz.wzy_mx_quantize(d.ptr, t, 96, rows, 96, q.ref(), None)
+    codes, scales = q.read()
+    wc, ws = R.quantize(x, fmt)
+    np.testing.assert_array_equal(scales, ws)
+    np.testing.assert_array_equal(codes, wc)
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_dequantize_every_code_and_scale(wz, gpu, fmt, t):
+    # every code under scale bytes from end to end, NaN among both
+    n = 16 if fmt == E2M1 else 256
+    scales = np.array([0, 1, 2, 9, 60, 100, 112, 120, 126, 127, 128, 135, 141, 200, 230, 245, 254, 255], np.uint8)
+    codes = np.tile(np.arange(n, dtype=np.uint8), (len(scales), 256 // n))
+    sc = np.repeat(scales[:, None], 8, 1)
+    q = Mat(len(scales), 256, fmt, gap=32, sgap=1, codes=codes, scales=sc)
+    y = out_rows(len(scales), 256, t, 8)
+    wz.wzy_mx_dequantize(q.ref(), len(scales), 256, y.ptr, t, 264, None)
+    got = read_rows(y, 256, t)
+    with np.errstate(over="ignore"):
+        want = R.typed(R.dequantize(codes, sc, fmt).astype(np.float32), t)[1]
+    np.testing.assert_array_equal(got, want)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 32), (5, 2560), (1000, 64)])
+def test_dequantize_inverts_quantize(wz, gpu, rows, cols):
+    rng = np.random.default_rng(rows)
+    for fmt in (E2M1, E4M3):
+        x = DA.from_numpy(activations(rng, rows, cols))
+        q, y = Mat(rows, cols, fmt), DA(rows * cols, np.float32)
+        wz.wzy_mx_quantize(x.ptr, F32, cols, rows, cols, q.ref(), None)
+        wz.wzy_mx_dequantize(q.ref(), rows, cols, y.ptr, F32, cols, None)
+        q2 = Mat(rows, cols, fmt)
+        wz.wzy_mx_quantize(y.ptr, F32, cols, rows, cols, q2.ref(), None)       # a fixed point
+        np.testing.assert_array_equal(y.numpy().reshape(rows, cols), R.dequantize(*q.read(), fmt).astype(np.float32))
+        y2 = R.dequantize(*q2.read(), fmt)
+        np.testing.assert_array_equal(y2, R.dequantize(*q.read(), fmt))
+
+
+def assert_quantized_near(codes, scales, v, rel):
+    """codes and scales are those of some values within rel (an array, relative) of v: each lies between the quantised
+    lower and upper ends.  A block whose scale could be either of two is checked under the scale it took."""
+    lo, hi = v - np.abs(v) * rel - 1e-36, v + np.abs(v) * rel + 1e-36
+    small, large = np.where(v > 0, lo, hi), np.where(v > 0, hi, lo)      # towards and away from zero
+    small = np.where(np.sign(small) != np.sign(v), 0.0, small)
+    s0, s1 = R.quantize(small, E4M3)[1], R.quantize(large, E4M3)[1]
+    assert ((scales >= s0) & (scales <= s1)).all()
+    got = R.element_values(E4M3)[codes]
+    up = np.exp2(127.0 - scales.astype(np.float64)).repeat(32, 1)
+    grid = R.element_values(E4M3)[:127]
+
+    def rounded(x):
+        x = np.clip(x, -448, 448)
+        step = np.exp2(np.maximum(np.frexp(x)[1] - 1, -6) - 3.0)
+        return np.rint(x / step) * step
+    assert np.isin(np.abs(got), grid).all()
+    assert (got >= rounded(lo * up)).all() and (got <= rounded(hi * up)).all()
+
+
+# the sum of squares: at most 32 terms a lane, 6 + 3 levels, every add off by 2^-24: 41 x 2^-24 of the sum, half of that
+# of its root, then mean, eps, root, reciprocal and two products at most 2^-23 each
+NORM_REL = 41 * 2.0 ** -25 + 6 * 2.0 ** -23
+
+
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,cols,gap,res", [(1, 32, 0, True), (1, 2048, 0, True), (3, 96, 8, False), (9, 2560, 0, True),
+                                               (5, 4128, 24, True), (2, 8192, 0, False), (3, 16384, 0, True), (2100, 320, 0, True)])
+def test_add_rmsnorm(wz, gpu, t, rows, cols, gap, res):
+    rng = np.random.default_rng(rows + cols + t)
+    xb, x = R.typed(activations(rng, rows, cols), t)
+    rb, r = R.typed(activations(rng, rows, cols), t)
+    gamma = (1 + 0.1 * rng.standard_normal(cols)).astype(np.float32)
+    h = R.typed((x.astype(np.float32) + r.astype(np.float32)) if res else x, t)[1]
+    n = h / np.sqrt((h * h).mean(1, keepdims=True) + np.float64(np.float32(1e-6))) * gamma
+    dx, dr, dg = DA.from_numpy(wide(xb, gap)), DA.from_numpy(wide(rb, gap)), DA.from_numpy(gamma)
+    s, y = out_rows(rows, cols, t, gap), out_rows(rows, cols, t, gap)
+    q = Mat(rows, cols, E4M3, gap=16, sgap=1)
+    wz.wzy_mx_add_rmsnorm(dx.ptr, dr.ptr if res else None, t, cols + gap, dg.ptr, 1e-6, rows, cols, s.ptr, y.ptr, q.ref(), None)
+    np.testing.assert_array_equal(read_rows(s, cols, t), h)
+    got = read_rows(y, cols, t)
+    assert (np.abs(got - n) <= np.abs(n) * (NORM_REL + R.HALF_STEP[t] * (1 + NORM_REL)) + 2.0 ** -25).all()
+    assert_quantized_near(*q.read(), n, NORM_REL)
+    # each output alone, and the sum in place of the residual or of x
+    s2, q2 = out_rows(rows, cols, t, gap), Mat(rows, cols, E4M3)
+    wz.wzy_mx_add_rmsnorm(dx.ptr, dr.ptr if res else None, t, cols + gap, dg.ptr, 1e-6, rows, cols, None, s2.ptr, None, None)
+    np.testing.assert_array_equal(s2.numpy(), y.numpy())
+    into = dr if res else dx
+    wz.wzy_mx_add_rmsnorm(dx.ptr, dr.ptr if res else None, t, cols + gap, dg.ptr, 1e-6, rows, cols, into.ptr, None, q2.ref(), None)
+    np.testing.assert_array_equal(into.numpy(), s.numpy())
+    for a, b in zip(q2.read(), q.read()):
+        np.testing.assert_array_equal(a, b)
+
+
+def test_add_rmsnorm_zero_and_nan_rows(wz, gpu):
+    x = np.ones((4, 64), np.float32)
+    x[0] = 0
+    x[2, 5] = np.nan
+    g = np.ones(64, np.float32)
+    dx, dg, y, q = DA.from_numpy(x), DA.from_numpy(g), out_rows(4, 64, F32), Mat(4, 64, E4M3)
+    wz.wzy_mx_add_rmsnorm(dx.ptr, None, F32, 64, dg.ptr, 1e-6, 4, 64, None, y.ptr, q.ref(), None)
+    got = read_rows(y, 64, F32)
+    assert (got[0] == 0).all() and np.isnan(got[2]).all() and np.isfinite(got[[1, 3]]).all()
+    codes, scales = q.read()
+    assert (scales[0] == 0).all() and (codes[0] == 0).all() and (scales[2] == 255).all() and (codes[2] == 0).all()
+    wz.wzy_mx_add_rmsnorm(dx.ptr, None, F32, 64, dg.ptr, 0.0, 4, 64, None, y.ptr, q.ref(), None)
+    assert np.isnan(read_rows(y, 64, F32)[0]).all() and (q.read()[1][0] == 255).all()
+
+
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,cols,gap", [(1, 32, 0), (40, 512, 0), (7, 640, 8), (300, 96, 24)])
+def test_swiglu(wz, gpu, t, rows, cols, gap):
+    rng = np.random.default_rng(rows + cols + t)
+    bits, x = R.typed(np.clip(activations(rng, rows, 2 * cols) * 3, -60, 60), t)
+    g, u = x[:, :cols], x[:, cols:]
+    d = DA.from_numpy(wide(bits, gap))
+    q = Mat(rows, cols, E4M3, gap=16, sgap=2)
+    wz.wzy_mx_swiglu(d.ptr, d.ptr + cols * (4 if t == F32 else 2), t, 2 * cols + gap, rows, cols, q.ref(), None)
+    # the exponent's argument is off by |g| 2^-23 at most, exp, the sum, the quotient and the product by 2^-22 each
+    assert_quantized_near(*q.read(), g * u / (1 + np.exp(-g)), (np.abs(g) + 8) * 2.0 ** -22)
+
+
+def test_swiglu_far_gates(wz, gpu):
+    """gates far below zero give zeros, not NaN; infinities and NaN spoil their block alone"""
+    x = np.ones((1, 128), np.float32)
+    x[0, :32] = -200.0
+    x[0, 33], x[0, 100] = np.inf, 0.0                             # inf * 0
+    d, q = DA.from_numpy(x), Mat(1, 64, E4M3)
+    x[0, 97] = 0.0
+    d = DA.from_numpy(x)
+    wz.wzy_mx_swiglu(d.ptr, d.ptr + 256, F32, 128, 1, 64, q.ref(), None)
+    codes, scales = q.read()
+    assert (R.element_values(E4M3)[codes[0, :32]] * R.scale_values(scales[0, :1]) == 0).all()
+    assert scales[0, 0] != 255 and scales[0, 1] == 255
+
+
+# ---- products -----------------------------------------------------------------------------------------
+def random_mx(rng, rows, cols, fmt, gap=0, sgap=0, spread=2):
+    codes = rng.integers(0, 16 if fmt == E2M1 else 256, (rows, cols)).astype(np.uint8)
+    if fmt == E4M3:
+        codes[(codes & 127) == 127] -= 1
+    scales = rng.integers(127 - spread, 128 + spread, (rows, cols // 32)).astype(np.uint8)
+    m = Mat(rows, cols, fmt, gap, sgap, codes, scales)
+    return m, R.dequantize(codes, scales, fmt)
+
+
+def quantized_mx(rng, rows, cols, fmt, gap=0, sgap=0):
+    codes, scales = R.quantize(activations(rng, rows, cols).astype(np.float64), fmt)
+    return Mat(rows, cols, fmt, gap, sgap, codes, scales), R.dequantize(codes, scales, fmt)
+
+
+def check_product(got, a, w, fmt, t):
+    want, tol = R.product(a, w, fmt, t)
+    off = np.abs(got - want) - tol
+    assert np.isfinite(got).all() and (off <= 0).all(), "off by %g past %g at %s" % (
+        np.abs(got - want).max(), tol.ravel()[off.argmax()], np.unravel_index(off.argmax(), off.shape))
+
+
+GEMM_SHAPES = [(1, 1, 32), (1, 16, 2048), (1, 257, 320), (2, 33, 96), (4, 100, 512), (5, 48, 2560), (8, 31, 544), (15, 17, 640),
+               (16, 130, 160), (17, 128, 128), (31, 65, 352), (64, 300, 96), (100, 129, 1056), (129, 127, 640), (257, 50, 160),
+               (130, 260, 64)]
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("M,N,K", GEMM_SHAPES)
+def test_gemm(wz, gpu, fmt, t, M, N, K):
+    rng = np.random.default_rng(M * 1000 + N + K)
+    pad = (M + N) % 3
+    a, av = quantized_mx(rng, M, K, fmt, 16 * pad, pad)
+    w, wv = quantized_mx(rng, N, K, E2M1, 32 * pad, 2 * pad)
+    y = out_rows(M, N, t, pad)
+    wz.wzy_mx_gemm(a.ref(), w.ref(), M, N, K, y.ptr, t, N + pad, None)
+    check_product(read_rows(y, N, t), av, wv, fmt, t)
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("M", [3, 40])
+def test_gemm_every_code(wz, gpu, fmt, M):
+    """codes and scales drawn evenly: the whole range of an element inside every block"""
+    rng = np.random.default_rng(M)
+    a, av = random_mx(rng, M, 288, fmt)
+    w, wv = random_mx(rng, 70, 288, E2M1)
+    for t in (F32, BF16):
+        y = out_rows(M, 70, t)
+        wz.wzy_mx_gemm(a.ref(), w.ref(), M, 70, 288, y.ptr, t, 70, None)
+        check_product(read_rows(y, 70, t), av, wv, fmt, t)
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("M", [2, 33])
+def test_gemm_scales_belong_to_their_block(wz, gpu, fmt, M):
+    """one element set in a and w at every k in turn, scales different in every block: powers of two come back exactly"""
+    K, N = 256, 256
+    a = np.zeros((M, K), np.uint8)
+    a[M - 1] = 2 if fmt == E2M1 else 0x38                         # ones
+    w = np.zeros((N, K), np.uint8)
+    w[np.arange(N), np.arange(K)] = 2
+    sa = (120 + np.arange(M * K // 32).reshape(M, -1) % 8).astype(np.uint8)
+    sw = (100 + np.arange(N * K // 32).reshape(N, -1) % 50).astype(np.uint8)
+    da, dw, y = Mat(M, K, fmt, codes=a, scales=sa), Mat(N, K, E2M1, codes=w, scales=sw), out_rows(M, N, F32)
+    wz.wzy_mx_gemm(da.ref(), dw.ref(), M, N, K, y.ptr, F32, N, None)
+    want = R.dequantize(a, sa, fmt) @ R.dequantize(w, sw, E2M1).T
+    np.testing.assert_array_equal(read_rows(y, N, F32), want)
+
+
+@pytest.mark.parametrize("M", [4, 50])
+def test_gemm_nan_stays_in_its_row_and_column(wz, gpu, M):
+    rng = np.random.default_rng(M)
+    codes, scales = R.quantize(activations(rng, M, 160).astype(np.float64), E4M3)
+    codes[1, 70] = 0x7F
+    scales[2, 4] = 255
+    a = Mat(M, 160, E4M3, codes=codes, scales=scales)
+    wc, ws = R.quantize(activations(rng, 40, 160).astype(np.float64), E2M1)
+    ws[7, 0] = 255
+    w = Mat(40, 160, E2M1, codes=wc, scales=ws)
+    for t in (F32, BF16):
+        y = out_rows(M, 40, t)
+        wz.wzy_mx_gemm(a.ref(), w.ref(), M, 40, 160, y.ptr, t, 40, None)
+        got = read_rows(y, 40, t)
+        want = np.zeros((M, 40), bool)
+        want[[1, 2]] = True
+        want[:, 7] = True
+        np.testing.assert_array_equal(np.isnan(got), want)
+
+
+def grouped(wz, rng, sizes, M, N, K, fmt, t, a_rows=None, ids=None, pad=0, stream=None):
+    off = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+    a, av = quantized_mx(rng, M if a_rows is None else a_rows, K, fmt, 16 * pad, pad)
+    w, wv = quantized_mx(rng, len(sizes) * N, K, E2M1)
+    y = out_rows(M, N, t, pad)
+    before = y.numpy()
+    do, di = DA.from_numpy(off), None if ids is None else DA.from_numpy(np.asarray(ids, np.int32))
+    wz.wzy_mx_grouped_gemm(a.ref(), a.rows, None if ids is None else di.ptr, w.ref(), do.ptr, len(sizes), M, N, K, y.ptr, t,
+                           N + pad, stream)
+    got = read_rows(y, N, t)
+    rows = np.arange(M) if ids is None else np.asarray(ids)
+    for g in range(len(sizes)):
+        sel = rows[off[g]:off[g + 1]]
+        if len(sel):
+            x = np.zeros((len(sel), K))
+            ok = (sel >= 0) & (sel < av.shape[0])
+            x[ok] = av[sel[ok]]
+            check_product(got[off[g]:off[g + 1]], x, wv[g * N:(g + 1) * N], fmt, t)
+    np.testing.assert_array_equal(y.numpy()[off[-1]:], before[off[-1]:])
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("sizes,N,K", [
+    ([1], 16, 32), ([0, 0, 3, 0], 40, 320), ([2, 1, 0, 5, 16, 17], 33, 160), ([300], 50, 96), ([0, 200, 1, 0, 128, 129], 130, 160),
+    ([40] * 7, 64, 640), ([33, 0, 31], 257, 64)])
+def test_grouped(wz, gpu, fmt, t, sizes, N, K):
+    rng = np.random.default_rng(sum(sizes) + N + K)
+    M = sum(sizes)
+    grouped(wz, rng, sizes, M, N, K, fmt, t)
+    # gathered from fewer rows, some twice; three rows behind the last group
+    grouped(wz, rng, sizes, M + 3, N, K, fmt, t, a_rows=M // 2 + 1, ids=rng.integers(0, M // 2 + 1, M + 3), pad=1)
+
+
+def test_grouped_many_groups(wz, gpu):
+    """more groups than one pass of the tile search holds, and nearly all empty"""
+    rng = np.random.default_rng(5)
+    sizes = np.zeros(1500, int)
+    sizes[[0, 511, 512, 513, 700, 1499]] = [1, 2, 20, 1, 3, 17]
+    grouped(wz, rng, list(sizes), int(sizes.sum()), 20, 64, E4M3, F32)
+    sizes[512] = 40000                                            # one group far larger than the average
+    grouped(wz, rng, list(sizes[:520]), int(sizes[:520].sum()), 3, 32, E2M1, F32)
+
+
+@pytest.mark.parametrize("M", [6, 90])
+def test_grouped_ids_out_of_range_read_zeros(wz, gpu, M):
+    rng = np.random.default_rng(M)
+    ids = rng.integers(0, 10, M)
+    ids[[0, 3]], ids[5] = [-1, 10], 2 ** 31 - 1
+    grouped(wz, rng, [M // 2, M - M // 2], M, 24, 96, E4M3, F32, a_rows=10, ids=ids)
+    grouped(wz, rng, [M], M, 24, 96, E2M1, BF16, a_rows=10, ids=ids)
+
+
+@pytest.mark.parametrize("off", [[0, 9, 4, 12], [-5, 3, 1000, 2], [12, 12, 0, 0], [2 ** 31 - 1, -2 ** 31, 5, 12]])
+@pytest.mark.parametrize("M", [12, 120])
+def test_grouped_broken_offsets_stay_in_y(wz, gpu, off, M):
+    rng = np.random.default_rng(1)
+    a, _ = quantized_mx(rng, M, 64, E4M3)
+    w, _ = quantized_mx(rng, 3 * 20, 64, E2M1)
+    y = DA.from_numpy(np.full((M + 300, 20), 7.0, np.float32))
+    do = DA.from_numpy(np.asarray(off, np.int64).astype(np.int32))
+    wz.wzy_mx_grouped_gemm(a.ref(), M, None, w.ref(), do.ptr, 3, M, 20, 64, y.ptr, F32, 20, None)
+    assert (y.numpy()[M:] == 7.0).all()
+
+
+# ---- as they are used together -------------------------------------------------------------------------
+@pytest.mark.parametrize("T", [1, 4, 40])
+def test_expert_block_run(wz, gpu, T):
+    """norm -> gathered gate|up per expert -> SwiGLU -> down per expert, each step checked on what the GPU handed it"""
+    rng = np.random.default_rng(T)
+    D, F, E, K = 256, 96, 6, 3
+    xb, x = R.typed(activations(rng, T, D), BF16)
+    rb, r = R.typed(activations(rng, T, D), BF16)
+    gamma = np.ones(D, np.float32)
+    ids = np.stack([rng.permutation(E)[:K] for _ in range(T)])
+    order = np.argsort(ids.ravel(), kind="stable")
+    off = np.concatenate([[0], np.cumsum(np.bincount(ids.ravel(), minlength=E))]).astype(np.int32)
+    M = T * K
+    w1, w1v = quantized_mx(rng, E * 2 * F, D, E2M1)
+    w2, w2v = quantized_mx(rng, E * D, F, E2M1)
+    dx, dr, dg, do = DA.from_numpy(xb), DA.from_numpy(rb), DA.from_numpy(gamma), DA.from_numpy(off)
+    dids = DA.from_numpy((order // K).astype(np.int32))
+    q1, q2 = Mat(T, D, E4M3), Mat(M, F, E4M3)
+    gu, y, sm = out_rows(M, 2 * F, BF16), out_rows(M, D, F32), out_rows(T, D, BF16)
+    st = C.c_void_p()
+    wz.wzy_stream_create(C.byref(st))
+    s = st.value
+    wz.wzy_mx_add_rmsnorm(dx.ptr, dr.ptr, BF16, D, dg.ptr, 1e-6, T, D, sm.ptr, None, q1.ref(), s)
+    wz.wzy_mx_grouped_gemm(q1.ref(), T, dids.ptr, w1.ref(), do.ptr, E, M, 2 * F, D, gu.ptr, BF16, 2 * F, s)
+    wz.wzy_mx_swiglu(gu.ptr, gu.ptr + 2 * F, BF16, 2 * F, M, F, q2.ref(), s)
+    wz.wzy_mx_grouped_gemm(q2.ref(), M, None, w2.ref(), do.ptr, E, M, D, F, y.ptr, F32, D, s)
+    wz.wzy_stream_sync(s)
+    wz.wzy_stream_destroy(s)
+    h = R.typed(x.astype(np.float32) + r.astype(np.float32), BF16)[1]
+    np.testing.assert_array_equal(read_rows(sm, D, BF16), h)
+    n = h / np.sqrt((h * h).mean(1, keepdims=True) + 1e-6)
+    assert_quantized_near(*q1.read(), n, NORM_REL)
+    a1, guv, a2, yv = R.dequantize(*q1.read(), E4M3), read_rows(gu, 2 * F, BF16), R.dequantize(*q2.read(), E4M3), read_rows(y, D, F32)
+    for e in range(E):
+        o = slice(off[e], off[e + 1])
+        if off[e] < off[e + 1]:
+            check_product(guv[o], a1[order[o] // K], w1v[e * 2 * F:(e + 1) * 2 * F], E4M3, BF16)
+            check_product(yv[o], a2[o], w2v[e * D:(e + 1) * D], E4M3, F32)
+    g, u = guv[:, :F], guv[:, F:]
+    assert_quantized_near(*q2.read(), g * u / (1 + np.exp(-g)), (np.abs(g) + 8) * 2.0 ** -22)
+
+
+def test_two_streams_and_graph_replays(wz, gpu):
+    """the same calls on two streams at once, then captured and replayed between eager calls: the same bits"""
+    hip = C.CDLL("libamdhip64.so")
+    rng = np.random.default_rng(9)
+    T, D, N, E = 24, 512, 320, 5
+    sizes = [3, 0, 11, 9, 1]
+    off = DA.from_numpy(np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32))
+    x, g = DA.from_numpy(activations(rng, T, D)), DA.from_numpy(np.ones(D, np.float32))
+    w, _ = quantized_mx(rng, E * N, D, E2M1)
+
+    def outputs():
+        return dict(q=Mat(T, D, E4M3), y=out_rows(T, N, F32), z=out_rows(T, N, BF16), q2=Mat(T, N, E2M1))
+
+    def enqueue(o, s):
+        wz.wzy_mx_add_rmsnorm(x.ptr, None, F32, D, g.ptr, 1e-6, T, D, None, None, o["q"].ref(), s)
+        wz.wzy_mx_gemm(o["q"].ref(), w.ref(), T, N, D, o["y"].ptr, F32, N, s)
+        wz.wzy_mx_grouped_gemm(o["q"].ref(), T, None, w.ref(), off.ptr, E, T, N, D, o["z"].ptr, BF16, N, s)
+        wz.wzy_mx_quantize(o["y"].ptr, F32, N, T, N, o["q2"].ref(), s)
+
+    def bits(o):
+        return [o["y"].numpy(), o["z"].numpy(), *o["q"].read(), *o["q2"].read()]
+
+    one, two = outputs(), outputs()
+    enqueue(one, None)
+    wz.wzy_device_sync()
+    want = bits(one)
+    st = [C.c_void_p(), C.c_void_p()]
+    for s in st:
+        wz.wzy_stream_create(C.byref(s))
+    o1, o2 = outputs(), outputs()
+    for _ in range(5):
+        enqueue(o1, st[0].value)
+        enqueue(o2, st[1].value)
+    wz.wzy_device_sync()
+    for o in (o1, o2):
+        for a, b in zip(bits(o), want):
+            np.testing.assert_array_equal(a, b)
+    graph, run = C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamBeginCapture(st[0], 2) == 0
+    enqueue(two, st[0].value)
+    assert hip.hipStreamEndCapture(st[0], C.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(C.byref(run), graph, None, None, C.c_size_t(0)) == 0
+    for _ in range(4):
+        for d in (two["y"], two["z"]):
+            wz.wzy_memset(d.ptr, 0, d.nbytes, None)
+        wz.wzy_device_sync()
+        assert hip.hipGraphLaunch(run, st[0]) == 0
+        wz.wzy_device_sync()
+        for a, b in zip(bits(two), want):
+            np.testing.assert_array_equal(a, b)
+        enqueue(one, None)
+        wz.wzy_device_sync()
+        for a, b in zip(bits(one), want):
+            np.testing.assert_array_equal(a, b)
+    assert hip.hipGraphExecDestroy(run) == 0 and hip.hipGraphDestroy(graph) == 0
+    for s in st:
+        wz.wzy_stream_destroy(s.value)
+
+
+def test_no_rows_launch_nothing(wz, gpu):
+    q = Mat(1, 64, E4M3)
+    wz.wzy_mx_quantize(None, F32, 64, 0, 64, None, None)
+    wz.wzy_mx_dequantize(None, 0, 64, None, F32, 64, None)
+    wz.wzy_mx_add_rmsnorm(None, None, F32, 64, None, 1e-6, 0, 64, None, None, q.ref(), None)
+    wz.wzy_mx_swiglu(None, None, BF16, 64, 0, 64, None, None)
+    wz.wzy_mx_gemm(None, None, 0, 5, 64, None, F32, 5, None)
+    wz.wzy_mx_gemm(None, None, 5, 0, 64, None, F32, 5, None)
+    wz.wzy_mx_grouped_gemm(None, 0, None, None, None, 4, 0, 5, 64, None, F32, 5, None)
+    wz.wzy_device_sync()
+    assert (q.read()[0] == FILL).all()

@@ -1,6 +1,6 @@
 """ctypes bindings of libwzy_amd.so, the MI355X decode-path library.
 
-The C ABI (include/wzy_kernels.h, include/wzy_synth.h, include/wzy_stage.h) takes plain pointers and
+The C ABI (include/wzy_kernels.h, include/wzy_mx.h, include/wzy_synth.h, include/wzy_stage.h) takes plain pointers and
 sizes; these bindings pass integers (device pointers from any allocator, numpy buffer addresses)
 and raise WzyError on a negative status.  Loading fails loudly when the shared library has not been
 built: there is no CPU fallback behind this module.
@@ -44,6 +44,16 @@ class GemvSeg(C.Structure):
 
 
 GEMV_Q8, GEMV_BF16 = 0, 1
+
+
+# microscaled (MX) matrices and the types of rows that are not quantised (include/wzy_mx.h)
+MX_E2M1, MX_E4M3 = 0, 1
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+
+
+class MxMat(C.Structure):
+    """struct wzy_mx_mat (include/wzy_mx.h)"""
+    _fields_ = [("codes", P), ("scales", P), ("ld_codes", I64), ("ld_scales", I64), ("fmt", I32)]
 
 
 class QsaDims(C.Structure):
@@ -203,6 +213,13 @@ _SIGS = {
     "wzy_ple_block": (I32, [P, P, P, P, P, P, P, P, P, P, P, I32, I32, F32, I32, P, P, SZ, P], True),
     "wzy_synth_ple_row": (None, [U64, U64, I32, P], False),
     "wzy_synth_ple_table_device": (I32, [U64, I32, P, P], True),
+    # microscaled operators
+    "wzy_mx_quantize": (I32, [P, I32, I64, I32, I32, C.POINTER(MxMat), P], True),
+    "wzy_mx_dequantize": (I32, [C.POINTER(MxMat), I32, I32, P, I32, I64, P], True),
+    "wzy_mx_add_rmsnorm": (I32, [P, P, I32, I64, P, F32, I32, I32, P, P, C.POINTER(MxMat), P], True),
+    "wzy_mx_swiglu": (I32, [P, P, I32, I64, I32, I32, C.POINTER(MxMat), P], True),
+    "wzy_mx_gemm": (I32, [C.POINTER(MxMat), C.POINTER(MxMat), I32, I32, I32, P, I32, I64, P], True),
+    "wzy_mx_grouped_gemm": (I32, [C.POINTER(MxMat), I32, P, C.POINTER(MxMat), P, I32, I32, I32, I32, P, I32, I64, P], True),
     # synth
     "wzy_synth_hash": (U64, [U64, U64, U64], False),
     "wzy_synth_stream": (U64, [U32, U32, U32], False),
