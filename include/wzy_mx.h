@@ -82,7 +82,7 @@ int wzy_mx_gemm(const wzy_mx_mat* a, const wzy_mx_mat* w, int M, int N, int K, v
  *   y[e] = a[row_ids[e]] . w_g^T,   w_g = rows g * N .. g * N + N - 1 of w (E2M1).
  * offsets [groups + 1] and row_ids [M] are device memory.  Groups may be empty; M is the number of rows of y and
  * at least offsets[groups], and rows of y in no group keep what they hold.  row_ids NULL: entry e reads row e.
- * An id outside 0 .. a_rows - 1 reads as a row of zeros.  offsets are taken as they are but limited to 0 .. M;
+ * a has a_rows >= 1 rows; an id outside 0 .. a_rows - 1 gives a row of zeros.  offsets are taken as they are but limited to 0 .. M;
  * where they decrease or overlap, which rows are computed is not specified (nothing outside y [M x N] is written).
  * 1 <= groups <= 65,536; shapes otherwise as wzy_mx_gemm. */
 int wzy_mx_grouped_gemm(const wzy_mx_mat* a, int a_rows, const int* row_ids, const wzy_mx_mat* w, const int* offsets,

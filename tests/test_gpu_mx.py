@@ -284,6 +284,26 @@ def test_gemm(wz, gpu, fmt, t, M, N, K):
     check_product(read_rows(y, N, t), av, wv, fmt, t)
 
 
+# K in whole steps of 128 and scale rows aligned to 4 bytes: the direct-to-LDS tiles, from one step to more than the buffers hold
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("M,N,K", [(17, 20, 512), (40, 50, 256), (33, 70, 1280), (64, 64, 896), (100, 513, 512), (128, 256, 640), (130, 260, 1152),
+                                   (257, 300, 640), (300, 97, 2048), (70, 90, 768)])
+def test_gemm_whole_steps(wz, gpu, fmt, t, M, N, K):
+    rng = np.random.default_rng(M * 1000 + N + K)
+    pad = M % 2
+    a, av = quantized_mx(rng, M, K, fmt, 16 * pad, 4 * pad)
+    w, wv = quantized_mx(rng, N, K, E2M1, 32 * pad, 8 * pad)
+    y = out_rows(M, N, t, pad)
+    wz.wzy_mx_gemm(a.ref(), w.ref(), M, N, K, y.ptr, t, N + pad, None)
+    got = read_rows(y, N, t)
+    step = max(1, M * N * K // 20000000)          # the bound needs every product: rows in a stride that meets every tile
+    rows = np.unique(np.concatenate([np.arange(0, M, step), [M - 1]]))
+    check_product(got[rows], av[rows], wv, fmt, t)
+    want, off = av @ wv.T, 1e-2
+    assert (np.abs(got - want) <= off * (np.abs(av) @ np.abs(wv).T)).all()      # and all rows in rough
+
+
 @pytest.mark.parametrize("fmt", [E2M1, E4M3])
 @pytest.mark.parametrize("M", [3, 40])
 def test_gemm_every_code(wz, gpu, fmt, M):
@@ -366,6 +386,18 @@ def test_grouped(wz, gpu, fmt, t, sizes, N, K):
     grouped(wz, rng, sizes, M, N, K, fmt, t)
     # gathered from fewer rows, some twice; three rows behind the last group
     grouped(wz, rng, sizes, M + 3, N, K, fmt, t, a_rows=M // 2 + 1, ids=rng.integers(0, M // 2 + 1, M + 3), pad=1)
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("sizes,N,K", [([300], 50, 128), ([0, 200, 1, 0, 128, 129], 130, 512), ([40] * 7, 64, 640), ([33, 0, 31], 257, 896)])
+def test_grouped_whole_steps(wz, gpu, fmt, t, sizes, N, K):
+    rng = np.random.default_rng(sum(sizes) + N + K)
+    M = sum(sizes)
+    grouped(wz, rng, sizes, M, N, K, fmt, t)
+    ids = rng.integers(0, M // 2 + 1, M + 3)
+    ids[rng.integers(0, M, 5)] = [-1, M // 2 + 1, 2 ** 31 - 1, -2 ** 31, 0]
+    grouped(wz, rng, sizes, M + 3, N, K, fmt, t, a_rows=M // 2 + 1, ids=ids)
 
 
 def test_grouped_many_groups(wz, gpu):

@@ -84,6 +84,7 @@ def test_bad_products_are_refused(wz):
     refused(wz, *g, 4, None, w, None, 2, 4, 8, 64, A, F32, 8, None)        # no offsets
     refused(wz, *g, 3, None, w, A, 2, 4, 8, 64, A, F32, 8, None)           # fewer rows than entries, not gathered
     refused(wz, *g, -1, A, w, A, 2, 4, 8, 64, A, F32, 8, None)
+    refused(wz, *g, 0, A, w, A, 2, 4, 8, 64, A, F32, 8, None)
     refused(wz, *g, 4, None, w, A, 0, 4, 8, 64, A, F32, 8, None)
     refused(wz, *g, 4, None, w, A, 65537, 4, 8, 64, A, F32, 8, None)
 

@@ -2,13 +2,13 @@
 //
 //   y[m, n] = sum over blocks b of 32:  2^(sa[m, b] + sw[n, b] - 254) * sum_i a[m, 32 b + i] * w[n, 32 b + i]
 //
-// v_mfma_scale_f32_{16x16x128, 32x32x64}_f8f6f4 multiply E2M1 by E2M1 or E4M3 codes as they lie in memory and
-// apply the two scale bytes of each block of 32, with fp32 accumulators; nothing is dequantised.  Operand
-// layouts (measured): a lane holds one row (lane % 16 or % 32) and one block of k (lane / 16 or / 32).  E2M1: the
-// block's 32 codes in order, 16 bytes.  E4M3: two 16-byte pieces, piece j of lane group q holding the 16 k from
-// 16 q + (half the instruction's k) j; the scale byte of group q still belongs to block q.  D: register r of lane l
-// is row 4 (l / 16) + r (16x16) or 8 (r / 4) + 4 (l / 32) + r % 4 (32x32) of the first operand, column l % 16 or
-// l % 32 of the second.
+// v_mfma_scale_f32_16x16x128_f8f6f4 multiplies E2M1 by E2M1 or E4M3 codes as they lie in memory and applies the two
+// scale bytes of each block of 32, with fp32 accumulators; nothing is dequantised.  Operand layout (measured): lane
+// (q = lane / 16, r = lane % 16) holds row r and block q of 128 k.  E2M1: the block's 32 codes in order, 16 bytes.  E4M3: two
+// 16-byte pieces, piece j holding the 16 k from 16 q + 64 j; the scale byte of lane group q still belongs to block q.  D:
+// register i of lane (q, r) is row 4 q + i of the first operand, column r of the second.  w comes first, so a lane holds
+// consecutive columns of y.  (32x32x64 does as much per cycle, and on data that is not zeros draws more power: registers
+// alone, random codes, 6,770 against 8,130 TFLOP/s in E2M1, 4,350 against 4,700 with E4M3.)
 //
 // Precision (measured): an instruction adds the products of 8 consecutive k after cutting each to 13 bits below the
 // largest of the eight, and the sums of eights in fp32.  E2M1 products span 9 bits: nothing is lost.  An E4M3 operand
@@ -16,10 +16,12 @@
 // 1/50 of an fp16 one, and are left there.  For fp32 outputs the operand is taken in two parts, codes with exponent bit 3
 // set and the others: each part spans 11 bits, so both products are whole, at twice the MFMA work.
 //
-//   mx_skinny  up to 16 rows (decode, small groups): a wave takes 16 weight rows over a share of K, operands
-//              straight from memory; the waves of a workgroup meet in LDS
-//   mx_tile    more rows: output tiles through LDS
-// Both serve the dense product and the product per group.
+// Three kernels, chosen in launch():
+//   mx_dma     tiles of 16 x 64 to 256 x 256 through LDS, filled by direct-to-LDS loads several steps ahead; K a multiple of 128
+//   mx_any     tiles of 32 x 64 to 128 x 128 through LDS and registers: any K, any alignment of the scales
+//   mx_skinny  up to 16 rows and few columns, or any K: operands straight from memory, K split over a workgroup's waves
+// mx_dma and mx_any serve the product per group too: a workgroup finds its group's tile from the offsets by itself, so
+// there is no preparing launch, no workspace and nothing for the host to know.
 #include <algorithm>
 
 #include "wzy_mx.h"
@@ -28,7 +30,6 @@ using namespace wzy;
 
 typedef int v8i_t __attribute__((ext_vector_type(8)));
 typedef float v4f_t __attribute__((ext_vector_type(4)));
-typedef float v16f_t __attribute__((ext_vector_type(16)));
 
 namespace {
 
@@ -39,24 +40,12 @@ struct MxGemm {
     void* y;
     int64_t ldy;
     int a_rows, groups, M, N, K, y_type;
-    int nt;                           // tiles along N
+    int mt, nt;                       // row and column tiles
 };
 
-// 16 bytes at any address
-struct __attribute__((packed, aligned(1))) Bytes16 { uint32_t x, y, z, w; };
+// 4 bytes at any address
 struct __attribute__((packed, aligned(1))) Bytes4 { uint32_t x; };
-// up to 16 scale bytes at p, n of them inside the row; bytes past it read as 0 (2^-127: not NaN)
-WZY_DEV uint4 load_scales16(const uint8_t* p, int n) {
-    if (n >= 16) {
-        const Bytes16 b = *(const Bytes16*) p;
-        return make_uint4(b.x, b.y, b.z, b.w);
-    }
-    uint32_t v[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (i < n) v[i >> 2] |= (uint32_t) p[i] << (8 * (i & 3));
-    return make_uint4(v[0], v[1], v[2], v[3]);
-}
+// up to 4 scale bytes at p, n of them inside the row; bytes past it read as 0 (2^-127: not NaN)
 WZY_DEV uint32_t load_scales4(const uint8_t* p, int n) {
     if (n >= 4) return ((const Bytes4*) p)->x;
     uint32_t v = 0;
@@ -77,12 +66,18 @@ WZY_DEV v8i_t operand8(uint4 a, uint4 b) {
     return v8i_t{(int) a.x, (int) a.y, (int) a.z, (int) a.w, (int) b.x, (int) b.y, (int) b.z, (int) b.w};
 }
 template <int FMT>
+WZY_DEV v8i_t operand_of(const uint4 (&v)[FMT == WZY_MX_E4M3 ? 2 : 1]) {
+    if constexpr (FMT == WZY_MX_E4M3) return operand8(v[0], v[1]);
+    else return operand4(v[0]);
+}
+template <int FMT>
 struct Code;                                                     // the instructions' format numbers
 template <> struct Code<WZY_MX_E4M3> { static constexpr int v = 0; };
 template <> struct Code<WZY_MX_E2M1> { static constexpr int v = 4; };
 
-template <int FMT, bool WHOLE, int OPA>
-WZY_DEV v4f_t mfma16(v8i_t a, v8i_t w, v4f_t c, int sa, int sw) {
+// w (E2M1) by a: D's rows are w's, its columns a's.  OW, OA: the scale's byte in its dword.
+template <int FMT, bool WHOLE, int OW, int OA>
+WZY_DEV v4f_t mfma16(v8i_t w, v8i_t a, v4f_t c, int sw, int sa) {
     if constexpr (FMT == WZY_MX_E4M3 && WHOLE) {
         v8i_t hi, lo;
 #pragma unroll
@@ -90,13 +85,12 @@ WZY_DEV v4f_t mfma16(v8i_t a, v8i_t w, v4f_t c, int sa, int sw) {
             hi[i] = (int) e4m3_large((uint32_t) a[i]);
             lo[i] = a[i] ^ hi[i];
         }
-        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(lo, w, c, 0, 4, OPA, sa, 0, sw);
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(hi, w, c, 0, 4, OPA, sa, 0, sw);
+        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, lo, c, 4, 0, OW, sw, OA, sa);
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, hi, c, 4, 0, OW, sw, OA, sa);
     } else {
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, w, c, Code<FMT>::v, 4, OPA, sa, 0, sw);
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 4, Code<FMT>::v, OW, sw, OA, sa);
     }
 }
-
 template <int OUT>
 WZY_DEV void put(void* y, size_t i, float v) {
     if constexpr (OUT == WZY_F32) ((float*) y)[i] = v;
@@ -108,6 +102,18 @@ WZY_DEV void put(void* y, size_t i, float v) {
 // Tiles of up to TM rows are numbered through the groups in order; the wave finds tile t: 64 lanes x 8 groups a
 // pass, a prefix sum over the lanes.  False where there are fewer tiles.  Offsets are limited to 0 .. M, so a
 // tile never leaves y.
+struct __attribute__((packed, aligned(4))) Ints4 { int x, y, z, w; };
+template <int CTRL, int ROWMASK>
+WZY_DEV int add_dpp(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWMASK, 0xF, true); }
+// sums of lanes 0 .. l: within 16-lane rows by shifts, then the rows' last lanes on to the next rows
+WZY_DEV int prefix_sum(int v) {
+    v = add_dpp<0x111, 0xF>(v);                                    // row_shr 1, 2, 4, 8
+    v = add_dpp<0x112, 0xF>(v);
+    v = add_dpp<0x114, 0xF>(v);
+    v = add_dpp<0x118, 0xF>(v);
+    v = add_dpp<DPP_ROW_BCAST15, 0xA>(v);
+    return add_dpp<DPP_ROW_BCAST31, 0xC>(v);
+}
 WZY_DEV int clamp_off(int o, int M) { return min(max(o, 0), M); }
 template <int TM>
 WZY_DEV bool find_tile(const MxGemm& g, int t, int& group, int& row0, int& rows) {
@@ -116,19 +122,23 @@ WZY_DEV bool find_tile(const MxGemm& g, int t, int& group, int& row0, int& rows)
     for (int base = 0; base < g.groups; base += 512) {
         const int g0 = base + 8 * lane;
         int off[9], cnt[8], sum = 0;
+        if (g0 + 8 <= g.groups) {
+            const Ints4 a = *(const Ints4*) (g.offsets + g0), b = *(const Ints4*) (g.offsets + g0 + 4);
+            off[0] = a.x; off[1] = a.y; off[2] = a.z; off[3] = a.w;
+            off[4] = b.x; off[5] = b.y; off[6] = b.z; off[7] = b.w;
+            off[8] = g.offsets[g0 + 8];
+        } else {
 #pragma unroll
-        for (int i = 0; i < 9; ++i) off[i] = clamp_off(g.offsets[min(g0 + i, g.groups)], g.M);
+            for (int i = 0; i < 9; ++i) off[i] = g.offsets[min(g0 + i, g.groups)];
+        }
+#pragma unroll
+        for (int i = 0; i < 9; ++i) off[i] = clamp_off(off[i], g.M);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             cnt[i] = (max(off[i + 1] - off[i], 0) + TM - 1) / TM;
             sum += cnt[i];
         }
-        int pre = sum;                                            // inclusive prefix over the lanes
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(pre, d);
-            if (lane >= d) pre += o;
-        }
+        const int pre = prefix_sum(sum);                          // over the lanes, its own included
         const int first = before + pre - sum;
         const uint64_t hit = __ballot(t >= first && t < first + sum);
         if (hit) {
@@ -153,6 +163,28 @@ WZY_DEV bool find_tile(const MxGemm& g, int t, int& group, int& row0, int& rows)
     return false;
 }
 
+// Tile of this workgroup.  Consecutive workgroups go to the 8 XCDs in turn, each with an L2 of its own.  Dense: the tiles are
+// numbered in bands of four row tiles, down the band and then along it, and XCD x takes the x-th eighth of them: the 32 or 64
+// tiles it works on at a time share 4 panels of a and 8 or 16 of w.  Grouped: the number of tiles is not known here, so an
+// XCD takes every eighth row tile and runs its column tiles one after another.  (Bands of four there, so that tiles of one group
+// share their weights: 3 % slower at 8,192 tokens of 10 of 512 experts, the row tiles being as many bytes.)
+template <bool GROUPED>
+WZY_DEV bool tile_of(const MxGemm& g, int& mi, int& ni) {
+    const int x = (int) blockIdx.x & 7, s = (int) blockIdx.x >> 3;
+    if constexpr (GROUPED) {
+        mi = (s / g.nt) * 8 + x;
+        ni = s % g.nt;
+    } else {
+        const int t = x * ((int) gridDim.x >> 3) + s, band = t / (4 * g.nt), r = t - band * 4 * g.nt, h = min(g.mt - 4 * band, 4);
+        if (h <= 0) return false;
+        ni = r / h;
+        mi = 4 * band + r % h;
+    }
+    mi = __builtin_amdgcn_readfirstlane(mi);                       // the divisions leave them in vector registers
+    ni = __builtin_amdgcn_readfirstlane(ni);
+    return ni < g.nt;
+}
+
 // row of a that entry e reads; -1: zeros
 WZY_DEV int entry_row(const MxGemm& g, int e) {
     if (!g.row_ids) return e;
@@ -161,90 +193,140 @@ WZY_DEV int entry_row(const MxGemm& g, int e) {
 }
 
 // ---- up to 16 rows -----------------------------------------------------------------------------------------
-// A workgroup of KS waves takes 16 weight rows; wave w the batches w, w + KS, ... of 512 k (four instructions, one
-// 16-byte read of scales a row), so neighbouring waves read neighbouring pieces of the same rows.
-template <int FMT, int OUT, bool GROUPED>
-__global__ void __launch_bounds__(256) mx_skinny_kernel(MxGemm g) {
-    __shared__ float s_acc[3][4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ks = blockDim.x >> 6;
-    const int q = lane >> 4, lr = lane & 15;
-    const int n0 = ((int) blockIdx.x % g.nt) * 16;
-    int row0 = 0, rows = g.M, group = 0;
-    if constexpr (GROUPED) {
-        if (!find_tile<16>(g, (int) blockIdx.x / g.nt, group, row0, rows)) return;
-    }
-    const int ar = entry_row(g, row0 + min(lr, rows - 1));
-    const bool has = ar >= 0;
-    const size_t wr = (size_t) group * g.N + min(n0 + lr, g.N - 1);
-    const uint8_t* const ap = g.a.codes + (size_t) max(ar, 0) * g.a.ldc;
-    const uint8_t* const asp = g.a.scales + (size_t) max(ar, 0) * g.a.lds;
+// A workgroup of up to 8 waves takes 16 weight rows; wave w the batches w, w + waves, ... of 512 k, so neighbouring waves read
+// neighbouring pieces of the same rows, and the waves' sums meet in LDS.  Of a batch's 16 blocks lane group q takes 4 q .. 4 q + 3 in
+// its four instructions: its scales are one dword a row, its weights 64 bytes.
+template <int FMT, int OUT>
+__global__ void __launch_bounds__(512) mx_skinny_kernel(MxGemm g) {
+    constexpr bool E8 = FMT == WZY_MX_E4M3;
+    __shared__ v4f_t s_acc[7][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ks = blockDim.x >> 6;
+    const int q = lane >> 4, lr = lane & 15, n0 = (int) blockIdx.x * 16;
+    const size_t ar = min(lr, g.M - 1), wr = min(n0 + lr, g.N - 1);
+    const uint8_t* const ap = g.a.codes + ar * g.a.ldc;
+    const uint8_t* const asp = g.a.scales + ar * g.a.lds;
     const uint8_t* const wp = g.w.codes + wr * g.w.ldc;
     const uint8_t* const wsp = g.w.scales + wr * g.w.lds;
     const int nblk = g.K / 32;
     v4f_t acc = {0.f, 0.f, 0.f, 0.f};
-    for (int b = 16 * wave; b < nblk; b += 16 * ks) {              // b: first block of the batch
-        uint4 wv[4], av[4][FMT == WZY_MX_E4M3 ? 2 : 1];
+    struct Batch { uint4 w[4], a[4][E8 ? 2 : 1]; uint32_t sw, sa; };
+    // E4M3: piece j of lane group q holds half q % 2 of the block of lane group q / 2 + 2 j
+    auto a_off = [&](int b, int s, int j) { return E8 ? 32 * (b + 4 * ((q >> 1) + 2 * j) + s) + 16 * (q & 1) : 16 * (b + 4 * q + s); };
+    auto load = [&](int b) {                                       // b: first block of the batch
+        Batch t;
+        if (b + 16 <= nblk) {                                      // wave-uniform
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int blk = b + 4 * s + q;
-            wv[s] = load16(wp + 16 * (size_t) blk, blk < nblk);
-            if constexpr (FMT == WZY_MX_E4M3) {
+            for (int s = 0; s < 4; ++s) t.w[s] = ld_stream_u4(wp + 16 * (b + 4 * q + s));
+            t.sw = ((const Bytes4*) (wsp + b + 4 * q))->x;
+            t.sa = ((const Bytes4*) (asp + b + 4 * q))->x;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int k16 = 2 * (b + 4 * s) + q + 4 * j;   // 16-byte piece of the row
-                    av[s][j] = load16(ap + 16 * (size_t) k16, has && k16 < 2 * nblk);
-                }
-            } else {
-                av[s][0] = load16(ap + 16 * (size_t) blk, has && blk < nblk);
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int j = 0; j < (E8 ? 2 : 1); ++j) t.a[s][j] = *(const uint4*) (ap + a_off(b, s, j));
+        } else {
+            const int left = nblk - b - 4 * q;                     // blocks of this lane group inside the row
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                t.w[s] = load16(wp + 16 * (b + 4 * q + s), s < left);
+#pragma unroll
+                for (int j = 0; j < (E8 ? 2 : 1); ++j) t.a[s][j] = load16(ap + a_off(b, s, j), E8 ? b + 4 * ((q >> 1) + 2 * j) + s < nblk : s < left);
             }
+            t.sw = load_scales4(wsp + b + 4 * q, left);
+            t.sa = load_scales4(asp + b + 4 * q, left);
         }
-        const uint4 sw = load_scales16(wsp + b, nblk - b);
-        const uint4 sa = has ? load_scales16(asp + b, nblk - b) : make_uint4(0, 0, 0, 0);
-        const uint32_t swd[4] = {sw.x, sw.y, sw.z, sw.w}, sad[4] = {sa.x, sa.y, sa.z, sa.w};
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            v8i_t a;
-            if constexpr (FMT == WZY_MX_E4M3) a = operand8(av[s][0], av[s][1]);
-            else a = operand4(av[s][0]);
-            acc = mfma16<FMT, OUT == WZY_F32, 0>(a, operand4(wv[s]), acc, (int) (sad[s] >> (8 * q)), (int) (swd[s] >> (8 * q)));
+        return t;
+    };
+    auto multiply = [&](const Batch& t) {
+        acc = mfma16<FMT, OUT == WZY_F32, 0, 0>(operand4(t.w[0]), operand_of<FMT>(t.a[0]), acc, (int) t.sw, (int) t.sa);
+        acc = mfma16<FMT, OUT == WZY_F32, 1, 1>(operand4(t.w[1]), operand_of<FMT>(t.a[1]), acc, (int) t.sw, (int) t.sa);
+        acc = mfma16<FMT, OUT == WZY_F32, 2, 2>(operand4(t.w[2]), operand_of<FMT>(t.a[2]), acc, (int) t.sw, (int) t.sa);
+        acc = mfma16<FMT, OUT == WZY_F32, 3, 3>(operand4(t.w[3]), operand_of<FMT>(t.a[3]), acc, (int) t.sw, (int) t.sa);
+    };
+    int b = 16 * wave;
+    if (b < nblk) {
+        Batch t = load(b);
+        for (b += 16 * ks; b < nblk; b += 16 * ks) {               // the next batch's loads leave before this one is used
+            const Batch n = load(b);
+            multiply(t);
+            t = n;
         }
+        multiply(t);
     }
-    if (wave) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s_acc[wave - 1][r][lane] = acc[r];
-    }
+    if (wave) s_acc[wave - 1][lane] = acc;
     __syncthreads();
     if (wave) return;
-    for (int w = 1; w < ks; ++w)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[r] += s_acc[w - 1][r][lane];
-    const int n = n0 + lr;
+    for (int w = 1; w < ks; ++w) acc += s_acc[w - 1][lane];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        const int m = 4 * q + r;
-        if (m < rows && n < g.N) put<OUT>(g.y, (size_t) (row0 + m) * g.ldy + n, acc[r]);
+        const int n = n0 + 4 * q + r;
+        if (lr < g.M && n < g.N) put<OUT>(g.y, (size_t) lr * g.ldy + n, acc[r]);
     }
 }
 
-// ---- tiles of TM x TN -----------------------------------------------------------------------------------------
-// Four waves share a tile; wave w takes all TM rows and TN / 4 columns of it.  K goes in steps of 128 through two
-// LDS buffers: the next step loads into registers while this one multiplies.  An LDS row holds a step's codes of one
-// row (64 bytes of E2M1, 128 of E4M3); its 16-byte pieces are permuted by the row, so that 16 lanes that read the same
-// piece of 16 rows touch all 64 banks once.
-template <int FMT, int OUT, int TM, int TN, bool GROUPED>
-__global__ void __launch_bounds__(256, 2) mx_tile_kernel(MxGemm g) {
-    constexpr int AP = FMT == WZY_MX_E4M3 ? 8 : 4, WP = 4;        // 16-byte pieces of a row per step
-    constexpr int RB = TM / 32, CB = TN / 128;                     // 32 x 32 blocks of a wave
-    constexpr int NA = TM * AP / 256, NW = TN * WP / 256, NS = (TM + TN + 255) / 256;
+// ---- tiles in LDS --------------------------------------------------------------------------------------------
+// Row of w behind row lr of column block j of a wave.  16-bit y: the four registers of blocks j and j + 1 of a lane are eight
+// columns in a row, one 16-byte store (PAIR); otherwise those of a block are four.
+template <bool PAIR>
+WZY_DEV int w_row(int j, int lr) { return PAIR ? 32 * (j / 2) + 8 * (lr >> 2) + 4 * (j % 2) + (lr & 3) : 16 * j + lr; }
+// A row of P 16-byte pieces keeps them exchanged by the bits of the row's number that differ among the 16 rows that 16 lanes
+// read one piece of at a time (16 i .. of a, w_row of w), so that these touch all 64 banks once: no conflicts counted.
+template <int P>
+WZY_DEV int swz_a(int r) { return P == 16 ? r & 15 : P == 8 ? (r >> 1) & 7 : (r >> 2) & 3; }
+template <int P, bool PAIR>
+WZY_DEV int swz_w(int r) {
+    if constexpr (PAIR) return P == 8 ? ((r >> 1) & 1) | ((r >> 3) & 3) << 1 : (r >> 3) & 3;
+    else return swz_a<P>(r);
+}
+// A wave's part of y: lane (q4, lr) holds rows wr + 16 i + lr, columns n + 16 j + 4 q4 .. + 3, or n + 16 j + 8 q4 .. + 7 of a pair
+// of blocks.  whole: no column of the tile lies past N and y's rows are aligned to 16 bytes.
+template <int OUT, int NI, int CB, bool PAIR>
+WZY_DEV void store_tile(const MxGemm& g, bool gather, bool whole, int row0, int rows, int wr, int n, const v4f_t (&acc)[NI][CB]) {
+    constexpr int NV = PAIR ? 8 : 4;
+    const int q4 = (threadIdx.x & 63) >> 4, lr = threadIdx.x & 15;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int m = wr + 16 * i + lr;
+        if (m >= rows) continue;
+        const bool zero = gather && (unsigned) g.row_ids[row0 + m] >= (unsigned) g.a_rows;
+        const size_t row = (size_t) (row0 + m) * g.ldy;
+#pragma unroll
+        for (int j = 0; j < CB; j += PAIR ? 2 : 1) {
+            const int c = n + 16 * j + NV * q4;
+            float v[8];
+#pragma unroll
+            for (int r = 0; r < NV; ++r) v[r] = zero ? 0.f : acc[i][j + (r >> 2)][r & 3];
+            if (whole) {
+                if constexpr (PAIR) store8<OUT>(g.y, row + c, v);
+                else if constexpr (OUT == WZY_F32) *(float4*) ((float*) g.y + row + c) = make_float4(v[0], v[1], v[2], v[3]);
+                else *(uint2*) ((uint16_t*) g.y + row + c) = make_uint2(pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3]));
+            } else {
+#pragma unroll
+                for (int r = 0; r < NV; ++r)
+                    if (c + r < g.N) put<OUT>(g.y, row + c + r, v[r]);
+            }
+        }
+    }
+}
+template <int OUT>
+WZY_DEV bool whole_tile(const MxGemm& g, int n0, int tn) {
+    return n0 + tn <= g.N && (((uintptr_t) g.y | (uintptr_t) g.ldy * (OUT == WZY_F32 ? 4 : 2)) & 15) == 0;
+}
+
+// Tiles of TM x TN for any K and any alignment of the scale rows.  WM x WN waves; wave (i, j) holds TM / WM rows by TN / WN columns.
+// K goes in steps of 128 through two LDS buffers and two register sets: step k + 2 loads while step k multiplies.
+template <int FMT, int OUT, int TM, int TN, int WM, int WN, bool GROUPED>
+__global__ void __launch_bounds__(64 * WM * WN, 2) mx_any_kernel(MxGemm g) {
+    constexpr bool E8 = FMT == WZY_MX_E4M3, PAIR = OUT != WZY_F32 && TN / 16 / WN % 2 == 0;
+    constexpr int T = 64 * WM * WN, RB = TM / 16 / WM, CB = TN / 16 / WN;
+    constexpr int AP = E8 ? 8 : 4, WP = 4;                         // 16-byte pieces of a row per step
+    constexpr int NA = (TM * AP + T - 1) / T, NW = (TN * WP + T - 1) / T, NS = (TM + TN + T - 1) / T;
     __shared__ uint4 s_a[2][TM * AP];
     __shared__ uint4 s_w[2][TN * WP];
     __shared__ uint32_t s_sc[2][TM + TN];
-    auto a_at = [](int r, int c) { return r * AP + (c ^ (AP == 8 ? (r >> 1) & 7 : (r >> 2) & 3)); };
-    auto w_at = [](int r, int c) { return r * WP + (c ^ ((r >> 2) & 3)); };
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, lr = lane & 31;
-    // consecutive workgroups go to the 8 XCDs in turn: XCD x takes the row tiles x, x + 8, ... and runs all column
-    // tiles of one after another, so that the tile's rows stay in its L2
-    const int s = (int) blockIdx.x >> 3, mi = (s / g.nt) * 8 + ((int) blockIdx.x & 7), n0 = (s % g.nt) * TN;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q4 = lane >> 4, lr = lane & 15;
+    int mi, ni;
+    if (!tile_of<GROUPED>(g, mi, ni)) return;
+    const int n0 = ni * TN;
     int row0 = mi * TM, rows = min(g.M - row0, TM), group = 0;
     if constexpr (GROUPED) {
         if (!find_tile<TM>(g, mi, group, row0, rows)) return;
@@ -253,153 +335,486 @@ __global__ void __launch_bounds__(256, 2) mx_tile_kernel(MxGemm g) {
     const uint8_t* const wbase = g.w.codes + ((size_t) group * g.N + n0) * g.w.ldc;
     const uint8_t* const wsbase = g.w.scales + ((size_t) group * g.N + n0) * g.w.lds;
     const uint8_t* ap[NA];
-    bool aok[NA];
+    const uint8_t* sp[NS];
     uint32_t wo[NW];
+    bool aok[NA], sok[NS];
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
-        const int p = tid + 256 * i, ar = entry_row(g, row0 + min(p / AP, rows - 1));
-        aok[i] = ar >= 0;
+        const int p = tid + T * i, ar = entry_row(g, row0 + min(p / AP, rows - 1));
+        aok[i] = ar >= 0 && p < TM * AP;
         ap[i] = g.a.codes + (size_t) max(ar, 0) * g.a.ldc + 16 * (p % AP);
     }
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
-        const int p = tid + 256 * i;
+        const int p = tid + T * i;
         wo[i] = (uint32_t) min(p / WP, g.N - 1 - n0) * (uint32_t) g.w.ldc + 16 * (p % WP);
     }
-    const uint8_t* sp[NS];
-    bool sok[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-        const int r = tid + 256 * i;
-        if (r < TM) {
-            const int ar = entry_row(g, row0 + min(r, rows - 1));
-            sok[i] = ar >= 0;
-            sp[i] = g.a.scales + (size_t) max(ar, 0) * g.a.lds;
-        } else {
-            sok[i] = r < TM + TN;
-            sp[i] = wsbase + (size_t) min(r - TM, g.N - 1 - n0) * g.w.lds;
-        }
+        const int r = tid + T * i;
+        const int ar = entry_row(g, row0 + min(min(r, TM - 1), rows - 1));
+        sok[i] = r < TM ? ar >= 0 : r < TM + TN;
+        sp[i] = r < TM ? g.a.scales + (size_t) max(ar, 0) * g.a.lds : wsbase + (size_t) min(r - TM, g.N - 1 - n0) * g.w.lds;
     }
-    uint4 ra[NA], rw[NW];
-    uint32_t rs[NS];
+    struct Regs { uint4 a[NA], w[NW]; uint32_t s[NS]; };
     auto load = [&](int k) {
-        const int left = nblk - 4 * k;                             // blocks from this step on
+        Regs t;
+        const int left = nblk - 4 * k;                             // blocks from this step on; none past the end
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
-            const int c = (tid + 256 * i) % AP;
-            ra[i] = load16(ap[i] + (size_t) k * (16 * AP), aok[i] && (AP == 8 ? c < 2 * left : c < left));
+            const int c = (tid + T * i) % AP;
+            t.a[i] = load16(ap[i] + (size_t) k * (16 * AP), aok[i] && (E8 ? c < 2 * left : c < left));
         }
 #pragma unroll
-        for (int i = 0; i < NW; ++i) rw[i] = load16(wbase + wo[i] + (size_t) k * 64, (tid + 256 * i) % WP < left);
+        for (int i = 0; i < NW; ++i) t.w[i] = load16(wbase + wo[i] + (size_t) k * 64, (tid + T * i) % WP < left);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) rs[i] = sok[i] ? load_scales4(sp[i] + 4 * (size_t) k, left) : 0;
+        for (int i = 0; i < NS; ++i) t.s[i] = sok[i] ? load_scales4(sp[i] + 4 * (size_t) k, left) : 0;
+        return t;
     };
-    auto store = [&](int b) {
+    auto store = [&](int b, const Regs& t) {
 #pragma unroll
-        for (int i = 0; i < NA; ++i) s_a[b][a_at((tid + 256 * i) / AP, (tid + 256 * i) % AP)] = ra[i];
+        for (int i = 0; i < NA; ++i) {
+            const int p = tid + T * i;
+            if (TM * AP % T == 0 || p < TM * AP) s_a[b][p / AP * AP + ((p % AP) ^ swz_a<AP>(p / AP))] = t.a[i];
+        }
 #pragma unroll
-        for (int i = 0; i < NW; ++i) s_w[b][w_at((tid + 256 * i) / WP, (tid + 256 * i) % WP)] = rw[i];
+        for (int i = 0; i < NW; ++i) {
+            const int p = tid + T * i;
+            if (TN * WP % T == 0 || p < TN * WP) s_w[b][p / WP * WP + ((p % WP) ^ swz_w<WP, PAIR>(p / WP))] = t.w[i];
+        }
 #pragma unroll
         for (int i = 0; i < NS; ++i)
-            if (tid + 256 * i < TM + TN) s_sc[b][tid + 256 * i] = rs[i];
+            if (tid + T * i < TM + TN) s_sc[b][tid + T * i] = t.s[i];
     };
-    v16f_t acc[RB][CB];
+    v4f_t acc[RB][CB];
 #pragma unroll
     for (int i = 0; i < RB; ++i)
 #pragma unroll
-        for (int j = 0; j < CB; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    const int nrb = (rows + 31) / 32;                              // row blocks that hold rows
-    const int wc = wave * (TN / 4);
-    load(0);
-    store(0);
-    __syncthreads();
-    for (int k = 0; k < steps; ++k) {
-        const int b = k & 1;
-        if (k + 1 < steps) load(k + 1);
+        for (int j = 0; j < CB; ++j) acc[i][j] = v4f_t{0.f, 0.f, 0.f, 0.f};
+    const int wr = (wave / WN) * (TM / WM), wc = (wave % WN) * (TN / WN), wl = w_row<PAIR>(0, lr);
+    const int nrb = (rows - wr + 15) / 16;                         // row blocks of this wave that hold rows
+    const int asw = swz_a<AP>(lr), wsw = swz_w<WP, PAIR>(wl);
+    auto multiply = [&](int b) {
+        uint4 wv[CB];
         int sw[CB];
 #pragma unroll
-        for (int j = 0; j < CB; ++j) sw[j] = (int) (s_sc[b][TM + wc + 32 * j + lr] >> (8 * h));
-        v8i_t wv[2][CB];
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-            for (int j = 0; j < CB; ++j) wv[kk][j] = operand4(s_w[b][w_at(wc + 32 * j + lr, 2 * kk + h)]);
+        for (int j = 0; j < CB; ++j) {
+            const int r = wc + w_row<PAIR>(j, 0) + wl;
+            wv[j] = s_w[b][r * WP + (q4 ^ wsw)];
+            sw[j] = (int) (s_sc[b][TM + r] >> (8 * q4));
+        }
 #pragma unroll
         for (int i = 0; i < RB; ++i) {
-            if (i >= nrb) break;                                   // workgroup-uniform
-            const int r = 32 * i + lr;
-            const int sa = (int) (s_sc[b][r] >> (8 * h));
+            if (i >= nrb) break;                                   // wave-uniform
+            const int r = wr + 16 * i + lr, sa = (int) (s_sc[b][r] >> (8 * q4));
+            uint4 av[E8 ? 2 : 1];
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                v8i_t av;
-                if constexpr (FMT == WZY_MX_E4M3) av = operand8(s_a[b][a_at(r, 4 * kk + h)], s_a[b][a_at(r, 4 * kk + 2 + h)]);
-                else av = operand4(s_a[b][a_at(r, 2 * kk + h)]);
+            for (int j = 0; j < (E8 ? 2 : 1); ++j) av[j] = s_a[b][r * AP + ((q4 + 4 * j) ^ asw)];
 #pragma unroll
-                for (int j = 0; j < CB; ++j) {
-                    // the step's four scale bytes, shifted by 8 h: block 2 kk + h is byte 2 kk
-                    if constexpr (FMT == WZY_MX_E4M3 && OUT == WZY_F32) {
-                        v8i_t hi, lo;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            hi[e] = (int) e4m3_large((uint32_t) av[e]);
-                            lo[e] = av[e] ^ hi[e];
-                        }
-                        if (kk == 0) {
-                            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(lo, wv[kk][j], acc[i][j], 0, 4, 0, sa, 0, sw[j]);
-                            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(hi, wv[kk][j], acc[i][j], 0, 4, 0, sa, 0, sw[j]);
-                        } else {
-                            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(lo, wv[kk][j], acc[i][j], 0, 4, 2, sa, 2, sw[j]);
-                            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(hi, wv[kk][j], acc[i][j], 0, 4, 2, sa, 2, sw[j]);
-                        }
-                    } else {
-                        constexpr int F = Code<FMT>::v;
-                        if (kk == 0) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, wv[kk][j], acc[i][j], F, 4, 0, sa, 0, sw[j]);
-                        else acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, wv[kk][j], acc[i][j], F, 4, 2, sa, 2, sw[j]);
-                    }
-                }
-            }
+            for (int j = 0; j < CB; ++j) acc[i][j] = mfma16<FMT, OUT == WZY_F32, 0, 0>(operand4(wv[j]), operand_of<FMT>(av), acc[i][j], sw[j], sa);
         }
-        if (k + 1 < steps) store(b ^ 1);
+    };
+    Regs t0 = load(0), t1 = load(1);
+    store(0, t0);
+    __syncthreads();
+    for (int k = 0; k < steps; k += 2) {
+        t0 = load(k + 2);
+        multiply(0);
+        if (k + 1 >= steps) break;                                 // workgroup-uniform
+        store(1, t1);
+        __syncthreads();
+        t1 = load(k + 3);
+        multiply(1);
+        store(0, t0);
         __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < RB; ++i)
-#pragma unroll
-        for (int j = 0; j < CB; ++j) {
-            const int n = n0 + wc + 32 * j + lr;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int m = 32 * i + 8 * (r >> 2) + 4 * h + (r & 3);
-                if (m < rows && n < g.N) put<OUT>(g.y, (size_t) (row0 + m) * g.ldy + n, acc[i][j][r]);
-            }
-        }
+    store_tile<OUT, RB, CB, PAIR>(g, GROUPED && g.row_ids, whole_tile<OUT>(g, n0, TN), row0, rows, wr, n0 + wc, acc);
 }
 
-constexpr int SKINNY_M = 16;
+// ---- tiles fed by direct-to-LDS loads -----------------------------------------------------------------------
+// K a multiple of 128 from 512 on, scale rows aligned to 4 bytes.  Codes and scales go from memory to LDS without registers, in
+// units of UK k through ST buffers.  The loads are counted, so a wave waits for the unit it needs and leaves the later ones
+// in flight, and one barrier a unit tells every wave that all parts of the next unit have landed and that this unit's
+// buffer is free.  (Inline assembly: the compiler would have every LDS read wait for every such load.  The loads have no
+// register result.)  Scales come 16 bytes a row, for 512 k: 4 bytes a row took as many cache requests as the codes (8,192 x 8,192 x
+// 8,192 in E2M1, 377 -> 342 us).  UK 256 makes a weight row's piece a whole cache line of 128 bytes (342 -> 314); E4M3 tiles of
+// 128 x 128 and more take 128, for want of LDS.
+//
+// Every operand is read from LDS one row block before it is used, across units too: before the last row block of a unit a wave
+// waits for the next unit's loads and meets the others; all its reads of this unit are done then, so the buffer takes the
+// loads of unit u + ST, and the next unit's first operands are read under the last row block's MFMAs (314 -> 303; tiles in
+// bands, tile_of: 285; 16x16x128 instructions: 271).
+//
+// WM x WN waves hold TM / WM rows by TN / WN columns each; KW 2: two such sets, one for each 128 of a unit, whose sums meet
+// at the end (16 x 64 tiles, where a unit's chain of LDS reads and MFMAs is what takes the time: 1 x 12,288 x 2,048 to fp32 6.8 ->
+// 5.7 us).
+//
+// What bounds it: 8,192 x 8,192 x 8,192, E2M1 271 us (4,060 TFLOP/s), E4M3 417 (2,640).  The same launch without its MFMAs takes
+// 224 (313), without its loads 231 (335): loads into LDS run at 10 TB/s over the chip whatever the tile, and the MFMAs with
+// their LDS reads at 5 PFLOP/s (3.3).  Bigger tiles than 256 x 256 do not fit the LDS.
+WZY_DEV uint32_t lds_offset(const void* p) { return (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) char*) p; }
+// 64 lanes x 16 bytes from base + off (per lane) to LDS lds .. lds + 1023, lane order; lds and base wave-uniform
+WZY_DEV void dma16(uint32_t lds, uint32_t off, const uint8_t* base) {
+    const uint64_t b = (uint64_t) (uintptr_t) base;
+    lds = (uint32_t) __builtin_amdgcn_readfirstlane((int) lds);      // nothing where they are in scalar registers already
+    base = (const uint8_t*) (uintptr_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (b >> 32)) << 32 |
+                                         (uint32_t) __builtin_amdgcn_readfirstlane((int) b));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+// this wave's loads but the last N have landed and its LDS reads are done; then all waves meet
+template <int N>
+WZY_DEV void dma_wait_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+template <int FMT, int OUT, int TM, int TN, int WM, int WN, int KW, int UK, int ST, int OCC, bool GROUPED>
+__global__ void __launch_bounds__(64 * WM * WN * KW, OCC) mx_dma_kernel(MxGemm g) {
+    constexpr bool E8 = FMT == WZY_MX_E4M3;
+    // waves; a wave's row blocks of RH x 16 rows, column blocks of 16
+    constexpr int NWV = WM * WN * KW, RH = TM / WM >= 32 ? 2 : 1, RB = TM / WM / (16 * RH), CB = TN / 16 / WN;
+    constexpr int AP = UK / (E8 ? 16 : 32), WP = UK / 32;            // 16-byte pieces of a row of a and of w per unit
+    constexpr int A_B = TM * AP * 16, W_B = TN * WP * 16, S_B = (TN + (TM + 63) / 64 * 64) * 16;
+    // wave-wide loads of a step; where they do not divide by the waves, some are issued twice (same bytes, same place), so
+    // that every wave has the same number in flight
+    constexpr int LA = A_B / 1024, LW = W_B / 1024, LS = S_B / 1024;
+    constexpr int NA = (LA + NWV - 1) / NWV, NW = (LW + NWV - 1) / NWV, NS = (LS + NWV - 1) / NWV, NI = NA + NW;
+    static_assert(TM % 16 == 0 && TN % 64 == 0 && A_B % 1024 == 0 && RB >= 1 && CB >= 1 && ST >= 2, "tile");
+    static_assert((ST - 2) * NI + NS < 64, "loads in flight are counted in six bits");
+    static_assert(KW == 1 || (KW == 2 && UK == 256 && RB == 1 && (KW - 1) * WM * WN * RH * CB * 1024 <= ST * (A_B + W_B)), "waves along k");
+    static_assert(ST - 2 < 512 / UK, "the count of scales in flight holds from the first unit on");
+    __shared__ __align__(1024) uint8_t s_buf[ST * (A_B + W_B) + 2 * S_B];
+    constexpr bool PAIR = OUT != WZY_F32 && CB % 2 == 0;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), q4 = lane >> 4, lr = lane & 15;
+    int mi, ni;
+    if (!tile_of<GROUPED>(g, mi, ni)) return;
+    const int n0 = ni * TN;
+    int row0 = mi * TM, rows = min(g.M - row0, TM), group = 0;
+    if constexpr (GROUPED) {
+        if (!find_tile<TM>(g, mi, group, row0, rows)) return;
+    } else if (rows <= 0) return;
+    const bool gather = GROUPED && g.row_ids;
+    const uint8_t* const abase = g.a.codes + (gather ? 0 : (size_t) row0 * g.a.ldc);
+    const uint8_t* const asbase = g.a.scales + (gather ? 0 : (size_t) row0 * g.a.lds);
+    const uint8_t* const wbase = g.w.codes + ((size_t) group * g.N + n0) * g.w.ldc;
+    const uint8_t* const wsbase = g.w.scales + ((size_t) group * g.N + n0) * g.w.lds;
+    auto a_row = [&](int r) {                                        // row r of the tile, counted from abase
+        r = min(r, rows - 1);
+        if (!gather) return (uint32_t) r;
+        const int id = g.row_ids[row0 + r];
+        return (unsigned) id < (unsigned) g.a_rows ? (uint32_t) id : 0u;
+    };
+    // Units of UH halves of 128 k; K of an odd number of halves: the last unit of two loads the row's last two and multiplies
+    // the second
+    constexpr int UH = UK / 128, GU = 4 / UH;                        // GU units to a group of scales
+    const int halves = g.K / 128;
+    const uint32_t lds0 = lds_offset(s_buf);
+    auto k_at = [&](int u) { return min(UH * u, halves - UH); };     // first half of unit u; past the end the last unit again
+    // LDS position p (16 bytes) of a buffer: row p / pieces, its piece p % pieces permuted by the row
+    uint32_t ao[NA], wo[NW], so[NS];
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        const int p = ((wave * NW + i) % LW) * 64 + lane, r = p / WP;
+        wo[i] = (uint32_t) min(r, g.N - 1 - n0) * (uint32_t) g.w.ldc + 16 * ((p % WP) ^ swz_w<WP, PAIR>(r));
+    }
+    auto issue_w = [&](int u, int buf) {                             // w's codes of unit u
+        const uint8_t* const b = wbase + (size_t) k_at(u) * 64;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) dma16(lds0 + ST * A_B + buf * W_B + ((wave * NW + i) % LW) * 1024, wo[i], b);
+    };
+    // The weights' first loads leave before the row ids, which a's addresses wait for, are there.
+    if constexpr (GROUPED) {
+#pragma unroll
+        for (int u = 0; u < ST; ++u) issue_w(u, u);
+    }
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+        const int p = ((wave * NA + i) % LA) * 64 + lane, r = p / AP;
+        ao[i] = a_row(r) * (uint32_t) g.a.ldc + 16 * ((p % AP) ^ swz_a<AP>(r));
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int r = ((wave * NS + i) % LS) * 64 + lane;
+        so[i] = r < TN ? (uint32_t) min(r, g.N - 1 - n0) * (uint32_t) g.w.lds : a_row(r - TN) * (uint32_t) g.a.lds;
+    }
+    auto issue_a = [&](int u, int buf) {
+        const uint8_t* const b = abase + (size_t) k_at(u) * (E8 ? 128 : 64);
+#pragma unroll
+        for (int i = 0; i < NA; ++i) dma16(lds0 + buf * A_B + ((wave * NA + i) % LA) * 1024, ao[i], b);
+    };
+    // scales of four halves: 16 bytes a row, the row's last 16 where fewer halves are left
+    auto scale_at = [&](int q) { return min(16 * q, 4 * halves - 16); };   // byte in a scale row
+    auto issue_scales = [&](int q) {
+        const uint32_t at = lds0 + ST * (A_B + W_B) + (q & 1) * S_B;
+        const int o = scale_at(q);
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int r = ((wave * NS + i) % LS) * 64;
+            dma16(at + r * 16, so[i], (r < TN ? wsbase : asbase) + o);
+        }
+    };
+    v4f_t acc[RH * RB][CB];
+#pragma unroll
+    for (int i = 0; i < RH * RB; ++i)
+#pragma unroll
+        for (int j = 0; j < CB; ++j) acc[i][j] = v4f_t{0.f, 0.f, 0.f, 0.f};
+    const int kg = wave / (WM * WN), wt = wave % (WM * WN);          // the wave's half of a unit (KW 2), its part of the tile
+    const int wr = (wt / WN) * (TM / WM), wc = (wt % WN) * (TN / WN);
+    const int nrb = (rows - wr + 16 * RH - 1) / (16 * RH);           // row blocks of this wave that hold rows
+    // lane (q4, lr) reads piece q4 of row 16 i + lr of a and of row w_row(j, lr) = w_row(j, 0) + wl of w
+    const int wl = w_row<PAIR>(0, lr), asw = swz_a<AP>(lr), wsw = swz_w<WP, PAIR>(wl);
+    const uint8_t* const la = s_buf + (wr + lr) * (AP * 16);
+    const uint8_t* const lw = s_buf + ST * A_B + (wc + wl) * (WP * 16);
+    const uint8_t* const lsw = s_buf + ST * (A_B + W_B) + (wc + wl) * 16;
+    const uint8_t* const lsa = s_buf + ST * (A_B + W_B) + (TN + wr + lr) * 16;
+    struct Wf { uint4 v[CB]; };                                      // a half's operands
+    struct Af { uint4 v[RH][E8 ? 2 : 1]; };                          // of one row block
+    struct Sf { int a[RH * RB], w[CB]; };                            // the scales of the lane's block in four halves, a byte each
+    auto load_w = [&](int buf, int half) {
+        Wf f;
+#pragma unroll
+        for (int j = 0; j < CB; ++j)
+            f.v[j] = *(const uint4*) (lw + buf * W_B + w_row<PAIR>(j, 0) * (WP * 16) + 16 * ((4 * half + q4) ^ wsw));
+        return f;
+    };
+    auto load_a = [&](int buf, int half, int i) {
+        Af f;
+#pragma unroll
+        for (int e = 0; e < RH; ++e) {
+            const uint8_t* const ra = la + buf * A_B + (AP * 16) * 16 * (RH * i + e);
+            if constexpr (E8) {
+                f.v[e][0] = *(const uint4*) (ra + 16 * ((8 * half + q4) ^ asw));
+                f.v[e][1] = *(const uint4*) (ra + 16 * ((8 * half + 4 + q4) ^ asw));
+            } else {
+                f.v[e][0] = *(const uint4*) (ra + 16 * ((4 * half + q4) ^ asw));
+            }
+        }
+        return f;
+    };
+    const uint32_t pick = 0x0C0C0400u + 0x0101u * (uint32_t) q4;     // byte q4 of one dword, then of another
+    auto load_s = [&](int q) {
+        Sf f;
+        const int o = (q & 1) * S_B, skip = (16 * q - scale_at(q)) / 4;   // 0, or what the row's last 16 bytes start early
+        auto one = [&](const uint8_t* p) {
+            uint4 d = *(const uint4*) p;
+            if (skip & 1) { d.x = d.y; d.y = d.z; d.z = d.w; }       // the last one is there twice then
+            if (skip & 2) { d.x = d.z; d.y = d.w; }
+            return (int) ((__builtin_amdgcn_perm(d.y, d.x, pick) | __builtin_amdgcn_perm(d.w, d.z, pick) << 16) >> (KW == 2 ? 8 * kg : 0));
+        };
+#pragma unroll
+        for (int j = 0; j < CB; ++j) f.w[j] = one(lsw + o + w_row<PAIR>(j, 0) * 16);
+#pragma unroll
+        for (int i = 0; i < RH * RB; ++i) f.a[i] = one(lsa + o + 16 * 16 * i);
+        return f;
+    };
+    issue_scales(0);
+    issue_scales(1);
+#pragma unroll
+    for (int u = 0; u < ST; ++u) {
+        issue_a(u, u);
+        if (!GROUPED) issue_w(u, u);
+    }
+    dma_wait_barrier<(ST - 1) * (GROUPED ? NA : NI)>();
+    Sf sc = load_s(0);
+    Wf wf = load_w(0, kg);                                           // kg: 0 unless KW 2
+    Af af = load_a(0, kg, 0);
+    int buf = 0;                                                     // of unit u
+    auto unit = [&](int u, auto p_, auto whole_) {                   // whole: both halves of a unit of two
+        constexpr int P = p_();                                      // u % GU
+        if (GU % ST == 0) buf = P % ST;                              // known here then
+        const int next = buf + 1 == ST ? 0 : buf + 1;
+        // younger than the codes of unit u + 1: those of ST - 2 units and the scales issued with them (after units of P 0)
+        constexpr int scales = [] { int n = 0; for (int j = 1; j <= ST - 2; ++j) n += (P + 2 * GU - j) % GU == 0; return n; }();
+        constexpr int young = (ST - 2) * NI + scales * NS;
+        auto block = [&](auto last_, int half, auto d_) {            // half: of the unit; d: of the group of scales
+            constexpr bool LAST = last_();
+            constexpr int D = d_();
+            Wf wn;
+#pragma unroll
+            for (int i = 0; i < RB; ++i) {
+                Af an;
+                Sf sn = sc;
+                if (i + 1 < RB) {
+                    an = load_a(buf, half, i + 1);
+                    if (!LAST && i == RB - 2) wn = load_w(buf, 1);
+                } else if (!LAST) {
+                    if (RB == 1) wn = load_w(buf, 1);
+                    an = load_a(buf, 1, 0);
+                } else {
+                    // (grouped: the first units' weights are older than they are counted here)
+                    if (GROUPED && ST > 2 && u < ST - 2) dma_wait_barrier<0>();
+                    else dma_wait_barrier<young>();
+                    if (P == 0) issue_scales(u / GU + 2);
+                    issue_a(u + ST, buf);
+                    issue_w(u + ST, buf);
+                    // half of its buffer that the next unit (or this wave in it) starts with
+                    const int f = KW == 2 ? kg : UH * (u + 1) - k_at(u + 1);
+                    wn = load_w(next, f);
+                    an = load_a(next, f, 0);
+                    if (P == GU - 1) sn = load_s(u / GU + 1);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (!GROUPED || i < nrb) {                           // wave-uniform
+#pragma unroll
+                    for (int e = 0; e < RH; ++e)
+#pragma unroll
+                        for (int j = 0; j < CB; ++j)
+                            acc[RH * i + e][j] = mfma16<FMT, OUT == WZY_F32, D, D>(operand4(wf.v[j]), operand_of<FMT>(af.v[e]), acc[RH * i + e][j],
+                                                                                   sc.w[j], sc.a[RH * i + e]);
+                }
+                af = an;
+                sc = sn;
+            }
+            wf = wn;
+        };
+        if constexpr (UH == 1) {
+            block(std::true_type(), 0, p_);
+        } else if constexpr (KW == 2) {
+            // a wave's byte of its scales is shifted to the even one; a unit with a second half only counts for the waves that take it
+            if constexpr (whole_()) block(std::true_type(), 0, std::integral_constant<int, 2 * P>());
+            else {
+                if (kg == 0) sc = Sf{}, af = Af{};                   // zeros (under scales of 2^-127)
+                block(std::true_type(), 0, std::integral_constant<int, 2 * P>());
+            }
+        } else {
+            // the last unit of an odd number of halves has a second half only; its scale is there twice (load_s)
+            if constexpr (whole_()) block(std::false_type(), 0, std::integral_constant<int, 2 * P>());
+            block(std::true_type(), 1, std::integral_constant<int, 2 * P + 1>());
+        }
+        buf = next;
+    };
+    // Whole groups of four halves, then what is left (branches inside the loop would cost copies of the accumulators).
+    constexpr std::integral_constant<int, 0> p0{};
+    constexpr std::integral_constant<int, 1> p1{};
+    constexpr std::integral_constant<int, 2> p2{};
+    constexpr std::integral_constant<int, 3> p3{};
+    int u = 0;
+    const int left = halves & 3;
+    for (int n = halves >> 2; n > 0; --n, u += GU) {
+        unit(u, p0, std::true_type());
+        unit(u + 1, p1, std::true_type());
+        if constexpr (UH == 1) {
+            unit(u + 2, p2, std::true_type());
+            unit(u + 3, p3, std::true_type());
+        }
+    }
+    if constexpr (UH == 1) {
+        if (left > 0) unit(u, p0, std::true_type());
+        if (left > 1) unit(u + 1, p1, std::true_type());
+        if (left > 2) unit(u + 2, p2, std::true_type());
+    } else {
+        if (left == 1) unit(u, p0, std::false_type());
+        if (left > 1) unit(u, p0, std::true_type());
+        if (left > 2) unit(u + 1, p1, std::false_type());
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                 // no load outlives the workgroup's LDS
+    if constexpr (KW == 2) {                                         // the two halves' sums meet
+        __syncthreads();
+        v4f_t* const part = (v4f_t*) s_buf + wt * (RH * CB * 64) + lane;
+        if (kg == 1) {
+#pragma unroll
+            for (int i = 0; i < RH; ++i)
+#pragma unroll
+                for (int j = 0; j < CB; ++j) part[(i * CB + j) * 64] = acc[i][j];
+        }
+        __syncthreads();
+        if (kg == 1) return;
+#pragma unroll
+        for (int i = 0; i < RH; ++i)
+#pragma unroll
+            for (int j = 0; j < CB; ++j) acc[i][j] += part[(i * CB + j) * 64];
+    }
+    store_tile<OUT, RH * RB, CB, PAIR>(g, gather, whole_tile<OUT>(g, n0, TN), row0, rows, wr, n0 + wc, acc);
+}
+
+constexpr int CUS = 256;
+
+// the direct-to-LDS form takes whole steps, aligned scale dwords and 32-bit offsets from its bases
+bool dma_ok(const MxGemm& g, bool grouped) {
+    const bool near = !(grouped && g.row_ids) || (int64_t) g.a_rows * std::max(g.a.ldc, g.a.lds) < (int64_t) 1 << 32;
+    return g.K % 128 == 0 && g.K >= 512 && near && (g.a.lds | g.w.lds) % 4 == 0 && ((uintptr_t) g.a.scales | (uintptr_t) g.w.scales) % 4 == 0;
+}
+
+enum Tile { T256x256, T128x128, T64x128, T64x64, T32x128, T32x64, T16x64 };
+constexpr int TILE_M[] = {256, 128, 64, 64, 32, 32, 16}, TILE_N[] = {256, 128, 128, 64, 128, 64, 64};
+
+// Tiles of a dense product: a CU's time for n tiles is that of n / 2 pairs beside each other and of an odd one (256 x 256
+// tiles have a CU to themselves); the least of them is taken.  Measured, us for 128 k, {alone, a pair}.  What it decides, for instance
+// (E4M3 to bf16, us): 250 x 2,048 x 6,144 32x64 9.8, 64x64 12.7, 64x128 18.6; 1,024 x 2,048 x 2,048 64x128 8.9, 64x64 9.2, 128x128 12.8;
+// 2,048 x 12,288 x 2,048 128x128 51, 256x256 61, 64x128 60; 8,192 x 6,144 x 2,048 256x256 93, 128x128 100.
+Tile dense_tile(const MxGemm& g, bool e8, bool f32) {
+    constexpr Tile kind[] = {T256x256, T128x128, T64x128, T64x64, T32x64};
+    constexpr float cost[3][5][2] = {{{1.62f, 3.24f}, {0.62f, 0.96f}, {0.36f, 0.58f}, {0.24f, 0.40f}, {0.17f, 0.28f}},   // E4M3
+                                     {{1.06f, 2.12f}, {0.40f, 0.67f}, {0.27f, 0.46f}, {0.19f, 0.29f}, {0.14f, 0.24f}},   // E2M1
+                                     {{9.00f, 9.00f}, {0.95f, 1.70f}, {0.65f, 1.10f}, {0.38f, 0.62f}, {0.25f, 0.37f}}};  // E4M3 to fp32
+    const auto& c = cost[!e8 ? 1 : f32 ? 2 : 0];
+    Tile best = T32x64;
+    float least = 0.f;
+    for (int i = e8 && f32 ? 1 : 0; i < 5; ++i) {                  // E4M3 to fp32 has no 256 x 256 (its registers spill)
+        const int64_t t = (int64_t) ((g.M + TILE_M[kind[i]] - 1) / TILE_M[kind[i]]) * ((g.N + TILE_N[kind[i]] - 1) / TILE_N[kind[i]]);
+        const int64_t n = (t + CUS - 1) / CUS;
+        const float us = (float) (n / 2) * c[i][1] + (float) (n % 2) * c[i][0];
+        if (least == 0.f || us < least) least = us, best = kind[i];
+    }
+    return best;
+}
+// Tiles of a product per group, by the rows of a group that has any.  Measured at 512 groups, N 1,024, K 2,048, E4M3 to bf16, us: 6 rows
+// 16x64 106, 32x128 108 (to fp32 117, 134); 12 rows 128, 118, 64x128 132; 20 rows 32x128 126, 64x128 134; 40 rows 168, 149, 128x128 164; 80
+// rows 64x128 213, 128x128 192; 160 rows 128x128 304, 256x256 367, but E2M1 253, 218.
+Tile grouped_tile(const MxGemm& g, bool e8) {
+    const int rows = g.M / std::min(g.M, g.groups);
+    if (rows <= 8) return T16x64;
+    if (rows <= 25) return T32x128;
+    if (rows <= 56) return T64x128;
+    const bool many = (int64_t) g.groups * ((g.N + 255) / 256) >= 2 * CUS;
+    return !e8 && rows >= 128 && many ? T256x256 : T128x128;
+}
 
 template <int FMT, int OUT, bool GROUPED>
 int launch(MxGemm g, hipStream_t st) {
-    // Grouped: average rows a group decide; every group may end in a part tile, so rows / tile + groups tiles cover
-    // any split (and no more tiles than rows exist).
-    const int avg = GROUPED ? (g.M + g.groups - 1) / g.groups : g.M;
-    auto tiles = [&](int tm) { return GROUPED ? (int) std::min<int64_t>(g.M, (int64_t) g.M / tm + g.groups) : (g.M + tm - 1) / tm; };
-    if (avg <= SKINNY_M) {
-        g.nt = (g.N + 15) / 16;
-        const int64_t grid = (int64_t) g.nt * tiles(16);
-        WZY_REQUIRE(grid < (int64_t) 1 << 31, "wzy_mx_gemm: %lld tiles", (long long) grid);
-        const int ks = std::min(4, (g.K + 511) / 512);
-        mx_skinny_kernel<FMT, OUT, GROUPED><<<(uint32_t) grid, 64 * ks, 0, st>>>(g);
-    } else {
-        constexpr int TM = 128, TN = 128;
-        g.nt = (g.N + TN - 1) / TN;
-        const int64_t grid = (int64_t) g.nt * align_up((size_t) tiles(TM), 8);
-        WZY_REQUIRE(grid < (int64_t) 1 << 31, "wzy_mx_gemm: %lld tiles", (long long) grid);
-        mx_tile_kernel<FMT, OUT, TM, TN, GROUPED><<<(uint32_t) grid, 256, 0, st>>>(g);
+    constexpr bool E8 = FMT == WZY_MX_E4M3;
+    auto go = [&](auto kernel, int tm, int tn, int threads) {
+        // every group may end in a part tile, so rows / tile + groups tiles cover any split (and no more than there are rows)
+        const int64_t mt = GROUPED ? std::min<int64_t>(g.M, (int64_t) g.M / tm + g.groups) : ((int64_t) g.M + tm - 1) / tm;
+        const int64_t nt = ((int64_t) g.N + tn - 1) / tn;
+        const int64_t grid = GROUPED ? (mt + 7) / 8 * 8 * nt : (mt * nt + 7) / 8 * 8;
+        WZY_REQUIRE(grid < (int64_t) 1 << 31, "wzy_mx_%sgemm: %lld tiles", GROUPED ? "grouped_" : "", (long long) grid);
+        g.mt = (int) mt;
+        g.nt = (int) nt;
+        kernel<<<(uint32_t) grid, threads, 0, st>>>(g);
+        WZY_LAUNCH_CHECK();
+        return WZY_OK;
+    };
+    const bool dma = dma_ok(g, GROUPED);
+    if constexpr (!GROUPED) {
+        // Up to 16 rows: 16 x 64 tiles where there are enough of them, or K split over the waves.  1 row, E4M3 to fp32, us: N 2,048, K
+        // 2,048 5.0 against 4.8; N 2,048, K 6,144 9.1, 5.9; N 12,288, K 2,048 5.7, 6.6; 4 x 151,936 x 2,048 35, 56.
+        if (g.M <= 16 && !(dma && g.N > 4096)) {
+            mx_skinny_kernel<FMT, OUT><<<(g.N + 15) / 16, 64 * std::min(8, (g.K + 511) / 512), 0, st>>>(g);
+            WZY_LAUNCH_CHECK();
+            return WZY_OK;
+        }
     }
-    WZY_LAUNCH_CHECK();
-    return WZY_OK;
+    if (!dma) {
+        // the largest tile that still gives every CU one
+        const int64_t m = GROUPED ? std::min(g.M, g.groups) : 1, r = GROUPED ? g.M / m : g.M;
+        auto enough = [&](int tm, int tn) { return r > tm / 2 && m * ((r + tm - 1) / tm) * ((g.N + tn - 1) / tn) >= CUS; };
+        if (enough(128, 128)) return go(mx_any_kernel<FMT, OUT, 128, 128, 2, 2, GROUPED>, 128, 128, 256);
+        if (enough(64, 64)) return go(mx_any_kernel<FMT, OUT, 64, 64, 2, 2, GROUPED>, 64, 64, 256);
+        return go(mx_any_kernel<FMT, OUT, 32, 64, 2, 2, GROUPED>, 32, 64, 256);
+    }
+    const Tile t = GROUPED ? grouped_tile(g, E8) : g.M <= 16 ? T16x64 : dense_tile(g, E8, OUT == WZY_F32);
+    if (t == T16x64) return go(mx_dma_kernel<FMT, OUT, 16, 64, 1, 2, 2, 256, 3, 2, GROUPED>, 16, 64, 256);
+    if (t == T64x128) return go(mx_dma_kernel<FMT, OUT, 64, 128, 1, 4, 1, 256, 2, 2, GROUPED>, 64, 128, 256);
+    if constexpr (GROUPED) {
+        if (t == T32x128) return go(mx_dma_kernel<FMT, OUT, 32, 128, 1, 4, 1, 256, 3, 2, GROUPED>, 32, 128, 256);
+    } else {
+        if (t == T32x64) return go(mx_dma_kernel<FMT, OUT, 32, 64, 2, 2, 1, 256, 3, 2, GROUPED>, 32, 64, 256);
+        if (t == T64x64) return go(mx_dma_kernel<FMT, OUT, 64, 64, 2, 2, 1, 256, 3, 2, GROUPED>, 64, 64, 256);
+    }
+    if constexpr (!E8 || (!GROUPED && OUT != WZY_F32)) {
+        if (t == T256x256) return go(mx_dma_kernel<FMT, OUT, 256, 256, 2, 4, 1, E8 ? 128 : 256, E8 ? 3 : 2, 2, GROUPED>, 256, 256, 512);
+    }
+    return go(mx_dma_kernel<FMT, OUT, 128, 128, 2, 2, 1, E8 ? 128 : 256, 2, 2, GROUPED>, 128, 128, 256);
 }
 template <bool GROUPED>
 int dispatch(const MxGemm& g, int fmt, hipStream_t st) {
@@ -438,9 +853,10 @@ extern "C" int wzy_mx_grouped_gemm(const wzy_mx_mat* a, int a_rows, const int* r
     MxGemm g{};
     g.y = y; g.ldy = ldy; g.M = M; g.N = N; g.K = K; g.y_type = y_type; g.a_rows = a_rows;
     g.row_ids = row_ids; g.offsets = offsets; g.groups = groups;
-    WZY_REQUIRE(groups >= 1 && groups <= 65536 && a_rows >= 0, "%s: %d groups (1 .. 65,536), %d rows of a", who, groups, a_rows);
+    WZY_REQUIRE(groups >= 1 && groups <= 65536, "%s: %d groups (1 .. 65,536)", who, groups);
     WZY_TRY(check_gemm(who, a, w, g));
     if (M == 0 || N == 0) return WZY_OK;
+    WZY_REQUIRE(a_rows >= 1, "%s: %d rows of a", who, a_rows);
     WZY_REQUIRE(offsets, "%s: offsets is null", who);
     WZY_REQUIRE(row_ids || a_rows >= M, "%s: %d rows of a for %d entries without row_ids", who, a_rows, M);
     return dispatch<true>(g, a->fmt, as_stream(stream));
