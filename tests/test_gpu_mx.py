@@ -543,3 +543,153 @@ def test_no_rows_launch_nothing(wz, gpu):
     wz.wzy_mx_grouped_gemm(None, 0, None, None, None, 4, 0, 5, 64, None, F32, 5, None)
     wz.wzy_device_sync()
     assert (q.read()[0] == FILL).all()
+
+
+# ---- every tile, whole units of K and any K ---------------------------------------------------------------
+def check_in_rough(got, a, w, t):
+    """all of y: 8 products are cut at 13 bits below the largest of them, so by 8 * 2^-12 of it at most; each of the sums of eights
+    rounds to 24 bits; the output to its type"""
+    want, s = a @ w.T, np.abs(a) @ np.abs(w).T
+    assert (np.abs(got - want) <= (2.0 ** -9 + a.shape[1] / 8 * 2.0 ** -23) * s + {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}[t] * np.abs(want)
+            + 2.0 ** -24).all()
+
+
+def check_large(got, a, w, fmt, t):
+    """the exact bound at rows and columns in strides that meet every place of a tile in turn, the rough one everywhere"""
+    m, n = max(1, a.shape[0] // 50), max(1, w.shape[0] // 60)
+    i, j = np.unique(np.r_[0:len(a):m, len(a) - 1]), np.unique(np.r_[0:len(w):n, len(w) - 1])
+    check_product(got[np.ix_(i, j)], a[i], w[j], fmt, t)
+    check_in_rough(got, a, w, t)
+
+
+TILE_SHAPES = [(5, 4100, 32), (16, 4200, 768), (1, 5000, 544), (9, 4097, 1056), (250, 600, 672), (250, 600, 512), (700, 1300, 608),
+               (700, 1300, 1024), (1030, 2060, 96), (1030, 2060, 768), (2050, 2100, 544), (2050, 2100, 512), (4100, 4090, 512)]
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("M,N,K", TILE_SHAPES)
+def test_gemm_every_tile(wz, gpu, fmt, t, M, N, K):
+    rng = np.random.default_rng(M + N + K)
+    a, av = random_mx(rng, M, K, fmt)
+    w, wv = random_mx(rng, N, K, E2M1)
+    y = out_rows(M, N, t)
+    wz.wzy_mx_gemm(a.ref(), w.ref(), M, N, K, y.ptr, t, N, None)
+    check_large(read_rows(y, N, t), av, wv, fmt, t)
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("K", list(range(32, 33 * 32, 32)))
+def test_gemm_every_tail(wz, gpu, fmt, K):
+    """every number of blocks up to two groups of scales: a skinny call, small tiles, 16 x 64 tiles; unaligned scale rows"""
+    rng = np.random.default_rng(K)
+    for M, N, sgap in [(3, 40, 1), (33, 65, 3), (40, 70, 0), (7, 4112, 0)]:
+        cols = np.r_[0:N:max(1, N // 20), N - 1]
+        a, av = random_mx(rng, M, K, fmt, sgap=sgap)
+        w, wv = random_mx(rng, N, K, E2M1, sgap=sgap)
+        for t in (F32, BF16):
+            y = out_rows(M, N, t)
+            wz.wzy_mx_gemm(a.ref(), w.ref(), M, N, K, y.ptr, t, N, None)
+            check_product(read_rows(y, N, t)[:, cols], av, wv[cols], fmt, t)
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("K", [512, 544, 768, 1120])
+def test_gemm_neighbours_of_a_row_do_not_show(wz, gpu, fmt, K):
+    """what lies behind a row's codes and scales, NaN codes and scales of 255, is not multiplied"""
+    rng = np.random.default_rng(K)
+    for M, N in [(3, 30), (9, 4100), (40, 70), (300, 520), (1100, 2100)]:
+        m, mv = random_mx(rng, M, K, fmt)
+        w, wv = random_mx(rng, N, K, E2M1)
+        for x in (m, w):
+            c, s = x.c.numpy(), x.s.numpy()
+            c, s = np.pad(c, ((0, 0), (0, 32)), constant_values=0xFF), np.pad(s, ((0, 0), (0, 5 if K % 256 else 4)), constant_values=0xFF)
+            x.c, x.s = DA.from_numpy(c), DA.from_numpy(s)
+            x.m = wzy_amd.MxMat(x.c.ptr, x.s.ptr, c.shape[1], s.shape[1], x.fmt)
+        y = out_rows(M, N, BF16)
+        wz.wzy_mx_gemm(m.ref(), w.ref(), M, N, K, y.ptr, BF16, N, None)
+        check_large(read_rows(y, N, BF16), mv, wv, fmt, BF16)
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("per,groups,N,K", [(5, 9, 130, 512), (5, 9, 130, 288), (20, 7, 260, 768), (20, 7, 260, 1056), (50, 5, 200, 512),
+                                            (50, 5, 200, 608), (90, 4, 300, 1024), (90, 4, 300, 96), (300, 3, 90, 544)])
+def test_grouped_every_tile(wz, gpu, fmt, t, per, groups, N, K):
+    rng = np.random.default_rng(per + N + K)
+    sizes = rng.multinomial(per * groups, np.arange(groups) / np.arange(groups).sum())    # an empty one first
+    M = int(sizes.sum())
+    grouped(wz, rng, list(sizes), M, N, K, fmt, t)
+    ids = rng.integers(-2, M // 2 + 3, M + 5)
+    grouped(wz, rng, list(sizes), M + 5, N, K, fmt, t, a_rows=M // 2 + 1, ids=ids, pad=1)
+
+
+@pytest.mark.parametrize("K", [512, 544])
+def test_grouped_largest_tiles(wz, gpu, K):
+    """enough rows and tiles for 256 x 256 (E2M1); a group's weights are the first one's, rolled by its number"""
+    rng = np.random.default_rng(K)
+    G, N, per = 64, 2048, 130
+    codes = rng.integers(0, 16, (N, K)).astype(np.uint8)
+    scales = rng.integers(125, 130, (N, K // 32)).astype(np.uint8)
+    wv = R.dequantize(codes, scales, E2M1)
+    w = Mat(G * N, K, E2M1, codes=np.concatenate([np.roll(codes, g, 0) for g in range(G)]),
+            scales=np.concatenate([np.roll(scales, g, 0) for g in range(G)]))
+    sizes = rng.multinomial(G * per, np.ones(G) / G)
+    M = int(sizes.sum())
+    off = np.r_[0, np.cumsum(sizes)].astype(np.int32)
+    a, av = random_mx(rng, M, K, E2M1)
+    y, do = out_rows(M, N, BF16), DA.from_numpy(off)
+    wz.wzy_mx_grouped_gemm(a.ref(), M, None, w.ref(), do.ptr, G, M, N, K, y.ptr, BF16, N, None)
+    got = read_rows(y, N, BF16)
+    for g in range(G):
+        i = slice(off[g], off[g + 1])
+        check_large(got[i], av[i], np.roll(wv, g, 0), E2M1, BF16)
+
+
+class FarRows:
+    """rows of a matrix `stride` bytes apart: only the rows themselves are written"""
+
+    def __init__(self, wz, codes, scales, fmt, stride):
+        p = R.pack(codes, fmt)
+        self.rows = len(p)
+        self.c, self.s = DA(((self.rows - 1) * stride + p.shape[1],), np.uint8), DA.from_numpy(scales)
+        for i, row in enumerate(np.ascontiguousarray(p)):
+            wz.wzy_memcpy_h2d(self.c.ptr + i * stride, row.ctypes.data, row.nbytes, None)
+        self.m = wzy_amd.MxMat(self.c.ptr, self.s.ptr, stride, scales.shape[1], fmt)
+
+    def ref(self):
+        return C.byref(self.m)
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("K", [512, 544])
+def test_rows_far_apart(wz, gpu, fmt, K):
+    """the widest rows allowed: offsets past 2^31 inside a tile, past 2^32 between tiles and among gathered rows"""
+    rng = np.random.default_rng(K)
+    stride, M, N = 2 ** 23 - 16, 600, 90
+    codes = rng.integers(0, 16 if fmt == E2M1 else 126, (M, K)).astype(np.uint8)
+    scales = rng.integers(125, 130, (M, K // 32)).astype(np.uint8)
+    a, av = FarRows(wz, codes, scales, fmt, stride), R.dequantize(codes, scales, fmt)
+    w, wv = random_mx(rng, 2 * N, K, E2M1)
+    far, farv = FarRows(wz, codes[:N] & 15, scales[:N], E2M1, stride), R.dequantize(codes[:N] & 15, scales[:N], E2M1)
+    for t in (F32, BF16):
+        y = out_rows(M, N, t)
+        wz.wzy_mx_gemm(a.ref(), far.ref(), M, N, K, y.ptr, t, N, None)
+        check_large(read_rows(y, N, t), av, farv, fmt, t)
+        ids = rng.integers(0, M, M)
+        ids[[0, 7]] = [-1, M]
+        y, di = out_rows(M, N, t), DA.from_numpy(ids.astype(np.int32))
+        do = DA.from_numpy(np.array([0, M // 3, M], np.int32))
+        wz.wzy_mx_grouped_gemm(a.ref(), M, di.ptr, w.ref(), do.ptr, 2, M, N, K, y.ptr, t, N, None)
+        got, x = read_rows(y, N, t), av[ids.clip(0, M - 1)]
+        x[[0, 7]] = 0
+        check_large(got[:M // 3], x[:M // 3], wv[:N], fmt, t)
+        check_large(got[M // 3:], x[M // 3:], wv[N:], fmt, t)
+        y = out_rows(300, N, t)                                   # not gathered: the second group's rows begin past 2^30
+        do = DA.from_numpy(np.array([0, 40, 300], np.int32))
+        wz.wzy_mx_grouped_gemm(a.ref(), M, None, w.ref(), do.ptr, 2, 300, N, K, y.ptr, t, N, None)
+        got = read_rows(y, N, t)
+        check_large(got[:40], av[:40], wv[:N], fmt, t)
+        check_large(got[40:], av[40:300], wv[N:], fmt, t)
+    for m in (a, far):
+        m.c.free()

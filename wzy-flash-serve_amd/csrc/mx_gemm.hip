@@ -17,11 +17,11 @@
 // set and the others: each part spans 11 bits, so both products are whole, at twice the MFMA work.
 //
 // Three kernels, chosen in launch():
-//   mx_dma     tiles of 16 x 64 to 256 x 256 through LDS, filled by direct-to-LDS loads several steps ahead; K a multiple of 128
-//   mx_any     tiles of 32 x 64 to 128 x 128 through LDS and registers: any K, any alignment of the scales
-//   mx_skinny  up to 16 rows and few columns, or any K: operands straight from memory, K split over a workgroup's waves
-// mx_dma and mx_any serve the product per group too: a workgroup finds its group's tile from the offsets by itself, so
-// there is no preparing launch, no workspace and nothing for the host to know.
+//   mx_dma     tiles of 16 x 64 to 256 x 256 through LDS, filled by direct-to-LDS loads several steps ahead
+//   mx_skinny  up to 16 rows and few columns: operands straight from memory, K split over a workgroup's waves
+//   mx_far     rows gathered from more than 4 GiB: 64 x 64 tiles through registers, with 64-bit addresses
+// mx_dma and mx_far serve the product per group: a workgroup finds its group's tile from the offsets by itself, so there is no
+// preparing launch, no workspace and nothing for the host to know.
 #include <algorithm>
 
 #include "wzy_mx.h"
@@ -156,7 +156,7 @@ WZY_DEV bool find_tile(const MxGemm& g, int t, int& group, int& row0, int& rows)
             group = __builtin_amdgcn_readlane(gg, src);
             row0 = __builtin_amdgcn_readlane(r0, src);
             rows = __builtin_amdgcn_readlane(n, src);
-            return true;
+            return rows > 0;                                       // (0: only where offsets that fall make the counts wrap)
         }
         before = __builtin_amdgcn_readlane(before + pre, 63);
     }
@@ -187,7 +187,6 @@ WZY_DEV bool tile_of(const MxGemm& g, int& mi, int& ni) {
 
 // row of a that entry e reads; -1: zeros
 WZY_DEV int entry_row(const MxGemm& g, int e) {
-    if (!g.row_ids) return e;
     const int r = g.row_ids[e];
     return (unsigned) r < (unsigned) g.a_rows ? r : -1;
 }
@@ -312,11 +311,12 @@ WZY_DEV bool whole_tile(const MxGemm& g, int n0, int tn) {
     return n0 + tn <= g.N && (((uintptr_t) g.y | (uintptr_t) g.ldy * (OUT == WZY_F32 ? 4 : 2)) & 15) == 0;
 }
 
-// Tiles of TM x TN for any K and any alignment of the scale rows.  WM x WN waves; wave (i, j) holds TM / WM rows by TN / WN columns.
-// K goes in steps of 128 through two LDS buffers and two register sets: step k + 2 loads while step k multiplies.
-template <int FMT, int OUT, int TM, int TN, int WM, int WN, bool GROUPED>
-__global__ void __launch_bounds__(64 * WM * WN, 2) mx_any_kernel(MxGemm g) {
-    constexpr bool E8 = FMT == WZY_MX_E4M3, PAIR = OUT != WZY_F32 && TN / 16 / WN % 2 == 0;
+// Product per group with rows gathered from more than 4 GiB.  Each wave holds 32 rows by 32 columns of the tile.  K goes in steps of 128
+// through two LDS buffers and two register sets: step k + 2 loads while step k multiplies.
+template <int FMT, int OUT>
+__global__ void __launch_bounds__(256, 2) mx_far_kernel(MxGemm g) {
+    constexpr int TM = 64, TN = 64, WM = 2, WN = 2;
+    constexpr bool E8 = FMT == WZY_MX_E4M3, PAIR = OUT != WZY_F32;
     constexpr int T = 64 * WM * WN, RB = TM / 16 / WM, CB = TN / 16 / WN;
     constexpr int AP = E8 ? 8 : 4, WP = 4;                         // 16-byte pieces of a row per step
     constexpr int NA = (TM * AP + T - 1) / T, NW = (TN * WP + T - 1) / T, NS = (TM + TN + T - 1) / T;
@@ -324,13 +324,9 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mx_any_kernel(MxGemm g) {
     __shared__ uint4 s_w[2][TN * WP];
     __shared__ uint32_t s_sc[2][TM + TN];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q4 = lane >> 4, lr = lane & 15;
-    int mi, ni;
-    if (!tile_of<GROUPED>(g, mi, ni)) return;
+    int mi, ni, group, row0, rows;
+    if (!tile_of<true>(g, mi, ni) || !find_tile<TM>(g, mi, group, row0, rows)) return;
     const int n0 = ni * TN;
-    int row0 = mi * TM, rows = min(g.M - row0, TM), group = 0;
-    if constexpr (GROUPED) {
-        if (!find_tile<TM>(g, mi, group, row0, rows)) return;
-    } else if (rows <= 0) return;
     const int nblk = g.K / 32, steps = (nblk + 3) / 4;
     const uint8_t* const wbase = g.w.codes + ((size_t) group * g.N + n0) * g.w.ldc;
     const uint8_t* const wsbase = g.w.scales + ((size_t) group * g.N + n0) * g.w.lds;
@@ -341,7 +337,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mx_any_kernel(MxGemm g) {
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
         const int p = tid + T * i, ar = entry_row(g, row0 + min(p / AP, rows - 1));
-        aok[i] = ar >= 0 && p < TM * AP;
+        aok[i] = ar >= 0;
         ap[i] = g.a.codes + (size_t) max(ar, 0) * g.a.ldc + 16 * (p % AP);
     }
 #pragma unroll
@@ -375,12 +371,12 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mx_any_kernel(MxGemm g) {
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
             const int p = tid + T * i;
-            if (TM * AP % T == 0 || p < TM * AP) s_a[b][p / AP * AP + ((p % AP) ^ swz_a<AP>(p / AP))] = t.a[i];
+            s_a[b][p / AP * AP + ((p % AP) ^ swz_a<AP>(p / AP))] = t.a[i];
         }
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
             const int p = tid + T * i;
-            if (TN * WP % T == 0 || p < TN * WP) s_w[b][p / WP * WP + ((p % WP) ^ swz_w<WP, PAIR>(p / WP))] = t.w[i];
+            s_w[b][p / WP * WP + ((p % WP) ^ swz_w<WP, PAIR>(p / WP))] = t.w[i];
         }
 #pragma unroll
         for (int i = 0; i < NS; ++i)
@@ -428,11 +424,11 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mx_any_kernel(MxGemm g) {
         store(0, t0);
         __syncthreads();
     }
-    store_tile<OUT, RB, CB, PAIR>(g, GROUPED && g.row_ids, whole_tile<OUT>(g, n0, TN), row0, rows, wr, n0 + wc, acc);
+    store_tile<OUT, RB, CB, PAIR>(g, true, whole_tile<OUT>(g, n0, TN), row0, rows, wr, n0 + wc, acc);
 }
 
 // ---- tiles fed by direct-to-LDS loads -----------------------------------------------------------------------
-// K a multiple of 128 from 512 on, scale rows aligned to 4 bytes.  Codes and scales go from memory to LDS without registers, in
+// Codes and scales go from memory to LDS without registers, in
 // units of UK k through ST buffers.  The loads are counted, so a wave waits for the unit it needs and leaves the later ones
 // in flight, and one barrier a unit tells every wave that all parts of the next unit have landed and that this unit's
 // buffer is free.  (Inline assembly: the compiler would have every LDS read wait for every such load.  The loads have no
@@ -444,6 +440,12 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mx_any_kernel(MxGemm g) {
 // waits for the next unit's loads and meets the others; all its reads of this unit are done then, so the buffer takes the
 // loads of unit u + ST, and the next unit's first operands are read under the last row block's MFMAs (314 -> 303; tiles in
 // bands, tile_of: 285; 16x16x128 instructions: 271).
+//
+// Two forms.  Where K is whole units, every row's scales begin at a dword and there are at least 16 bytes of them, nothing is checked.
+// ANY takes every K and alignment: loads are kept inside the matrix, blocks past a row's end count as zeros, and scales come a
+// dword a lane and are shifted into place on the way out of LDS.  (That form for aligned calls too: 5 to 10 % slower, up to 60 % where
+// its registers spill, 256 x 256, so it has no such tile.  ANY against 64 x 64 and 128 x 128 tiles through registers, E4M3 to bf16, K 2,080, us:
+// 4 x 151,936 45, 89; 100 x 2,048 5.9, 7.2; 300 x 2,048 x 6,176 15, 28; 8,192 x 6,144 129, 142; per group, 512 groups, 6,000 rows 157, 192.)
 //
 // WM x WN waves hold TM / WM rows by TN / WN columns each; KW 2: two such sets, one for each 128 of a unit, whose sums meet
 // at the end (16 x 64 tiles, where a unit's chain of LDS reads and MFMAs is what takes the time: 1 x 12,288 x 2,048 to fp32 6.8 ->
@@ -461,28 +463,40 @@ WZY_DEV void dma16(uint32_t lds, uint32_t off, const uint8_t* base) {
                                          (uint32_t) __builtin_amdgcn_readfirstlane((int) b));
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
+// 64 lanes x 4 bytes, likewise
+WZY_DEV void dma4(uint32_t lds, uint32_t off, const uint8_t* base) {
+    const uint64_t b = (uint64_t) (uintptr_t) base;
+    lds = (uint32_t) __builtin_amdgcn_readfirstlane((int) lds);
+    base = (const uint8_t*) (uintptr_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (b >> 32)) << 32 |
+                                         (uint32_t) __builtin_amdgcn_readfirstlane((int) b));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
 // this wave's loads but the last N have landed and its LDS reads are done; then all waves meet
 template <int N>
 WZY_DEV void dma_wait_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-template <int FMT, int OUT, int TM, int TN, int WM, int WN, int KW, int UK, int ST, int OCC, bool GROUPED>
+template <int FMT, int OUT, int TM, int TN, int WM, int WN, int KW, int UK, int ST, int OCC, bool GROUPED, bool ANY>
 __global__ void __launch_bounds__(64 * WM * WN * KW, OCC) mx_dma_kernel(MxGemm g) {
     constexpr bool E8 = FMT == WZY_MX_E4M3;
     // waves; a wave's row blocks of RH x 16 rows, column blocks of 16
     constexpr int NWV = WM * WN * KW, RH = TM / WM >= 32 ? 2 : 1, RB = TM / WM / (16 * RH), CB = TN / 16 / WN;
     constexpr int AP = UK / (E8 ? 16 : 32), WP = UK / 32;            // 16-byte pieces of a row of a and of w per unit
-    constexpr int A_B = TM * AP * 16, W_B = TN * WP * 16, S_B = (TN + (TM + 63) / 64 * 64) * 16;
+    constexpr int A_B = TM * AP * 16, W_B = TN * WP * 16, S_B = (TN + (ANY ? TM : (TM + 63) / 64 * 64)) * 16;
     // wave-wide loads of a step; where they do not divide by the waves, some are issued twice (same bytes, same place), so
     // that every wave has the same number in flight
-    constexpr int LA = A_B / 1024, LW = W_B / 1024, LS = S_B / 1024;
+    constexpr int LA = A_B / 1024, LW = W_B / 1024, LS = S_B / (ANY ? 256 : 1024);
     constexpr int NA = (LA + NWV - 1) / NWV, NW = (LW + NWV - 1) / NWV, NS = (LS + NWV - 1) / NWV, NI = NA + NW;
     static_assert(TM % 16 == 0 && TN % 64 == 0 && A_B % 1024 == 0 && RB >= 1 && CB >= 1 && ST >= 2, "tile");
     static_assert((ST - 2) * NI + NS < 64, "loads in flight are counted in six bits");
     static_assert(KW == 1 || (KW == 2 && UK == 256 && RB == 1 && (KW - 1) * WM * WN * RH * CB * 1024 <= ST * (A_B + W_B)), "waves along k");
     static_assert(ST - 2 < 512 / UK, "the count of scales in flight holds from the first unit on");
-    __shared__ __align__(1024) uint8_t s_buf[ST * (A_B + W_B) + 2 * S_B];
+    // ANY: a group of scales also takes the next one's first dwords: two buffers will do where those are older than the codes waited
+    // for with them
+    constexpr int SB = !ANY || ST - 2 < 512 / UK - 1 ? 2 : 3;
+    static_assert(ST * (A_B + W_B) + SB * S_B <= 160 * 1024, "LDS");
+    __shared__ __align__(1024) uint8_t s_buf[ST * (A_B + W_B) + SB * S_B];
     constexpr bool PAIR = OUT != WZY_F32 && CB % 2 == 0;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), q4 = lane >> 4, lr = lane & 15;
     int mi, ni;
@@ -495,20 +509,25 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, OCC) mx_dma_kernel(MxGemm g
     const bool gather = GROUPED && g.row_ids;
     const uint8_t* const abase = g.a.codes + (gather ? 0 : (size_t) row0 * g.a.ldc);
     const uint8_t* const asbase = g.a.scales + (gather ? 0 : (size_t) row0 * g.a.lds);
-    const uint8_t* const wbase = g.w.codes + ((size_t) group * g.N + n0) * g.w.ldc;
-    const uint8_t* const wsbase = g.w.scales + ((size_t) group * g.N + n0) * g.w.lds;
+    const size_t wrow0 = (size_t) group * g.N + n0;
+    const uint8_t* const wbase = g.w.codes + wrow0 * g.w.ldc;
+    const uint8_t* const wsbase = g.w.scales + wrow0 * g.w.lds;
     auto a_row = [&](int r) {                                        // row r of the tile, counted from abase
         r = min(r, rows - 1);
         if (!gather) return (uint32_t) r;
         const int id = g.row_ids[row0 + r];
         return (unsigned) id < (unsigned) g.a_rows ? (uint32_t) id : 0u;
     };
-    // Units of UH halves of 128 k; K of an odd number of halves: the last unit of two loads the row's last two and multiplies
-    // the second
-    constexpr int UH = UK / 128, GU = 4 / UH;                        // GU units to a group of scales
-    const int halves = g.K / 128;
+    // ANY: loads that pass the end of a row read on in the matrix, up to its end, and what they bring is replaced by zeros.  Offsets from the bases of the last 16 bytes of codes and the last dword
+    // that holds a scale:
+    const int nblk = g.K / 32;
+    const size_t a_left = (size_t) (g.a_rows - 1 - (gather ? 0 : row0)), w_left = (size_t) (GROUPED ? g.groups : 1) * g.N - 1 - wrow0;
+    const uint32_t as0 = (uint32_t) (uintptr_t) asbase & 3u, ws0 = (uint32_t) (uintptr_t) wsbase & 3u;
+    auto low32 = [](size_t x) { return (uint32_t) min(x, (size_t) 0xFFFFFFF0u); };
+    const uint32_t a_end = low32(a_left * g.a.ldc + (size_t) nblk * (E8 ? 32 : 16) - 16), w_end = low32(w_left * g.w.ldc + (size_t) nblk * 16 - 16);
+    const uint32_t as_end = low32(a_left * g.a.lds + as0 + nblk - 1) & ~3u, ws_end = low32(w_left * g.w.lds + ws0 + nblk - 1) & ~3u;
+    constexpr int UH = UK / 128, GU = 4 / UH;                        // units have UH halves of 128 k, groups of scales GU units
     const uint32_t lds0 = lds_offset(s_buf);
-    auto k_at = [&](int u) { return min(UH * u, halves - UH); };     // first half of unit u; past the end the last unit again
     // LDS position p (16 bytes) of a buffer: row p / pieces, its piece p % pieces permuted by the row
     uint32_t ao[NA], wo[NW], so[NS];
 #pragma unroll
@@ -516,10 +535,15 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, OCC) mx_dma_kernel(MxGemm g
         const int p = ((wave * NW + i) % LW) * 64 + lane, r = p / WP;
         wo[i] = (uint32_t) min(r, g.N - 1 - n0) * (uint32_t) g.w.ldc + 16 * ((p % WP) ^ swz_w<WP, PAIR>(r));
     }
+    const int units = (nblk + 4 * UH - 1) / (4 * UH);
+    auto dma_codes = [&](uint32_t at, uint32_t off, int u, int bytes, uint32_t end, const uint8_t* base) {
+        const uint32_t k = (uint32_t) min(u, units - 1) * bytes;     // past the end the last unit again
+        dma16(at, ANY ? min(off, end - k) : off, base + k);
+    };
     auto issue_w = [&](int u, int buf) {                             // w's codes of unit u
-        const uint8_t* const b = wbase + (size_t) k_at(u) * 64;
 #pragma unroll
-        for (int i = 0; i < NW; ++i) dma16(lds0 + ST * A_B + buf * W_B + ((wave * NW + i) % LW) * 1024, wo[i], b);
+        for (int i = 0; i < NW; ++i)
+            dma_codes(lds0 + ST * A_B + buf * W_B + ((wave * NW + i) % LW) * 1024, wo[i], u, 64 * UH, w_end, wbase);
     };
     // The weights' first loads leave before the row ids, which a's addresses wait for, are there.
     if constexpr (GROUPED) {
@@ -531,25 +555,31 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, OCC) mx_dma_kernel(MxGemm g
         const int p = ((wave * NA + i) % LA) * 64 + lane, r = p / AP;
         ao[i] = a_row(r) * (uint32_t) g.a.ldc + 16 * ((p % AP) ^ swz_a<AP>(r));
     }
+    // Scales.  Aligned rows: a row a lane, 16 bytes for the four halves of a group, the row's last 16 where fewer are left.  ANY: 16 rows
+    // a load, a dword a lane, 4 in a row; a row may begin at any byte, so dwords are counted from the one with its first scale.
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-        const int r = ((wave * NS + i) % LS) * 64 + lane;
-        so[i] = r < TN ? (uint32_t) min(r, g.N - 1 - n0) * (uint32_t) g.w.lds : a_row(r - TN) * (uint32_t) g.a.lds;
+        const int r = ((wave * NS + i) % LS) * (ANY ? 16 : 64) + (ANY ? lane >> 2 : lane);
+        uint32_t t;
+        if (r < TN) t = (uint32_t) min(r, g.N - 1 - n0) * (uint32_t) g.w.lds + (ANY ? ws0 : 0);
+        else t = a_row(r - TN) * (uint32_t) g.a.lds + (ANY ? as0 : 0);   // (only here: a_row reads row_ids)
+        so[i] = ANY ? (t & ~3u) + 4 * (lane & 3) : t;
     }
+    auto scale_at = [&](int q) { return min(16 * q, nblk - 16); };   // byte in an aligned row
     auto issue_a = [&](int u, int buf) {
-        const uint8_t* const b = abase + (size_t) k_at(u) * (E8 ? 128 : 64);
 #pragma unroll
-        for (int i = 0; i < NA; ++i) dma16(lds0 + buf * A_B + ((wave * NA + i) % LA) * 1024, ao[i], b);
+        for (int i = 0; i < NA; ++i)
+            dma_codes(lds0 + buf * A_B + ((wave * NA + i) % LA) * 1024, ao[i], u, (E8 ? 128 : 64) * UH, a_end, abase);
     };
-    // scales of four halves: 16 bytes a row, the row's last 16 where fewer halves are left
-    auto scale_at = [&](int q) { return min(16 * q, 4 * halves - 16); };   // byte in a scale row
-    auto issue_scales = [&](int q) {
-        const uint32_t at = lds0 + ST * (A_B + W_B) + (q & 1) * S_B;
-        const int o = scale_at(q);
+    auto scales_at = [&](int q) { return ST * (A_B + W_B) + (SB == 2 ? q & 1 : q % 3) * S_B; };
+    auto issue_scales = [&](int q) {                                 // of group q
+        const uint32_t at = lds0 + scales_at(q);
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            const int r = ((wave * NS + i) % LS) * 64;
-            dma16(at + r * 16, so[i], (r < TN ? wsbase : asbase) + o);
+            const int r = ((wave * NS + i) % LS) * (ANY ? 16 : 64);
+            const bool w = r < TN;                                   // wave-uniform
+            if constexpr (ANY) dma4(at + r * 16, min(so[i] + 16u * (uint32_t) min(q, nblk / 16 + 1), w ? ws_end : as_end), w ? wsbase - ws0 : asbase - as0);
+            else dma16(at + r * 16, so[i], (w ? wsbase : asbase) + scale_at(q));
         }
     };
     v4f_t acc[RH * RB][CB];
@@ -564,8 +594,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, OCC) mx_dma_kernel(MxGemm g
     const int wl = w_row<PAIR>(0, lr), asw = swz_a<AP>(lr), wsw = swz_w<WP, PAIR>(wl);
     const uint8_t* const la = s_buf + (wr + lr) * (AP * 16);
     const uint8_t* const lw = s_buf + ST * A_B + (wc + wl) * (WP * 16);
-    const uint8_t* const lsw = s_buf + ST * (A_B + W_B) + (wc + wl) * 16;
-    const uint8_t* const lsa = s_buf + ST * (A_B + W_B) + (TN + wr + lr) * 16;
+    const int lsw = (wc + wl) * 16, lsa = (TN + wr + lr) * 16;      // rows of scales
     struct Wf { uint4 v[CB]; };                                      // a half's operands
     struct Af { uint4 v[RH][E8 ? 2 : 1]; };                          // of one row block
     struct Sf { int a[RH * RB], w[CB]; };                            // the scales of the lane's block in four halves, a byte each
@@ -590,35 +619,60 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, OCC) mx_dma_kernel(MxGemm g
         }
         return f;
     };
+    // first byte in its dword of each row of scales that the lane reads, 2 bits each
+    uint32_t first = 0;
+    if constexpr (ANY) {
+#pragma unroll
+        for (int j = 0; j < CB; ++j) first |= ((ws0 + (uint32_t) min(wc + w_row<PAIR>(j, 0) + wl, g.N - 1 - n0) * (uint32_t) g.w.lds) & 3u) << (2 * j);
+#pragma unroll
+        for (int i = 0; i < RH * RB; ++i) first |= ((as0 + a_row(wr + 16 * i + lr) * (uint32_t) g.a.lds) & 3u) << (2 * (CB + i));
+    }
+    static_assert(CB + RH * RB <= 16, "two bits a row");
     const uint32_t pick = 0x0C0C0400u + 0x0101u * (uint32_t) q4;     // byte q4 of one dword, then of another
-    auto load_s = [&](int q) {
-        Sf f;
-        const int o = (q & 1) * S_B, skip = (16 * q - scale_at(q)) / 4;   // 0, or what the row's last 16 bytes start early
-        auto one = [&](const uint8_t* p) {
-            uint4 d = *(const uint4*) p;
-            if (skip & 1) { d.x = d.y; d.y = d.z; d.z = d.w; }       // the last one is there twice then
-            if (skip & 2) { d.x = d.z; d.y = d.w; }
-            return (int) ((__builtin_amdgcn_perm(d.y, d.x, pick) | __builtin_amdgcn_perm(d.w, d.z, pick) << 16) >> (KW == 2 ? 8 * kg : 0));
-        };
-#pragma unroll
-        for (int j = 0; j < CB; ++j) f.w[j] = one(lsw + o + w_row<PAIR>(j, 0) * 16);
-#pragma unroll
-        for (int i = 0; i < RH * RB; ++i) f.a[i] = one(lsa + o + 16 * 16 * i);
-        return f;
+    struct Reader { const uint8_t *here, *next; bool skip; uint32_t in; };   // of a group of scales
+    auto scales_of = [&](int q) {
+        const int n = min(max(nblk - 16 * q - q4 + 3, 0) >> 2, 4);    // the lane's blocks inside the row; the others' scales are 0
+        // skip: the row's last 16 bytes begin two dwords before the group
+        return Reader{s_buf + scales_at(q), s_buf + scales_at(q + 1), scale_at(q) < 16 * q, n == 4 ? ~0u : (1u << (8 * n)) - 1};
     };
-    issue_scales(0);
-    issue_scales(1);
+    auto load_s = [&](const Reader& s, int at, int i) {              // scales of the lane's block in four halves
+        uint4 d = *(const uint4*) (s.here + at);
+        uint32_t in = ~0u;
+        if constexpr (ANY) {
+            const uint32_t e = *(const uint32_t*) (s.next + at), f = first >> (2 * i);   // (its low two bits count)
+            d.x = __builtin_amdgcn_alignbyte(d.y, d.x, f);
+            d.y = __builtin_amdgcn_alignbyte(d.z, d.y, f);
+            d.z = __builtin_amdgcn_alignbyte(d.w, d.z, f);
+            d.w = __builtin_amdgcn_alignbyte(e, d.w, f);
+            in = s.in;
+        } else {
+            if (s.skip) { d.x = d.z; d.y = d.w; }
+        }
+        return (int) (((__builtin_amdgcn_perm(d.y, d.x, pick) | __builtin_amdgcn_perm(d.w, d.z, pick) << 16) & in) >> (KW == 2 ? 8 * kg : 0));
+    };
+    auto load_sw = [&](const Reader& s, Sf& f) {
+#pragma unroll
+        for (int j = 0; j < CB; ++j) f.w[j] = load_s(s, lsw + w_row<PAIR>(j, 0) * 16, j);
+    };
+    auto load_sa = [&](const Reader& s, Sf& f, int i) {               // of row block i
+#pragma unroll
+        for (int e = 0; e < RH; ++e) f.a[RH * i + e] = load_s(s, lsa + 16 * 16 * (RH * i + e), CB + RH * i + e);
+    };
+#pragma unroll
+    for (int q = 0; q < SB; ++q) issue_scales(q);
 #pragma unroll
     for (int u = 0; u < ST; ++u) {
         issue_a(u, u);
         if (!GROUPED) issue_w(u, u);
     }
     dma_wait_barrier<(ST - 1) * (GROUPED ? NA : NI)>();
-    Sf sc = load_s(0);
+    Sf sc;
+    load_sw(scales_of(0), sc);
+    load_sa(scales_of(0), sc, 0);
     Wf wf = load_w(0, kg);                                           // kg: 0 unless KW 2
     Af af = load_a(0, kg, 0);
     int buf = 0;                                                     // of unit u
-    auto unit = [&](int u, auto p_, auto whole_) {                   // whole: both halves of a unit of two
+    auto unit = [&](int u, auto p_, auto tail_, auto one_) {         // tail: the row may end in it; one: in its first half
         constexpr int P = p_();                                      // u % GU
         if (GU % ST == 0) buf = P % ST;                              // known here then
         const int next = buf + 1 == ST ? 0 : buf + 1;
@@ -632,9 +686,10 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, OCC) mx_dma_kernel(MxGemm g
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
                 Af an;
-                Sf sn = sc;
+                Sf sn;
                 if (i + 1 < RB) {
                     an = load_a(buf, half, i + 1);
+                    if (D == 0) load_sa(scales_of(u / GU), sc, i + 1);
                     if (!LAST && i == RB - 2) wn = load_w(buf, 1);
                 } else if (!LAST) {
                     if (RB == 1) wn = load_w(buf, 1);
@@ -643,16 +698,25 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, OCC) mx_dma_kernel(MxGemm g
                     // (grouped: the first units' weights are older than they are counted here)
                     if (GROUPED && ST > 2 && u < ST - 2) dma_wait_barrier<0>();
                     else dma_wait_barrier<young>();
-                    if (P == 0) issue_scales(u / GU + 2);
+                    if (P == 0) issue_scales(u / GU + SB);
                     issue_a(u + ST, buf);
                     issue_w(u + ST, buf);
-                    // half of its buffer that the next unit (or this wave in it) starts with
-                    const int f = KW == 2 ? kg : UH * (u + 1) - k_at(u + 1);
-                    wn = load_w(next, f);
-                    an = load_a(next, f, 0);
-                    if (P == GU - 1) sn = load_s(u / GU + 1);
+                    wn = load_w(next, kg);
+                    an = load_a(next, kg, 0);
+                    if (P == GU - 1) {
+                        load_sw(scales_of(u / GU + 1), sn);
+                        load_sa(scales_of(u / GU + 1), sn, 0);
+                    }
                 }
                 __builtin_amdgcn_sched_barrier(0);
+                if constexpr (ANY && tail_()) {                             // codes past the row's end are zeros
+                    const int in = nblk - 4 * (UH * u + half);       // blocks of this half inside the row
+#pragma unroll
+                    for (int e = 0; e < RH; ++e)
+#pragma unroll
+                        for (int j = 0; j < (E8 ? 2 : 1); ++j)
+                            if ((E8 ? (q4 >> 1) + 2 * j : q4) >= in) af.v[e][j] = make_uint4(0, 0, 0, 0);
+                }
                 if (!GROUPED || i < nrb) {                           // wave-uniform
 #pragma unroll
                     for (int e = 0; e < RH; ++e)
@@ -662,22 +726,20 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, OCC) mx_dma_kernel(MxGemm g
                                                                                    sc.w[j], sc.a[RH * i + e]);
                 }
                 af = an;
-                sc = sn;
+                if (LAST && P == GU - 1 && i == RB - 1) {
+#pragma unroll
+                    for (int j = 0; j < CB; ++j) sc.w[j] = sn.w[j];
+#pragma unroll
+                    for (int e = 0; e < RH; ++e) sc.a[e] = sn.a[e];
+                }
             }
             wf = wn;
         };
-        if constexpr (UH == 1) {
-            block(std::true_type(), 0, p_);
-        } else if constexpr (KW == 2) {
-            // a wave's byte of its scales is shifted to the even one; a unit with a second half only counts for the waves that take it
-            if constexpr (whole_()) block(std::true_type(), 0, std::integral_constant<int, 2 * P>());
-            else {
-                if (kg == 0) sc = Sf{}, af = Af{};                   // zeros (under scales of 2^-127)
-                block(std::true_type(), 0, std::integral_constant<int, 2 * P>());
-            }
-        } else {
-            // the last unit of an odd number of halves has a second half only; its scale is there twice (load_s)
-            if constexpr (whole_()) block(std::false_type(), 0, std::integral_constant<int, 2 * P>());
+        if constexpr (UH == 1) block(std::true_type(), 0, p_);
+        else if constexpr (KW == 2) block(std::true_type(), kg, std::integral_constant<int, 2 * P>());   // (its scales are shifted to this byte)
+        else if constexpr (one_()) block(std::true_type(), 0, std::integral_constant<int, 2 * P>());
+        else {
+            block(std::false_type(), 0, std::integral_constant<int, 2 * P>());
             block(std::true_type(), 1, std::integral_constant<int, 2 * P + 1>());
         }
         buf = next;
@@ -687,24 +749,35 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, OCC) mx_dma_kernel(MxGemm g
     constexpr std::integral_constant<int, 1> p1{};
     constexpr std::integral_constant<int, 2> p2{};
     constexpr std::integral_constant<int, 3> p3{};
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
     int u = 0;
-    const int left = halves & 3;
-    for (int n = halves >> 2; n > 0; --n, u += GU) {
-        unit(u, p0, std::true_type());
-        unit(u + 1, p1, std::true_type());
+    const int left = ((nblk & 15) + 3) >> 2;                           // halves
+    for (int n = nblk >> 4; n > 0; --n, u += GU) {
+        unit(u, p0, no, no);
+        unit(u + 1, p1, no, no);
         if constexpr (UH == 1) {
-            unit(u + 2, p2, std::true_type());
-            unit(u + 3, p3, std::true_type());
+            unit(u + 2, p2, no, no);
+            unit(u + 3, p3, no, no);
         }
     }
     if constexpr (UH == 1) {
-        if (left > 0) unit(u, p0, std::true_type());
-        if (left > 1) unit(u + 1, p1, std::true_type());
-        if (left > 2) unit(u + 2, p2, std::true_type());
+        if (left > 0) unit(u, p0, yes, no);
+        if (left > 1) unit(u + 1, p1, yes, no);
+        if constexpr (ANY) {
+            if (left > 2) unit(u + 2, p2, yes, no);
+            if (left > 3) unit(u + 3, p3, yes, no);
+        }
+    } else if constexpr (!ANY) {
+        if (left > 0) unit(u, p0, yes, no);
+    } else if constexpr (KW == 2) {
+        if (left > 0) unit(u, p0, yes, no);
+        if (left > 2) unit(u + 1, p1, yes, no);
     } else {
-        if (left == 1) unit(u, p0, std::false_type());
-        if (left > 1) unit(u, p0, std::true_type());
-        if (left > 2) unit(u + 1, p1, std::false_type());
+        if (left == 1) unit(u, p0, yes, yes);
+        if (left > 1) unit(u, p0, yes, no);
+        if (left == 3) unit(u + 1, p1, yes, yes);
+        if (left > 3) unit(u + 1, p1, yes, no);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                 // no load outlives the workgroup's LDS
     if constexpr (KW == 2) {                                         // the two halves' sums meet
@@ -728,10 +801,13 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, OCC) mx_dma_kernel(MxGemm g
 
 constexpr int CUS = 256;
 
-// the direct-to-LDS form takes whole steps, aligned scale dwords and 32-bit offsets from its bases
-bool dma_ok(const MxGemm& g, bool grouped) {
-    const bool near = !(grouped && g.row_ids) || (int64_t) g.a_rows * std::max(g.a.ldc, g.a.lds) < (int64_t) 1 << 32;
-    return g.K % 128 == 0 && g.K >= 512 && near && (g.a.lds | g.w.lds) % 4 == 0 && ((uintptr_t) g.a.scales | (uintptr_t) g.w.scales) % 4 == 0;
+// mx_dma has 32-bit offsets from its bases: rows gathered (and what a row's loads may pass its end by) lie in 4 GiB
+bool far_rows(const MxGemm& g) {
+    return g.row_ids && (int64_t) g.a_rows * std::max(g.a.ldc, g.a.lds) >= ((int64_t) 1 << 32) - 4096;
+}
+// whole units of 256 k, a scale row of 16 bytes at least, dwords of scales aligned; otherwise the form ANY
+bool whole_steps(const MxGemm& g) {
+    return g.K % 256 == 0 && g.K >= 512 && (g.a.lds | g.w.lds) % 4 == 0 && ((uintptr_t) g.a.scales | (uintptr_t) g.w.scales) % 4 == 0;
 }
 
 enum Tile { T256x256, T128x128, T64x128, T64x64, T32x128, T32x64, T16x64 };
@@ -741,7 +817,7 @@ constexpr int TILE_M[] = {256, 128, 64, 64, 32, 32, 16}, TILE_N[] = {256, 128, 1
 // tiles have a CU to themselves); the least of them is taken.  Measured, us for 128 k, {alone, a pair}.  What it decides, for instance
 // (E4M3 to bf16, us): 250 x 2,048 x 6,144 32x64 9.8, 64x64 12.7, 64x128 18.6; 1,024 x 2,048 x 2,048 64x128 8.9, 64x64 9.2, 128x128 12.8;
 // 2,048 x 12,288 x 2,048 128x128 51, 256x256 61, 64x128 60; 8,192 x 6,144 x 2,048 256x256 93, 128x128 100.
-Tile dense_tile(const MxGemm& g, bool e8, bool f32) {
+Tile dense_tile(const MxGemm& g, bool e8, bool f32, bool whole) {
     constexpr Tile kind[] = {T256x256, T128x128, T64x128, T64x64, T32x64};
     constexpr float cost[3][5][2] = {{{1.62f, 3.24f}, {0.62f, 0.96f}, {0.36f, 0.58f}, {0.24f, 0.40f}, {0.17f, 0.28f}},   // E4M3
                                      {{1.06f, 2.12f}, {0.40f, 0.67f}, {0.27f, 0.46f}, {0.19f, 0.29f}, {0.14f, 0.24f}},   // E2M1
@@ -749,8 +825,8 @@ Tile dense_tile(const MxGemm& g, bool e8, bool f32) {
     const auto& c = cost[!e8 ? 1 : f32 ? 2 : 0];
     Tile best = T32x64;
     float least = 0.f;
-    for (int i = e8 && f32 ? 1 : 0; i < 5; ++i) {                  // E4M3 to fp32 has no 256 x 256 (its registers spill)
-        const int64_t t = (int64_t) ((g.M + TILE_M[kind[i]] - 1) / TILE_M[kind[i]]) * ((g.N + TILE_N[kind[i]] - 1) / TILE_N[kind[i]]);
+    for (int i = (e8 && f32) || !whole ? 1 : 0; i < 5; ++i) {      // E4M3 to fp32 and ANY have no 256 x 256 (their registers spill)
+        const int64_t t = ((int64_t) g.M + TILE_M[kind[i]] - 1) / TILE_M[kind[i]] * (((int64_t) g.N + TILE_N[kind[i]] - 1) / TILE_N[kind[i]]);
         const int64_t n = (t + CUS - 1) / CUS;
         const float us = (float) (n / 2) * c[i][1] + (float) (n % 2) * c[i][0];
         if (least == 0.f || us < least) least = us, best = kind[i];
@@ -760,13 +836,13 @@ Tile dense_tile(const MxGemm& g, bool e8, bool f32) {
 // Tiles of a product per group, by the rows of a group that has any.  Measured at 512 groups, N 1,024, K 2,048, E4M3 to bf16, us: 6 rows
 // 16x64 106, 32x128 108 (to fp32 117, 134); 12 rows 128, 118, 64x128 132; 20 rows 32x128 126, 64x128 134; 40 rows 168, 149, 128x128 164; 80
 // rows 64x128 213, 128x128 192; 160 rows 128x128 304, 256x256 367, but E2M1 253, 218.
-Tile grouped_tile(const MxGemm& g, bool e8) {
+Tile grouped_tile(const MxGemm& g, bool e8, bool whole) {
     const int rows = g.M / std::min(g.M, g.groups);
     if (rows <= 8) return T16x64;
     if (rows <= 25) return T32x128;
     if (rows <= 56) return T64x128;
     const bool many = (int64_t) g.groups * ((g.N + 255) / 256) >= 2 * CUS;
-    return !e8 && rows >= 128 && many ? T256x256 : T128x128;
+    return whole && !e8 && rows >= 128 && many ? T256x256 : T128x128;
 }
 
 template <int FMT, int OUT, bool GROUPED>
@@ -784,37 +860,34 @@ int launch(MxGemm g, hipStream_t st) {
         WZY_LAUNCH_CHECK();
         return WZY_OK;
     };
-    const bool dma = dma_ok(g, GROUPED);
-    if constexpr (!GROUPED) {
+    if constexpr (GROUPED) {
+        if (far_rows(g)) return go(mx_far_kernel<FMT, OUT>, 64, 64, 256);
+    } else {
         // Up to 16 rows: 16 x 64 tiles where there are enough of them, or K split over the waves.  1 row, E4M3 to fp32, us: N 2,048, K
         // 2,048 5.0 against 4.8; N 2,048, K 6,144 9.1, 5.9; N 12,288, K 2,048 5.7, 6.6; 4 x 151,936 x 2,048 35, 56.
-        if (g.M <= 16 && !(dma && g.N > 4096)) {
+        if (g.M <= 16 && g.N <= 4096) {
             mx_skinny_kernel<FMT, OUT><<<(g.N + 15) / 16, 64 * std::min(8, (g.K + 511) / 512), 0, st>>>(g);
             WZY_LAUNCH_CHECK();
             return WZY_OK;
         }
     }
-    if (!dma) {
-        // the largest tile that still gives every CU one
-        const int64_t m = GROUPED ? std::min(g.M, g.groups) : 1, r = GROUPED ? g.M / m : g.M;
-        auto enough = [&](int tm, int tn) { return r > tm / 2 && m * ((r + tm - 1) / tm) * ((g.N + tn - 1) / tn) >= CUS; };
-        if (enough(128, 128)) return go(mx_any_kernel<FMT, OUT, 128, 128, 2, 2, GROUPED>, 128, 128, 256);
-        if (enough(64, 64)) return go(mx_any_kernel<FMT, OUT, 64, 64, 2, 2, GROUPED>, 64, 64, 256);
-        return go(mx_any_kernel<FMT, OUT, 32, 64, 2, 2, GROUPED>, 32, 64, 256);
-    }
-    const Tile t = GROUPED ? grouped_tile(g, E8) : g.M <= 16 ? T16x64 : dense_tile(g, E8, OUT == WZY_F32);
-    if (t == T16x64) return go(mx_dma_kernel<FMT, OUT, 16, 64, 1, 2, 2, 256, 3, 2, GROUPED>, 16, 64, 256);
-    if (t == T64x128) return go(mx_dma_kernel<FMT, OUT, 64, 128, 1, 4, 1, 256, 2, 2, GROUPED>, 64, 128, 256);
-    if constexpr (GROUPED) {
-        if (t == T32x128) return go(mx_dma_kernel<FMT, OUT, 32, 128, 1, 4, 1, 256, 3, 2, GROUPED>, 32, 128, 256);
-    } else {
-        if (t == T32x64) return go(mx_dma_kernel<FMT, OUT, 32, 64, 2, 2, 1, 256, 3, 2, GROUPED>, 32, 64, 256);
-        if (t == T64x64) return go(mx_dma_kernel<FMT, OUT, 64, 64, 2, 2, 1, 256, 3, 2, GROUPED>, 64, 64, 256);
-    }
-    if constexpr (!E8 || (!GROUPED && OUT != WZY_F32)) {
-        if (t == T256x256) return go(mx_dma_kernel<FMT, OUT, 256, 256, 2, 4, 1, E8 ? 128 : 256, E8 ? 3 : 2, 2, GROUPED>, 256, 256, 512);
-    }
-    return go(mx_dma_kernel<FMT, OUT, 128, 128, 2, 2, 1, E8 ? 128 : 256, 2, 2, GROUPED>, 128, 128, 256);
+    auto tiles = [&](auto any_) {
+        constexpr bool ANY = any_();
+        const Tile t = GROUPED ? grouped_tile(g, E8, !ANY) : g.M <= 16 ? T16x64 : dense_tile(g, E8, OUT == WZY_F32, !ANY);
+        if (t == T16x64) return go(mx_dma_kernel<FMT, OUT, 16, 64, 1, 2, 2, 256, 3, 2, GROUPED, ANY>, 16, 64, 256);
+        if (t == T64x128) return go(mx_dma_kernel<FMT, OUT, 64, 128, 1, 4, 1, 256, 2, 2, GROUPED, ANY>, 64, 128, 256);
+        if constexpr (GROUPED) {
+            if (t == T32x128) return go(mx_dma_kernel<FMT, OUT, 32, 128, 1, 4, 1, 256, 3, 2, GROUPED, ANY>, 32, 128, 256);
+        } else {
+            if (t == T32x64) return go(mx_dma_kernel<FMT, OUT, 32, 64, 2, 2, 1, 256, 3, 2, GROUPED, ANY>, 32, 64, 256);
+            if (t == T64x64) return go(mx_dma_kernel<FMT, OUT, 64, 64, 2, 2, 1, 256, 3, 2, GROUPED, ANY>, 64, 64, 256);
+        }
+        if constexpr (!ANY && (!E8 || (!GROUPED && OUT != WZY_F32))) {
+            if (t == T256x256) return go(mx_dma_kernel<FMT, OUT, 256, 256, 2, 4, 1, E8 ? 128 : 256, E8 ? 3 : 2, 2, GROUPED, ANY>, 256, 256, 512);
+        }
+        return go(mx_dma_kernel<FMT, OUT, 128, 128, 2, 2, 1, E8 ? 128 : 256, 2, 2, GROUPED, ANY>, 128, 128, 256);
+    };
+    return whole_steps(g) ? tiles(std::false_type()) : tiles(std::true_type());
 }
 template <bool GROUPED>
 int dispatch(const MxGemm& g, int fmt, hipStream_t st) {
