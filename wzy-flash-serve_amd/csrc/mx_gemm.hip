@@ -451,9 +451,10 @@ __global__ void __launch_bounds__(256, 2) mx_far_kernel(MxGemm g) {
 // at the end (16 x 64 tiles, where a unit's chain of LDS reads and MFMAs is what takes the time: 1 x 12,288 x 2,048 to fp32 6.8 ->
 // 5.7 us).
 //
-// What bounds it: 8,192 x 8,192 x 8,192, E2M1 271 us (4,060 TFLOP/s), E4M3 417 (2,640).  The same launch without its MFMAs takes
-// 224 (313), without its loads 231 (335): loads into LDS run at 10 TB/s over the chip whatever the tile, and the MFMAs with
-// their LDS reads at 5 PFLOP/s (3.3).  Bigger tiles than 256 x 256 do not fit the LDS.
+// What bounds it: 8,192 x 8,192 x 8,192 to bf16, E2M1 276 us (3,980 TFLOP/s), E4M3 422 (2,610).  The same launch without its MFMAs
+// took 224 (313), without its loads 231 (335): loads into LDS run at 10 TB/s over the chip whatever the tile, and the MFMAs with
+// their LDS reads at 5 PFLOP/s (3.3).  Bigger tiles than 256 x 256 do not fit the LDS; a fourth buffer for 32 x 64 tiles, where the
+// loads are all there is (250 x 2,048 x 6,144 9.6 us), changes nothing.
 WZY_DEV uint32_t lds_offset(const void* p) { return (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) char*) p; }
 // 64 lanes x 16 bytes from base + off (per lane) to LDS lds .. lds + 1023, lane order; lds and base wave-uniform
 WZY_DEV void dma16(uint32_t lds, uint32_t off, const uint8_t* base) {
@@ -815,7 +816,7 @@ constexpr int TILE_M[] = {256, 128, 64, 64, 32, 32, 16}, TILE_N[] = {256, 128, 1
 
 // Tiles of a dense product: a CU's time for n tiles is that of n / 2 pairs beside each other and of an odd one (256 x 256
 // tiles have a CU to themselves); the least of them is taken.  Measured, us for 128 k, {alone, a pair}.  What it decides, for instance
-// (E4M3 to bf16, us): 250 x 2,048 x 6,144 32x64 9.8, 64x64 12.7, 64x128 18.6; 1,024 x 2,048 x 2,048 64x128 8.9, 64x64 9.2, 128x128 12.8;
+// (E4M3 to bf16, us): 250 x 2,048 x 6,144 32x64 9.6, 64x64 12.7, 64x128 18.6; 1,024 x 2,048 x 2,048 64x128 8.9, 64x64 9.2, 128x128 12.8;
 // 2,048 x 12,288 x 2,048 128x128 51, 256x256 61, 64x128 60; 8,192 x 6,144 x 2,048 256x256 93, 128x128 100.
 Tile dense_tile(const MxGemm& g, bool e8, bool f32, bool whole) {
     constexpr Tile kind[] = {T256x256, T128x128, T64x128, T64x64, T32x64};
@@ -879,6 +880,12 @@ int launch(MxGemm g, hipStream_t st) {
         if constexpr (GROUPED) {
             if (t == T32x128) return go(mx_dma_kernel<FMT, OUT, 32, 128, 1, 4, 1, 256, 3, 2, GROUPED, ANY>, 32, 128, 256);
         } else {
+            // E4M3 to fp32, at most a tile a CU: both halves of a unit at once.  32 x 2,048 x 6,144 13.9 -> 12.1 us, 250 x 2,048 x 2,048 7.1 ->
+            // 6.7; the other types 4 to 15 % slower, ANY no faster.
+            if constexpr (!ANY && E8 && OUT == WZY_F32) {
+                if (t == T32x64 && ((int64_t) g.M + 31) / 32 * (((int64_t) g.N + 63) / 64) <= CUS)
+                    return go(mx_dma_kernel<FMT, OUT, 32, 64, 2, 2, 2, 256, 3, 2, GROUPED, ANY>, 32, 64, 512);
+            }
             if (t == T32x64) return go(mx_dma_kernel<FMT, OUT, 32, 64, 2, 2, 1, 256, 3, 2, GROUPED, ANY>, 32, 64, 256);
             if (t == T64x64) return go(mx_dma_kernel<FMT, OUT, 64, 64, 2, 2, 1, 256, 3, 2, GROUPED, ANY>, 64, 64, 256);
         }
