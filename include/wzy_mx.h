@@ -61,11 +61,11 @@ int wzy_mx_dequantize(const wzy_mx_mat* q, int rows, int cols, void* y, int y_ty
  * sum = h, y = n rounded to `type`, q = n as MX E4M3 (from fp32, as wzy_mx_quantize quantises).
  * x, residual, sum and y are [rows x cols] of `type` with one row stride ld (elements); gamma [cols] fp32.
  * Any of sum, y, q may be NULL, not all three; sum may be x or residual, and so may y where sum is NULL or another buffer.
- * Rows aligned to 16 bytes, gamma too; cols at most 16,384; eps >= 0 (a row of zeros with eps 0 is NaN). */
+ * Rows aligned to 16 bytes, gamma too; cols at most 16,384; at most 8,388,607 rows, and up to 2^26 - 1 of them where cols <= 512; eps >= 0 (a row of zeros with eps 0 is NaN). */
 int wzy_mx_add_rmsnorm(const void* x, const void* residual, int type, int64_t ld, const float* gamma, float eps,
                        int rows, int cols, void* sum, void* y, const wzy_mx_mat* q, void* stream);
 
-/* q = MX E4M3 of gate * up / (1 + exp(-gate)), computed in fp32; gate and up [rows x cols] of `type` with row
+/* q = MX E4M3 of gate / (1 + exp(-gate)) * up, computed in fp32; gate and up [rows x cols] of `type` with row
  * stride ld (elements), for instance the halves of one gate|up row (up = gate + cols).  Rows aligned to 16 bytes;
  * rows * cols / 32 below 2^31. */
 int wzy_mx_swiglu(const void* gate, const void* up, int type, int64_t ld, int rows, int cols, const wzy_mx_mat* q,

@@ -244,6 +244,17 @@ def test_swiglu_far_gates(wz, gpu):
     assert scales[0, 0] != 255 and scales[0, 1] == 255
 
 
+def test_swiglu_product_of_large_factors(wz, gpu):
+    """gate * up is past fp32's range, the result is not"""
+    x = np.ones((1, 128), np.float32)
+    x[0, :32], x[0, 64:96] = -80.0, np.float32(1e37) * (1 + np.arange(32) / 32)
+    x[0, 32:64], x[0, 96:] = 30 + np.arange(32) / 4, np.float32(4e36)
+    d, q = DA.from_numpy(x), Mat(1, 64, E4M3)
+    wz.wzy_mx_swiglu(d.ptr, d.ptr + 256, F32, 128, 1, 64, q.ref(), None)
+    g, u = x[:, :64].astype(np.float64), x[:, 64:].astype(np.float64)
+    assert_quantized_near(*q.read(), g / (1 + np.exp(-g)) * u, (np.abs(g) + 8) * 2.0 ** -22)
+
+
 # ---- products -----------------------------------------------------------------------------------------
 def random_mx(rng, rows, cols, fmt, gap=0, sgap=0, spread=2):
     codes = rng.integers(0, 16 if fmt == E2M1 else 256, (rows, cols)).astype(np.uint8)

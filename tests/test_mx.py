@@ -64,6 +64,8 @@ def test_bad_rows_types_and_options_are_refused(wz):
     refused(wz, *n, 64, A, -1e-6, 4, 64, None, A, None, None)
     refused(wz, *n, 64, A, float("nan"), 4, 64, None, A, None, None)
     refused(wz, *n, 16416, A, 1e-6, 4, 16416, None, A, None, None)         # too wide
+    refused(wz, *n, 32, A, 1e-6, 2 ** 26, 32, None, A, None, None)         # more rows than a launch holds
+    refused(wz, *n, 16384, A, 1e-6, 2 ** 23, 16384, None, A, None, None)
     refused(wz, *n, 64, A, 1e-6, 4, 64, A, A, None, None)                  # sum and y in one buffer
     refused(wz, *n, 64, A, 1e-6, 4, 64, None, None, mat(E2M1), None)
     refused(wz, "wzy_mx_add_rmsnorm", A, A + 8, F32, 64, A, 1e-6, 4, 64, None, A, None, None)

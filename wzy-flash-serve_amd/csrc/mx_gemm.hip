@@ -854,7 +854,7 @@ int launch(MxGemm g, hipStream_t st) {
         const int64_t mt = GROUPED ? std::min<int64_t>(g.M, (int64_t) g.M / tm + g.groups) : ((int64_t) g.M + tm - 1) / tm;
         const int64_t nt = ((int64_t) g.N + tn - 1) / tn;
         const int64_t grid = GROUPED ? (mt + 7) / 8 * 8 * nt : (mt * nt + 7) / 8 * 8;
-        WZY_REQUIRE(grid < (int64_t) 1 << 31, "wzy_mx_%sgemm: %lld tiles", GROUPED ? "grouped_" : "", (long long) grid);
+        WZY_REQUIRE(grid * threads < (int64_t) 1 << 32, "wzy_mx_%sgemm: %lld tiles", GROUPED ? "grouped_" : "", (long long) grid);
         g.mt = (int) mt;
         g.nt = (int) nt;
         kernel<<<(uint32_t) grid, threads, 0, st>>>(g);

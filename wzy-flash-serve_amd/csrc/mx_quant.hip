@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(QT) mx_quant_kernel(const void* __restrict__ x
     for (int i = 0; i < QU; ++i) {
         if constexpr (GLU) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * u[i][j] / (1.0f + __expf(-v[i][j]));
+            for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] / (1.0f + __expf(-v[i][j])) * u[i][j];   // gate * up first would overflow
         }
         const int byte = mx_block_scale<FMT>(v[i]);
         const uint2 c = mx_block_codes<FMT>(v[i], byte);
@@ -226,15 +226,14 @@ extern "C" int wzy_mx_add_rmsnorm(const void* x, const void* residual, int type,
         WZY_REQUIRE(q->fmt == WZY_MX_E4M3, "%s: q is E4M3", who);
     }
     a.x = x; a.res = residual; a.gamma = gamma; a.sum = sum; a.y = y; a.ld = ld; a.eps = eps; a.cols = cols;
-    const int pieces = cols / 8;
+    const int pieces = cols / 8, nv = pieces <= 512 ? 1 : pieces <= 1024 ? 2 : 4;
+    const int threads = (int) align_up((size_t) (pieces + nv - 1) / nv, 64);
+    WZY_REQUIRE((int64_t) rows * threads < (int64_t) 1 << 32, "%s: %d rows of %d (at most %lld in a call)", who, rows, cols,
+                ((1LL << 32) - 1) / threads);
     return mx_with_type(type, [&](auto t) {
-        auto go = [&](auto nv) {
-            const int threads = (int) align_up((size_t) (pieces + nv() - 1) / nv(), 64);
-            mx_norm_kernel<t(), nv()><<<rows, threads, 0, as_stream(stream)>>>(a);
-        };
-        if (pieces <= 512) go(std::integral_constant<int, 1>());
-        else if (pieces <= 1024) go(std::integral_constant<int, 2>());
-        else go(std::integral_constant<int, 4>());
+        if (nv == 1) mx_norm_kernel<t(), 1><<<rows, threads, 0, as_stream(stream)>>>(a);
+        else if (nv == 2) mx_norm_kernel<t(), 2><<<rows, threads, 0, as_stream(stream)>>>(a);
+        else mx_norm_kernel<t(), 4><<<rows, threads, 0, as_stream(stream)>>>(a);
         WZY_LAUNCH_CHECK();
         return WZY_OK;
     });
