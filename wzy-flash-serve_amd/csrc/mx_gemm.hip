@@ -29,6 +29,7 @@
 using namespace wzy;
 
 typedef int v8i_t __attribute__((ext_vector_type(8)));
+typedef uint32_t v4u_t __attribute__((ext_vector_type(4)));
 typedef float v4f_t __attribute__((ext_vector_type(4)));
 
 namespace {
@@ -282,6 +283,42 @@ template <int OUT, int NI, int CB, bool PAIR>
 WZY_DEV void store_tile(const MxGemm& g, bool gather, bool whole, int row0, int rows, int wr, int n, const v4f_t (&acc)[NI][CB]) {
     constexpr int NV = PAIR ? 8 : 4;
     const int q4 = (threadIdx.x & 63) >> 4, lr = threadIdx.x & 15;
+    // Whole cache lines: a lane has two 16-byte pieces of its row 64 bytes apart.  Lanes lr and lr + 8 exchange one of theirs, and a store writes
+    // 8 rows of 128 bytes, past the caches (half lines stored so cost up to 18 %, whole ones through the caches nothing).  us, before and
+    // after: 8,192 x 6,144 x 2,048 E2M1 to bf16 68 and 65, to fp32 101 and 82, E4M3 to fp32 207 and 182; 8,192 x 12,288 x 2,048 E2M1 142 and 127,
+    // 220 and 158; per group, 82,000 rows of K 512, E4M3 257 and 234; but 8,192 x 8,192 x 320 to bf16 50 and 52.
+    constexpr int LINE = OUT == WZY_F32 ? 2 : 4;                      // column blocks of 128 bytes
+    if constexpr (CB % LINE == 0) {
+        if (whole) {
+            const bool up = lr >= 8;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int r0 = wr + 16 * i;
+                const bool zero = gather && r0 + lr < rows && (unsigned) g.row_ids[row0 + r0 + lr] >= (unsigned) g.a_rows;
+#pragma unroll
+                for (int j = 0; j < CB; j += LINE) {
+                    v4u_t p[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            if constexpr (OUT == WZY_F32) p[h][r] = zero ? 0u : __float_as_uint(acc[i][j + h][r]);
+                            else p[h][r] = zero ? 0u : pack2<OUT>(acc[i][j + 2 * h + (r >> 1)][2 * (r & 1)], acc[i][j + 2 * h + (r >> 1)][2 * (r & 1) + 1]);
+                        }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const uint32_t t = (uint32_t) __builtin_amdgcn_update_dpp(0, (int) (up ? p[0][r] : p[1][r]), 0x128, 0xF, 0xF, true);   // row_ror 8
+                        if (up) p[0][r] = t;
+                        else p[1][r] = t;
+                    }
+                    uint8_t* const at = (uint8_t*) g.y + ((size_t) (row0 + r0 + (lr & 7)) * g.ldy + n + 16 * j) * (OUT == WZY_F32 ? 4 : 2) + (up ? 64 : 0) + 16 * q4;
+                    if (r0 + (lr & 7) < rows) __builtin_nontemporal_store(p[0], (v4u_t*) at);
+                    if (r0 + (lr & 7) + 8 < rows) __builtin_nontemporal_store(p[1], (v4u_t*) (at + 8 * g.ldy * (OUT == WZY_F32 ? 4 : 2)));
+                }
+            }
+            return;
+        }
+    }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
         const int m = wr + 16 * i + lr;
@@ -451,7 +488,7 @@ __global__ void __launch_bounds__(256, 2) mx_far_kernel(MxGemm g) {
 // at the end (16 x 64 tiles, where a unit's chain of LDS reads and MFMAs is what takes the time: 1 x 12,288 x 2,048 to fp32 6.8 ->
 // 5.7 us).
 //
-// What bounds it: 8,192 x 8,192 x 8,192 to bf16, E2M1 276 us (3,980 TFLOP/s), E4M3 422 (2,610).  The same launch without its MFMAs
+// What bounds it: 8,192 x 8,192 x 8,192 to bf16, E2M1 263 us (4,180 TFLOP/s), E4M3 405 (2,710).  The same launch without its MFMAs
 // took 224 (313), without its loads 231 (335): loads into LDS run at 10 TB/s over the chip whatever the tile, and the MFMAs with
 // their LDS reads at 5 PFLOP/s (3.3).  Bigger tiles than 256 x 256 do not fit the LDS; a fourth buffer for 32 x 64 tiles, where the
 // loads are all there is (250 x 2,048 x 6,144 9.6 us), changes nothing.
