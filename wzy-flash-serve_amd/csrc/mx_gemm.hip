@@ -499,7 +499,7 @@ WZY_DEV void dma16(uint32_t lds, uint32_t off, const uint8_t* base) {
     lds = (uint32_t) __builtin_amdgcn_readfirstlane((int) lds);      // nothing where they are in scalar registers already
     base = (const uint8_t*) (uintptr_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (b >> 32)) << 32 |
                                          (uint32_t) __builtin_amdgcn_readfirstlane((int) b));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 // 64 lanes x 4 bytes, likewise
 WZY_DEV void dma4(uint32_t lds, uint32_t off, const uint8_t* base) {
@@ -507,7 +507,7 @@ WZY_DEV void dma4(uint32_t lds, uint32_t off, const uint8_t* base) {
     lds = (uint32_t) __builtin_amdgcn_readfirstlane((int) lds);
     base = (const uint8_t*) (uintptr_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (b >> 32)) << 32 |
                                          (uint32_t) __builtin_amdgcn_readfirstlane((int) b));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 // this wave's loads but the last N have landed and its LDS reads are done; then all waves meet
 template <int N>
