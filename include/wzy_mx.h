@@ -72,7 +72,10 @@ int wzy_mx_swiglu(const void* gate, const void* up, int type, int64_t ld, int ro
                   void* stream);
 
 /* y [M x N] (y_type, row stride ldy >= N) = a [M x K] . w [N x K]^T, a of either format, w E2M1, K a multiple of
- * 32.  Sums are fp32 on the scaled MFMA instructions.  A NaN scale or code makes its row of y (a) or its column (w) NaN.
+ * 32.  Sums are fp32, on the scaled MFMA instructions; products are whole, but for E4M3 rows with bf16 output: of each eight
+ * consecutive k the seven smaller products lose up to 2^-13 of the largest (1e-5 of a sum of the usual size, below the output's
+ * rounding unless the sum cancels).  E4M3 rows to fp32 and fp16 take up to twice that one's time for it.  A NaN scale or code makes its
+ * row of y (a) or its column (w) NaN.
  * M = 1 .. 16 is the decode form: the weights stream once, at memory speed.  y is aligned to its element.
  * K at most 2^20. */
 int wzy_mx_gemm(const wzy_mx_mat* a, const wzy_mx_mat* w, int M, int N, int K, void* y, int y_type, int64_t ldy,

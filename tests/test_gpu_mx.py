@@ -704,3 +704,25 @@ def test_rows_far_apart(wz, gpu, fmt, K):
         check_large(got[40:], av[40:300], wv[N:], fmt, t)
     for m in (a, far):
         m.c.free()
+
+
+@pytest.mark.parametrize("M,N", [(3, 40), (40, 70), (7, 4112), (300, 200)])
+@pytest.mark.parametrize("K", [512, 288])
+def test_gemm_fp16_sums_that_cancel(wz, gpu, M, N, K):
+    """a small rest of large products, of E4M3 rows: the bound of fp32 sums and one rounding"""
+    rng = np.random.default_rng(M + K)
+    small = rng.integers(0, 24, (M, K)) | rng.integers(0, 2, (M, K)) << 7       # up to 2^-4
+    codes = small.astype(np.uint8)
+    codes[:, 0::16] = codes[:, 1::16] = 0x7E                      # 448 twice in an eight, by weights that cancel
+    wc = rng.integers(0, 16, (N, K)).astype(np.uint8)
+    wc[:, 1::16] = wc[:, 0::16] ^ 8
+    scales = np.full((M, K // 32), 127, np.uint8)
+    wsc = np.full((N, K // 32), 127, np.uint8)
+    a, w = Mat(M, K, E4M3, codes=codes, scales=scales), Mat(N, K, E2M1, codes=wc, scales=wsc)
+    at = np.r_[0:N:max(1, N // 20), N - 1]
+    av, wv = R.dequantize(codes, scales, E4M3), R.dequantize(wc, wsc, E2M1)[at]
+    y, z, off = out_rows(M, N, F16), out_rows(M, N, F16), DA.from_numpy(np.array([0, M], np.int32))
+    wz.wzy_mx_gemm(a.ref(), w.ref(), M, N, K, y.ptr, F16, N, None)
+    wz.wzy_mx_grouped_gemm(a.ref(), M, None, w.ref(), off.ptr, 1, M, N, K, z.ptr, F16, N, None)
+    for d in (y, z):                              # (E2M1 names the bound without cut products)
+        check_product(read_rows(d, N, F16)[:, at], av, wv, E2M1, F16)

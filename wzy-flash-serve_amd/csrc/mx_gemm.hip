@@ -12,9 +12,11 @@
 //
 // Precision (measured): an instruction adds the products of 8 consecutive k after cutting each to 13 bits below the
 // largest of the eight, and the sums of eights in fp32.  E2M1 products span 9 bits: nothing is lost.  An E4M3 operand
-// spans 19 bits; over activations the cuts come to 1e-5 of a sum's size, 1/200 of the rounding of a bf16 output and
-// 1/50 of an fp16 one, and are left there.  For fp32 outputs the operand is taken in two parts, codes with exponent bit 3
-// set and the others: each part spans 11 bits, so both products are whole, at twice the MFMA work.
+// spans 19 bits.  For fp32 and fp16 outputs it is taken in two parts, codes with exponent bit 3 set and the others: each
+// part spans 11 bits, so both products are whole, at twice the MFMA work.  For bf16 outputs the cuts stay: over activations they come to
+// 1e-5 of a sum's size, 1/200 of the output's rounding, and show where a sum cancels (1 output in 200 is off by more than half a step, K
+// 2,048); two parts would cost up to 100 % (8,192 x 6,144 x 2,048 89 -> 165 us, 250 x 2,048 x 6,144 9.6 -> 14.8, 4 x 151,936 x 2,048 33.2 -> 33.5,
+// per group 81,920 x 1,024 x 2,048 280 -> 400).  An fp16 step is 8 times finer: of cut sums 1 in 35 is off by more than half of one.
 //
 // Three kernels, chosen in launch():
 //   mx_dma     tiles of 16 x 64 to 256 x 256 through LDS, filled by direct-to-LDS loads several steps ahead
@@ -71,15 +73,17 @@ WZY_DEV v8i_t operand_of(const uint4 (&v)[FMT == WZY_MX_E4M3 ? 2 : 1]) {
     if constexpr (FMT == WZY_MX_E4M3) return operand8(v[0], v[1]);
     else return operand4(v[0]);
 }
+// products taken in two parts, none cut
+constexpr bool two_parts(int fmt, int out) { return fmt == WZY_MX_E4M3 && out != WZY_BF16; }
 template <int FMT>
 struct Code;                                                     // the instructions' format numbers
 template <> struct Code<WZY_MX_E4M3> { static constexpr int v = 0; };
 template <> struct Code<WZY_MX_E2M1> { static constexpr int v = 4; };
 
 // w (E2M1) by a: D's rows are w's, its columns a's.  OW, OA: the scale's byte in its dword.
-template <int FMT, bool WHOLE, int OW, int OA>
+template <int FMT, int OUT, int OW, int OA>
 WZY_DEV v4f_t mfma16(v8i_t w, v8i_t a, v4f_t c, int sw, int sa) {
-    if constexpr (FMT == WZY_MX_E4M3 && WHOLE) {
+    if constexpr (two_parts(FMT, OUT)) {
         v8i_t hi, lo;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -237,10 +241,10 @@ __global__ void __launch_bounds__(512) mx_skinny_kernel(MxGemm g) {
         return t;
     };
     auto multiply = [&](const Batch& t) {
-        acc = mfma16<FMT, OUT == WZY_F32, 0, 0>(operand4(t.w[0]), operand_of<FMT>(t.a[0]), acc, (int) t.sw, (int) t.sa);
-        acc = mfma16<FMT, OUT == WZY_F32, 1, 1>(operand4(t.w[1]), operand_of<FMT>(t.a[1]), acc, (int) t.sw, (int) t.sa);
-        acc = mfma16<FMT, OUT == WZY_F32, 2, 2>(operand4(t.w[2]), operand_of<FMT>(t.a[2]), acc, (int) t.sw, (int) t.sa);
-        acc = mfma16<FMT, OUT == WZY_F32, 3, 3>(operand4(t.w[3]), operand_of<FMT>(t.a[3]), acc, (int) t.sw, (int) t.sa);
+        acc = mfma16<FMT, OUT, 0, 0>(operand4(t.w[0]), operand_of<FMT>(t.a[0]), acc, (int) t.sw, (int) t.sa);
+        acc = mfma16<FMT, OUT, 1, 1>(operand4(t.w[1]), operand_of<FMT>(t.a[1]), acc, (int) t.sw, (int) t.sa);
+        acc = mfma16<FMT, OUT, 2, 2>(operand4(t.w[2]), operand_of<FMT>(t.a[2]), acc, (int) t.sw, (int) t.sa);
+        acc = mfma16<FMT, OUT, 3, 3>(operand4(t.w[3]), operand_of<FMT>(t.a[3]), acc, (int) t.sw, (int) t.sa);
     };
     int b = 16 * wave;
     if (b < nblk) {
@@ -444,7 +448,7 @@ __global__ void __launch_bounds__(256, 2) mx_far_kernel(MxGemm g) {
 #pragma unroll
             for (int j = 0; j < (E8 ? 2 : 1); ++j) av[j] = s_a[b][r * AP + ((q4 + 4 * j) ^ asw)];
 #pragma unroll
-            for (int j = 0; j < CB; ++j) acc[i][j] = mfma16<FMT, OUT == WZY_F32, 0, 0>(operand4(wv[j]), operand_of<FMT>(av), acc[i][j], sw[j], sa);
+            for (int j = 0; j < CB; ++j) acc[i][j] = mfma16<FMT, OUT, 0, 0>(operand4(wv[j]), operand_of<FMT>(av), acc[i][j], sw[j], sa);
         }
     };
     Regs t0 = load(0), t1 = load(1);
@@ -760,8 +764,8 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, OCC) mx_dma_kernel(MxGemm g
                     for (int e = 0; e < RH; ++e)
 #pragma unroll
                         for (int j = 0; j < CB; ++j)
-                            acc[RH * i + e][j] = mfma16<FMT, OUT == WZY_F32, D, D>(operand4(wf.v[j]), operand_of<FMT>(af.v[e]), acc[RH * i + e][j],
-                                                                                   sc.w[j], sc.a[RH * i + e]);
+                            acc[RH * i + e][j] = mfma16<FMT, OUT, D, D>(operand4(wf.v[j]), operand_of<FMT>(af.v[e]), acc[RH * i + e][j], sc.w[j],
+                                                                       sc.a[RH * i + e]);
                 }
                 af = an;
                 if (LAST && P == GU - 1 && i == RB - 1) {
@@ -855,12 +859,14 @@ constexpr int TILE_M[] = {256, 128, 64, 64, 32, 32, 16}, TILE_N[] = {256, 128, 1
 // tiles have a CU to themselves); the least of them is taken.  Measured, us for 128 k, {alone, a pair}.  What it decides, for instance
 // (E4M3 to bf16, us): 250 x 2,048 x 6,144 32x64 9.6, 64x64 12.7, 64x128 18.6; 1,024 x 2,048 x 2,048 64x128 8.9, 64x64 9.2, 128x128 12.8;
 // 2,048 x 12,288 x 2,048 128x128 51, 256x256 61, 64x128 60; 8,192 x 6,144 x 2,048 256x256 93, 128x128 100.
-Tile dense_tile(const MxGemm& g, bool e8, bool f32, bool whole) {
+Tile dense_tile(const MxGemm& g, bool e8, bool whole) {
     constexpr Tile kind[] = {T256x256, T128x128, T64x128, T64x64, T32x64};
-    constexpr float cost[3][5][2] = {{{1.62f, 3.24f}, {0.62f, 0.96f}, {0.36f, 0.58f}, {0.24f, 0.40f}, {0.17f, 0.28f}},   // E4M3
+    constexpr float cost[4][5][2] = {{{1.62f, 3.24f}, {0.62f, 0.96f}, {0.36f, 0.58f}, {0.24f, 0.40f}, {0.17f, 0.28f}},   // E4M3
                                      {{1.06f, 2.12f}, {0.40f, 0.67f}, {0.27f, 0.46f}, {0.19f, 0.29f}, {0.14f, 0.24f}},   // E2M1
-                                     {{9.00f, 9.00f}, {0.95f, 1.70f}, {0.65f, 1.10f}, {0.38f, 0.62f}, {0.25f, 0.37f}}};  // E4M3 to fp32
-    const auto& c = cost[!e8 ? 1 : f32 ? 2 : 0];
+                                     {{9.00f, 9.00f}, {0.95f, 1.70f}, {0.65f, 1.10f}, {0.38f, 0.62f}, {0.25f, 0.37f}},    // E4M3 to fp32
+                                     {{3.15f, 6.30f}, {1.15f, 1.80f}, {0.85f, 1.25f}, {0.55f, 0.70f}, {0.38f, 0.45f}}};  // E4M3 to fp16
+    const bool f32 = g.y_type == WZY_F32;
+    const auto& c = cost[!e8 ? 1 : f32 ? 2 : g.y_type == WZY_F16 ? 3 : 0];
     Tile best = T32x64;
     float least = 0.f;
     for (int i = (e8 && f32) || !whole ? 1 : 0; i < 5; ++i) {      // E4M3 to fp32 and ANY have no 256 x 256 (their registers spill)
@@ -911,15 +917,15 @@ int launch(MxGemm g, hipStream_t st) {
     }
     auto tiles = [&](auto any_) {
         constexpr bool ANY = any_();
-        const Tile t = GROUPED ? grouped_tile(g, E8, !ANY) : g.M <= 16 ? T16x64 : dense_tile(g, E8, OUT == WZY_F32, !ANY);
+        const Tile t = GROUPED ? grouped_tile(g, E8, !ANY) : g.M <= 16 ? T16x64 : dense_tile(g, E8, !ANY);
         if (t == T16x64) return go(mx_dma_kernel<FMT, OUT, 16, 64, 1, 2, 2, 256, 3, 2, GROUPED, ANY>, 16, 64, 256);
         if (t == T64x128) return go(mx_dma_kernel<FMT, OUT, 64, 128, 1, 4, 1, 256, 2, 2, GROUPED, ANY>, 64, 128, 256);
         if constexpr (GROUPED) {
             if (t == T32x128) return go(mx_dma_kernel<FMT, OUT, 32, 128, 1, 4, 1, 256, 3, 2, GROUPED, ANY>, 32, 128, 256);
         } else {
-            // E4M3 to fp32, at most a tile a CU: both halves of a unit at once.  32 x 2,048 x 6,144 13.9 -> 12.1 us, 250 x 2,048 x 2,048 7.1 ->
-            // 6.7; the other types 4 to 15 % slower, ANY no faster.
-            if constexpr (!ANY && E8 && OUT == WZY_F32) {
+            // Products in two parts, at most a tile a CU: both halves of a unit at once.  To fp32, 32 x 2,048 x 6,144 13.9 -> 12.1 us, 250 x 2,048 x
+            // 2,048 7.1 -> 6.7; the other types 4 to 15 % slower, ANY no faster.
+            if constexpr (!ANY && two_parts(FMT, OUT)) {
                 if (t == T32x64 && ((int64_t) g.M + 31) / 32 * (((int64_t) g.N + 63) / 64) <= CUS)
                     return go(mx_dma_kernel<FMT, OUT, 32, 64, 2, 2, 2, 256, 3, 2, GROUPED, ANY>, 32, 64, 512);
             }
