@@ -726,3 +726,31 @@ def test_gemm_fp16_sums_that_cancel(wz, gpu, M, N, K):
     wz.wzy_mx_grouped_gemm(a.ref(), M, None, w.ref(), off.ptr, 1, M, N, K, z.ptr, F16, N, None)
     for d in (y, z):                              # (E2M1 names the bound without cut products)
         check_product(read_rows(d, N, F16)[:, at], av, wv, E2M1, F16)
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("rows,cols", [(24, 2048), (24, 96), (24, 8192)])
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-6])
+def test_add_rmsnorm_rows_whose_squares_leave_fp32(wz, gpu, t, rows, cols, eps):
+    rng = np.random.default_rng(cols)
+    size = np.array([1e37, 1e30, 1e25, 2e20, 1e19, 3e18, 1e17, 1.0, 1e-10, 1e-13, 1e-17, 1e-20, 1e-22, 1e-25, 1e-30, 1e-36])
+    x = rng.standard_normal((rows, cols))
+    x[:len(size)] *= size[:, None]
+    x[16] = 1.0
+    x[16, 5] = 3e38                                               # one value far above the others
+    x[17] = 1e-18
+    x[17, 7] = 2e19
+    x[18] = 0.0
+    x[18, 9] = 1e-30
+    x[19:] *= 10.0 ** rng.uniform(-36, 36, (5, 1))
+    bits, h = R.typed(x, t)
+    gamma = (1 + 0.1 * rng.standard_normal(cols)).astype(np.float32)
+    n = h / np.sqrt((h * h).mean(1, keepdims=True) + np.float64(np.float32(eps))) * gamma
+    d, g = DA.from_numpy(bits), DA.from_numpy(gamma)
+    s, y, q = out_rows(rows, cols, t), out_rows(rows, cols, t), Mat(rows, cols, E4M3)
+    wz.wzy_mx_add_rmsnorm(d.ptr, None, t, cols, g.ptr, eps, rows, cols, s.ptr, y.ptr, q.ref(), None)
+    np.testing.assert_array_equal(read_rows(s, cols, t), h)
+    got = read_rows(y, cols, t)
+    # below 2^-126 steps are 2^-149 (fp32) or 2^-133 (bf16)
+    assert (np.abs(got - n) <= np.abs(n) * (NORM_REL + R.HALF_STEP[t] * (1 + NORM_REL)) + (2.0 ** -149 if t == F32 else 2.0 ** -134)).all()
+    assert_quantized_near(*q.read(), n, NORM_REL)

@@ -4,6 +4,8 @@
 // A block of 32 values sits on the four lanes of a DPP quad, 8 consecutive values a lane: 16- or 32-byte loads, the
 // block's maximum by two quad permutations, 4 or 8 bytes of codes stored per lane.  (A large copy on this card reads and
 // writes 5.0 TB/s.)
+#include <cfloat>
+
 #include "wzy_mx.h"
 
 using namespace wzy;
@@ -121,12 +123,32 @@ __global__ void __launch_bounds__(512) mx_norm_kernel(NormArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(v[i][j], v[i][j], ss);
     }
-    ss = wave_sum(ss);
-    if ((tid & 63) == 0) s_red[tid >> 6] = ss;
-    __syncthreads();
-    float tot = 0.f;
-    for (int w = 0; w < nt / 64; ++w) tot += s_red[w];
-    const float sc = 1.0f / sqrtf(tot / (float) a.cols + a.eps);
+    auto over_row = [&](float part) {
+        part = wave_sum(part);
+        if ((tid & 63) == 0) s_red[tid >> 6] = part;
+        __syncthreads();
+        float tot = 0.f;
+        for (int w = 0; w < nt / 64; ++w) tot += s_red[w];
+        return tot;
+    };
+    float tot = over_row(ss), eps = a.eps, before = 1.f, after = 1.f;
+    // Squares past fp32's range, or so far below it that few bits of them are left and eps does not hide it (the same for the whole
+    // workgroup, and no row of ordinary size): once more, of values scaled by a power of two.  Each value is scaled with them before it is
+    // divided (small ones), or after (large ones), so no step leaves the range that the result does not.
+    const bool large = !(tot <= FLT_MAX), small = tot < 0x1p-80f && eps < 0x1p-73f;
+    if (large || small) {
+        const float k = large ? 0x1p-80f : 0x1p100f;
+        ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss = fmaf(v[i][j] * k, v[i][j] * k, ss);
+        __syncthreads();
+        tot = over_row(ss);
+        eps = eps * k * k;
+        (large ? after : before) = k;
+    }
+    const float sc = 1.0f / sqrtf(tot / (float) a.cols + eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int p = tid + i * nt;
@@ -135,7 +157,7 @@ __global__ void __launch_bounds__(512) mx_norm_kernel(NormArgs a) {
         float g[8];
         load8<WZY_F32>(a.gamma, 8 * (size_t) p, g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = v[i][j] * sc * g[j];
+        for (int j = 0; j < 8; ++j) g[j] = v[i][j] * before * sc * after * g[j];
         if (a.y) store8<TYPE>(a.y, at0 + 8 * (size_t) p, g);
         if (a.q.codes) {
             const int byte = mx_block_scale<WZY_MX_E4M3>(g);
