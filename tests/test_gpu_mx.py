@@ -754,3 +754,23 @@ def test_add_rmsnorm_rows_whose_squares_leave_fp32(wz, gpu, t, rows, cols, eps):
     # below 2^-126 steps are 2^-149 (fp32) or 2^-133 (bf16)
     assert (np.abs(got - n) <= np.abs(n) * (NORM_REL + R.HALF_STEP[t] * (1 + NORM_REL)) + (2.0 ** -149 if t == F32 else 2.0 ** -134)).all()
     assert_quantized_near(*q.read(), n, NORM_REL)
+
+
+def test_swiglu_small_gates_times_large_factors(wz, gpu):
+    """exp(-gate) is past fp32's range from gates of -88.8 on; the products come out down to the format's smallest element"""
+    rng = np.random.default_rng(3)
+    x = np.empty((64, 128), np.float32)
+    x[:, :64] = -np.linspace(80, 187, 64, dtype=np.float32)[:, None] - rng.random((64, 64), np.float32) * 0.5
+    g = x[:, :64].astype(np.float64)
+    x[:, 64:] = np.sign(rng.standard_normal((64, 64))) * np.minimum(2.0 ** rng.integers(-20, 8, (64, 64)) / (-g * np.exp(g)), 3e38)
+    u = x[:, 64:].astype(np.float64)
+    d, q = DA.from_numpy(x), Mat(64, 64, E4M3)
+    wz.wzy_mx_swiglu(d.ptr, d.ptr + 256, F32, 128, 64, 64, q.ref(), None)
+    codes, scales = q.read()
+    v = g * u / (1 + np.exp(-g))
+    # the bound of test_swiglu, and of a product that passes through fp32's denormals half a step of those, 2^-150, before a factor
+    # exp(gate / 2) of 2^-57 at most takes the rest of its way: nothing beside the 1e-36 of assert_quantized_near, nor that beside 2^-9
+    # of the smallest scale 2^-127
+    assert_quantized_near(codes, scales, v, (np.abs(g) + 8) * 2.0 ** -22)
+    big = np.abs(v).reshape(64, 2, 32).max(2) > 1e-30
+    assert big.sum() > 60 and (scales[big] > 8).all()
