@@ -497,13 +497,16 @@ __global__ void __launch_bounds__(256, 2) mx_far_kernel(MxGemm g) {
 // their LDS reads at 5 PFLOP/s (3.3).  Bigger tiles than 256 x 256 do not fit the LDS; a fourth buffer for 32 x 64 tiles, where the
 // loads are all there is (250 x 2,048 x 6,144 9.6 us), changes nothing.
 WZY_DEV uint32_t lds_offset(const void* p) { return (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) char*) p; }
-// 64 lanes x 16 bytes from base + off (per lane) to LDS lds .. lds + 1023, lane order; lds and base wave-uniform
+// 64 lanes x 16 bytes from base + off (per lane) to LDS lds .. lds + 1023, lane order; lds and base wave-uniform.  The LDS address is in m0,
+// an output of the statement, so that the compiler knows it changed (it is a register of the compiler's own: a clobber of it means nothing; as an
+// input, E4M3 tiles of 256 x 256 spilled inside their loop, 8,192 x 8,192 x 8,192 to bf16 398 -> 422 us).
 WZY_DEV void dma16(uint32_t lds, uint32_t off, const uint8_t* base) {
     const uint64_t b = (uint64_t) (uintptr_t) base;
     lds = (uint32_t) __builtin_amdgcn_readfirstlane((int) lds);      // nothing where they are in scalar registers already
     base = (const uint8_t*) (uintptr_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (b >> 32)) << 32 |
                                          (uint32_t) __builtin_amdgcn_readfirstlane((int) b));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+    uint32_t m0;
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %2, %3" : "={m0}"(m0) : "s"(lds), "v"(off), "s"(base) : "memory");
 }
 // 64 lanes x 4 bytes, likewise
 WZY_DEV void dma4(uint32_t lds, uint32_t off, const uint8_t* base) {
@@ -511,7 +514,8 @@ WZY_DEV void dma4(uint32_t lds, uint32_t off, const uint8_t* base) {
     lds = (uint32_t) __builtin_amdgcn_readfirstlane((int) lds);
     base = (const uint8_t*) (uintptr_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (b >> 32)) << 32 |
                                          (uint32_t) __builtin_amdgcn_readfirstlane((int) b));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+    uint32_t m0;
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dword %2, %3" : "={m0}"(m0) : "s"(lds), "v"(off), "s"(base) : "memory");
 }
 // this wave's loads but the last N have landed and its LDS reads are done; then all waves meet
 template <int N>
