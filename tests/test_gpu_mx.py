@@ -774,3 +774,133 @@ def test_swiglu_small_gates_times_large_factors(wz, gpu):
     assert_quantized_near(codes, scales, v, (np.abs(g) + 8) * 2.0 ** -22)
     big = np.abs(v).reshape(64, 2, 32).max(2) > 1e-30
     assert big.sum() > 60 and (scales[big] > 8).all()
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("M", [2, 33])
+def test_gemm_scales_from_end_to_end(wz, gpu, fmt, M):
+    """every scale byte of a against the one of w that brings the product back near 1; a block that is NaN as the quantiser writes it"""
+    K, N = 256, 256
+    a = np.zeros((M, K), np.uint8)
+    a[:, 3::32] = 2 if fmt == E2M1 else 0x38                      # a one in each block
+    w = np.zeros((N, K), np.uint8)
+    w[np.arange(N), np.arange(N) % 8 * 32 + 3] = 2
+    sw = (np.arange(N)[:, None] * np.ones(K // 32, int)).clip(0, 254).astype(np.uint8)
+    for sa in (0, 1, 120, 253, 254):
+        s = np.full((M, K // 32), sa, np.uint8)
+        da, dw, y = Mat(M, K, fmt, codes=a, scales=s), Mat(N, K, E2M1, codes=w, scales=sw), out_rows(M, N, F32)
+        wz.wzy_mx_gemm(da.ref(), dw.ref(), M, N, K, y.ptr, F32, N, None)
+        want = np.exp2(sa + sw[:, 0].astype(np.float64) - 254)[None].repeat(M, 0)
+        got, inside = read_rows(y, N, F32), (want >= 2.0 ** -126) & (want < 2.0 ** 128)
+        np.testing.assert_array_equal(got[inside], want[inside])
+        assert (got[want >= 2.0 ** 128] == np.inf).all() and (got[want < 2.0 ** -126] <= 2.0 ** -126).all()
+    codes, scales = np.zeros((M, K), np.uint8), np.full((M, K // 32), 127, np.uint8)
+    scales[1, 5] = 255
+    ws = np.full((N, K // 32), 127, np.uint8)
+    ws[9, 2] = 255
+    wc = w.copy()
+    wc[9] = 0
+    for t in (F32, BF16, F16):
+        da, dw, y = Mat(M, K, fmt, codes=codes, scales=scales), Mat(N, K, E2M1, codes=wc, scales=ws), out_rows(M, N, t)
+        wz.wzy_mx_gemm(da.ref(), dw.ref(), M, N, K, y.ptr, t, N, None)
+        want = np.zeros((M, N), bool)
+        want[1], want[:, 9] = True, True
+        np.testing.assert_array_equal(np.isnan(read_rows(y, N, t)), want)
+
+
+def within_fp16(got, a, w, t):
+    """got with the infinities that fp16 rounds to from 65,520 on, halfway past its last value, in place of what they stand for; none elsewhere"""
+    if t == F16:
+        want, most = a @ w.T, 2.0 ** -9 * (np.abs(a) @ np.abs(w).T)   # (check_in_rough bounds a sum's error by that and less than as much again)
+        assert not (np.isinf(got) & (np.abs(want) + 2 * most < 65520)).any() and np.isinf(got[np.abs(want) - 2 * most > 65520]).all()
+        inf = np.isinf(got)
+        assert (np.sign(got[inf]) == np.sign(want[inf])).all()
+        got = np.where(inf, want, got)
+    return got
+
+
+# Tiles that the shapes take:   E4M3 to bf16   E2M1             E4M3 to fp32   E4M3 to fp16   (256 x 256: whole units of K; otherwise in brackets)
+#   200 x 320                   32x64          32x64            32x64          32x64
+#   10 x 4,224                  16x64          16x64            16x64          16x64
+#   4,100 x 80                  64x64          64x64            32x64          32x64
+#   4,100 x 200                 64x128         64x128           64x64          64x64
+#   900 x 4,104                 64x128         64x128           64x128         64x128
+#   4,100 x 464                 64x128         128x128          128x128        128x128
+#   3,800 x 1,552               128x128        128x128          128x128        128x128
+#   3,100 x 3,848               256x256 (64x128)  256x256 (128x128)  64x128    256x256 (128x128)
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("M,N", [(200, 320), (10, 4224), (4100, 80), (4100, 200), (900, 4104), (4100, 464), (3800, 1552), (3100, 3848)])
+def test_gemm_tiles_whole_and_any(wz, gpu, fmt, t, M, N):
+    """whole units and any K; rows of y aligned (whole lines stored) and not"""
+    rng = np.random.default_rng(M + N)
+    for n, K in [(N, 768), (N + 1, 512), (N, 608), (N + 1, 544)]:
+        a, av = random_mx(rng, M, K, fmt)
+        w, wv = random_mx(rng, n, K, E2M1)
+        y = out_rows(M, n, t)
+        wz.wzy_mx_gemm(a.ref(), w.ref(), M, n, K, y.ptr, t, n, None)
+        check_large(within_fp16(read_rows(y, n, t), av, wv, t), av, wv, fmt, t)
+
+
+# rows per group: 16x64, 32x128, 64x128, 128x128 tiles
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("per,groups", [(2, 12), (7, 9), (20, 7), (50, 5), (90, 4)])
+def test_grouped_gathered_tiles(wz, gpu, fmt, t, per, groups):
+    """whole units and any K, rows gathered, ids outside a among them, whole lines of y stored and not; the same not gathered"""
+    rng = np.random.default_rng(per + groups)
+    sizes = rng.multinomial(per * groups, np.arange(groups) / np.arange(groups).sum())
+    M = int(sizes.sum())
+    for N, K in [(256, 512), (264, 768), (129, 768), (256, 608)]:
+        ids = rng.integers(-1, M // 2 + 2, M)
+        ids[rng.integers(0, M, 2)] = [2 ** 31 - 1, -2 ** 31]
+        grouped(wz, rng, list(sizes), M, N, K, fmt, t, a_rows=M // 2 + 1, ids=ids)
+        grouped(wz, rng, list(sizes), M, N, K, fmt, t)
+
+
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("K", [512, 768])
+def test_grouped_largest_tiles_gathered(wz, gpu, t, K):
+    """256 x 256 tiles of gathered rows, ids outside a among them; a group's weights are the first one's, rolled by its number"""
+    rng = np.random.default_rng(K)
+    G, N, per, T = 64, 2048, 130, 900
+    codes = rng.integers(0, 16, (N, K)).astype(np.uint8)
+    scales = rng.integers(125, 130, (N, K // 32)).astype(np.uint8)
+    wv = R.dequantize(codes, scales, E2M1)
+    w = Mat(G * N, K, E2M1, codes=np.concatenate([np.roll(codes, g, 0) for g in range(G)]),
+            scales=np.concatenate([np.roll(scales, g, 0) for g in range(G)]))
+    sizes = rng.multinomial(G * per, np.ones(G) / G)
+    M = int(sizes.sum())
+    off = np.r_[0, np.cumsum(sizes)].astype(np.int32)
+    ids = rng.integers(-5, T + 5, M)
+    ids[[0, M - 1]] = [-2 ** 31, 2 ** 31 - 1]
+    a, av = random_mx(rng, T, K, E2M1)
+    x = np.where(((ids >= 0) & (ids < T))[:, None], av[ids.clip(0, T - 1)], 0.0)
+    y, do, di = out_rows(M, N, t), DA.from_numpy(off), DA.from_numpy(ids.astype(np.int32))
+    wz.wzy_mx_grouped_gemm(a.ref(), T, di.ptr, w.ref(), do.ptr, G, M, N, K, y.ptr, t, N, None)
+    got = read_rows(y, N, t)
+    for g in range(G):
+        i = slice(off[g], off[g + 1])
+        check_large(got[i], x[i], np.roll(wv, g, 0), E2M1, t)
+
+
+@pytest.mark.parametrize("fmt", [E2M1, E4M3])
+def test_rows_gathered_from_far_fp16(wz, gpu, fmt):
+    """rows gathered from more than 4 GiB to fp16, ids outside a among them, rows of y aligned and not"""
+    rng = np.random.default_rng(fmt)
+    stride, T, M, K = 2 ** 23 - 16, 520, 150, 544
+    codes = rng.integers(0, 16 if fmt == E2M1 else 126, (T, K)).astype(np.uint8)
+    scales = rng.integers(118, 122, (T, K // 32)).astype(np.uint8)
+    a, av = FarRows(wz, codes, scales, fmt, stride), R.dequantize(codes, scales, fmt)
+    ids = rng.integers(0, T, M)
+    ids[[0, 9, M - 1]] = [-1, T, T - 1]
+    x = np.where(((ids >= 0) & (ids < T))[:, None], av[ids.clip(0, T - 1)], 0.0)
+    do, di = DA.from_numpy(np.array([0, 70, M], np.int32)), DA.from_numpy(ids.astype(np.int32))
+    for N in (128, 75):
+        w, wv = random_mx(rng, 2 * N, K, E2M1)
+        y = out_rows(M, N, F16)
+        wz.wzy_mx_grouped_gemm(a.ref(), T, di.ptr, w.ref(), do.ptr, 2, M, N, K, y.ptr, F16, N, None)
+        got = read_rows(y, N, F16)
+        check_product(got[:70], x[:70], wv[:N], fmt, F16)
+        check_product(got[70:], x[70:], wv[N:], fmt, F16)
+    a.c.free()
