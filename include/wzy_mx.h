@@ -57,7 +57,7 @@ int wzy_mx_quantize(const void* x, int x_type, int64_t ldx, int rows, int cols, 
 int wzy_mx_dequantize(const wzy_mx_mat* q, int rows, int cols, void* y, int y_type, int64_t ldy, void* stream);
 
 /* h = x + residual (added in fp32, rounded to `type`; residual NULL: h = x),
- * n = h * 1 / sqrt(mean(h^2) + eps) * gamma   (fp32; the mean over the row's cols, also where its squares leave fp32's range),
+ * n = h * 1 / sqrt(mean(h^2) + eps) * gamma   (the mean over the row's cols; in 64 bits, rounded to fp32 once),
  * sum = h, y = n rounded to `type`, q = n as MX E4M3 (from fp32, as wzy_mx_quantize quantises).
  * x, residual, sum and y are [rows x cols] of `type` with one row stride ld (elements); gamma [cols] fp32.
  * Any of sum, y, q may be NULL, not all three; sum may be x or residual, and so may y where sum is NULL or another buffer.

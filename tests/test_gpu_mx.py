@@ -904,3 +904,20 @@ def test_rows_gathered_from_far_fp16(wz, gpu, fmt):
         check_product(got[:70], x[:70], wv[:N], fmt, F16)
         check_product(got[70:], x[70:], wv[N:], fmt, F16)
     a.c.free()
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("rows,cols", [(300, 2048), (40, 16384), (2000, 96)])
+def test_add_rmsnorm_sums_in_64_bits(wz, gpu, t, rows, cols):
+    """n is right to one rounding: the sum of squares, its root and the product keep more than fp32"""
+    rng = np.random.default_rng(rows)
+    xb, x = R.typed(activations(rng, rows, cols), t)
+    gamma = (1 + 0.1 * rng.standard_normal(cols)).astype(np.float32)
+    n = x / np.sqrt((x * x).mean(1, keepdims=True) + np.float64(np.float32(1e-6))) * gamma
+    dx, dg, y, q = DA.from_numpy(xb), DA.from_numpy(gamma), out_rows(rows, cols, t), Mat(rows, cols, E4M3)
+    wz.wzy_mx_add_rmsnorm(dx.ptr, None, t, cols, dg.ptr, 1e-6, rows, cols, None, y.ptr, q.ref(), None)
+    # 64-bit steps: at most 16,384 additions and a Newton step from 22 bits on, 2^-38 together; then fp32's half step, and bf16's of that
+    rel = 2.0 ** -24 * (1 + 2.0 ** -13)
+    half = np.exp2(np.frexp(n)[1] - (24.0 if t == F32 else 8.0) - 1) if t == F32 else R.HALF_STEP[t] * np.abs(n)
+    assert (np.abs(read_rows(y, cols, t) - n) <= (half * (1 + 2.0 ** -13) if t == F32 else half + rel * np.abs(n))).all()
+    assert_quantized_near(*q.read(), n, rel)

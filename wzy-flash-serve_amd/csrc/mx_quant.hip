@@ -4,8 +4,6 @@
 // A block of 32 values sits on the four lanes of a DPP quad, 8 consecutive values a lane: 16- or 32-byte loads, the
 // block's maximum by two quad permutations, 4 or 8 bytes of codes stored per lane.  (A large copy on this card reads and
 // writes 5.0 TB/s.)
-#include <cfloat>
-
 #include "wzy_mx.h"
 
 using namespace wzy;
@@ -97,24 +95,45 @@ __global__ void __launch_bounds__(QT) mx_dequant_kernel(MxView q, uint32_t block
 
 // ---- residual addition + RMSNorm: one workgroup a row -------------------------------------------------------
 // Thread t holds the 8-value pieces t, t + threads, ... of the row in registers: one read, the sum of squares over the
-// workgroup, one write.  NV pieces a thread, 64 .. 512 threads.  8,191 x 2,560 bf16 with residual, sum, y and E4M3 out 37 us
-// (5.1 TB/s); one row of 2,048 2.1 us on the GPU, 4.3 a call.
+// workgroup, one write.  NV pieces a thread, 64 .. 512 threads.  The sum and what follows are in 64 bits: squares of fp32 values are exact
+// there and in range, and a normed value is rounded once before it becomes a code; beside the memory traffic the operations are free
+// (fp32 sums: the same times).  8,191 x 2,560 bf16 with residual, sum, y and E4M3 out 37 us (5.1 TB/s); one row of 2,048 2.1 us on the GPU,
+// 4.3 a call.
 constexpr int NORM_MAX = 16384;
 struct NormArgs {
     const void* x; const void* res; const float* gamma;
     void* sum; void* y;
     MxView q;
     int64_t ld;
+    double inv_cols;
     float eps;
     int cols;
 };
+template <int CTRL>
+WZY_DEV double add_dpp64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t) dpp_i<CTRL>((int) b), hi = (uint32_t) dpp_i<CTRL>((int) (b >> 32));
+    return v + __builtin_bit_cast(double, (uint64_t) hi << 32 | lo);
+}
+WZY_DEV double lane64(double v, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t) (uint32_t) __builtin_amdgcn_readlane((int) (b >> 32), lane) << 32 |
+                                          (uint32_t) __builtin_amdgcn_readlane((int) b, lane));
+}
+WZY_DEV double wave_sum64(double v) {
+    v = add_dpp64<DPP_XOR1>(v);
+    v = add_dpp64<DPP_XOR2>(v);
+    v = add_dpp64<DPP_HALF_MIRROR>(v);
+    v = add_dpp64<DPP_MIRROR>(v);
+    return (lane64(v, 0) + lane64(v, 16)) + (lane64(v, 32) + lane64(v, 48));
+}
 template <int TYPE, int NV>
 __global__ void __launch_bounds__(512) mx_norm_kernel(NormArgs a) {
-    __shared__ float s_red[8];
+    __shared__ double s_red[8];
     const size_t at0 = (size_t) blockIdx.x * a.ld;
     const int tid = threadIdx.x, nt = blockDim.x, pieces = a.cols / 8;
     float v[NV][8];
-    float ss = 0.f;
+    double ss = 0.;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int p = tid + i * nt;
@@ -130,34 +149,16 @@ __global__ void __launch_bounds__(512) mx_norm_kernel(NormArgs a) {
             }
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(v[i][j], v[i][j], ss);
+        for (int j = 0; j < 8; ++j) ss = fma((double) v[i][j], (double) v[i][j], ss);
     }
-    auto over_row = [&](float part) {
-        part = wave_sum(part);
-        if ((tid & 63) == 0) s_red[tid >> 6] = part;
-        __syncthreads();
-        float tot = 0.f;
-        for (int w = 0; w < nt / 64; ++w) tot += s_red[w];
-        return tot;
-    };
-    float tot = over_row(ss), eps = a.eps, before = 1.f, after = 1.f;
-    // Squares past fp32's range, or so far below it that few bits of them are left and eps does not hide it (the same for the whole
-    // workgroup, and no row of ordinary size): once more, of values scaled by a power of two.  Each value is scaled with them before it is
-    // divided (small ones), or after (large ones), so no step leaves the range that the result does not.
-    const bool large = !(tot <= FLT_MAX), small = tot < 0x1p-80f && eps < 0x1p-73f;
-    if (large || small) {
-        const float k = large ? 0x1p-80f : 0x1p100f;
-        ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) ss = fmaf(v[i][j] * k, v[i][j] * k, ss);
-        __syncthreads();
-        tot = over_row(ss);
-        eps = eps * k * k;
-        (large ? after : before) = k;
-    }
-    const float sc = 1.0f / sqrtf(tot / (float) a.cols + eps);
+    ss = wave_sum64(ss);
+    if ((tid & 63) == 0) s_red[tid >> 6] = ss;
+    __syncthreads();
+    double tot = 0.;
+    for (int w = 0; w < nt / 64; ++w) tot += s_red[w];
+    // one Newton step from the instruction's approximation, but where that is 0, infinite or NaN
+    const double m = fma(tot, a.inv_cols, (double) a.eps), r0 = __builtin_amdgcn_rsq(m);
+    const double r = m > 0. && m < __builtin_inf() ? fma(0.5 * r0, fma(-m * r0, r0, 1.0), r0) : r0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int p = tid + i * nt;
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(512) mx_norm_kernel(NormArgs a) {
         float g[8];
         load8<WZY_F32>(a.gamma, 8 * (size_t) p, g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = v[i][j] * before * sc * after * g[j];
+        for (int j = 0; j < 8; ++j) g[j] = (float) ((double) v[i][j] * r * (double) g[j]);
         if (a.y) store8<TYPE>(a.y, at0 + 8 * (size_t) p, g);
         if (a.q.codes) {
             const int byte = mx_block_scale<WZY_MX_E4M3>(g);
@@ -261,7 +262,7 @@ extern "C" int wzy_mx_add_rmsnorm(const void* x, const void* residual, int type,
         WZY_TRY(mx_check_mat(who, "q", q, cols, a.q));
         WZY_REQUIRE(q->fmt == WZY_MX_E4M3, "%s: q is E4M3", who);
     }
-    a.x = x; a.res = residual; a.gamma = gamma; a.sum = sum; a.y = y; a.ld = ld; a.eps = eps; a.cols = cols;
+    a.x = x; a.res = residual; a.gamma = gamma; a.sum = sum; a.y = y; a.ld = ld; a.inv_cols = 1.0 / cols; a.eps = eps; a.cols = cols;
     const int pieces = cols / 8, nv = pieces <= 512 ? 1 : pieces <= 1024 ? 2 : 4;
     const int threads = (int) align_up((size_t) (pieces + nv - 1) / nv, 64);
     WZY_REQUIRE((int64_t) rows * threads < (int64_t) 1 << 32, "%s: %d rows of %d (at most %lld in a call)", who, rows, cols,
