@@ -921,3 +921,18 @@ def test_add_rmsnorm_sums_in_64_bits(wz, gpu, t, rows, cols):
     half = np.exp2(np.frexp(n)[1] - (24.0 if t == F32 else 8.0) - 1) if t == F32 else R.HALF_STEP[t] * np.abs(n)
     assert (np.abs(read_rows(y, cols, t) - n) <= (half * (1 + 2.0 ** -13) if t == F32 else half + rel * np.abs(n))).all()
     assert_quantized_near(*q.read(), n, rel)
+
+
+@pytest.mark.parametrize("low,high", [(-60, 0), (-6, 6), (-185, -40)])
+def test_swiglu_right_to_few_last_bits(wz, gpu, low, high):
+    """the exponential keeps fp32's bits at every gate: p and the reciprocal are off by one last bit, five roundings by half of one, and
+    (rounded up) what f = -|g| log2(e) - n loses to its own rounding, 2^-26, which 2^f turns into as much"""
+    rng = np.random.default_rng(max(high, 0))
+    rows, cols = 2000, 256
+    x = rng.uniform(low, high, (rows, 2 * cols)).astype(np.float32)
+    g = x[:, :cols].astype(np.float64)
+    x[:, cols:] = (rng.uniform(0.5, 2, (rows, cols)) * np.minimum(np.exp(np.maximum(-g, 0)), 1e38) / np.maximum(np.abs(g), 1e-3)).astype(np.float32)
+    u = x[:, cols:].astype(np.float64)
+    d, q = DA.from_numpy(x), Mat(rows, cols, E4M3)
+    wz.wzy_mx_swiglu(d.ptr, d.ptr + 4 * cols, F32, 2 * cols, rows, cols, q.ref(), None)
+    assert_quantized_near(*q.read(), g / (1 + np.exp(-g)) * u, 5 * 2.0 ** -23)

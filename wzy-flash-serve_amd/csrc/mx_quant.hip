@@ -13,18 +13,29 @@ namespace {
 constexpr int QT = 256;                       // threads of the flat kernels: 64 blocks at a time
 constexpr int QU = 4;                         // blocks a quad holds at once: their loads are in flight together
 
-// g / (1 + exp(-g)) * u.  For g < 0 that is g * exp(g) * u / (1 + exp(g)): exp(-g) is past fp32's range from -88.8 on, where a large u still
-// makes values that E4M3 under a scale of 2^-127 holds.  exp(g) comes as four factors exp(g / 4) (its hardware instruction gives no
-// denormals), two of them on either side of u, and u after the quotient, so that no step leaves the range before the result does.  (The reciprocal, of 1 .. 2, is
-// off by one last bit.)
-WZY_DEV float swiglu(float g, float u) {
-    const float t = __expf(-0.25f * fabsf(g)), t2 = t * t, m = g < 0.f ? t2 : 1.f;
-    return g * m * __builtin_amdgcn_rcpf(fmaf(t2, t2, 1.0f)) * u * m;
+// SwiGLU, g / (1 + exp(-g)) * u.  exp(x) = 2^n * p: x * log2(e) = n + f taken to 48 bits, p = 2^f by the hardware's instruction.  Right to 4 * 2^-23
+// (p and the reciprocal one last bit each, half of one for each of three roundings); __expf alone is off by |g| * 2^-24.
+WZY_DEV float exp_parts(float x, int& n) {
+    const float r = rintf(x * 0x1.715476p+0f);
+    n = (int) r;
+    return __builtin_amdgcn_exp2f(fmaf(x, 0x1.4ae0cp-26f, fmaf(x, 0x1.715476p+0f, -r)));
+}
+WZY_DEV float swiglu(float g, float u) {                          // g >= -87
+    int n;
+    const float p = exp_parts(fmaxf(-g, -100.0f), n);             // (a NaN of g comes back below)
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_ldexpf(p, n)) * u;
+}
+// g < -87, as g * exp(g) / (1 + exp(g)) * u: exp(-g) is past fp32's range from -88.8 on, where a large u still makes values that E4M3 under a
+// scale of 2^-127 holds.  2^n multiplies half before u and half after it, so that no step leaves the range before the result does.
+WZY_DEV float swiglu_far(float g, float u) {
+    int n;
+    const float p = exp_parts(fmaxf(g, -400.0f), n);              // the product is 0 long before; 1 + exp(g) is 1
+    return __builtin_ldexpf(__builtin_ldexpf(g * p, n >> 1) * u, n - (n >> 1));
 }
 
 // ---- quantise and SwiGLU: blocks in flat order over rows x cols / 32 ------------------------------------
 // Flat, so that any shape fills the chip: a row is a division, no workgroup belongs to one.  151,936 x 2,048 bf16 to E2M1 164 us
-// (4.8 TB/s); SwiGLU of 81,920 x 512 bf16 42 us (5.0 TB/s); 4 x 2,048 fp32 2.1 us on the GPU, 3.6 a call.
+// (4.8 TB/s); SwiGLU of 81,920 x 512 bf16 41 us (5.1 TB/s); 4 x 2,048 fp32 2.1 us on the GPU, 3.6 a call.
 template <int TYPE, int FMT, bool GLU>
 __global__ void __launch_bounds__(QT) mx_quant_kernel(const void* __restrict__ x, const void* __restrict__ up, int64_t ld,
                                                       uint32_t blocks, FastDiv per_row, MxView q) {
@@ -44,8 +55,16 @@ __global__ void __launch_bounds__(QT) mx_quant_kernel(const void* __restrict__ x
 #pragma unroll
     for (int i = 0; i < QU; ++i) {
         if constexpr (GLU) {
+            float low = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = swiglu(v[i][j], u[i][j]);
+            for (int j = 0; j < 8; ++j) low = fminf(low, v[i][j]);
+            if (low >= -87.0f) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] = swiglu(v[i][j], u[i][j]);
+            } else {                                              // rare: not worth the common path's time
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] < -87.0f ? swiglu_far(v[i][j], u[i][j]) : swiglu(v[i][j], u[i][j]);
+            }
         }
         const int byte = mx_block_scale<FMT>(v[i]);
         const uint2 c = mx_block_codes<FMT>(v[i], byte);
