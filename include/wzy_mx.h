@@ -6,6 +6,7 @@
  * passed as void* (NULL = the null stream), a status code comes back and wzy_last_error() says why a call was
  * refused.  Nothing here synchronizes, allocates, uses a workspace or keeps state between calls: calls on
  * several streams may overlap, and every call can be captured into a graph.  A refused call launches nothing.
+ * An output shares no byte with an input or another output, but where its operator says so.
  * A call with no rows (rows, M or N of 0) is valid and launches nothing.
  *
  * Together: wzy_mx_add_rmsnorm hands its rows in 8 bits to wzy_mx_gemm (projections, LM head) or, gathered by

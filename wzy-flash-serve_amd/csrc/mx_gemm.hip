@@ -273,7 +273,8 @@ __global__ void __launch_bounds__(512) mx_skinny_kernel(MxGemm g) {
 template <bool PAIR>
 WZY_DEV int w_row(int j, int lr) { return PAIR ? 32 * (j / 2) + 8 * (lr >> 2) + 4 * (j % 2) + (lr & 3) : 16 * j + lr; }
 // A row of P 16-byte pieces keeps them exchanged by the bits of the row's number that differ among the 16 rows that 16 lanes
-// read one piece of at a time (16 i .. of a, w_row of w), so that these touch all 64 banks once: no conflicts counted.
+// read one piece of at a time (16 i .. of a, w_row of w), so that these touch all 64 banks once.  Conflict cycles counted, of the LDS's active ones:
+// 16 x 64 tiles none, 256 x 256 E2M1 to bf16 0.07, 32 x 64 E4M3 to bf16 0.10, 128 x 128 the same per group 0.27.
 template <int P>
 WZY_DEV int swz_a(int r) { return P == 16 ? r & 15 : P == 8 ? (r >> 1) & 7 : (r >> 2) & 3; }
 template <int P, bool PAIR>
@@ -290,7 +291,7 @@ WZY_DEV void store_tile(const MxGemm& g, bool gather, bool whole, int row0, int 
     // Whole cache lines: a lane has two 16-byte pieces of its row 64 bytes apart.  Lanes lr and lr + 8 exchange one of theirs, and a store writes
     // 8 rows of 128 bytes, past the caches (half lines stored so cost up to 18 %, whole ones through the caches nothing).  us, before and
     // after: 8,192 x 6,144 x 2,048 E2M1 to bf16 68 and 65, to fp32 101 and 82, E4M3 to fp32 207 and 182; 8,192 x 12,288 x 2,048 E2M1 142 and 127,
-    // 220 and 158; per group, 82,000 rows of K 512, E4M3 257 and 234; but 8,192 x 8,192 x 320 to bf16 50 and 52.
+    // 220 and 158; per group, gathered, 81,920 x 2,048 x 512, E4M3 to bf16 257 and 234; but 8,192 x 8,192 x 320 to bf16 50 and 52.
     constexpr int LINE = OUT == WZY_F32 ? 2 : 4;                      // column blocks of 128 bytes
     if constexpr (CB % LINE == 0) {
         if (whole) {
@@ -873,7 +874,7 @@ Tile dense_tile(const MxGemm& g, bool e8, bool whole) {
     const auto& c = cost[!e8 ? 1 : f32 ? 2 : g.y_type == WZY_F16 ? 3 : 0];
     Tile best = T32x64;
     float least = 0.f;
-    for (int i = (e8 && f32) || !whole ? 1 : 0; i < 5; ++i) {      // E4M3 to fp32 and ANY have no 256 x 256 (their registers spill)
+    for (int i = (e8 && f32) || !whole ? 1 : 0; i < 5; ++i) {      // E4M3 to fp32 and ANY have no 256 x 256: their registers spill inside the loop (E4M3 to 16 bits spills 4 or 5, before and after it)
         const int64_t t = ((int64_t) g.M + TILE_M[kind[i]] - 1) / TILE_M[kind[i]] * (((int64_t) g.N + TILE_N[kind[i]] - 1) / TILE_N[kind[i]]);
         const int64_t n = (t + CUS - 1) / CUS;
         const float us = (float) (n / 2) * c[i][1] + (float) (n % 2) * c[i][0];
@@ -883,7 +884,8 @@ Tile dense_tile(const MxGemm& g, bool e8, bool whole) {
 }
 // Tiles of a product per group, by the rows of a group that has any.  Measured at 512 groups, N 1,024, K 2,048, E4M3 to bf16, us: 6 rows
 // 16x64 106, 32x128 108 (to fp32 117, 134); 12 rows 128, 118, 64x128 132; 20 rows 32x128 126, 64x128 134; 40 rows 168, 149, 128x128 164; 80
-// rows 64x128 213, 128x128 192; 160 rows 128x128 304, 256x256 367, but E2M1 253, 218.
+// rows 64x128 213, 128x128 192; 160 rows 128x128 304, 256x256 367, but E2M1 253, 218.  (Which groups have entries is not known here: where a few of
+// many hold all rows, tiles are smaller than they would best be, 8,192 rows in 4 of 512 groups 35.5 us, in 4 of 4 27.5.)
 Tile grouped_tile(const MxGemm& g, bool e8, bool whole) {
     const int rows = g.M / std::min(g.M, g.groups);
     if (rows <= 8) return T16x64;
