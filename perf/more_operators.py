@@ -351,7 +351,8 @@ def calls(s):
         s["q_start"], s["kv_len"], s["served"] = int32(requests + 1), int32(requests), int32(requests)
         s["row_positions"], s["row_slots"] = int32(s["max_tokens"]), int32(s["max_tokens"])
         return W.PagedBatch(requests, s["max_tokens"], s["max_pages"], at(s["n_cached"]), at(s["n_new"]), at(s["table"]),
-                            at(s["q_start"]), at(s["kv_len"]), at(s["served"]), at(s["row_positions"]), at(s["row_slots"]))
+                            at(s["q_start"]), at(s["kv_len"]), at(s["served"]), at(s["row_positions"]), at(s["row_slots"]),
+                            max(lengths(c)[1]))
 
     def work(b, qh, kvh, hd, window):
         w = W.PagedWork(qh, kvh, hd, window, None, 0)
@@ -378,7 +379,7 @@ def calls(s):
         cfg = W.RopeCfg(m["theta"], m["factor"], m["low"], m["high"], m["amplitude"], m["ctx"], c["n_rot"], kind)
         s["freqs"] = torch.empty(c["n_rot"] // 2 + 1, device=DEV, dtype=torch.float64)
         lib.wzy_rope_freqs(C.byref(cfg), at(s["freqs"]), st)
-        r = W.Rope(at(s["freqs"]), c["n_rot"], W.ROPE_PAIRS if c["layout"] == "pairs" else W.ROPE_HALVES)
+        r = W.RopeTab(at(s["freqs"]), c["n_rot"], W.ROPE_PAIRS if c["layout"] == "pairs" else W.ROPE_HALVES)
         if op == "rope":
             x, y = heads(s["x"]), heads(s["out"])
             todo = [(lib.wzy_rope, (C.byref(r), C.byref(x), types[s["x"].dtype], c["rows"], c["heads"], c["hd"], at(s["positions"]),
