@@ -1,0 +1,561 @@
+// paged_attn.hip -- attention of new tokens over a paged key-value cache.
+//
+//   o = sum_j 2^(t_j - m) v_j / sum_j 2^(t_j - m),   t_j = scale log2(e) q . k_j,   m the running maximum of t
+//
+// One pass over the keys, 32 at a time, on v_mfma_f32_32x32x16: S^T = K Q^T, then O^T += V^T P^T.  The products are taken
+// transposed so that a lane holds one query row throughout: of S^T it has 16 keys' scores (the other 16 are in the lane 32
+// away), so maximum and sum cost one exchange between the halves, rescaling is by a lane's own factor, and the accumulator
+// registers of S^T, rounded, are P^T's operand as they stand: register i of lane half h is key 8 (i / 4) + 4 h + i % 4, which
+// is the order in which V^T's operand then takes its keys (the product's sum may run over them in any order).  V lies in LDS
+// as in memory, a row a key, and ds_read_b64_tr_b16 hands each lane four keys of one column.
+//
+// Rows are (token, head of the group) pairs of one key head, so a group's heads share every byte of K and V.
+//   narrow  up to 32 rows: the waves of a workgroup take every fourth block of 32 keys each, through buffers of their own,
+//           with no barrier until their results are joined
+//   wide    128 rows, 32 a wave: the workgroup's waves share each block
+// The maximum follows the scores only when one has come 2^8 above it, so most blocks leave the accumulators alone; weights
+// then reach 2^8, and in fp16, whose numbers end at 2^-24, all are taken 2^6 larger.
+#include "wzy_paged.h"
+
+using namespace wzy;
+
+typedef short v4s_t __attribute__((ext_vector_type(4)));
+typedef __bf16 v8b_t __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h_t __attribute__((ext_vector_type(8)));
+typedef float v16f_t __attribute__((ext_vector_type(16)));
+typedef uint32_t v4w_t __attribute__((ext_vector_type(4)));
+
+namespace {
+
+struct AttnArgs {
+    const char* k;
+    const char* v;
+    int64_t ld_page, ld_cell, ld_head;       // bytes
+    const int* table;
+    const char* q;
+    char* out;
+    int64_t ldq, ldq_head, ldo, ldo_head;    // bytes
+    const PgHead* head;
+    float* part_o;                           // [part][kvh][tile rows][hd]
+    float2* part_ml;                         // [part][kvh][tile rows]: maximum, sum
+    FastDiv div_g;
+    float c;                                 // scale * log2(e)
+    int n_pages, lp, max_pages, n_req, max_tokens;
+    int g, kvh, window, geometry;
+    int item_at, cap_items, cap_parts, merge_at, cap_merges;
+};
+
+template <int T> struct Half;                // of the cache's type
+template <> struct Half<WZY_BF16> {
+    static constexpr float SHIFT = 0.0f;
+    static WZY_DEV v16f_t mfma(v4w_t a, v4w_t b, v16f_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b_t, a), __builtin_bit_cast(v8b_t, b), c, 0, 0, 0);
+    }
+};
+template <> struct Half<WZY_F16> {
+    static constexpr float SHIFT = 6.0f;
+    static WZY_DEV v16f_t mfma(v4w_t a, v4w_t b, v16f_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h_t, a), __builtin_bit_cast(v8h_t, b), c, 0, 0, 0);
+    }
+};
+constexpr float RISE = 8.0f;
+
+WZY_DEV uint32_t lds_offset(const void* p) { return (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) char*) p; }
+// 64 lanes x 16 bytes to LDS lds .. lds + 1023 in lane order, from a wave-uniform base + off, or from an address a lane
+WZY_DEV void dma16(uint32_t lds, uint32_t off, const char* base) {
+    uint32_t m0;
+    lds = (uint32_t) __builtin_amdgcn_readfirstlane((int) lds);          // nothing where it is in a scalar register already
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %2, %3" : "={m0}"(m0) : "s"(lds), "v"(off), "s"(base) : "memory");
+}
+WZY_DEV void dma16(uint32_t lds, const char* p) {
+    uint32_t m0;
+    lds = (uint32_t) __builtin_amdgcn_readfirstlane((int) lds);          // nothing where it is in a scalar register already
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %2, off" : "={m0}"(m0) : "s"(lds), "v"(p) : "memory");
+}
+// this wave's loads but the last N have landed
+template <int N>
+WZY_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+WZY_DEV void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// this wave's loads have landed and its LDS reads are done; then all waves meet
+WZY_DEV void wait_all_and_meet() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+WZY_DEV const char* uniform(const char* p) {
+    const uint64_t b = (uint64_t) (uintptr_t) p;
+    return (const char*) (uintptr_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (b >> 32)) << 32 |
+                                      (uint32_t) __builtin_amdgcn_readfirstlane((int) b));
+}
+// the other lane half's value
+WZY_DEV float other_half(float v) { return __shfl_xor(v, 32); }
+
+// K and V of 32 keys in LDS: a row a key, its 16-byte pieces permuted by the key.  K is read by 32 lanes, a row each, the same
+// piece: pieces p ^ f(row) are spread over the banks.  V is read by 16 lanes as 4 keys x 32 bytes, twice side by side: the
+// 64-byte groups of 4 neighbouring keys change places.
+template <int HD>
+struct Block {
+    static constexpr int PIECES = HD / 8, ROW = HD * 2, BYTES = 32 * ROW, LOADS = BYTES / 1024, ROWS = 64 / PIECES;   // rows a load
+    static WZY_DEV int swz_k(int row) { return HD == 64 ? (row >> 1) & 7 : row & (PIECES - 1); }
+    static WZY_DEV int swz_v(int row) { return HD == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
+    // K's operand: row l % 32, piece 2 s + l / 32
+    static WZY_DEV v4w_t k_at(const char* lds, int lane, int s) {
+        const int row = lane & 31;
+        return *(const v4w_t*) (lds + row * ROW + (((2 * s + (lane >> 5)) ^ swz_k(row)) << 4));
+    }
+    // V^T's operand for columns 32 d + l % 32: keys 16 s + 4 h + 0 .. 3 and 8 more than those, h = l / 32
+    static WZY_DEV v4w_t v_at(const char* lds, int lane, int s, int d) {
+        const int i = lane & 15;
+        v4w_t r;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const int row = 16 * s + 8 * p + 4 * (lane >> 5) + (i >> 2);
+            const int piece = 4 * d + 2 * (lane >> 4 & 1) + (i >> 1 & 1);
+            const char* const at = lds + row * ROW + ((piece ^ swz_v(row)) << 4) + 8 * (i & 1);
+            const v4s_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*) at);
+            const uint2 w = __builtin_bit_cast(uint2, x);
+            r[2 * p] = w.x;
+            r[2 * p + 1] = w.y;
+        }
+        return r;
+    }
+};
+
+// A tile's place in the step
+struct TileCtx {
+    PgItem it;
+    int head;                                // key head
+    const int* pages;                        // the request's row of the table
+};
+
+// Loads of one block's K or V.  Rows of a block are 32 neighbouring cells from a multiple of 32, so a page holds all of them or
+// (16 cells a page) a half.  Blocks that reach past the part's cells repeat its first or last: what lies there in memory may be
+// anything, a NaN too, and a weight of 0 does not silence it.
+template <int HD>
+struct Loader {
+    using B = Block<HD>;
+    const AttnArgs& a;
+    const TileCtx& t;
+    int lane;
+    const char* base[2];                     // of K's halves; V's are as far off
+    int64_t to_v;
+    bool whole;
+    int first, last;                         // rows that are there, where not all are
+    WZY_DEV Loader(const AttnArgs& a_, const TileCtx& t_, int lane_) : a(a_), t(t_), lane(lane_), to_v(a_.v - a_.k) {}
+    WZY_DEV const char* cell(int c) const {
+        int id = t.pages[c >> a.lp];
+        id = (unsigned) id < (unsigned) a.n_pages ? id : 0;
+        return a.k + (int64_t) id * a.ld_page + (int64_t) (c & ((1 << a.lp) - 1)) * a.ld_cell + (int64_t) t.head * a.ld_head;
+    }
+    // the block of cells 32 b .. 32 b + 31, at least one of them the part's
+    WZY_DEV void at(int b) {
+        const int c = 32 * b;
+        whole = c >= t.it.lo && c + 32 <= t.it.hi;
+        first = max(t.it.lo - c, 0);
+        last = min(t.it.hi - c, 32) - 1;
+        // cells of a half that has none of the part are not looked up
+        const int h0 = first < 16 ? 0 : 16, h1 = last >= 16 ? 16 : 0;
+        base[0] = uniform(cell(c + h0));
+        base[1] = uniform(h1 == h0 ? base[0] : cell(c + h1));
+    }
+    // loads i0 .. i1 - 1 (of LOADS, each B::ROWS rows) into lds
+    template <bool V, int I0, int I1>
+    WZY_DEV void issue(uint32_t lds, int start) const {
+        const int r0 = lane / B::PIECES, piece = lane & (B::PIECES - 1);
+        const int64_t add = V ? to_v : 0;
+        if (whole) {
+#pragma unroll
+            for (int i = I0; i < I1; ++i) {
+                const int row = (start + i) * B::ROWS + r0;
+                const uint32_t off = (uint32_t) (row & 15) * (uint32_t) a.ld_cell + (uint32_t) ((piece ^ (V ? B::swz_v(row) : B::swz_k(row))) << 4);
+                dma16(lds + (uint32_t) (start + i) * 1024, off, uniform(((start + i) * B::ROWS < 16 ? base[0] : base[1]) + add));
+            }
+        } else {
+#pragma unroll
+            for (int i = I0; i < I1; ++i) {
+                const int row = (start + i) * B::ROWS + r0, from = min(max(row, first), last);
+                const char* const p = (from < 16 ? base[0] : base[1]) + add + (int64_t) (from & 15) * a.ld_cell +
+                                      ((piece ^ (V ? B::swz_v(row) : B::swz_k(row))) << 4);
+                dma16(lds + (uint32_t) (start + i) * 1024, p);
+            }
+        }
+    }
+};
+
+// A wave's 32 query rows
+template <int HD, int T>
+struct Wave {
+    static constexpr int KS = HD / 16, DT = HD / 32;
+    v4w_t q[KS];
+    v16f_t o[DT];
+    float m, l;
+    int pos, pos_min, pos_max;               // of the lane's row; of the wave's
+    int row, rows;                           // the lane's row of the tile's request; rows of the request
+
+    WZY_DEV void start(const AttnArgs& a, const TileCtx& t, int row0, int lane) {
+        rows = t.it.n_new * a.g;
+        row = row0 + (lane & 31);
+        const int r = min(row, rows - 1), token = (int) fast_div((uint32_t) r, a.div_g), h = r - token * a.g;
+        pos = t.it.n_cached + token;
+        pos_min = t.it.n_cached + (int) fast_div((uint32_t) min(row0, rows - 1), a.div_g);
+        pos_max = t.it.n_cached + (int) fast_div((uint32_t) min(row0 + 31, rows - 1), a.div_g);
+        const char* const p = a.q + (int64_t) (t.it.q0 + token) * a.ldq + (int64_t) (t.head * a.g + h) * a.ldq_head + (lane >> 5) * 16;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[s] = row < rows ? *(const v4w_t*) (p + 32 * s) : v4w_t{0, 0, 0, 0};
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] = v16f_t{};
+        m = -INFINITY;
+        l = 0.0f;
+    }
+    // does the wave see any cell of block b, and does it see all of them?
+    WZY_DEV bool sees(const AttnArgs& a, int b) const {
+        return 32 * b <= pos_max && (a.window == 0 || 32 * b + 31 > pos_min - a.window);
+    }
+    WZY_DEV bool masked(const AttnArgs& a, int b) const {
+        return 32 * b + 31 > pos_min || (a.window != 0 && 32 * b <= pos_max - a.window);
+    }
+    WZY_DEV v16f_t scores(const char* kb, int lane) const {
+        v16f_t s = v16f_t{};
+#pragma unroll
+        for (int i = 0; i < KS; ++i) s = Half<T>::mfma(Block<HD>::k_at(kb, lane, i), q[i], s);
+        return s;
+    }
+    // scores to weights, rounded and packed
+    WZY_DEV void weights(const AttnArgs& a, int b, int lane, v16f_t& s, v4w_t (&p)[2]) {
+        if (masked(a, b)) {
+            const int low = a.window ? pos - a.window : -1;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = 32 * b + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+                s[i] = key <= pos && key > low ? s[i] : -INFINITY;
+            }
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        mx = fmaxf(mx, other_half(mx)) * a.c;
+        if (__any(mx > m + RISE)) {
+            const float to = fmaxf(m, mx), f = to > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] *= f;
+        }
+        const float less = m > -INFINITY ? Half<T>::SHIFT - m : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, less));
+            l += s[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i / 4][i % 4] = pack2<T>(s[2 * i], s[2 * i + 1]);
+    }
+    WZY_DEV void add(const char* vb, int lane, const v4w_t (&p)[2]) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) o[d] = Half<T>::mfma(Block<HD>::v_at(vb, lane, s, d), p[s], o[d]);
+    }
+};
+
+// the workgroup's item and key head; false where there is none, or the list is not one of this step
+WZY_DEV bool tile_ctx(const AttnArgs& a, int kind, TileCtx& t) {
+    const int at = (int) (blockIdx.x / (unsigned) a.kvh);
+    t.head = (int) (blockIdx.x - (unsigned) at * (unsigned) a.kvh);
+    if (a.head->magic != PG_MAGIC || a.head->geometry != a.geometry || at >= a.head->n_items[kind]) return false;
+    t.it = ((const PgItem*) (a.head + 1))[a.item_at + at];
+    const PgItem& i = t.it;
+    if ((unsigned) i.req >= (unsigned) a.n_req || i.q0 < 0 || i.n_new < 1 || i.q0 > a.max_tokens - i.n_new || i.row0 < 0 || i.row0 >= i.n_new * a.g ||
+        i.lo < 0 || i.hi > a.max_pages << a.lp || i.part >= a.cap_parts)
+        return false;
+    t.pages = a.table + (size_t) i.req * a.max_pages;
+    return true;
+}
+WZY_DEV char* out_row(const AttnArgs& a, const TileCtx& t, int row) {
+    const int token = (int) fast_div((uint32_t) row, a.div_g);
+    return a.out + (int64_t) (t.it.q0 + token) * a.ldo + (int64_t) (t.head * a.g + row - token * a.g) * a.ldo_head;
+}
+
+template <int HD, int T>
+__global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
+    using B = Block<HD>;
+    __shared__ __align__(1024) char s_buf[4][2 * B::BYTES];             // a wave's K and V; then its results in fp32
+    __shared__ float s_m[4][32], s_l[4][32];
+    static_assert(2 * B::BYTES == 32 * HD * 4, "a wave's results take its buffers");
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    TileCtx t;
+    if (!tile_ctx(a, 0, t)) return;
+    if (t.it.lo >= t.it.hi) {                                           // not served: all its rows become 0
+        for (int i = tid; i < t.it.n_new * a.g * (HD / 8); i += 256) {
+            const int row = i / (HD / 8);
+            *(v4w_t*) (out_row(a, t, row) + 16 * (i % (HD / 8))) = v4w_t{0, 0, 0, 0};
+        }
+        return;
+    }
+    Wave<HD, T> w;
+    w.start(a, t, 0, lane);
+    Loader<HD> ld(a, t, lane);
+    char* const kb = s_buf[wave];
+    char* const vb = kb + B::BYTES;
+    const uint32_t lk = lds_offset(kb), lv = lds_offset(vb);
+    const int end = (t.it.hi + 31) >> 5;
+    int b = (t.it.lo >> 5) + wave;
+    if (b < end) {
+        wait_loads<0>();                                                // what the compiler still has in flight: q
+        ld.at(b);
+        ld.template issue<false, 0, B::LOADS>(lk, 0);
+        ld.template issue<true, 0, B::LOADS>(lv, 0);
+        for (;; b += 4) {
+            const bool more = b + 4 < end;
+            wait_loads<B::LOADS>();                                     // K is there
+            v16f_t s = w.scores(kb, lane);
+            wait_lds();                                                 // and read
+            if (more) {
+                ld.at(b + 4);
+                ld.template issue<false, 0, B::LOADS>(lk, 0);
+            }
+            v4w_t p[2];
+            w.weights(a, b, lane, s, p);
+            if (more) wait_loads<B::LOADS>();
+            else wait_loads<0>();
+            w.add(vb, lane, p);
+            if (!more) break;
+            wait_lds();
+            ld.template issue<true, 0, B::LOADS>(lv, 0);
+        }
+    }
+    w.l += other_half(w.l);
+    if (lane < 32) {
+        s_m[wave][lane] = w.m;
+        s_l[wave][lane] = w.l;
+    }
+    // results as [column / 4][row][4]: neighbouring lanes side by side
+    wait_lds();
+    float4* const r = (float4*) s_buf[wave];
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            r[(8 * d + 2 * i + (lane >> 5)) * 32 + (lane & 31)] = make_float4(w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]);
+    __syncthreads();
+    const int rows = w.rows;
+    for (int i = tid; i < rows * (HD / 4); i += 256) {
+        const int row = i / (HD / 4), col = i % (HD / 4);
+        float m = s_m[0][row], l = 0.0f;
+#pragma unroll
+        for (int k = 1; k < 4; ++k) m = fmaxf(m, s_m[k][row]);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float f = s_l[k][row] != 0.0f ? __builtin_amdgcn_exp2f(s_m[k][row] - m) : 0.0f;
+            const float4 x = ((const float4*) s_buf[k])[col * 32 + row];
+            l += f * s_l[k][row];
+            o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
+        }
+        if (t.it.part < 0) {
+            const float n = l != 0.0f ? 1.0f / l : 0.0f;
+            *(uint2*) (out_row(a, t, row) + 8 * col) = make_uint2(pack2<T>(o.x * n, o.y * n), pack2<T>(o.z * n, o.w * n));
+        } else {
+            const size_t at = ((size_t) t.it.part * a.kvh + t.head) * PG_NARROW + row;
+            ((float4*) (a.part_o + at * HD))[col] = o;
+            if (col == 0) a.part_ml[at] = make_float2(m, l);
+        }
+    }
+}
+
+template <int HD, int T>
+__global__ void __launch_bounds__(256) paged_wide_kernel(AttnArgs a) {
+    using B = Block<HD>;
+    __shared__ __align__(1024) char s_buf[2][2 * B::BYTES];             // two blocks' K and V
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    TileCtx t;
+    if (!tile_ctx(a, 1, t)) return;
+    Wave<HD, T> w;
+    w.start(a, t, t.it.row0 + 32 * wave, lane);
+    Loader<HD> ld(a, t, lane);
+    const uint32_t lk = lds_offset(s_buf);
+    const int end = (t.it.hi + 31) >> 5;
+    int b = t.it.lo >> 5, buf = 0;
+    constexpr int MINE = B::LOADS / 4;                                  // of each matrix, a wave
+    wait_loads<0>();
+    if (b < end) {
+        ld.at(b);
+        ld.template issue<false, 0, MINE>(lk, wave * MINE);
+        ld.template issue<true, 0, MINE>(lk + B::BYTES, wave * MINE);
+    }
+    for (; b < end; ++b, buf ^= 1) {
+        wait_all_and_meet();                                            // the block is there; the other buffer has been read
+        if (b + 1 < end) {
+            ld.at(b + 1);
+            const uint32_t to = lk + (uint32_t) (buf ^ 1) * 2 * B::BYTES;
+            ld.template issue<false, 0, MINE>(to, wave * MINE);
+            ld.template issue<true, 0, MINE>(to + B::BYTES, wave * MINE);
+        }
+        if (w.sees(a, b)) {
+            v16f_t s = w.scores(s_buf[buf], lane);
+            v4w_t p[2];
+            w.weights(a, b, lane, s, p);
+            w.add(s_buf[buf] + B::BYTES, lane, p);
+        }
+    }
+    const float l = w.l + other_half(w.l);
+    if (w.row >= w.rows) return;
+    if (t.it.part < 0) {
+        const float n = l != 0.0f ? 1.0f / l : 0.0f;
+        char* const p = out_row(a, t, w.row) + 8 * (lane >> 5);
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *(uint2*) (p + 64 * d + 16 * i) = make_uint2(pack2<T>(w.o[d][4 * i] * n, w.o[d][4 * i + 1] * n),
+                                                             pack2<T>(w.o[d][4 * i + 2] * n, w.o[d][4 * i + 3] * n));
+    } else {
+        const size_t at = ((size_t) t.it.part * a.kvh + t.head) * PG_WIDE + (w.row - t.it.row0);
+        float4* const p = (float4*) (a.part_o + at * HD) + (lane >> 5);
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[8 * d + 2 * i] = make_float4(w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]);
+        if (lane < 32) a.part_ml[at] = make_float2(w.m, l);
+    }
+}
+
+// Parts of a tile joined.  HD / 4 lanes hold a row; of a workgroup's groups of lanes, several take one row's parts in turn where
+// there are many, so that all of a row's loads are under way at once.  blockIdx.y goes through the tile's rows.
+template <int HD, int T, int ROWS>
+__global__ void __launch_bounds__(512) paged_merge_kernel(AttnArgs a, int kind) {
+    constexpr int L = HD / 4, GROUPS = 512 / L;
+    __shared__ float4 s_o[512];
+    __shared__ float2 s_ml[GROUPS];
+    const int at = (int) (blockIdx.x / (unsigned) a.kvh), head = (int) (blockIdx.x - (unsigned) at * (unsigned) a.kvh);
+    if (a.head->magic != PG_MAGIC || a.head->geometry != a.geometry || at >= a.head->n_merges[kind]) return;
+    const PgMerge e = ((const PgMerge*) (a.head + 1))[a.merge_at + at];
+    if (e.part < 0 || e.n < 1 || e.part > a.cap_parts - e.n || e.rows < 1 || e.rows > ROWS || e.row0 < 0 || e.q0 < 0) return;
+    int per = 1;                                                        // groups a row
+    while (per < GROUPS && per * 4 < e.n) per *= 2;
+    const int rows_here = GROUPS / per, group = threadIdx.x / L, col = threadIdx.x % L, sub = group & (per - 1);
+    for (int r0 = blockIdx.y * rows_here; r0 < e.rows; r0 += gridDim.y * rows_here) {
+        const int r = min(r0 + group / per, e.rows - 1);
+        float m = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = sub; i < e.n; i += 4 * per) {
+            float2 ml[4];
+            float4 x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k = i + j * per;
+                const size_t p = ((size_t) (e.part + min(k, e.n - 1)) * a.kvh + head) * ROWS + r;
+                ml[j] = a.part_ml[p];
+                x[j] = ((const float4*) (a.part_o + p * HD))[col];
+                if (k >= e.n) ml[j] = make_float2(-INFINITY, 0.0f);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (ml[j].y != 0.0f) {
+                    const float to = fmaxf(m, ml[j].x), f = l != 0.0f ? __builtin_amdgcn_exp2f(m - to) : 0.0f, g = __builtin_amdgcn_exp2f(ml[j].x - to);
+                    m = to;
+                    l = l * f + ml[j].y * g;
+                    o.x = o.x * f + x[j].x * g; o.y = o.y * f + x[j].y * g; o.z = o.z * f + x[j].z * g; o.w = o.w * f + x[j].w * g;
+                }
+        }
+        if (per > 1) {
+            s_o[threadIdx.x] = o;
+            if (col == 0) s_ml[group] = make_float2(m, l);
+            __syncthreads();
+            if (sub == 0) {
+                for (int j = 1; j < per; ++j) {
+                    const float2 ml = s_ml[group + j];
+                    const float4 x = s_o[threadIdx.x + j * L];
+                    if (ml.y != 0.0f) {
+                        const float to = fmaxf(m, ml.x), f = l != 0.0f ? __builtin_amdgcn_exp2f(m - to) : 0.0f, g = __builtin_amdgcn_exp2f(ml.x - to);
+                        m = to;
+                        l = l * f + ml.y * g;
+                        o.x = o.x * f + x.x * g; o.y = o.y * f + x.y * g; o.z = o.z * f + x.z * g; o.w = o.w * f + x.w * g;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (sub == 0 && r0 + group / per < e.rows) {
+            const float n = l != 0.0f ? 1.0f / l : 0.0f;
+            const int row = e.row0 + r, token = (int) fast_div((uint32_t) row, a.div_g);
+            if (e.q0 + token < a.max_tokens)
+                *(uint2*) (a.out + (int64_t) (e.q0 + token) * a.ldo + (int64_t) (head * a.g + row - token * a.g) * a.ldo_head + 8 * col) =
+                    make_uint2(pack2<T>(o.x * n, o.y * n), pack2<T>(o.z * n, o.w * n));
+        }
+    }
+}
+
+struct Space { size_t o, ml, total; };
+Space space_of(const PgLayout& l, const wzy_paged_work* w) {
+    const size_t n = (size_t) l.parts[0] * PG_NARROW, wide = (size_t) l.parts[1] * PG_WIDE, rows = (n > wide ? n : wide) * w->kvh;
+    Space s;
+    s.o = 0;
+    s.ml = align_up(rows * w->hd * 4, 256);
+    s.total = s.ml + align_up(rows * sizeof(float2), 256);
+    return s;
+}
+
+template <int HD, int T>
+int launch(AttnArgs a, const PgLayout& l, void* stream) {
+    const auto st = as_stream(stream);
+    for (int kind = 0; kind < 2; ++kind) {
+        if (l.items[kind] == 0) continue;
+        a.item_at = l.item_at[kind]; a.cap_items = l.items[kind]; a.cap_parts = l.parts[kind];
+        a.merge_at = l.merge_at[kind]; a.cap_merges = l.merges[kind];
+        const unsigned grid = (unsigned) l.items[kind] * (unsigned) a.kvh;
+        if (kind == 0) paged_narrow_kernel<HD, T><<<grid, 256, 0, st>>>(a);
+        else paged_wide_kernel<HD, T><<<grid, 256, 0, st>>>(a);
+        WZY_LAUNCH_CHECK();
+        if (l.merges[kind] == 0) continue;
+        const unsigned tiles = (unsigned) l.merges[kind] * (unsigned) a.kvh;
+        if (kind == 0) paged_merge_kernel<HD, T, PG_NARROW><<<dim3(tiles, 32), 512, 0, st>>>(a, kind);
+        else paged_merge_kernel<HD, T, PG_WIDE><<<dim3(tiles, 16), 512, 0, st>>>(a, kind);
+        WZY_LAUNCH_CHECK();
+    }
+    return WZY_OK;
+}
+}  // namespace
+
+extern "C" size_t wzy_paged_attend_workspace_bytes(const wzy_paged_batch* b, const wzy_paged_work* w) {
+    if (pg_check_batch("wzy_paged_attend_workspace_bytes", b, 1) != WZY_OK || pg_check_work("wzy_paged_attend_workspace_bytes", w) != WZY_OK) return 0;
+    return space_of(pg_layout_of(b, w), w).total;
+}
+
+extern "C" int wzy_paged_attend(const wzy_paged_cache* c, const wzy_paged_batch* b, const wzy_paged_work* w, const wzy_heads* q,
+                                const wzy_heads* out, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* const who = "wzy_paged_attend";
+    WZY_TRY(pg_check_cache(who, c));
+    WZY_TRY(pg_check_batch(who, b, c->page));
+    WZY_TRY(pg_check_work(who, w));
+    WZY_REQUIRE(w->kvh == c->kvh && w->hd == c->hd, "%s: work list of %d heads of %d, cache of %d of %d", who, w->kvh, w->hd, c->kvh, c->hd);
+    WZY_REQUIRE(b->table, "%s: table is null", who);
+    const PgLayout l = pg_layout_of(b, w);
+    WZY_REQUIRE(w->items && (uintptr_t) w->items % 16 == 0 && w->bytes >= sizeof(PgHead) + sizeof(PgItem) * (size_t) l.total,
+                "%s: work list of %zu bytes at %p", who, w->bytes, w->items);
+    WZY_TRY(pg_check_heads(who, "q", q, c->type, w->qh, c->hd));
+    WZY_TRY(pg_check_heads(who, "out", out, c->type, w->qh, c->hd));
+    for (const wzy_heads* h : {q, out})
+        WZY_REQUIRE((uintptr_t) h->p % 16 == 0 && h->ld % 8 == 0 && h->ld_head % 8 == 0, "%s: %s has rows without 16-byte alignment", who,
+                    h == q ? "q" : "out");
+    WZY_REQUIRE(q->p != out->p, "%s: out is q", who);
+    WZY_REQUIRE(scale > 0.0f && scale < 1e30f, "%s: scale %g", who, (double) scale);
+    const Space s = space_of(l, w);
+    WZY_REQUIRE(workspace && (uintptr_t) workspace % 16 == 0 && workspace_bytes >= s.total, "%s: workspace of %zu bytes at %p (%zu, 16-byte aligned)",
+                who, workspace_bytes, workspace, s.total);
+    AttnArgs a{};
+    a.k = (const char*) c->k; a.v = (const char*) c->v;
+    a.ld_page = 2 * c->ld_page; a.ld_cell = 2 * c->ld_cell; a.ld_head = 2 * c->ld_head;
+    a.table = b->table;
+    a.q = (const char*) q->p; a.ldq = 2 * q->ld; a.ldq_head = 2 * q->ld_head;
+    a.out = (char*) out->p; a.ldo = 2 * out->ld; a.ldo_head = 2 * out->ld_head;
+    a.head = (const PgHead*) w->items;
+    a.part_o = (float*) ((char*) workspace + s.o);
+    a.part_ml = (float2*) ((char*) workspace + s.ml);
+    a.g = w->qh / w->kvh; a.kvh = w->kvh; a.window = w->window; a.geometry = pg_geometry(w);
+    a.div_g = FastDiv((uint32_t) a.g);
+    a.c = scale * 1.44269504088896340736f;
+    a.n_pages = c->n_pages; a.lp = pg_log2(c->page); a.max_pages = b->max_pages; a.n_req = b->n_req; a.max_tokens = b->max_tokens;
+    const bool bf = c->type == WZY_BF16;
+    switch (c->hd) {
+        case 64: return bf ? launch<64, WZY_BF16>(a, l, stream) : launch<64, WZY_F16>(a, l, stream);
+        case 128: return bf ? launch<128, WZY_BF16>(a, l, stream) : launch<128, WZY_F16>(a, l, stream);
+        default: return bf ? launch<256, WZY_BF16>(a, l, stream) : launch<256, WZY_F16>(a, l, stream);
+    }
+}

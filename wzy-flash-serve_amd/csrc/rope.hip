@@ -1,0 +1,285 @@
+// rope.hip -- rotary positions: frequencies, rows of heads, and rows on their way into a paged cache.
+//
+//   (a, b) -> A (a cos t - b sin t, b cos t + a sin t),   t = 2 pi * frac(position * f_i / 2 pi)
+//
+// Angles: position * (f / 2 pi) in 64 bits, less its nearest eighth of a turn's multiple; what is left, at most pi / 4 either
+// way, goes into the Taylor polynomials of sine and cosine in 64 bits (to x^13 and x^14: 2e-14).  They are made once a row, by
+// one thread an angle, and kept in LDS for all heads of the row: at far positions fp32 angles would be off by whole turns.
+// The rows are read and written once, 8 elements (and their partners) a thread where alignment allows 16-byte accesses, a pair
+// a thread elsewhere.  Bound by memory at large sizes, by the launch at one row.
+#include "wzy_paged.h"
+
+using namespace wzy;
+
+namespace {
+constexpr int RT = 256, ROPE_MAX = 512;
+
+struct View { const void* p; int64_t ld, ldh; };
+struct RopeArgs {
+    // three sets of heads: q (or the only one), k, v; the last two go to the cache's slots
+    View in[3], out[3];
+    int heads[3];                         // 0: absent
+    const double* freqs;                  // null: nothing is turned
+    const int* positions;
+    const int* slots;
+    int rows, hd, n_rot, n_sets;
+    int per_row, per_head;                // pieces of work: of all heads of a row, of a head
+    FastDiv div_row, div_head;
+    int64_t ld_page, n_cells;
+    int lp, rows_block;
+};
+
+// cos and sin of 2 pi x, amplitude in
+WZY_DEV float2 turn(double x, double amplitude) {
+    x -= floor(x);                                             // 0 .. 1
+    const int oct = (int) (x * 8.0 + 0.5) & ~1;                 // nearest quarter turn, in eighths
+    const double y = (x - (double) oct * 0.125) * 6.283185307179586476925, z = y * y;
+    double c = -1.0 / 87178291200.0, s = 1.0 / 6227020800.0;
+    c = fma(c, z, 1.0 / 479001600.0); s = fma(s, z, -1.0 / 39916800.0);
+    c = fma(c, z, -1.0 / 3628800.0);  s = fma(s, z, 1.0 / 362880.0);
+    c = fma(c, z, 1.0 / 40320.0);     s = fma(s, z, -1.0 / 5040.0);
+    c = fma(c, z, -1.0 / 720.0);      s = fma(s, z, 1.0 / 120.0);
+    c = fma(c, z, 1.0 / 24.0);        s = fma(s, z, -1.0 / 6.0);
+    c = fma(c, z, -0.5);              s = fma(s, z, 1.0) * y;
+    c = fma(c, z, 1.0);
+    const int q = (oct >> 1) & 3;                               // quarter turns
+    const double cc = q & 1 ? s : c, ss = q & 1 ? c : s;
+    return make_float2((float) (amplitude * (q == 1 || q == 2 ? -cc : cc)), (float) (amplitude * (q >= 2 ? -ss : ss)));
+}
+
+template <int T>
+WZY_DEV float load1(const void* p, size_t i) {
+    if constexpr (T == WZY_F32) return ((const float*) p)[i];
+    else if constexpr (T == WZY_BF16) return bf16_to_f(((const uint16_t*) p)[i]);
+    else return h16_to_f(((const uint16_t*) p)[i]);
+}
+template <int T>
+WZY_DEV void store1(void* p, size_t i, float v) {
+    if constexpr (T == WZY_F32) ((float*) p)[i] = v;
+    else if constexpr (T == WZY_BF16) ((uint16_t*) p)[i] = (uint16_t) pack2<WZY_BF16>(v, v);
+    else ((uint16_t*) p)[i] = f_to_h16(v);
+}
+
+// One workgroup does rows_block rows: their angles, then all pieces of all heads.  WIDE pieces: 8 elements and, in rotated
+// halves, the 8 they pair with; others: one pair or one element.
+template <int TI, int TO, bool PAIRS, bool WIDE>
+__global__ void __launch_bounds__(RT) rope_kernel(RopeArgs a) {
+    __shared__ float2 s_cs[ROPE_MAX];
+    const int tid = threadIdx.x, row0 = blockIdx.x * a.rows_block, rows = min(a.rows - row0, a.rows_block);
+    const int half = a.n_rot >> 1;
+    if (a.freqs) {
+        for (int i = tid; i < rows * half; i += RT) {
+            const int r = i / half, j = i - r * half;
+            s_cs[i] = turn((double) a.positions[row0 + r] * a.freqs[j], a.freqs[half]);
+        }
+        __syncthreads();
+    }
+    for (int i = tid; i < rows * a.per_row; i += RT) {
+        const int r = (int) fast_div((uint32_t) i, a.div_row), x = i - r * a.per_row;
+        int h = (int) fast_div((uint32_t) x, a.div_head);
+        const int piece = x - h * a.per_head;
+        int set = 0;
+        if (a.n_sets > 1) {
+            if (h >= a.heads[0]) { h -= a.heads[0]; set = 1; }
+            if (set == 1 && h >= a.heads[1]) { h -= a.heads[1]; set = 2; }
+        }
+        const int row = row0 + r;
+        const void* const src = set == 0 ? a.in[0].p : set == 1 ? a.in[1].p : a.in[2].p;
+        void* const dst = (void*) (set == 0 ? a.out[0].p : set == 1 ? a.out[1].p : a.out[2].p);
+        const size_t at = (size_t) row * (set == 0 ? a.in[0].ld : set == 1 ? a.in[1].ld : a.in[2].ld) +
+                          (size_t) h * (set == 0 ? a.in[0].ldh : set == 1 ? a.in[1].ldh : a.in[2].ldh);
+        size_t to;
+        if (set == 0) to = (size_t) row * a.out[0].ld + (size_t) h * a.out[0].ldh;
+        else {
+            const int slot = a.slots[row];
+            if (slot < 0 || slot >= a.n_cells) continue;
+            to = (size_t) (slot >> a.lp) * a.ld_page + (size_t) (slot & ((1 << a.lp) - 1)) * a.out[1].ld + (size_t) h * a.out[1].ldh;
+        }
+        const float2* const cs = s_cs + r * half;
+        const int n_rot = set < 2 && a.freqs ? a.n_rot : 0;        // values are not turned
+        if constexpr (WIDE) {
+            // pieces: of a turned half layout first the pairs of eights, then what is left, then (values) what the pairs covered
+            float u[8], v[8];
+            if constexpr (!PAIRS) {
+                if (piece < half >> 3) {
+                    const int e = 8 * piece;
+                    load8<TI>(src, at + e, u);
+                    load8<TI>(src, at + half + e, v);
+                    if (n_rot) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float2 t = cs[e + j];
+                            const float p = u[j] * t.x - v[j] * t.y, q = v[j] * t.x + u[j] * t.y;
+                            u[j] = p;
+                            v[j] = q;
+                        }
+                    }
+                    store8<TO>(dst, to + e, u);
+                    store8<TO>(dst, to + half + e, v);
+                } else {
+                    const int e = a.n_rot + 8 * (piece - (half >> 3));
+                    load8<TI>(src, at + e, u);
+                    store8<TO>(dst, to + e, u);
+                }
+            } else {
+                const int e = 8 * piece;
+                load8<TI>(src, at + e, u);
+                if (e < n_rot) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 t = cs[(e >> 1) + j];
+                        const float p = u[2 * j] * t.x - u[2 * j + 1] * t.y, q = u[2 * j + 1] * t.x + u[2 * j] * t.y;
+                        u[2 * j] = p;
+                        u[2 * j + 1] = q;
+                    }
+                }
+                store8<TO>(dst, to + e, u);
+            }
+        } else {
+            if (piece < half) {
+                const int e0 = PAIRS ? 2 * piece : piece, e1 = PAIRS ? e0 + 1 : piece + half;
+                float u = load1<TI>(src, at + e0), v = load1<TI>(src, at + e1);
+                if (n_rot) {
+                    const float2 t = cs[piece];
+                    const float p = u * t.x - v * t.y;
+                    v = v * t.x + u * t.y;
+                    u = p;
+                }
+                store1<TO>(dst, to + e0, u);
+                store1<TO>(dst, to + e1, v);
+            } else {
+                const int e = a.n_rot + piece - half;
+                store1<TO>(dst, to + e, load1<TI>(src, at + e));
+            }
+        }
+    }
+}
+
+__global__ void rope_freqs_kernel(wzy_rope_cfg c, double* __restrict__ f) {
+    const int i = threadIdx.x, half = c.n_rot / 2;
+    const double two_pi = 6.283185307179586476925, ln = log(c.theta);
+    if (i < half) {
+        const double base = exp(-2.0 * (double) i / (double) c.n_rot * ln);
+        double keep = 1.0;
+        if (c.scaling == WZY_ROPE_LINEAR) keep = 0.0;
+        if (c.scaling == WZY_ROPE_ROTATIONS) keep = ((double) c.ctx * base / two_pi - c.low) / (c.high - c.low);
+        if (c.scaling == WZY_ROPE_INDEX) {
+            const double at_high = (double) c.n_rot * log((double) c.ctx / (two_pi * c.high)) / (2.0 * ln);
+            const double at_low = (double) c.n_rot * log((double) c.ctx / (two_pi * c.low)) / (2.0 * ln);
+            const double a = fmax(floor(at_high), 0.0), b = fmin(ceil(at_low), (double) c.n_rot - 1.0);
+            // both ends on one pair: it and those below keep their frequency
+            keep = b > a ? 1.0 - ((double) i - a) / (b - a) : (double) i <= a ? 1.0 : 0.0;
+        }
+        keep = fmin(fmax(keep, 0.0), 1.0);
+        f[i] = base * (keep + (1.0 - keep) / c.factor) / two_pi;
+    }
+    if (i == half) f[half] = c.amplitude == 0.0 ? 1.0 : c.amplitude;
+}
+
+int check_tab(const char* who, const wzy_rope_tab* t, int hd) {
+    WZY_REQUIRE(t && t->freqs && (uintptr_t) t->freqs % 8 == 0, "%s: the rotary table is null", who);
+    WZY_REQUIRE(t->n_rot >= 2 && t->n_rot % 2 == 0 && t->n_rot <= hd, "%s: n_rot %d of heads of %d", who, t->n_rot, hd);
+    WZY_REQUIRE(t->layout == WZY_ROPE_HALVES || t->layout == WZY_ROPE_PAIRS, "%s: layout %d", who, t->layout);
+    return WZY_OK;
+}
+bool rows16(const void* p, int64_t ld, int64_t ldh, int type) {
+    const int n = mx_type_bytes(type);
+    return (uintptr_t) p % 16 == 0 && ld * n % 16 == 0 && ldh * n % 16 == 0;
+}
+
+// Rows a workgroup takes: enough pieces for its 256 threads, while there are rows for all CUs, as far as the angles' room goes.
+template <int TI, int TO>
+int launch(RopeArgs a, bool pairs, bool wide, void* stream) {
+    const int heads = a.heads[0] + a.heads[1] + a.heads[2], half = a.n_rot / 2;
+    a.per_head = !wide ? half + a.hd - a.n_rot : pairs ? a.hd / 8 : half / 8 + (a.hd - a.n_rot) / 8;
+    a.per_row = heads * a.per_head;
+    a.div_row = FastDiv((uint32_t) a.per_row);
+    a.div_head = FastDiv((uint32_t) a.per_head);
+    int rb = 1;
+    while (rb * a.per_row < 4 * RT && 2 * rb * half <= ROPE_MAX && a.rows / (2 * rb) >= 512) rb *= 2;
+    a.rows_block = rb;
+    const int grid = (a.rows + rb - 1) / rb;
+    const auto st = as_stream(stream);
+    if (pairs && wide) rope_kernel<TI, TO, true, true><<<grid, RT, 0, st>>>(a);
+    else if (pairs) rope_kernel<TI, TO, true, false><<<grid, RT, 0, st>>>(a);
+    else if (wide) rope_kernel<TI, TO, false, true><<<grid, RT, 0, st>>>(a);
+    else rope_kernel<TI, TO, false, false><<<grid, RT, 0, st>>>(a);
+    WZY_LAUNCH_CHECK();
+    return WZY_OK;
+}
+}  // namespace
+
+extern "C" int wzy_rope_freqs(const wzy_rope_cfg* c, double* freqs, void* stream) {
+    const char* const who = "wzy_rope_freqs";
+    WZY_REQUIRE(c && freqs && (uintptr_t) freqs % 8 == 0, "%s: null", who);
+    WZY_REQUIRE(c->n_rot >= 2 && c->n_rot <= ROPE_MAX && c->n_rot % 2 == 0, "%s: n_rot %d (even, 2 .. %d)", who, c->n_rot, ROPE_MAX);
+    WZY_REQUIRE(c->theta > 1.0 && c->theta <= 1e300, "%s: theta %g (above 1)", who, c->theta);
+    WZY_REQUIRE(c->scaling >= WZY_ROPE_PLAIN && c->scaling <= WZY_ROPE_INDEX, "%s: scaling %d", who, c->scaling);
+    WZY_REQUIRE(c->amplitude > -1e30 && c->amplitude < 1e30, "%s: amplitude %g", who, c->amplitude);
+    if (c->scaling != WZY_ROPE_PLAIN) WZY_REQUIRE(c->factor >= 1.0 && c->factor <= 1e300, "%s: factor %g (at least 1)", who, c->factor);
+    if (c->scaling >= WZY_ROPE_ROTATIONS)
+        WZY_REQUIRE(c->low > 0.0 && c->high > c->low && c->high <= 1e300 && c->ctx >= 1, "%s: low %g, high %g, ctx %d", who, c->low, c->high, c->ctx);
+    rope_freqs_kernel<<<1, ROPE_MAX / 2 + 64, 0, as_stream(stream)>>>(*c, freqs);
+    WZY_LAUNCH_CHECK();
+    return WZY_OK;
+}
+
+extern "C" int wzy_rope(const wzy_rope_tab* t, const wzy_heads* x, int type, int rows, int heads, int hd, const int* positions,
+                        const wzy_heads* out, void* stream) {
+    const char* const who = "wzy_rope";
+    WZY_TRY(mx_check_type(who, type));
+    WZY_REQUIRE(rows >= 0 && heads >= 1 && heads <= 1024 && hd >= 2 && hd <= ROPE_MAX, "%s: %d rows of %d heads of %d", who, rows, heads, hd);
+    WZY_TRY(check_tab(who, t, hd));
+    if (rows == 0) return WZY_OK;
+    WZY_TRY(pg_check_heads(who, "x", x, type, heads, hd));
+    WZY_TRY(pg_check_heads(who, "out", out, type, heads, hd));
+    WZY_REQUIRE(positions, "%s: positions is null", who);
+    WZY_REQUIRE(x->p != out->p || (x->ld == out->ld && x->ld_head == out->ld_head), "%s: in place with other strides", who);
+    RopeArgs a{};
+    a.in[0] = View{x->p, x->ld, x->ld_head};
+    a.out[0] = View{out->p, out->ld, out->ld_head};
+    a.heads[0] = heads;
+    a.n_sets = 1;
+    a.freqs = t->freqs; a.positions = positions; a.rows = rows; a.hd = hd; a.n_rot = t->n_rot;
+    const bool wide = hd % 8 == 0 && t->n_rot % 16 == 0 && rows16(x->p, x->ld, x->ld_head, type) && rows16(out->p, out->ld, out->ld_head, type);
+    return mx_with_type(type, [&](auto ti) { return launch<ti(), ti()>(a, t->layout == WZY_ROPE_PAIRS, wide, stream); });
+}
+
+extern "C" int wzy_paged_append(const wzy_paged_cache* c, const wzy_rope_tab* t, const wzy_heads* q, int qh, const wzy_heads* q_out,
+                                const wzy_heads* k, const wzy_heads* v, int type, int rows, const int* positions, const int* slots,
+                                void* stream) {
+    const char* const who = "wzy_paged_append";
+    WZY_TRY(mx_check_type(who, type));
+    WZY_TRY(pg_check_cache(who, c));
+    WZY_REQUIRE(rows >= 0 && qh >= 0 && qh <= 1024, "%s: %d rows, %d query heads", who, rows, qh);
+    WZY_REQUIRE((qh == 0) == (q == nullptr) && (qh == 0) == (q_out == nullptr), "%s: %d query heads with q %p, q_out %p", who, qh,
+                (const void*) q, (const void*) q_out);
+    if (t) WZY_TRY(check_tab(who, t, c->hd));
+    if (rows == 0) return WZY_OK;
+    WZY_REQUIRE(slots && (positions || !t), "%s: positions or slots are null", who);
+    WZY_TRY(pg_check_heads(who, "k", k, type, c->kvh, c->hd));
+    WZY_TRY(pg_check_heads(who, "v", v, type, c->kvh, c->hd));
+    RopeArgs a{};
+    if (q) {
+        WZY_TRY(pg_check_heads(who, "q", q, type, qh, c->hd));
+        WZY_TRY(pg_check_heads(who, "q_out", q_out, c->type, qh, c->hd));
+        WZY_REQUIRE(q->p != q_out->p || (type == c->type && q->ld == q_out->ld && q->ld_head == q_out->ld_head), "%s: q in place with other rows", who);
+        a.in[0] = View{q->p, q->ld, q->ld_head};
+        a.out[0] = View{q_out->p, q_out->ld, q_out->ld_head};
+    }
+    a.in[1] = View{k->p, k->ld, k->ld_head};
+    a.in[2] = View{v->p, v->ld, v->ld_head};
+    a.out[1] = View{c->k, c->ld_cell, c->ld_head};
+    a.out[2] = View{c->v, c->ld_cell, c->ld_head};
+    a.heads[0] = qh; a.heads[1] = a.heads[2] = c->kvh;
+    a.n_sets = 3;
+    a.freqs = t ? t->freqs : nullptr;
+    a.positions = positions; a.slots = slots; a.rows = rows; a.hd = c->hd; a.n_rot = t ? t->n_rot : 0;
+    a.ld_page = c->ld_page; a.n_cells = (int64_t) c->n_pages * c->page; a.lp = pg_log2(c->page);
+    const bool wide = a.n_rot % 16 == 0 && rows16(k->p, k->ld, k->ld_head, type) && rows16(v->p, v->ld, v->ld_head, type) &&
+                      (!q || (rows16(q->p, q->ld, q->ld_head, type) && rows16(q_out->p, q_out->ld, q_out->ld_head, c->type)));
+    const bool pairs = t && t->layout == WZY_ROPE_PAIRS;
+    return mx_with_type(type, [&](auto ti) {
+        return c->type == WZY_BF16 ? launch<ti(), WZY_BF16>(a, pairs, wide, stream) : launch<ti(), WZY_F16>(a, pairs, wide, stream);
+    });
+}

@@ -1,6 +1,7 @@
 """ctypes bindings of libwzy_amd.so, the MI355X decode-path library.
 
-The C ABI (include/wzy_kernels.h, include/wzy_mx.h, include/wzy_synth.h, include/wzy_stage.h) takes plain pointers and
+The C ABI (include/wzy_kernels.h, include/wzy_mx.h, include/wzy_paged.h, include/wzy_synth.h,
+include/wzy_stage.h) takes plain pointers and
 sizes; these bindings pass integers (device pointers from any allocator, numpy buffer addresses)
 and raise WzyError on a negative status.  Loading fails loudly when the shared library has not been
 built: there is no CPU fallback behind this module.
@@ -54,6 +55,49 @@ TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
 class MxMat(C.Structure):
     """struct wzy_mx_mat (include/wzy_mx.h)"""
     _fields_ = [("codes", P), ("scales", P), ("ld_codes", I64), ("ld_scales", I64), ("fmt", I32)]
+
+
+# several requests at once (include/wzy_paged.h)
+ROPE_HALVES, ROPE_PAIRS = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_ROTATIONS, ROPE_INDEX = 0, 1, 2, 3
+
+
+class PagedPool(C.Structure):
+    """struct wzy_paged_pool (include/wzy_paged.h)"""
+    _fields_ = [("free_pages", P), ("n_free", P), ("n_free_out", P), ("n_pages", I32), ("page", I32)]
+
+
+class PagedBatch(C.Structure):
+    """struct wzy_paged_batch (include/wzy_paged.h)"""
+    _fields_ = [("n_req", I32), ("max_tokens", I32), ("max_pages", I32), ("n_cached", P), ("n_new", P), ("table", P),
+                ("q_start", P), ("kv_len", P), ("served", P), ("positions", P), ("slots", P), ("max_new", I32)]
+
+
+class PagedWork(C.Structure):
+    """struct wzy_paged_work (include/wzy_paged.h)"""
+    _fields_ = [("qh", I32), ("kvh", I32), ("hd", I32), ("window", I32), ("items", P), ("bytes", SZ)]
+
+
+class Heads(C.Structure):
+    """struct wzy_heads (include/wzy_paged.h)"""
+    _fields_ = [("p", P), ("ld", I64), ("ld_head", I64)]
+
+
+class RopeCfg(C.Structure):
+    """struct wzy_rope_cfg (include/wzy_paged.h)"""
+    _fields_ = [("theta", C.c_double), ("factor", C.c_double), ("low", C.c_double), ("high", C.c_double),
+                ("amplitude", C.c_double), ("ctx", I32), ("n_rot", I32), ("scaling", I32)]
+
+
+class RopeTab(C.Structure):
+    """struct wzy_rope_tab (include/wzy_paged.h)"""
+    _fields_ = [("freqs", P), ("n_rot", I32), ("layout", I32)]
+
+
+class PagedCache(C.Structure):
+    """struct wzy_paged_cache (include/wzy_paged.h)"""
+    _fields_ = [("k", P), ("v", P), ("ld_page", I64), ("ld_cell", I64), ("ld_head", I64), ("n_pages", I32), ("page", I32),
+                ("kvh", I32), ("hd", I32), ("type", I32)]
 
 
 class QsaDims(C.Structure):
@@ -220,6 +264,19 @@ _SIGS = {
     "wzy_mx_swiglu": (I32, [P, P, I32, I64, I32, I32, C.POINTER(MxMat), P], True),
     "wzy_mx_gemm": (I32, [C.POINTER(MxMat), C.POINTER(MxMat), I32, I32, I32, P, I32, I64, P], True),
     "wzy_mx_grouped_gemm": (I32, [C.POINTER(MxMat), I32, P, C.POINTER(MxMat), P, I32, I32, I32, I32, P, I32, I64, P], True),
+    # several requests at once
+    "wzy_paged_work_bytes": (SZ, [C.POINTER(PagedBatch), C.POINTER(PagedWork)], False),
+    "wzy_paged_plan": (I32, [C.POINTER(PagedPool), C.POINTER(PagedBatch), C.POINTER(PagedWork), I32, P], True),
+    "wzy_paged_release": (I32, [C.POINTER(PagedPool), C.POINTER(PagedBatch), P, P], True),
+    "wzy_rope_freqs": (I32, [C.POINTER(RopeCfg), P, P], True),
+    "wzy_rope": (I32, [C.POINTER(RopeTab), C.POINTER(Heads), I32, I32, I32, I32, P, C.POINTER(Heads), P], True),
+    "wzy_paged_append": (I32, [C.POINTER(PagedCache), C.POINTER(RopeTab), C.POINTER(Heads), I32, C.POINTER(Heads), C.POINTER(Heads),
+                               C.POINTER(Heads), I32, I32, P, P, P], True),
+    "wzy_paged_attend_workspace_bytes": (SZ, [C.POINTER(PagedBatch), C.POINTER(PagedWork)], False),
+    "wzy_paged_attend": (I32, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedWork), C.POINTER(Heads), C.POINTER(Heads),
+                               F32, P, SZ, P], True),
+    "wzy_sample_workspace_bytes": (SZ, [I32, I32], False),
+    "wzy_sample": (I32, [P, I32, I64, I32, I32, P, P, P, P, P, P, P, P, SZ, P], True),
     # synth
     "wzy_synth_hash": (U64, [U64, U64, U64], False),
     "wzy_synth_stream": (U64, [U32, U32, U32], False),
