@@ -83,33 +83,49 @@ WZY_DEV const char* uniform(const char* p) {
     return (const char*) (uintptr_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (b >> 32)) << 32 |
                                       (uint32_t) __builtin_amdgcn_readfirstlane((int) b));
 }
-// the other lane half's value
-WZY_DEV float other_half(float v) { return __shfl_xor(v, 32); }
+// lane l's value and lane l ^ 32's, in either order
+WZY_DEV float2 both_halves(float v) {
+    uint32_t x = __builtin_bit_cast(uint32_t, v), y = x;
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(x), "+v"(y));
+    return make_float2(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
+WZY_DEV float half_max(float v) { const float2 b = both_halves(v); return fmaxf(b.x, b.y); }
+WZY_DEV float half_sum(float v) { const float2 b = both_halves(v); return b.x + b.y; }
 
-// K and V of 32 keys in LDS: a row a key, its 16-byte pieces permuted by the key.  K is read by 32 lanes, a row each, the same
-// piece: pieces p ^ f(row) are spread over the banks.  V is read by 16 lanes as 4 keys x 32 bytes, twice side by side: the
-// 64-byte groups of 4 neighbouring keys change places.
-template <int HD>
+// K or V of 32 keys in LDS: a row a key, as the loads leave them, 1 KiB (ROWS keys) each.  Within those the 16-byte pieces of
+// a row change places by its number (an exclusive or), and the loads lie PAD apart, so that the lanes that read at once find
+// all banks: K is read as 32 rows' same piece, V as 4 rows x 64 bytes.  Both permutations leave all but a few bits of a piece's
+// number alone: a lane needs SETS addresses, the rest are offsets in the instructions.
+template <int HD, bool V>
 struct Block {
-    static constexpr int PIECES = HD / 8, ROW = HD * 2, BYTES = 32 * ROW, LOADS = BYTES / 1024, ROWS = 64 / PIECES;   // rows a load
-    static WZY_DEV int swz_k(int row) { return HD == 64 ? (row >> 1) & 7 : row & (PIECES - 1); }
-    static WZY_DEV int swz_v(int row) { return HD == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
-    // K's operand: row l % 32, piece 2 s + l / 32
-    static WZY_DEV v4w_t k_at(const char* lds, int lane, int s) {
-        const int row = lane & 31;
-        return *(const v4w_t*) (lds + row * ROW + (((2 * s + (lane >> 5)) ^ swz_k(row)) << 4));
+    static constexpr int PIECES = HD / 8, ROW = HD * 2, LOADS = 32 * ROW / 1024, ROWS = 64 / PIECES;
+    static constexpr int PAD = V && HD == 256 ? 64 : 16, STEP = 1024 + PAD, BYTES = LOADS * STEP;
+    // pieces change places in units of 1 << SHIFT pieces
+    static constexpr int SHIFT = HD == 256 ? 3 : HD == 128 || V ? 2 : 1, SETS = HD == 256 || (HD == 64 && V) ? 2 : 4;
+    static WZY_DEV int swap(int row) { return HD == 64 ? (row >> 1) & (SETS - 1) : row & (SETS - 1); }
+    static WZY_DEV int row_at(int row) { return row / ROWS * STEP + row % ROWS * ROW; }
+    // addresses of a lane: set j for pieces whose bits at SHIFT are j
+    static WZY_DEV void addresses(uint32_t (&at)[SETS], int lane) {
+        const int i = lane & 15, row = V ? 4 * (lane >> 5) + (i >> 2) : lane & 31;
+        const int low = V ? (2 * (lane >> 4 & 1) + (i >> 1 & 1)) * 16 + 8 * (i & 1) : (lane >> 5) * 16;
+#pragma unroll
+        for (int j = 0; j < SETS; ++j) at[j] = (uint32_t) (row_at(row) + low + ((j ^ swap(row)) << (SHIFT + 4)));
     }
-    // V^T's operand for columns 32 d + l % 32: keys 16 s + 4 h + 0 .. 3 and 8 more than those, h = l / 32
-    static WZY_DEV v4w_t v_at(const char* lds, int lane, int s, int d) {
-        const int i = lane & 15;
+    // K's operand of columns 16 s ..: row l % 32, piece 2 s + l / 32
+    static WZY_DEV v4w_t k_operand(const char* lds, const uint32_t (&at)[SETS], int s) {
+        constexpr int M = (SETS - 1) << SHIFT;
+        const int piece = 2 * s;
+        return *(const v4w_t*) (lds + at[(piece & M) >> SHIFT] + (piece & ~M) * 16);
+    }
+    // V^T's operand of columns 32 d + l % 32: keys 16 s + 4 h + 0 .. 3 and 8 more than those, h = l / 32
+    static WZY_DEV v4w_t v_operand(const char* lds, const uint32_t (&at)[SETS], int s, int d) {
+        constexpr int M = (SETS - 1) << SHIFT;
+        const int piece = 4 * d;
         v4w_t r;
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-            const int row = 16 * s + 8 * p + 4 * (lane >> 5) + (i >> 2);
-            const int piece = 4 * d + 2 * (lane >> 4 & 1) + (i >> 1 & 1);
-            const char* const at = lds + row * ROW + ((piece ^ swz_v(row)) << 4) + 8 * (i & 1);
-            const v4s_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*) at);
-            const uint2 w = __builtin_bit_cast(uint2, x);
+            const char* const from = lds + at[(piece & M) >> SHIFT] + (piece & ~M) * 16 + row_at(16 * s + 8 * p);
+            const uint2 w = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*) from));
             r[2 * p] = w.x;
             r[2 * p + 1] = w.y;
         }
@@ -129,15 +145,22 @@ struct TileCtx {
 // anything, a NaN too, and a weight of 0 does not silence it.
 template <int HD>
 struct Loader {
-    using B = Block<HD>;
+    using BK = Block<HD, false>;
+    using BV = Block<HD, true>;
     const AttnArgs& a;
     const TileCtx& t;
-    int lane;
+    int r0;                                  // the lane's row of a load
+    int piece_k, piece_v;                    // and the bytes of that row it takes
     const char* base[2];                     // of K's halves; V's are as far off
     int64_t to_v;
     bool whole;
     int first, last;                         // rows that are there, where not all are
-    WZY_DEV Loader(const AttnArgs& a_, const TileCtx& t_, int lane_) : a(a_), t(t_), lane(lane_), to_v(a_.v - a_.k) {}
+    WZY_DEV Loader(const AttnArgs& a_, const TileCtx& t_, int lane) : a(a_), t(t_), to_v(a_.v - a_.k) {
+        r0 = lane / BK::PIECES;
+        const int piece = lane % BK::PIECES;
+        piece_k = (piece ^ (BK::swap(r0) << BK::SHIFT)) * 16;
+        piece_v = (piece ^ (BV::swap(r0) << BV::SHIFT)) * 16;
+    }
     WZY_DEV const char* cell(int c) const {
         int id = t.pages[c >> a.lp];
         id = (unsigned) id < (unsigned) a.n_pages ? id : 0;
@@ -154,25 +177,24 @@ struct Loader {
         base[0] = uniform(cell(c + h0));
         base[1] = uniform(h1 == h0 ? base[0] : cell(c + h1));
     }
-    // loads i0 .. i1 - 1 (of LOADS, each B::ROWS rows) into lds
-    template <bool V, int I0, int I1>
+    // loads start .. start + N - 1 of the block's into lds
+    template <bool V, int N>
     WZY_DEV void issue(uint32_t lds, int start) const {
-        const int r0 = lane / B::PIECES, piece = lane & (B::PIECES - 1);
+        using B = Block<HD, V>;
+        const int piece = V ? piece_v : piece_k;
         const int64_t add = V ? to_v : 0;
         if (whole) {
+            const uint32_t off = (uint32_t) r0 * (uint32_t) a.ld_cell + (uint32_t) piece;
 #pragma unroll
-            for (int i = I0; i < I1; ++i) {
-                const int row = (start + i) * B::ROWS + r0;
-                const uint32_t off = (uint32_t) (row & 15) * (uint32_t) a.ld_cell + (uint32_t) ((piece ^ (V ? B::swz_v(row) : B::swz_k(row))) << 4);
-                dma16(lds + (uint32_t) (start + i) * 1024, off, uniform(((start + i) * B::ROWS < 16 ? base[0] : base[1]) + add));
+            for (int i = 0; i < N; ++i) {
+                const int row = (start + i) * B::ROWS;
+                dma16(lds + (uint32_t) ((start + i) * B::STEP), off, uniform((row < 16 ? base[0] : base[1]) + add + (int64_t) (row & 15) * a.ld_cell));
             }
         } else {
 #pragma unroll
-            for (int i = I0; i < I1; ++i) {
-                const int row = (start + i) * B::ROWS + r0, from = min(max(row, first), last);
-                const char* const p = (from < 16 ? base[0] : base[1]) + add + (int64_t) (from & 15) * a.ld_cell +
-                                      ((piece ^ (V ? B::swz_v(row) : B::swz_k(row))) << 4);
-                dma16(lds + (uint32_t) (start + i) * 1024, p);
+            for (int i = 0; i < N; ++i) {
+                const int from = min(max((start + i) * B::ROWS + r0, first), last);
+                dma16(lds + (uint32_t) ((start + i) * B::STEP), (from < 16 ? base[0] : base[1]) + add + (int64_t) (from & 15) * a.ld_cell + piece);
             }
         }
     }
@@ -182,19 +204,24 @@ struct Loader {
 template <int HD, int T>
 struct Wave {
     static constexpr int KS = HD / 16, DT = HD / 32;
+    using BK = Block<HD, false>;
+    using BV = Block<HD, true>;
+    uint32_t at_k[BK::SETS], at_v[BV::SETS];
     v4w_t q[KS];
     v16f_t o[DT];
     float m, l;
     int pos, pos_min, pos_max;               // of the lane's row; of the wave's
-    int row, rows;                           // the lane's row of the tile's request; rows of the request
+    int row, rows;                           // the lane's row of the request's; how many those are
 
     WZY_DEV void start(const AttnArgs& a, const TileCtx& t, int row0, int lane) {
+        BK::addresses(at_k, lane);
+        BV::addresses(at_v, lane);
         rows = t.it.n_new * a.g;
         row = row0 + (lane & 31);
-        const int r = min(row, rows - 1), token = (int) fast_div((uint32_t) r, a.div_g), h = r - token * a.g;
-        pos = t.it.n_cached + token;
         pos_min = t.it.n_cached + (int) fast_div((uint32_t) min(row0, rows - 1), a.div_g);
         pos_max = t.it.n_cached + (int) fast_div((uint32_t) min(row0 + 31, rows - 1), a.div_g);
+        const int r = min(row, rows - 1), token = (int) fast_div((uint32_t) r, a.div_g), h = r - token * a.g;
+        pos = t.it.n_cached + token;
         const char* const p = a.q + (int64_t) (t.it.q0 + token) * a.ldq + (int64_t) (t.head * a.g + h) * a.ldq_head + (lane >> 5) * 16;
 #pragma unroll
         for (int s = 0; s < KS; ++s) q[s] = row < rows ? *(const v4w_t*) (p + 32 * s) : v4w_t{0, 0, 0, 0};
@@ -203,21 +230,29 @@ struct Wave {
         m = -INFINITY;
         l = 0.0f;
     }
-    // does the wave see any cell of block b, and does it see all of them?
-    WZY_DEV bool sees(const AttnArgs& a, int b) const {
-        return 32 * b <= pos_max && (a.window == 0 || 32 * b + 31 > pos_min - a.window);
-    }
+    // are there cells of block b that some row does not see?
     WZY_DEV bool masked(const AttnArgs& a, int b) const {
         return 32 * b + 31 > pos_min || (a.window != 0 && 32 * b <= pos_max - a.window);
     }
-    WZY_DEV v16f_t scores(const char* kb, int lane) const {
+    // Operands are read AHEAD steps before their product, and the order is held: left alone, the compiler reads them all first, into
+    // registers that there are not.
+    static constexpr int AHEAD = 3;
+    WZY_DEV v16f_t scores(const char* kb) const {
+        v4w_t k[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) k[i] = BK::k_operand(kb, at_k, i);
         v16f_t s = v16f_t{};
 #pragma unroll
-        for (int i = 0; i < KS; ++i) s = Half<T>::mfma(Block<HD>::k_at(kb, lane, i), q[i], s);
+        for (int i = 0; i < KS; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            s = Half<T>::mfma(k[i % AHEAD], q[i], s);
+            if (i + AHEAD < KS) k[i % AHEAD] = BK::k_operand(kb, at_k, i + AHEAD);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         return s;
     }
     // scores to weights, rounded and packed
-    WZY_DEV void weights(const AttnArgs& a, int b, int lane, v16f_t& s, v4w_t (&p)[2]) {
+    WZY_DEV void weights(const AttnArgs& a, int b, int lane, v16f_t s, v4w_t (&p)[2]) {
         if (masked(a, b)) {
             const int low = a.window ? pos - a.window : -1;
 #pragma unroll
@@ -229,7 +264,7 @@ struct Wave {
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-        mx = fmaxf(mx, other_half(mx)) * a.c;
+        mx = half_max(mx) * a.c;
         if (__any(mx > m + RISE)) {
             const float to = fmaxf(m, mx), f = to > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
             m = to;
@@ -246,11 +281,17 @@ struct Wave {
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i / 4][i % 4] = pack2<T>(s[2 * i], s[2 * i + 1]);
     }
-    WZY_DEV void add(const char* vb, int lane, const v4w_t (&p)[2]) {
+    WZY_DEV void add(const char* vb, const v4w_t (&p)[2]) {
+        v4w_t v[AHEAD];
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int i = 0; i < AHEAD; ++i) v[i] = BV::v_operand(vb, at_v, i % 2, i / 2);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) o[d] = Half<T>::mfma(Block<HD>::v_at(vb, lane, s, d), p[s], o[d]);
+        for (int i = 0; i < 2 * DT; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            o[i / 2] = Half<T>::mfma(v[i % AHEAD], p[i % 2], o[i / 2]);
+            if (i + AHEAD < 2 * DT) v[i % AHEAD] = BV::v_operand(vb, at_v, (i + AHEAD) % 2, (i + AHEAD) / 2);
+        }
+        __builtin_amdgcn_sched_barrier(0);
     }
 };
 
@@ -274,10 +315,12 @@ WZY_DEV char* out_row(const AttnArgs& a, const TileCtx& t, int row) {
 
 template <int HD, int T>
 __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
-    using B = Block<HD>;
-    __shared__ __align__(1024) char s_buf[4][2 * B::BYTES];             // a wave's K and V; then its results in fp32
+    using BK = Block<HD, false>;
+    using BV = Block<HD, true>;
+    constexpr int MINE = BK::BYTES + BV::BYTES;
+    __shared__ __align__(1024) char s_buf[4][MINE];                     // a wave's K and V; then its results in fp32
     __shared__ float s_m[4][32], s_l[4][32];
-    static_assert(2 * B::BYTES == 32 * HD * 4, "a wave's results take its buffers");
+    static_assert(MINE >= 32 * HD * 4 && MINE % 16 == 0, "a wave's results take its buffers");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     TileCtx t;
     if (!tile_ctx(a, 0, t)) return;
@@ -292,35 +335,35 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
     w.start(a, t, 0, lane);
     Loader<HD> ld(a, t, lane);
     char* const kb = s_buf[wave];
-    char* const vb = kb + B::BYTES;
+    char* const vb = kb + BK::BYTES;
     const uint32_t lk = lds_offset(kb), lv = lds_offset(vb);
     const int end = (t.it.hi + 31) >> 5;
     int b = (t.it.lo >> 5) + wave;
     if (b < end) {
         wait_loads<0>();                                                // what the compiler still has in flight: q
         ld.at(b);
-        ld.template issue<false, 0, B::LOADS>(lk, 0);
-        ld.template issue<true, 0, B::LOADS>(lv, 0);
+        ld.template issue<false, BK::LOADS>(lk, 0);
+        ld.template issue<true, BV::LOADS>(lv, 0);
         for (;; b += 4) {
             const bool more = b + 4 < end;
-            wait_loads<B::LOADS>();                                     // K is there
-            v16f_t s = w.scores(kb, lane);
+            wait_loads<BV::LOADS>();                                    // K is there
+            const v16f_t s = w.scores(kb);
             wait_lds();                                                 // and read
             if (more) {
                 ld.at(b + 4);
-                ld.template issue<false, 0, B::LOADS>(lk, 0);
+                ld.template issue<false, BK::LOADS>(lk, 0);
             }
             v4w_t p[2];
             w.weights(a, b, lane, s, p);
-            if (more) wait_loads<B::LOADS>();
+            if (more) wait_loads<BK::LOADS>();
             else wait_loads<0>();
-            w.add(vb, lane, p);
+            w.add(vb, p);
             if (!more) break;
             wait_lds();
-            ld.template issue<true, 0, B::LOADS>(lv, 0);
+            ld.template issue<true, BV::LOADS>(lv, 0);
         }
     }
-    w.l += other_half(w.l);
+    w.l = half_sum(w.l);
     if (lane < 32) {
         s_m[wave][lane] = w.m;
         s_l[wave][lane] = w.l;
@@ -332,7 +375,8 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
     for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            r[(8 * d + 2 * i + (lane >> 5)) * 32 + (lane & 31)] = make_float4(w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]);
+            r[(8 * d + 2 * i + (lane >> 5)) * 32 + (lane & 31)] =
+                make_float4(w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]);
     __syncthreads();
     const int rows = w.rows;
     for (int i = tid; i < rows * (HD / 4); i += 256) {
@@ -360,9 +404,11 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
 }
 
 template <int HD, int T>
-__global__ void __launch_bounds__(256) paged_wide_kernel(AttnArgs a) {
-    using B = Block<HD>;
-    __shared__ __align__(1024) char s_buf[2][2 * B::BYTES];             // two blocks' K and V
+__global__ void __launch_bounds__(256, 2) paged_wide_kernel(AttnArgs a) {
+    using BK = Block<HD, false>;
+    using BV = Block<HD, true>;
+    constexpr int BOTH = BK::BYTES + BV::BYTES;
+    __shared__ __align__(1024) char s_buf[2][BOTH];                     // two blocks' K and V
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     TileCtx t;
     if (!tile_ctx(a, 1, t)) return;
@@ -372,29 +418,32 @@ __global__ void __launch_bounds__(256) paged_wide_kernel(AttnArgs a) {
     const uint32_t lk = lds_offset(s_buf);
     const int end = (t.it.hi + 31) >> 5;
     int b = t.it.lo >> 5, buf = 0;
-    constexpr int MINE = B::LOADS / 4;                                  // of each matrix, a wave
+    auto load = [&](int block, int into) {
+        constexpr int MINE = BK::LOADS / 4;                             // of each matrix, a wave
+        const uint32_t at = lk + (uint32_t) (into * BOTH);
+        ld.at(block);
+        ld.template issue<false, MINE>(at, wave * MINE);
+        ld.template issue<true, MINE>(at + BK::BYTES, wave * MINE);
+    };
     wait_loads<0>();
-    if (b < end) {
-        ld.at(b);
-        ld.template issue<false, 0, MINE>(lk, wave * MINE);
-        ld.template issue<true, 0, MINE>(lk + B::BYTES, wave * MINE);
-    }
-    for (; b < end; ++b, buf ^= 1) {
+    if (b < end) load(b, 0);
+    // the blocks that the wave's rows see: others' it helps to load and waits for.  (A loop each: a branch around the work in one loop
+    // costs a second set of accumulators.)
+    const int from = a.window ? max(b, (max(w.pos_min - a.window + 1, 0)) >> 5) : b, to = min(end, (w.pos_max >> 5) + 1);
+    auto next = [&] {
         wait_all_and_meet();                                            // the block is there; the other buffer has been read
-        if (b + 1 < end) {
-            ld.at(b + 1);
-            const uint32_t to = lk + (uint32_t) (buf ^ 1) * 2 * B::BYTES;
-            ld.template issue<false, 0, MINE>(to, wave * MINE);
-            ld.template issue<true, 0, MINE>(to + B::BYTES, wave * MINE);
-        }
-        if (w.sees(a, b)) {
-            v16f_t s = w.scores(s_buf[buf], lane);
-            v4w_t p[2];
-            w.weights(a, b, lane, s, p);
-            w.add(s_buf[buf] + B::BYTES, lane, p);
-        }
+        if (b + 1 < end) load(b + 1, buf ^ 1);
+    };
+    for (; b < from && b < end; ++b, buf ^= 1) next();
+    for (; b < to; ++b, buf ^= 1) {
+        next();
+        const v16f_t s = w.scores(s_buf[buf]);
+        v4w_t p[2];
+        w.weights(a, b, lane, s, p);
+        w.add(s_buf[buf] + BK::BYTES, p);
     }
-    const float l = w.l + other_half(w.l);
+    for (; b < end; ++b, buf ^= 1) next();
+    const float l = half_sum(w.l);
     if (w.row >= w.rows) return;
     if (t.it.part < 0) {
         const float n = l != 0.0f ? 1.0f / l : 0.0f;

@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(PT) paged_plan_kernel(PlanArgs a, PlanWorks wo
                 cells += (uint64_t) (x.hi - (x.lo & ~31));
             }
             block_scan(cells, s_scan, total);
-            // parts of len cells (a multiple of 32): at most per_head of them, and one more a tile
+            // parts of at most len cells (a multiple of 32): at most per_head of them, and one more a tile
             uint64_t len = (total + (uint64_t) w.per_head - 1) / (uint64_t) w.per_head;
             len = (len + 31) & ~(uint64_t) 31;
             const int part = (int) max(len, (uint64_t) w.l.min_len[kind]);
@@ -236,8 +236,10 @@ __global__ void __launch_bounds__(PT) paged_plan_kernel(PlanArgs a, PlanWorks wo
                 for (int i = tid; i < n && n_items + i < w.l.items[kind]; i += PT) {
                     const int o = find_last(s_item, here, i), j = i - s_item[o];
                     const Tile y = tile_at(base + o, r);
-                    const int from = (y.lo & ~31) + j * part;
-                    items[w.l.item_at[kind] + n_items + i] = PgItem{r, y.row0, max(y.lo, from), min(y.hi, from + part), s_part[o] < 0 ? -1 : s_part[o] + j,
+                    // a tile's parts are of one length, but for the blocks of 32 cells
+                    const int parts = (o + 1 < here ? s_item[o + 1] : n) - s_item[o], first = y.lo >> 5, blocks = ((y.hi + 31) >> 5) - first;
+                    const int from = 32 * (first + (int) ((int64_t) blocks * j / parts)), to = 32 * (first + (int) ((int64_t) blocks * (j + 1) / parts));
+                    items[w.l.item_at[kind] + n_items + i] = PgItem{r, y.row0, max(y.lo, from), min(y.hi, to), s_part[o] < 0 ? -1 : s_part[o] + j,
                                                                     s_start[r], s_start[r + 1] - s_start[r], s_cached[r] & 0x7FFFFFFF};
                 }
                 n_items += n;
