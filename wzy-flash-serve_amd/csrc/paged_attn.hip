@@ -15,6 +15,8 @@
 //   wide    128 rows, 32 a wave: the workgroup's waves share each block
 // The maximum follows the scores only when one has come 2^8 above it, so most blocks leave the accumulators alone; weights
 // then reach 2^8, and in fp16, whose numbers end at 2^-24, all are taken 2^6 larger.
+#include <algorithm>
+
 #include "wzy_paged.h"
 
 using namespace wzy;
@@ -42,7 +44,7 @@ struct AttnArgs {
     float c;                                 // scale * log2(e)
     int n_pages, lp, max_pages, n_req, max_tokens;
     int g, kvh, window, geometry;
-    int item_at, cap_items, cap_parts, merge_at, cap_merges;
+    int item_at, cap_parts;
 };
 
 template <int T> struct Half;                // of the cache's type
@@ -299,9 +301,10 @@ struct Wave {
 WZY_DEV bool tile_ctx(const AttnArgs& a, int kind, TileCtx& t) {
     const int at = (int) (blockIdx.x / (unsigned) a.kvh);
     t.head = (int) (blockIdx.x - (unsigned) at * (unsigned) a.kvh);
-    if (a.head->magic != PG_MAGIC || a.head->geometry != a.geometry || at >= a.head->n_items[kind]) return false;
+    const PgHead h = *a.head;                                           // both loads at once: the list has room for every workgroup
     t.it = ((const PgItem*) (a.head + 1))[a.item_at + at];
     const PgItem& i = t.it;
+    if (h.magic != PG_MAGIC || h.geometry != a.geometry || at >= h.n_items[kind]) return false;
     if ((unsigned) i.req >= (unsigned) a.n_req || i.q0 < 0 || i.n_new < 1 || i.q0 > a.max_tokens - i.n_new || i.row0 < 0 || i.row0 >= i.n_new * a.g ||
         i.lo < 0 || i.hi > a.max_pages << a.lp || i.part >= a.cap_parts)
         return false;
@@ -332,18 +335,21 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
         return;
     }
     Wave<HD, T> w;
-    w.start(a, t, 0, lane);
     Loader<HD> ld(a, t, lane);
     char* const kb = s_buf[wave];
     char* const vb = kb + BK::BYTES;
     const uint32_t lk = lds_offset(kb), lv = lds_offset(vb);
     const int end = (t.it.hi + 31) >> 5;
     int b = (t.it.lo >> 5) + wave;
+    // the first block's loads before those of q, which the compiler counts as the only ones: it waits for all of them
     if (b < end) {
-        wait_loads<0>();                                                // what the compiler still has in flight: q
         ld.at(b);
         ld.template issue<false, BK::LOADS>(lk, 0);
         ld.template issue<true, BV::LOADS>(lv, 0);
+    }
+    w.start(a, t, 0, lane);
+    if (b < end) {
+        wait_loads<0>();
         for (;; b += 4) {
             const bool more = b + 4 < end;
             wait_loads<BV::LOADS>();                                    // K is there
@@ -413,7 +419,6 @@ __global__ void __launch_bounds__(256, 2) paged_wide_kernel(AttnArgs a) {
     TileCtx t;
     if (!tile_ctx(a, 1, t)) return;
     Wave<HD, T> w;
-    w.start(a, t, t.it.row0 + 32 * wave, lane);
     Loader<HD> ld(a, t, lane);
     const uint32_t lk = lds_offset(s_buf);
     const int end = (t.it.hi + 31) >> 5;
@@ -425,8 +430,9 @@ __global__ void __launch_bounds__(256, 2) paged_wide_kernel(AttnArgs a) {
         ld.template issue<false, MINE>(at, wave * MINE);
         ld.template issue<true, MINE>(at + BK::BYTES, wave * MINE);
     };
-    wait_loads<0>();
     if (b < end) load(b, 0);
+    w.start(a, t, t.it.row0 + 32 * wave, lane);
+    wait_loads<0>();                                                    // q too, which the compiler counts without the others
     // the blocks that the wave's rows see: others' it helps to load and waits for.  (A loop each: a branch around the work in one loop
     // costs a second set of accumulators.)
     const int from = a.window ? max(b, (max(w.pos_min - a.window + 1, 0)) >> 5) : b, to = min(end, (w.pos_max >> 5) + 1);
@@ -466,20 +472,32 @@ __global__ void __launch_bounds__(256, 2) paged_wide_kernel(AttnArgs a) {
 }
 
 // Parts of a tile joined.  HD / 4 lanes hold a row; of a workgroup's groups of lanes, several take one row's parts in turn where
-// there are many, so that all of a row's loads are under way at once.  blockIdx.y goes through the tile's rows.
-template <int HD, int T, int ROWS>
-__global__ void __launch_bounds__(512) paged_merge_kernel(AttnArgs a, int kind) {
+// there are many, so that all of a row's loads are under way at once.
+struct MergeArgs {
+    unsigned blocks;                         // of narrow tiles
+    int rows_y[2], at[2], parts[2];          // workgroups a tile, first entry, parts: narrow, wide
+    const float* wide_o;
+    const float2* wide_ml;
+};
+template <int HD, int T>
+__global__ void __launch_bounds__(512) paged_merge_kernel(AttnArgs a, MergeArgs g) {
     constexpr int L = HD / 4, GROUPS = 512 / L;
     __shared__ float4 s_o[512];
     __shared__ float2 s_ml[GROUPS];
-    const int at = (int) (blockIdx.x / (unsigned) a.kvh), head = (int) (blockIdx.x - (unsigned) at * (unsigned) a.kvh);
-    if (a.head->magic != PG_MAGIC || a.head->geometry != a.geometry || at >= a.head->n_merges[kind]) return;
-    const PgMerge e = ((const PgMerge*) (a.head + 1))[a.merge_at + at];
-    if (e.part < 0 || e.n < 1 || e.part > a.cap_parts - e.n || e.rows < 1 || e.rows > ROWS || e.row0 < 0 || e.q0 < 0) return;
+    // narrow tiles' workgroups first, by rows_y of them a tile; then wide ones'
+    const int kind = blockIdx.x >= g.blocks ? 1 : 0, rows_y = g.rows_y[kind], ROWS = kind ? PG_WIDE : PG_NARROW;
+    const unsigned in = blockIdx.x - (kind ? g.blocks : 0), tile = in / (unsigned) rows_y, y = in - tile * (unsigned) rows_y;
+    const int at = (int) (tile / (unsigned) a.kvh), head = (int) (tile - (unsigned) at * (unsigned) a.kvh);
+    const PgHead h = *a.head;
+    const PgMerge e = ((const PgMerge*) (a.head + 1))[g.at[kind] + at];
+    if (h.magic != PG_MAGIC || h.geometry != a.geometry || at >= h.n_merges[kind]) return;
+    if (e.part < 0 || e.n < 1 || e.part > g.parts[kind] - e.n || e.rows < 1 || e.rows > ROWS || e.row0 < 0 || e.q0 < 0) return;
+    const float* const part_o = kind ? g.wide_o : a.part_o;
+    const float2* const part_ml = kind ? g.wide_ml : a.part_ml;
     int per = 1;                                                        // groups a row
     while (per < GROUPS && per * 4 < e.n) per *= 2;
     const int rows_here = GROUPS / per, group = threadIdx.x / L, col = threadIdx.x % L, sub = group & (per - 1);
-    for (int r0 = blockIdx.y * rows_here; r0 < e.rows; r0 += gridDim.y * rows_here) {
+    for (int r0 = (int) y * rows_here; r0 < e.rows; r0 += rows_y * rows_here) {
         const int r = min(r0 + group / per, e.rows - 1);
         float m = -INFINITY, l = 0.0f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -490,8 +508,8 @@ __global__ void __launch_bounds__(512) paged_merge_kernel(AttnArgs a, int kind) 
             for (int j = 0; j < 4; ++j) {
                 const int k = i + j * per;
                 const size_t p = ((size_t) (e.part + min(k, e.n - 1)) * a.kvh + head) * ROWS + r;
-                ml[j] = a.part_ml[p];
-                x[j] = ((const float4*) (a.part_o + p * HD))[col];
+                ml[j] = part_ml[p];
+                x[j] = ((const float4*) (part_o + p * HD))[col];
                 if (k >= e.n) ml[j] = make_float2(-INFINITY, 0.0f);
             }
 #pragma unroll
@@ -531,33 +549,47 @@ __global__ void __launch_bounds__(512) paged_merge_kernel(AttnArgs a, int kind) 
     }
 }
 
-struct Space { size_t o, ml, total; };
+// narrow tiles' partial results, then wide ones'
+struct Space { size_t o[2], ml[2], total; };
 Space space_of(const PgLayout& l, const wzy_paged_work* w) {
-    const size_t n = (size_t) l.parts[0] * PG_NARROW, wide = (size_t) l.parts[1] * PG_WIDE, rows = (n > wide ? n : wide) * w->kvh;
     Space s;
-    s.o = 0;
-    s.ml = align_up(rows * w->hd * 4, 256);
-    s.total = s.ml + align_up(rows * sizeof(float2), 256);
+    s.total = 0;
+    for (int k = 0; k < 2; ++k) {
+        const size_t rows = (size_t) l.parts[k] * (k ? PG_WIDE : PG_NARROW) * w->kvh;
+        s.o[k] = s.total;
+        s.ml[k] = s.o[k] + align_up(rows * w->hd * 4, 256);
+        s.total = s.ml[k] + align_up(rows * sizeof(float2), 256);
+    }
     return s;
 }
 
 template <int HD, int T>
-int launch(AttnArgs a, const PgLayout& l, void* stream) {
+int launch(AttnArgs a, const PgLayout& l, const Space& s, char* space, int max_rows, void* stream) {
     const auto st = as_stream(stream);
+    MergeArgs g{};
+    unsigned blocks[2] = {0, 0};
     for (int kind = 0; kind < 2; ++kind) {
         if (l.items[kind] == 0) continue;
-        a.item_at = l.item_at[kind]; a.cap_items = l.items[kind]; a.cap_parts = l.parts[kind];
-        a.merge_at = l.merge_at[kind]; a.cap_merges = l.merges[kind];
+        a.item_at = l.item_at[kind]; a.cap_parts = l.parts[kind];
+        a.part_o = (float*) (space + s.o[kind]);
+        a.part_ml = (float2*) (space + s.ml[kind]);
         const unsigned grid = (unsigned) l.items[kind] * (unsigned) a.kvh;
         if (kind == 0) paged_narrow_kernel<HD, T><<<grid, 256, 0, st>>>(a);
         else paged_wide_kernel<HD, T><<<grid, 256, 0, st>>>(a);
         WZY_LAUNCH_CHECK();
-        if (l.merges[kind] == 0) continue;
-        const unsigned tiles = (unsigned) l.merges[kind] * (unsigned) a.kvh;
-        if (kind == 0) paged_merge_kernel<HD, T, PG_NARROW><<<dim3(tiles, 32), 512, 0, st>>>(a, kind);
-        else paged_merge_kernel<HD, T, PG_WIDE><<<dim3(tiles, 16), 512, 0, st>>>(a, kind);
-        WZY_LAUNCH_CHECK();
+        g.rows_y[kind] = kind ? 16 : std::min(PG_NARROW, max_rows);
+        g.at[kind] = l.merge_at[kind];
+        g.parts[kind] = l.parts[kind];
+        blocks[kind] = (unsigned) l.merges[kind] * (unsigned) a.kvh * (unsigned) g.rows_y[kind];
     }
+    if (blocks[0] + blocks[1] == 0) return WZY_OK;
+    a.part_o = (float*) (space + s.o[0]);
+    a.part_ml = (float2*) (space + s.ml[0]);
+    g.blocks = blocks[0];
+    g.wide_o = (const float*) (space + s.o[1]);
+    g.wide_ml = (const float2*) (space + s.ml[1]);
+    paged_merge_kernel<HD, T><<<blocks[0] + blocks[1], 512, 0, st>>>(a, g);
+    WZY_LAUNCH_CHECK();
     return WZY_OK;
 }
 }  // namespace
@@ -595,16 +627,16 @@ extern "C" int wzy_paged_attend(const wzy_paged_cache* c, const wzy_paged_batch*
     a.q = (const char*) q->p; a.ldq = 2 * q->ld; a.ldq_head = 2 * q->ld_head;
     a.out = (char*) out->p; a.ldo = 2 * out->ld; a.ldo_head = 2 * out->ld_head;
     a.head = (const PgHead*) w->items;
-    a.part_o = (float*) ((char*) workspace + s.o);
-    a.part_ml = (float2*) ((char*) workspace + s.ml);
     a.g = w->qh / w->kvh; a.kvh = w->kvh; a.window = w->window; a.geometry = pg_geometry(w);
     a.div_g = FastDiv((uint32_t) a.g);
     a.c = scale * 1.44269504088896340736f;
     a.n_pages = c->n_pages; a.lp = pg_log2(c->page); a.max_pages = b->max_pages; a.n_req = b->n_req; a.max_tokens = b->max_tokens;
     const bool bf = c->type == WZY_BF16;
+    const int max_rows = (int) std::min<int64_t>((int64_t) pg_max_new(b) * a.g, 1 << 20);
+    char* const sp = (char*) workspace;
     switch (c->hd) {
-        case 64: return bf ? launch<64, WZY_BF16>(a, l, stream) : launch<64, WZY_F16>(a, l, stream);
-        case 128: return bf ? launch<128, WZY_BF16>(a, l, stream) : launch<128, WZY_F16>(a, l, stream);
-        default: return bf ? launch<256, WZY_BF16>(a, l, stream) : launch<256, WZY_F16>(a, l, stream);
+        case 64: return bf ? launch<64, WZY_BF16>(a, l, s, sp, max_rows, stream) : launch<64, WZY_F16>(a, l, s, sp, max_rows, stream);
+        case 128: return bf ? launch<128, WZY_BF16>(a, l, s, sp, max_rows, stream) : launch<128, WZY_F16>(a, l, s, sp, max_rows, stream);
+        default: return bf ? launch<256, WZY_BF16>(a, l, s, sp, max_rows, stream) : launch<256, WZY_F16>(a, l, s, sp, max_rows, stream);
     }
 }

@@ -33,7 +33,7 @@ struct PlanArgs {
 struct PlanWork {
     PgHead* head;
     PgLayout l;
-    int g, window, geometry, per_head;
+    int g, window, geometry, per_head[2], more;
 };
 struct PlanWorks { PlanWork w[8]; };
 
@@ -211,7 +211,10 @@ __global__ void __launch_bounds__(PT) paged_plan_kernel(PlanArgs a, PlanWorks wo
             }
             block_scan(cells, s_scan, total);
             // parts of at most len cells (a multiple of 32): at most per_head of them, and one more a tile
-            uint64_t len = (total + (uint64_t) w.per_head - 1) / (uint64_t) w.per_head;
+            // few tiles: together with a tile's own last part they are what the chip holds at once
+            const int slots = w.per_head[kind];
+            const uint32_t per_head = (uint32_t) (4 * n_tiles <= slots ? slots - n_tiles : slots + (kind ? 0 : min(n_tiles, w.more)));
+            uint64_t len = (total + per_head - 1) / per_head;
             len = (len + 31) & ~(uint64_t) 31;
             const int part = (int) max(len, (uint64_t) w.l.min_len[kind]);
             int n_items = 0, n_parts = 0, n_merges = 0;
@@ -352,7 +355,8 @@ extern "C" int wzy_paged_plan(const wzy_paged_pool* pool, const wzy_paged_batch*
         WZY_REQUIRE(w->items && (uintptr_t) w->items % 16 == 0 && w->bytes >= want, "%s: work list %d: %zu bytes at %p (%zu, 16-byte aligned)",
                     who, i, w->bytes, w->items, want);
         for (int j = 0; j < i; ++j) WZY_REQUIRE(works[j].items != w->items, "%s: work lists %d and %d are one", who, j, i);
-        pw.w[i] = PlanWork{(PgHead*) w->items, l, w->qh / w->kvh, w->window, pg_geometry(w), pg_div_up(PG_PARTS, w->kvh)};
+        pw.w[i] = PlanWork{(PgHead*) w->items, l, w->qh / w->kvh, w->window, pg_geometry(w),
+                           {pg_div_up(pg_parts(0, w->hd), w->kvh), pg_div_up(pg_parts(1, w->hd), w->kvh)}, PG_MORE / w->kvh};
     }
     PlanArgs a{pool->free_pages, pool->n_free, pool->n_free_out, b->n_cached, b->n_new, b->table, b->q_start, b->kv_len, b->served,
                b->positions, b->slots, pool->n_pages, pg_log2(pool->page), b->n_req, b->max_tokens, b->max_pages, pg_max_new(b), n_works,

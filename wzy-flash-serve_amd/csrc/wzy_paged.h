@@ -15,7 +15,10 @@ namespace wzy {
 // says which belong together.  The same list serves every key head.
 constexpr int PG_NARROW = 32, PG_WIDE = 128;
 constexpr int PG_MAX_REQ = 4096, PG_MAX_TOKENS = 1 << 20, PG_MAX_CELLS = 1 << 24;
-constexpr int PG_PARTS = 512;                   // parts a step is cut into, over all key heads
+// Parts that a step is cut into, over all key heads: as many workgroups as the chip holds at once (by the LDS they take), and of
+// narrow tiles one more a tile, as far as PG_MORE, so that requests of different lengths come out even.
+constexpr int pg_parts(int kind, int hd) { return kind || hd == 128 ? 512 : hd == 64 ? 1024 : 256; }
+constexpr int PG_MORE = 512;
 constexpr int PG_MAGIC = 0x70616765;
 
 struct PgItem {
@@ -49,7 +52,7 @@ inline int pg_max_new(const wzy_paged_batch* b) { return b->max_new > 0 && b->ma
 // 4 * hd bytes of each cell's key and value; a wide tile's as much a row, for 128 rows.
 inline PgLayout pg_layout(int n_req, int max_tokens, int max_new, int max_cells, const wzy_paged_work* w) {
     PgLayout l{};
-    const int g = w->qh / w->kvh, per_head = pg_div_up(PG_PARTS, w->kvh);
+    const int g = w->qh / w->kvh;
     const bool any_wide = (int64_t) max_new * g > PG_NARROW;
     const int64_t tiles[2] = {n_req, any_wide ? (int64_t) max_tokens * g / PG_WIDE + n_req : 0};
     l.min_len[0] = 64;
@@ -57,6 +60,8 @@ inline PgLayout pg_layout(int n_req, int max_tokens, int max_new, int max_cells,
     int at = 0;
     for (int k = 0; k < 2; ++k) {
         // n = ceil(span / len) with the sum of span / len at most per_head: all tiles' parts, and those of tiles that have several
+        const int64_t more = k ? 0 : n_req < PG_MORE / w->kvh ? n_req : PG_MORE / w->kvh;
+        const int64_t per_head = pg_div_up(pg_parts(k, w->hd), w->kvh) + more;
         const int64_t most = tiles[k] * pg_div_up(max_cells, l.min_len[k]);
         l.items[k] = (int) (most < tiles[k] + per_head ? most : tiles[k] + per_head);
         l.parts[k] = (int) (most < 2 * per_head ? most : 2 * per_head);
