@@ -46,7 +46,7 @@ typedef struct wzy_paged_pool {
 typedef struct wzy_paged_batch {
     int n_req;                   /* 1 .. 4,096 */
     int max_tokens;              /* rows of the packed arrays, 1 .. 1,048,576 */
-    int max_pages;               /* columns of the table; max_pages * page at most 2^24 cells */
+    int max_pages;               /* columns of the table; max_pages * page at most 2^24 cells, n_req * max_pages below 2^31 */
     const int* n_cached;         /* [n_req]; negative counts as 0 */
     const int* n_new;            /* [n_req]; negative counts as 0 */
     int* table;                  /* [n_req x max_pages] page ids, in and out */

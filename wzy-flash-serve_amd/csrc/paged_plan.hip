@@ -13,7 +13,7 @@
 using namespace wzy;
 
 namespace {
-constexpr int PT = 1024, PLAN_ROWS = 4096, PER = PG_MAX_REQ / PT;
+constexpr int PT = 1024, PLAN_ROWS = 4096;
 
 struct PlanArgs {
     int* free_pages;
@@ -39,27 +39,36 @@ struct PlanWorks { PlanWork w[8]; };
 
 WZY_DEV int div_up_log2(int v, int l) { return (int) (((uint32_t) v + (1u << l) - 1) >> l); }
 
-// exclusive prefix sums over the workgroup's threads; total to all.  s: 17 words; a barrier before the next use is the function's own.
-WZY_DEV uint64_t block_scan(uint64_t v, uint64_t* s, uint64_t& total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    uint64_t x = v;
+// sums of lanes 0 .. l: within 16-lane rows by shifts, then the rows' last lanes on to the next rows
+template <int CTRL, int ROWMASK>
+WZY_DEV int add_dpp(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWMASK, 0xF, true); }
+WZY_DEV int prefix_sum(int v) {
+    v = add_dpp<0x111, 0xF>(v);                                    // row_shr 1, 2, 4, 8
+    v = add_dpp<0x112, 0xF>(v);
+    v = add_dpp<0x114, 0xF>(v);
+    v = add_dpp<0x118, 0xF>(v);
+    v = add_dpp<DPP_ROW_BCAST15, 0xA>(v);
+    return add_dpp<DPP_ROW_BCAST31, 0xC>(v);
+}
+// N exclusive prefix sums over the workgroup's NT threads at once, v in and out; the totals to all.  Sums below 2^31.
+template <int NT, int N>
+WZY_DEV void block_scan(int (&v)[N], int (*s)[NT / 64], int (&total)[N]) {
+    constexpr int NW = NT / 64;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int x[N];
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t y = (uint64_t) __shfl_up((unsigned long long) x, d);
-        if (lane >= d) x += y;
+    for (int i = 0; i < N; ++i) {
+        x[i] = prefix_sum(v[i]);
+        if (lane == 63) s[i][w] = x[i];
     }
-    if (lane == 63) s[w] = x;
     __syncthreads();
-    uint64_t before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < PT / 64; ++i) {
-        const uint64_t t = s[i];
-        before += i < w ? t : 0;
-        all += t;
+    for (int i = 0; i < N; ++i) {
+        const int t = prefix_sum(lane < NW ? s[i][lane & (NW - 1)] : 0);
+        total[i] = __builtin_amdgcn_readlane(t, NW - 1);
+        v[i] = x[i] - v[i] + (w > 0 ? __builtin_amdgcn_readlane(t, w > 0 ? w - 1 : 0) : 0);
     }
     __syncthreads();
-    total = all;
-    return before + x - v;
 }
 // the last r of 0 .. n - 1 with a[r] <= v (a ascending, a[0] = 0)
 WZY_DEV int find_last(const int* a, int n, int v) {
@@ -100,72 +109,70 @@ WZY_DEV void put_row(const PlanArgs& a, int t, const int* s_start, const int* s_
     a.slots[t] = slot;
 }
 
-__global__ void __launch_bounds__(PT) paged_plan_kernel(PlanArgs a, PlanWorks works) {
+template <int NT, int PER>
+__global__ void __launch_bounds__(NT) paged_plan_kernel(PlanArgs a, PlanWorks works) {
+    constexpr int REQ = NT * PER;
     // by request: cached cells (top bit: not served), first row, pages taken before it, tiles before it (one list's)
-    __shared__ int s_cached[PG_MAX_REQ], s_start[PG_MAX_REQ + 1], s_pages[PG_MAX_REQ], s_tiles[PG_MAX_REQ];
-    __shared__ int s_item[PT], s_part[PT];                     // by tile of a pass: items and parts before it
-    __shared__ uint64_t s_scan[PT / 64 + 1];
+    __shared__ int s_cached[REQ], s_start[REQ + 1], s_pages[REQ], s_tiles[2][REQ];
+    __shared__ int s_item[NT], s_part[NT];                     // by tile of a pass: items and parts before it
+    __shared__ int s_scan[3][NT / 64];
     const int tid = threadIdx.x;
     const int n_free = min(max(*a.n_free, 0), a.n_pages);
-    // requests PER * tid .. : rows, then pages
-    int c[PER], n[PER], need[PER];
-    int64_t sum = 0;
+    // requests PER * tid .. : rows.  A thread's are counted up to one more than there is room for, so that sums stay in 32 bits.
+    int c[PER], n[PER], sum = 0, v1[1], t1[1];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int r = PER * tid + i;
         c[i] = r < a.n_req ? max(a.n_cached[r], 0) : 0;
-        n[i] = r < a.n_req ? max(a.n_new[r], 0) : 0;
-        sum += n[i];
+        n[i] = r < a.n_req ? min(max(a.n_new[r], 0), a.max_tokens + 1) : 0;
+        sum = min(sum + n[i], a.max_tokens + 1);
     }
-    uint64_t total;
-    int64_t start = (int64_t) block_scan((uint64_t) sum, s_scan, total);
-    const int rows_total = (int) min((int64_t) total, (int64_t) a.max_tokens);
-    int64_t pages = 0;
+    v1[0] = sum;
+    block_scan<NT>(v1, s_scan, t1);
+    const int rows_total = min(t1[0], a.max_tokens);
+    int start = v1[0], need[PER];
     bool ok[PER];
+    v1[0] = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int r = PER * tid + i;
-        const int64_t cells = (int64_t) c[i] + n[i];
-        // c and n below 2^24 where the request fits; the others are not served, and their cells are not counted
-        ok[i] = r < a.n_req && cells <= (int64_t) a.max_pages << a.lp && n[i] <= a.max_new && (n[i] == 0 || start + n[i] <= a.max_tokens);
-        need[i] = ok[i] ? div_up_log2((int) cells, a.lp) - div_up_log2(c[i], a.lp) : 0;
-        if (r < a.n_req) s_start[r] = (int) min(start, (int64_t) a.max_tokens);
-        start += n[i];
-        pages += need[i];
+        // where the request fits, its cells are at most 2^24
+        ok[i] = r < a.n_req && (int64_t) c[i] + n[i] <= (int64_t) a.max_pages << a.lp && n[i] <= a.max_new && (n[i] == 0 || start + n[i] <= a.max_tokens);
+        need[i] = ok[i] ? div_up_log2(c[i] + n[i], a.lp) - div_up_log2(c[i], a.lp) : 0;
+        if (r < a.n_req) s_start[r] = min(start, a.max_tokens);
+        start = min(start + n[i], 1 << 30);
+        v1[0] += need[i];
     }
-    int64_t before = (int64_t) block_scan((uint64_t) pages, s_scan, total);
-    int64_t taken = 0;
+    block_scan<NT>(v1, s_scan, t1);
+    int before = v1[0], taken[1] = {0}, n_taken[1];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int r = PER * tid + i;
-        const bool fits = need[i] == 0 || before + need[i] <= n_free;
-        ok[i] = ok[i] && fits;
+        ok[i] = ok[i] && (need[i] == 0 || before + need[i] <= n_free);
         if (r < a.n_req) {
-            s_pages[r] = (int) min(before, (int64_t) n_free);
+            s_pages[r] = min(before, n_free);
             s_cached[r] = ok[i] ? c[i] : (int) ((uint32_t) c[i] | 0x80000000u);
             a.served[r] = ok[i] ? 1 : 0;
             a.kv_len[r] = ok[i] ? c[i] + n[i] : 0;
             a.q_start[r] = s_start[r];
         }
         before += need[i];
-        taken += ok[i] ? need[i] : 0;
+        taken[0] += ok[i] ? need[i] : 0;
     }
-    block_scan((uint64_t) taken, s_scan, total);               // those served are the first that need any
-    const int n_taken = (int) total;
     if (tid == 0) {
         s_start[a.n_req] = rows_total;
         a.q_start[a.n_req] = rows_total;
-        *a.n_free_out = n_free - n_taken;
     }
-    __syncthreads();
+    block_scan<NT>(taken, s_scan, n_taken);                    // those served are the first that need any
+    if (tid == 0) *a.n_free_out = n_free - n_taken[0];
     // pages into the table.  Page ids are limited, so that a slot is always one of the cache's.
     auto pool = [&](int i) { return min(max(a.free_pages[n_free - 1 - i], 0), a.n_pages - 1); };
-    for (int i = tid; i < n_taken; i += PT) {
+    for (int i = tid; i < n_taken[0]; i += NT) {
         const int r = find_last(s_pages, a.n_req, i);
         a.table[(size_t) r * a.max_pages + div_up_log2(s_cached[r], a.lp) + i - s_pages[r]] = pool(i);
     }
     if (a.fill_rows)
-        for (int t = tid; t < a.max_tokens; t += PT)
+        for (int t = tid; t < a.max_tokens; t += NT)
             put_row(a, t, s_start, s_cached, rows_total, [&](int r, int p) {
                 const int held = div_up_log2(s_cached[r], a.lp);
                 return p < held ? min(max(a.table[(size_t) r * a.max_pages + p], 0), a.n_pages - 1) : pool(s_pages[r] + p - held);
@@ -174,80 +181,85 @@ __global__ void __launch_bounds__(PT) paged_plan_kernel(PlanArgs a, PlanWorks wo
     for (int i = 0; i < a.n_works; ++i) {
         const PlanWork& w = works.w[i];
         PgItem* const items = (PgItem*) (w.head + 1);
+        // tiles before each request, narrow and wide.  A request that is not served has one narrow tile without cells, whatever its
+        // rows: they become 0.
+        int tiles[PER][2], at[2] = {0, 0}, n_tiles[2];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int r = PER * tid + j;
+            const int rows = r < a.n_req ? (s_start[r + 1] - s_start[r]) * w.g : 0;        // as far as there are any
+            const bool narrow = rows <= PG_NARROW || !ok[j];
+            tiles[j][0] = rows > 0 && narrow ? 1 : 0;
+            tiles[j][1] = narrow ? 0 : (rows + PG_WIDE - 1) / PG_WIDE;
+            at[0] += tiles[j][0];
+            at[1] += tiles[j][1];
+        }
+        block_scan<NT>(at, s_scan, n_tiles);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int r = PER * tid + j;
+#pragma unroll
+            for (int kind = 0; kind < 2; ++kind) {
+                if (r < a.n_req) s_tiles[kind][r] = at[kind];
+                at[kind] += tiles[j][kind];
+            }
+        }
+        __syncthreads();
         for (int kind = 0; kind < 2; ++kind) {
-            // tiles before each request.  A request that is not served has one narrow tile without cells, whatever its rows:
-            // they become 0.
-            int tiles[PER], mine = 0;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int r = PER * tid + j;
-                // its rows, as far as there are any
-                const int rows = r < a.n_req ? (s_start[r + 1] - s_start[r]) * w.g : 0;
-                const bool narrow = rows <= PG_NARROW || !ok[j];
-                tiles[j] = rows == 0 ? 0 : kind == 0 ? (narrow ? 1 : 0) : narrow ? 0 : (rows + PG_WIDE - 1) / PG_WIDE;
-                mine += tiles[j];
-            }
-            int at = (int) block_scan((uint64_t) mine, s_scan, total);
-            const int n_tiles = (int) total;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int r = PER * tid + j;
-                if (r < a.n_req) s_tiles[r] = at;
-                at += tiles[j];
-            }
-            __syncthreads();
+            const int nt = n_tiles[kind];
             // a request's last tile sees the most cells and comes first
             auto tile_at = [&](int t, int& r) {
-                r = find_last(s_tiles, a.n_req, t);
-                const int end = r + 1 < a.n_req ? s_tiles[r + 1] : n_tiles;
-                const int cc = s_cached[r];
+                r = find_last(s_tiles[kind], a.n_req, t);
+                const int end = r + 1 < a.n_req ? s_tiles[kind][r + 1] : nt, cc = s_cached[r];
                 return tile_of(w, kind, end - 1 - t, cc & 0x7FFFFFFF, s_start[r + 1] - s_start[r], cc >= 0);
             };
-            uint64_t cells = 0;
-            for (int t = tid; t < n_tiles; t += PT) {
-                int r;
-                const Tile x = tile_at(t, r);
-                cells += (uint64_t) (x.hi - (x.lo & ~31));
-            }
-            block_scan(cells, s_scan, total);
-            // parts of at most len cells (a multiple of 32): at most per_head of them, and one more a tile
-            // few tiles: together with a tile's own last part they are what the chip holds at once
-            const int slots = w.per_head[kind];
-            const uint32_t per_head = (uint32_t) (4 * n_tiles <= slots ? slots - n_tiles : slots + (kind ? 0 : min(n_tiles, w.more)));
-            uint64_t len = (total + per_head - 1) / per_head;
-            len = (len + 31) & ~(uint64_t) 31;
-            const int part = (int) max(len, (uint64_t) w.l.min_len[kind]);
+            auto blocks_of = [](const Tile& x) { return ((x.hi + 31) >> 5) - (x.lo >> 5); };
             int n_items = 0, n_parts = 0, n_merges = 0;
-            for (int base = 0; base < n_tiles; base += PT) {
-                const int t = base + tid, here = min(n_tiles - base, PT);
-                int r = 0, k = 0;
-                Tile x{};
-                if (t < n_tiles) {
-                    x = tile_at(t, r);
-                    k = max(1, (x.hi - (x.lo & ~31) + part - 1) / part);
+            if (nt > 0) {
+                int64_t blocks = 0;
+                for (int t = tid; t < nt; t += NT) {
+                    int r;
+                    blocks += blocks_of(tile_at(t, r));
                 }
-                const uint64_t v = (uint64_t) k | (uint64_t) (k > 1 ? k : 0) << 24 | (uint64_t) (k > 1 ? 1 : 0) << 48;
-                const uint64_t p = block_scan(v, s_scan, total);
-                const int pt = n_parts + (int) (p >> 24 & 0xFFFFFF), me = n_merges + (int) (p >> 48);
-                s_item[tid] = (int) (p & 0xFFFFFF);
-                s_part[tid] = k > 1 ? pt : -1;
-                if (k > 1 && me < w.l.merges[kind])
-                    ((PgMerge*) items)[w.l.merge_at[kind] + me] =
-                        PgMerge{pt, k, s_start[r], x.row0, min((s_start[r + 1] - s_start[r]) * w.g - x.row0, kind ? PG_WIDE : PG_NARROW), {0, 0, 0}};
-                __syncthreads();
-                const int n = (int) (total & 0xFFFFFF);
-                for (int i = tid; i < n && n_items + i < w.l.items[kind]; i += PT) {
-                    const int o = find_last(s_item, here, i), j = i - s_item[o];
-                    const Tile y = tile_at(base + o, r);
-                    // a tile's parts are of one length, but for the blocks of 32 cells
-                    const int parts = (o + 1 < here ? s_item[o + 1] : n) - s_item[o], first = y.lo >> 5, blocks = ((y.hi + 31) >> 5) - first;
-                    const int from = 32 * (first + (int) ((int64_t) blocks * j / parts)), to = 32 * (first + (int) ((int64_t) blocks * (j + 1) / parts));
-                    items[w.l.item_at[kind] + n_items + i] = PgItem{r, y.row0, max(y.lo, from), min(y.hi, to), s_part[o] < 0 ? -1 : s_part[o] + j,
-                                                                    s_start[r], s_start[r + 1] - s_start[r], s_cached[r] & 0x7FFFFFFF};
+                int half[2] = {(int) (blocks >> 16), (int) (blocks & 0xFFFF)}, sums[2];
+                block_scan<NT>(half, s_scan, sums);
+                // parts of at most part blocks of 32 cells: at most per_head of them, and one more a tile; few tiles: together with a
+                // tile's own last part they are what the chip holds at once
+                const int64_t all = ((int64_t) sums[0] << 16) + sums[1];
+                const int slots = w.per_head[kind];
+                const int per_head = 4 * nt <= slots ? slots - nt : slots + (kind ? 0 : min(nt, w.more));
+                const int part = (int) max((all + per_head - 1) / per_head, (int64_t) w.l.min_len[kind] / 32);
+                for (int base = 0; base < nt; base += NT) {
+                    const int t = base + tid, here = min(nt - base, NT);
+                    int r = 0, k = 0;
+                    Tile x{};
+                    if (t < nt) {
+                        x = tile_at(t, r);
+                        k = max(1, (blocks_of(x) + part - 1) / part);
+                    }
+                    int v[3] = {k, k > 1 ? k : 0, k > 1 ? 1 : 0}, tot[3];
+                    block_scan<NT>(v, s_scan, tot);
+                    const int pt = n_parts + v[1], me = n_merges + v[2];
+                    s_item[tid] = v[0];
+                    s_part[tid] = k > 1 ? pt : -1;
+                    if (k > 1 && me < w.l.merges[kind])
+                        ((PgMerge*) items)[w.l.merge_at[kind] + me] = PgMerge{pt, k, s_start[r], x.row0,
+                                                                              min((s_start[r + 1] - s_start[r]) * w.g - x.row0, kind ? PG_WIDE : PG_NARROW), {0, 0, 0}};
+                    __syncthreads();
+                    const int n = tot[0];
+                    for (int j = tid; j < n && n_items + j < w.l.items[kind]; j += NT) {
+                        const int o = find_last(s_item, here, j), k0 = s_item[o], parts = (o + 1 < here ? s_item[o + 1] : n) - k0;
+                        const Tile y = tile_at(base + o, r);
+                        // a tile's parts are of one length, but for the blocks of 32 cells
+                        const int first = y.lo >> 5, nb = blocks_of(y);
+                        const int from = 32 * (first + (int) ((int64_t) nb * (j - k0) / parts)), to = 32 * (first + (int) ((int64_t) nb * (j - k0 + 1) / parts));
+                        items[w.l.item_at[kind] + n_items + j] = PgItem{r, y.row0, max(y.lo, from), min(y.hi, to), s_part[o] < 0 ? -1 : s_part[o] + j - k0,
+                                                                        s_start[r], s_start[r + 1] - s_start[r], s_cached[r] & 0x7FFFFFFF};
+                    }
+                    n_items += n;
+                    n_parts += tot[1];
+                    n_merges += tot[2];
                 }
-                n_items += n;
-                n_parts += (int) (total >> 24 & 0xFFFFFF);
-                n_merges += (int) (total >> 48);
             }
             if (tid == 0) {
                 w.head->n_items[kind] = min(n_items, w.l.items[kind]);
@@ -278,41 +290,41 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(PlanArgs a) {
 
 // One workgroup: pages to push are counted a request, summed over requests, and numbered through.
 __global__ void __launch_bounds__(PT) paged_release_kernel(PlanArgs a, const int* __restrict__ ended) {
-    __shared__ int s_pages[PG_MAX_REQ + 1];
-    __shared__ uint64_t s_scan[PT / 64 + 1];
+    constexpr int PER = PG_MAX_REQ / PT;
+    __shared__ int s_pages[PG_MAX_REQ];
+    __shared__ int s_scan[1][PT / 64];
     const int tid = threadIdx.x, n_free = min(max(*a.n_free, 0), a.n_pages);
-    int held[PER];
-    uint64_t sum = 0, total;
+    int held[PER], at[1] = {0}, n[1];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int r = PER * tid + i;
-        held[i] = 0;
-        if (r < a.n_req && ended[r]) held[i] = min(div_up_log2(max(a.n_cached[r], 0), a.lp), a.max_pages);
-        sum += (uint64_t) held[i];
+        held[i] = r < a.n_req && ended[r] ? min(div_up_log2(max(a.n_cached[r], 0), a.lp), a.max_pages) : 0;
+        at[0] += held[i];                                      // the table has fewer than 2^31 entries
     }
-    uint64_t at = block_scan(sum, s_scan, total);
+    block_scan<PT>(at, s_scan, n);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int r = PER * tid + i;
-        if (r < a.n_req) s_pages[r] = (int) at;
-        at += (uint64_t) held[i];
+        if (r < a.n_req) s_pages[r] = at[0];
+        at[0] += held[i];
     }
     __syncthreads();
-    const int n = (int) total;
     int n_out = n_free;
-    for (int base = 0; base < n; base += PT) {
+    for (int base = 0; base < n[0]; base += PT) {
         const int i = base + tid;
         int id = -1;
-        if (i < n) {
+        if (i < n[0]) {
             const int r = find_last(s_pages, a.n_req, i);
             int* const e = a.table + (size_t) r * a.max_pages + i - s_pages[r];
             id = *e;
             *e = -1;
         }
         const bool ok = id >= 0 && id < a.n_pages;
-        const int to = n_out + (int) block_scan(ok ? 1 : 0, s_scan, total);
+        int v[1] = {ok ? 1 : 0}, all[1];
+        block_scan<PT>(v, s_scan, all);
+        const int to = n_out + v[0];
         if (ok && to < a.n_pages) a.free_pages[to] = id;
-        n_out = (int) min((int64_t) n_out + (int64_t) total, (int64_t) a.n_pages);
+        n_out = min(n_out + all[0], a.n_pages);
     }
     if (tid == 0) *a.n_free_out = n_out;
 }
@@ -361,10 +373,14 @@ extern "C" int wzy_paged_plan(const wzy_paged_pool* pool, const wzy_paged_batch*
     PlanArgs a{pool->free_pages, pool->n_free, pool->n_free_out, b->n_cached, b->n_new, b->table, b->q_start, b->kv_len, b->served,
                b->positions, b->slots, pool->n_pages, pg_log2(pool->page), b->n_req, b->max_tokens, b->max_pages, pg_max_new(b), n_works,
                b->max_tokens <= PLAN_ROWS};
-    paged_plan_kernel<<<1, PT, 0, as_stream(stream)>>>(a, pw);
+    // few requests and rows: fewer waves to bring together
+    const auto st = as_stream(stream);
+    if (b->n_req <= 256 && b->max_tokens <= 256) paged_plan_kernel<256, 1><<<1, 256, 0, st>>>(a, pw);
+    else if (b->n_req <= 1024) paged_plan_kernel<1024, 1><<<1, 1024, 0, st>>>(a, pw);
+    else paged_plan_kernel<1024, 4><<<1, 1024, 0, st>>>(a, pw);
     WZY_LAUNCH_CHECK();
     if (!a.fill_rows) {
-        paged_rows_kernel<<<pg_div_up(b->max_tokens, 256), 256, 0, as_stream(stream)>>>(a);
+        paged_rows_kernel<<<pg_div_up(b->max_tokens, 256), 256, 0, st>>>(a);
         WZY_LAUNCH_CHECK();
     }
     return WZY_OK;
@@ -374,7 +390,8 @@ extern "C" int wzy_paged_release(const wzy_paged_pool* pool, const wzy_paged_bat
     const char* const who = "wzy_paged_release";
     WZY_TRY(check_pool(who, pool));
     WZY_REQUIRE(b && b->n_req >= 1 && b->n_req <= PG_MAX_REQ, "%s: requests (1 .. %d)", who, PG_MAX_REQ);
-    WZY_REQUIRE(b->max_pages >= 1 && (int64_t) b->max_pages * pool->page <= PG_MAX_CELLS, "%s: max_pages %d", who, b->max_pages);
+    WZY_REQUIRE(b->max_pages >= 1 && (int64_t) b->max_pages * pool->page <= PG_MAX_CELLS && (int64_t) b->max_pages * b->n_req < 1ll << 31,
+                "%s: max_pages %d", who, b->max_pages);
     WZY_REQUIRE(b->n_cached && b->table && ended, "%s: an array is null", who);
     PlanArgs a{};
     a.free_pages = pool->free_pages; a.n_free = pool->n_free; a.n_free_out = pool->n_free_out; a.n_cached = b->n_cached; a.table = b->table;

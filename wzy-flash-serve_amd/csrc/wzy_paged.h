@@ -88,8 +88,8 @@ inline int pg_check_batch(const char* who, const wzy_paged_batch* b, int page) {
     WZY_REQUIRE(b->n_req >= 1 && b->n_req <= PG_MAX_REQ, "%s: %d requests (1 .. %d)", who, b->n_req, PG_MAX_REQ);
     WZY_REQUIRE(b->max_tokens >= 1 && b->max_tokens <= PG_MAX_TOKENS, "%s: max_tokens %d (1 .. %d)", who, b->max_tokens, PG_MAX_TOKENS);
     WZY_REQUIRE(b->max_new >= 0, "%s: max_new %d", who, b->max_new);
-    WZY_REQUIRE(b->max_pages >= 1 && (int64_t) b->max_pages * page <= PG_MAX_CELLS, "%s: max_pages %d (at most %d cells)", who,
-                b->max_pages, PG_MAX_CELLS);
+    WZY_REQUIRE(b->max_pages >= 1 && (int64_t) b->max_pages * page <= PG_MAX_CELLS && (int64_t) b->max_pages * b->n_req < 1ll << 31,
+                "%s: max_pages %d (at most %d cells, fewer than 2^31 entries)", who, b->max_pages, PG_MAX_CELLS);
     return WZY_OK;
 }
 inline int pg_check_work(const char* who, const wzy_paged_work* w) {
