@@ -5,9 +5,9 @@
 //
 // A few integers a request and a row: what bounds it is the chain from the lengths to the last slot, not bytes.  One workgroup
 // of 16 waves does requests, tables and work lists: the prefix sums over requests (4 a thread: wave shifts, then the 16 waves'
-// sums) stay in LDS, and everything that is counted in pages, tiles or rows is numbered through and dealt to the threads, each
+// sums) stay in LDS, and everything that is counted in pages, parts or rows is numbered through and dealt to the threads, each
 // finding its request by a search in those sums, so that one long prompt does not make one thread's loop long.  Up to PLAN_ROWS
-// rows the same launch fills positions and slots; more rows take a second one with a workgroup per 256 of them.
+// rows the same launch fills positions, slots and work lists; more rows take a second one with a workgroup per 256 of them.
 #include "wzy_paged.h"
 
 using namespace wzy;
@@ -70,28 +70,55 @@ WZY_DEV void block_scan(int (&v)[N], int (*s)[NT / 64], int (&total)[N]) {
     }
     __syncthreads();
 }
-// the last r of 0 .. n - 1 with a[r] <= v (a ascending, a[0] = 0)
-WZY_DEV int find_last(const int* a, int n, int v) {
+// the last r of 0 .. n - 1 with a(r) <= v (a ascending, a(0) = 0)
+template <class F>
+WZY_DEV int find_last_of(int n, int v, F&& a) {
     int lo = 0, hi = n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (a[mid] <= v) lo = mid;
+        if (a(mid) <= v) lo = mid;
         else hi = mid;
     }
     return lo;
 }
+WZY_DEV int find_last(const int* a, int n, int v) {
+    return find_last_of(n, v, [&](int r) { return a[r]; });
+}
 
-// a tile's cells: of its first token's window, to its last token's own
-struct Tile { int row0, lo, hi; };
-WZY_DEV Tile tile_of(const PlanWork& w, int kind, int j, int c, int n, bool served) {
-    Tile t;
+// A request in one list: its tiles, and the parts each is cut into.  A request that is not served has one narrow tile without
+// cells, whatever its rows: they become 0.
+struct Cut { int kind, tiles, parts, blocks; };
+WZY_DEV Cut cut_of(const PlanWork& w, int c, int n, bool served, const int (&part)[2]) {
+    Cut x;
     const int rows = n * w.g;
-    t.row0 = kind ? PG_WIDE * j : 0;
-    const int first = (int) ((uint32_t) t.row0 / (uint32_t) w.g);
-    const int last = (int) ((uint32_t) (min(t.row0 + (kind ? PG_WIDE : PG_NARROW), rows) - 1) / (uint32_t) w.g);
-    t.hi = served ? c + last + 1 : 0;
-    t.lo = served && w.window > 0 ? max(c + first + 1 - w.window, 0) : 0;
-    return t;
+    x.kind = rows <= PG_NARROW || !served ? 0 : 1;
+    x.tiles = rows == 0 ? 0 : x.kind ? (rows + PG_WIDE - 1) / PG_WIDE : 1;
+    // blocks of 32 cells that a tile sees, at most: the last one's end, or as many as its tokens' windows span
+    x.blocks = served ? (c + n + 31) >> 5 : 0;
+    if (w.window > 0) x.blocks = min(x.blocks, ((w.window + (int) ((uint32_t) (x.kind ? PG_WIDE : PG_NARROW) / (uint32_t) w.g)) >> 5) + 2);
+    const int p = part[x.kind];
+    x.parts = p > 0 && x.blocks > p ? (x.blocks + p - 1) / p : 1;
+    return x;
+}
+// item i of a kind, which is the request's i - before.items[kind]-th, and with a tile's first part its merge entry
+WZY_DEV void put_item(const PlanWork& w, int kind, int i, int r, const PgBefore& before, int c, int n, bool served, int q0, const int (&part)[2]) {
+    const Cut x = cut_of(w, c, n, served, part);
+    const int j = i - before.items[kind], tile = (int) ((uint32_t) j / (uint32_t) x.parts), k = j - tile * x.parts, rows = n * w.g;
+    // a request's last tile sees the most cells and comes first
+    const int row0 = kind ? PG_WIDE * (x.tiles - 1 - tile) : 0, row1 = min(row0 + (kind ? PG_WIDE : PG_NARROW), rows);
+    const int hi = served ? c + (int) ((uint32_t) (row1 - 1) / (uint32_t) w.g) + 1 : 0;
+    const int lo = served && w.window > 0 ? max(c + (int) ((uint32_t) row0 / (uint32_t) w.g) + 1 - w.window, 0) : 0;
+    // parts of one length, but for the blocks of 32 cells
+    const int first = lo >> 5, blocks = ((hi + 31) >> 5) - first;
+    // (below 2^32: 2^19 blocks, and parts are at most pg_parts() + PG_MORE)
+    const uint32_t nb = (uint32_t) blocks, np = (uint32_t) x.parts;
+    const int from = 32 * (first + (int) (nb * (uint32_t) k / np)), to = 32 * (first + (int) (nb * (uint32_t) (k + 1) / np));
+    const int pt = before.parts + tile * x.parts;
+    PgItem* const items = (PgItem*) (w.head + 1);
+    if (i >= w.l.items[kind] || (x.parts > 1 && pt + x.parts > w.l.parts[kind])) return;
+    items[w.l.item_at[kind] + i] = PgItem{r, row0, max(lo, from), min(hi, to), x.parts > 1 ? pt + k : -1, q0, n, c};
+    if (x.parts > 1 && k == 0 && before.merges + tile < w.l.merges[kind])
+        ((PgMerge*) items)[w.l.merge_at[kind] + before.merges + tile] = PgMerge{pt, x.parts, q0, row0, row1 - row0, {0, 0, 0}};
 }
 
 // positions and slots of row t, from the sums in LDS
@@ -112,10 +139,10 @@ WZY_DEV void put_row(const PlanArgs& a, int t, const int* s_start, const int* s_
 template <int NT, int PER>
 __global__ void __launch_bounds__(NT) paged_plan_kernel(PlanArgs a, PlanWorks works) {
     constexpr int REQ = NT * PER;
-    // by request: cached cells (top bit: not served), first row, pages taken before it, tiles before it (one list's)
-    __shared__ int s_cached[REQ], s_start[REQ + 1], s_pages[REQ], s_tiles[2][REQ];
-    __shared__ int s_item[NT], s_part[NT];                     // by tile of a pass: items and parts before it
-    __shared__ int s_scan[3][NT / 64];
+    // by request: cached cells (top bit: not served), first row, pages taken before it, what is before it in a list
+    __shared__ int s_cached[REQ], s_start[REQ + 1], s_pages[REQ];
+    __shared__ PgBefore s_before[REQ];
+    __shared__ int s_scan[6][NT / 64];
     const int tid = threadIdx.x;
     const int n_free = min(max(*a.n_free, 0), a.n_pages);
     // requests PER * tid .. : rows.  A thread's are counted up to one more than there is room for, so that sums stay in 32 bits.
@@ -180,112 +207,109 @@ __global__ void __launch_bounds__(NT) paged_plan_kernel(PlanArgs a, PlanWorks wo
 
     for (int i = 0; i < a.n_works; ++i) {
         const PlanWork& w = works.w[i];
-        PgItem* const items = (PgItem*) (w.head + 1);
-        // tiles before each request, narrow and wide.  A request that is not served has one narrow tile without cells, whatever its
-        // rows: they become 0.
-        int tiles[PER][2], at[2] = {0, 0}, n_tiles[2];
+        // the longest parts: tiles, and blocks of all tiles (in two halves, so that sums stay in 32 bits)
+        int part[2] = {0, 0}, v[6] = {0, 0, 0, 0, 0, 0}, sums[6];
+        int64_t blocks[2] = {0, 0};
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int r = PER * tid + j;
-            const int rows = r < a.n_req ? (s_start[r + 1] - s_start[r]) * w.g : 0;        // as far as there are any
-            const bool narrow = rows <= PG_NARROW || !ok[j];
-            tiles[j][0] = rows > 0 && narrow ? 1 : 0;
-            tiles[j][1] = narrow ? 0 : (rows + PG_WIDE - 1) / PG_WIDE;
-            at[0] += tiles[j][0];
-            at[1] += tiles[j][1];
-        }
-        block_scan<NT>(at, s_scan, n_tiles);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int r = PER * tid + j;
-#pragma unroll
-            for (int kind = 0; kind < 2; ++kind) {
-                if (r < a.n_req) s_tiles[kind][r] = at[kind];
-                at[kind] += tiles[j][kind];
+            if (r < a.n_req) {
+                const Cut x = cut_of(w, c[j], s_start[r + 1] - s_start[r], ok[j], part);
+                v[x.kind] += x.tiles;
+                blocks[x.kind] += (int64_t) x.tiles * x.blocks;
             }
+        }
+        v[2] = (int) (blocks[0] >> 16); v[3] = (int) (blocks[0] & 0xFFFF);
+        v[4] = (int) (blocks[1] >> 16); v[5] = (int) (blocks[1] & 0xFFFF);
+        block_scan<NT>(v, s_scan, sums);
+#pragma unroll
+        for (int kind = 0; kind < 2; ++kind) {
+            // at most per_head parts of that length, and one more a tile; few tiles: together with a tile's own last part they are what
+            // the chip holds at once
+            const int64_t all = ((int64_t) sums[2 + 2 * kind] << 16) + sums[3 + 2 * kind];
+            const int slots = w.per_head[kind], nt = sums[kind];
+            const int per_head = 4 * nt <= slots ? slots - nt : slots + (kind ? 0 : min(nt, w.more));
+            part[kind] = max((int) ceil((double) all / (double) per_head), w.l.min_len[kind] / 32);
+        }
+        // items, parts and merges before each request
+        Cut x[PER];
+#pragma unroll
+        for (int j = 0; j < 6; ++j) v[j] = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int r = PER * tid + j;
+            x[j] = r < a.n_req ? cut_of(w, c[j], s_start[r + 1] - s_start[r], ok[j], part) : Cut{0, 0, 1, 0};
+            const int k = x[j].kind, its = x[j].tiles * x[j].parts;
+            v[k] += its;
+            if (x[j].parts > 1) {
+                v[2 + 2 * k] += its;
+                v[3 + 2 * k] += x[j].tiles;
+            }
+        }
+        block_scan<NT>(v, s_scan, sums);
+        PgBefore* const out = (PgBefore*) ((PgItem*) (w.head + 1) + w.l.before_at);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int r = PER * tid + j, k = x[j].kind, its = x[j].tiles * x[j].parts;
+            if (r < a.n_req) {
+                const PgBefore b{{v[0], v[1]}, v[2 + 2 * k], v[3 + 2 * k]};
+                if (a.fill_rows) s_before[r] = b;
+                else out[r] = b;
+            }
+            v[k] += its;
+            if (x[j].parts > 1) {
+                v[2 + 2 * k] += its;
+                v[3 + 2 * k] += x[j].tiles;
+            }
+        }
+        if (tid == 0) *w.head = PgHead{PG_MAGIC, w.geometry, {min(sums[0], w.l.items[0]), min(sums[1], w.l.items[1])},
+                                       {min(sums[3], w.l.merges[0]), min(sums[5], w.l.merges[1])}, {part[0], part[1]}, {}};
+        if (!a.fill_rows) continue;
+        __syncthreads();
+        for (int j = tid; j < sums[0] + sums[1]; j += NT) {
+            const int kind = j < sums[0] ? 0 : 1, it = j - (kind ? sums[0] : 0);
+            const int r = find_last_of(a.n_req, it, [&](int q) { return s_before[q].items[kind]; });
+            const int cc = s_cached[r];
+            put_item(w, kind, it, r, s_before[r], cc & 0x7FFFFFFF, s_start[r + 1] - s_start[r], cc >= 0, s_start[r], part);
         }
         __syncthreads();
-        for (int kind = 0; kind < 2; ++kind) {
-            const int nt = n_tiles[kind];
-            // a request's last tile sees the most cells and comes first
-            auto tile_at = [&](int t, int& r) {
-                r = find_last(s_tiles[kind], a.n_req, t);
-                const int end = r + 1 < a.n_req ? s_tiles[kind][r + 1] : nt, cc = s_cached[r];
-                return tile_of(w, kind, end - 1 - t, cc & 0x7FFFFFFF, s_start[r + 1] - s_start[r], cc >= 0);
-            };
-            auto blocks_of = [](const Tile& x) { return ((x.hi + 31) >> 5) - (x.lo >> 5); };
-            int n_items = 0, n_parts = 0, n_merges = 0;
-            if (nt > 0) {
-                int64_t blocks = 0;
-                for (int t = tid; t < nt; t += NT) {
-                    int r;
-                    blocks += blocks_of(tile_at(t, r));
-                }
-                int half[2] = {(int) (blocks >> 16), (int) (blocks & 0xFFFF)}, sums[2];
-                block_scan<NT>(half, s_scan, sums);
-                // parts of at most part blocks of 32 cells: at most per_head of them, and one more a tile; few tiles: together with a
-                // tile's own last part they are what the chip holds at once
-                const int64_t all = ((int64_t) sums[0] << 16) + sums[1];
-                const int slots = w.per_head[kind];
-                const int per_head = 4 * nt <= slots ? slots - nt : slots + (kind ? 0 : min(nt, w.more));
-                const int part = (int) max((all + per_head - 1) / per_head, (int64_t) w.l.min_len[kind] / 32);
-                for (int base = 0; base < nt; base += NT) {
-                    const int t = base + tid, here = min(nt - base, NT);
-                    int r = 0, k = 0;
-                    Tile x{};
-                    if (t < nt) {
-                        x = tile_at(t, r);
-                        k = max(1, (blocks_of(x) + part - 1) / part);
-                    }
-                    int v[3] = {k, k > 1 ? k : 0, k > 1 ? 1 : 0}, tot[3];
-                    block_scan<NT>(v, s_scan, tot);
-                    const int pt = n_parts + v[1], me = n_merges + v[2];
-                    s_item[tid] = v[0];
-                    s_part[tid] = k > 1 ? pt : -1;
-                    if (k > 1 && me < w.l.merges[kind])
-                        ((PgMerge*) items)[w.l.merge_at[kind] + me] = PgMerge{pt, k, s_start[r], x.row0,
-                                                                              min((s_start[r + 1] - s_start[r]) * w.g - x.row0, kind ? PG_WIDE : PG_NARROW), {0, 0, 0}};
-                    __syncthreads();
-                    const int n = tot[0];
-                    for (int j = tid; j < n && n_items + j < w.l.items[kind]; j += NT) {
-                        const int o = find_last(s_item, here, j), k0 = s_item[o], parts = (o + 1 < here ? s_item[o + 1] : n) - k0;
-                        const Tile y = tile_at(base + o, r);
-                        // a tile's parts are of one length, but for the blocks of 32 cells
-                        const int first = y.lo >> 5, nb = blocks_of(y);
-                        const int from = 32 * (first + (int) ((int64_t) nb * (j - k0) / parts)), to = 32 * (first + (int) ((int64_t) nb * (j - k0 + 1) / parts));
-                        items[w.l.item_at[kind] + n_items + j] = PgItem{r, y.row0, max(y.lo, from), min(y.hi, to), s_part[o] < 0 ? -1 : s_part[o] + j - k0,
-                                                                        s_start[r], s_start[r + 1] - s_start[r], s_cached[r] & 0x7FFFFFFF};
-                    }
-                    n_items += n;
-                    n_parts += tot[1];
-                    n_merges += tot[2];
-                }
-            }
-            if (tid == 0) {
-                w.head->n_items[kind] = min(n_items, w.l.items[kind]);
-                w.head->n_merges[kind] = min(n_merges, w.l.merges[kind]);
-                if (kind == 0) {
-                    w.head->magic = PG_MAGIC;
-                    w.head->geometry = w.geometry;
-                }
-            }
-        }
     }
 }
 
-// rows of larger steps: the table and q_start are as the plan left them
-__global__ void __launch_bounds__(256) paged_rows_kernel(PlanArgs a) {
-    __shared__ int s_start[PG_MAX_REQ + 1], s_cached[PG_MAX_REQ];
+// Rows and work lists of larger steps, a workgroup per 256 of them: the table, q_start and the sums are as the plan left them.
+struct RowBlocks { int at[9]; };                               // first workgroup of each list; those before are rows'
+__global__ void __launch_bounds__(256) paged_rows_kernel(PlanArgs a, PlanWorks works, RowBlocks blocks) {
+    __shared__ int s_start[PG_MAX_REQ + 1], s_cached[PG_MAX_REQ], s_items[2][PG_MAX_REQ];
+    const int block = blockIdx.x;
+    int list = -1;
+    while (list + 1 < a.n_works && block >= blocks.at[list + 1]) ++list;
+    const PgBefore* before = nullptr;
+    if (list >= 0) before = (const PgBefore*) ((const PgItem*) (works.w[list].head + 1) + works.w[list].l.before_at);
     for (int r = threadIdx.x; r < a.n_req; r += 256) {
         const int c = max(a.n_cached[r], 0);
         s_start[r] = a.q_start[r];
         s_cached[r] = a.served[r] ? c : (int) ((uint32_t) c | 0x80000000u);
+        if (list >= 0) {
+            const PgBefore b = before[r];
+            s_items[0][r] = b.items[0];
+            s_items[1][r] = b.items[1];
+        }
     }
+    if (threadIdx.x == 0) s_start[a.n_req] = a.q_start[a.n_req];
     __syncthreads();
-    const int t = blockIdx.x * 256 + threadIdx.x;
-    if (t >= a.max_tokens) return;
-    put_row(a, t, s_start, s_cached, a.q_start[a.n_req],
-            [&](int r, int p) { return min(max(a.table[(size_t) r * a.max_pages + p], 0), a.n_pages - 1); });
+    if (list < 0) {
+        const int t = block * 256 + threadIdx.x;
+        if (t < a.max_tokens)
+            put_row(a, t, s_start, s_cached, s_start[a.n_req],
+                    [&](int r, int p) { return min(max(a.table[(size_t) r * a.max_pages + p], 0), a.n_pages - 1); });
+        return;
+    }
+    const PlanWork& w = works.w[list];
+    const PgHead h = *w.head;
+    const int part[2] = {h.part[0], h.part[1]}, j = (block - blocks.at[list]) * 256 + (int) threadIdx.x;
+    if (j >= h.n_items[0] + h.n_items[1]) return;
+    const int kind = j < h.n_items[0] ? 0 : 1, it = j - (kind ? h.n_items[0] : 0), r = find_last(s_items[kind], a.n_req, it), cc = s_cached[r];
+    put_item(w, kind, it, r, before[r], cc & 0x7FFFFFFF, s_start[r + 1] - s_start[r], cc >= 0, s_start[r], part);
 }
 
 // One workgroup: pages to push are counted a request, summed over requests, and numbered through.
@@ -380,7 +404,13 @@ extern "C" int wzy_paged_plan(const wzy_paged_pool* pool, const wzy_paged_batch*
     else paged_plan_kernel<1024, 4><<<1, 1024, 0, st>>>(a, pw);
     WZY_LAUNCH_CHECK();
     if (!a.fill_rows) {
-        paged_rows_kernel<<<pg_div_up(b->max_tokens, 256), 256, 0, st>>>(a);
+        RowBlocks rb{};
+        int at = pg_div_up(b->max_tokens, 256);
+        for (int i = 0; i < n_works; ++i) {
+            rb.at[i] = at;
+            at += pg_div_up((int64_t) pw.w[i].l.items[0] + pw.w[i].l.items[1], 256);
+        }
+        paged_rows_kernel<<<at, 256, 0, st>>>(a, pw, rb);
         WZY_LAUNCH_CHECK();
     }
     return WZY_OK;

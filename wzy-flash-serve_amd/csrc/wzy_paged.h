@@ -11,8 +11,8 @@ namespace wzy {
 // The rows of one request and key head are its (token, head of the group) pairs, token-major: row m is token m / g, head
 // m % g, g = qh / kvh.  They are cut into tiles: requests of up to PG_NARROW rows are one narrow tile, others have wide tiles
 // of PG_WIDE rows.  A tile's cells (from the first that its first token sees to its last token's own) are cut into parts of
-// equal length where the tiles alone do not fill the chip; parts leave partial results in the workspace, and a merge entry
-// says which belong together.  The same list serves every key head.
+// equal length where the tiles alone do not fill the chip, all tiles of a request into as many as its longest needs; parts leave
+// partial results in the workspace, and a merge entry says which belong together.  The same list serves every key head.
 constexpr int PG_NARROW = 32, PG_WIDE = 128;
 constexpr int PG_MAX_REQ = 4096, PG_MAX_TOKENS = 1 << 20, PG_MAX_CELLS = 1 << 24;
 // Parts that a step is cut into, over all key heads: as many workgroups as the chip holds at once (by the LDS they take), and of
@@ -34,15 +34,17 @@ struct PgMerge {
 struct PgHead {
     int magic, geometry;
     int n_items[2], n_merges[2];                // narrow, wide
-    int pad[10];
+    int part[2];                                // longest part, blocks of 32 cells
+    int pad[8];
 };
-static_assert(sizeof(PgItem) == 32 && sizeof(PgMerge) == 32 && sizeof(PgHead) == 64, "work list");
+struct PgBefore { int items[2], parts, merges; };   // what the requests before one have; parts and merges of its own kind
+static_assert(sizeof(PgItem) == 32 && sizeof(PgMerge) == 32 && sizeof(PgHead) == 64 && sizeof(PgBefore) == 16, "work list");
 
-// What one list holds at most, and where (in entries of 32 bytes behind the head).
+// What one list holds at most, and where (in entries of 32 bytes behind the head; the requests' sums come last).
 struct PgLayout {
     int items[2], parts[2], merges[2];          // capacities: narrow, wide
     int min_len[2];                             // shortest part, cells
-    int item_at[2], merge_at[2], total;
+    int item_at[2], merge_at[2], before_at, total;
 };
 
 inline int pg_div_up(int64_t a, int64_t b) { return (int) ((a + b - 1) / b); }
@@ -73,7 +75,8 @@ inline PgLayout pg_layout(int n_req, int max_tokens, int max_new, int max_cells,
         l.merge_at[k] = at;
         at += l.merges[k];
     }
-    l.total = at;
+    l.before_at = at;
+    l.total = at + (n_req + 1) / 2;
     return l;
 }
 PgLayout pg_layout_of(const wzy_paged_batch* b, const wzy_paged_work* w);
