@@ -174,7 +174,7 @@ int wzy_paged_attend(const wzy_paged_cache* cache, const wzy_paged_batch* batch,
  *   id           the first whose running sum reaches u * (the sum of what is left); prob = its share of that sum
  * as the host sampler of wzy_engine.h does, over any number of logits.  temp at or below 1e-5: the first of the order,
  * prob 1.  A row without a logit above -infinity gives id -1, prob 0; +infinity takes all there is, shared by those that
- * have it.  Sums are integers of 2^-40 to 2^-62 of w_0, so results do not depend on the order of additions.
+ * have it.  Sums are integers of 2^-40 to 2^-51 of w_0, so results do not depend on the order of additions.
  * temp, top_k, top_p, min_p [rows] may each be NULL: 1, all, all, all; u [rows] in 0 .. 1 (below 0 counts as 0, above 1 as 1,
  * NaN as 0).  probs may be NULL.  1 <= vocab <= 2^22; any alignment of an element. */
 size_t wzy_sample_workspace_bytes(int rows, int vocab);

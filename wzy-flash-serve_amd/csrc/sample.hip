@@ -3,14 +3,19 @@
 // The order of a row is (logit descending, id ascending).  Every cut keeps a prefix of it, and the draw takes the first
 // token whose running sum of w = 2^-x, x = (max - l) log2(e) / temp, reaches a target; so all that is needed are places in
 // that order: by count (top-k), by sum (top-p, the draw), by value (min-p).  No sort of the row: a histogram over x in bins of
-// 1/16 (count and sum of w) says in which bin a place lies, and only the tokens of that bin, or of all up to it where they are
-// few, are gathered and sorted.  Three launches:
-//   sample_max   a slice of a row a workgroup: its best token
-//   sample_hist  the same slices: x against the row's best, histogram in LDS, then added to the row's
-//   sample_pick  a workgroup a row: the places, with a pass over the row for each gathered range (one for top-k and small
-//                nuclei, two for large ones)
+// 1/16 (count and sum of w) says in which few bins the places lie, and only those bins' tokens are gathered and sorted.
+//   sample_max     a slice of a row a workgroup: its best token
+//   sample_hist    the same slices: x against the row's best, histogram in LDS, added to the row's
+//   sample_plan    a workgroup a row: which bins are wanted.  (The row's last workgroup of sample_hist, told by a counter, could do it:
+//                  the fences between their atomics and its loads took 200 us at 256 rows.)
+//   sample_gather  the slices again: tokens of those bins to the row's list
+//   sample_pick    a workgroup a row: the list sorted, sums, places
+// Rows whose bins hold more than CAP tokens (thousands of equal logits) are done by sample_pick alone, from the row.
 // w is taken in 64 bits (fp32's 1e-7 would move one draw in a thousand of a flat row) and summed as integers of 2^-F, F = 62 -
-// log2(vocab): sums do not depend on their order, so LDS and memory atomics may add them as they come.
+// log2(vocab), at most 51: sums do not depend on their order, so LDS and memory atomics may add them as they come.  Where top-k is
+// small, everything it leaves is gathered, and the histogram counts only.
+#include <algorithm>
+
 #include "wzy_paged.h"
 
 using namespace wzy;
@@ -18,15 +23,29 @@ using namespace wzy;
 namespace {
 constexpr int ST = 256, PER = 32, SLICE = ST * PER;      // sample_max, sample_hist
 constexpr int PT = 1024, CAP = 4096;                     // sample_pick; tokens gathered at most
+constexpr int SMALL_K = 2048;                            // top-k up to which all that it leaves is gathered
 constexpr int BINS = 1024;                               // 64 octaves of w
 constexpr float BIN_OCT = 16.0f;
 constexpr float GREEDY = 1e-5f;
 constexpr uint32_t KEY_NONE = 0x007FFFFFu;               // order key of -infinity
 
+// What sample_plan leaves to the next kernels.
+enum { ROW_FIRST, ROW_LIST, ROW_ALONE };
+struct RowPlan {
+    int mode;                                            // the best token (or none at all); a list; neither
+    int n, lo[4], hi[4];                                 // intervals of bins that are gathered, in order
+    float most[4], least[4];                             // the logits at their ends
+    uint64_t before_mass[4], list_mass[4];               // sums before each, of the row and of the list
+    uint32_t before_count[4], count;                     // tokens before each; of the row (where top-k wants them)
+    uint64_t mass;                                       // of the row
+    int m0, m1;                                          // bins in which min-p ends; -1: it does not matter
+    uint64_t m_mass;                                     // sum before bin m0
+};
+
 struct SampleArgs {
     const void* logits;
     int64_t ld;
-    int rows, vocab, slices, F;
+    int rows, vocab, slices, units, F;                   // slices of `units` x SLICE logits
     const float* temp;
     const int* top_k;
     const float* top_p;
@@ -37,6 +56,9 @@ struct SampleArgs {
     uint64_t* best;                                      // [rows x slices]
     uint64_t* mass;                                      // [rows x BINS]
     uint32_t* count;                                     // [rows x BINS]
+    RowPlan* plan;                                       // [rows]
+    uint32_t* listed;                                    // [rows] tokens in the list
+    uint64_t* list;                                      // [rows x CAP]
 };
 
 // a logit's bits in numeric order (both zeros alike); a NaN as -infinity
@@ -49,93 +71,105 @@ WZY_DEV float key_value(uint32_t k) {
 }
 WZY_DEV uint64_t order_u64(float v, int i) { return (uint64_t) order_key(v) << 32 | (uint32_t) ~i; }
 
-// 2^(-j / 64)
+// 2^(-j / STEPS)
+constexpr int LSTEPS = 8, STEPS = 1 << LSTEPS;
 WZY_DEV void fill_table(double* s) {
-    for (int i = threadIdx.x; i < 64; i += blockDim.x) s[i] = exp2(-(double) i / 64.0);
+    for (int i = threadIdx.x; i < STEPS; i += blockDim.x) s[i] = exp2(-(double) i / STEPS);
 }
 // A row's weights: m its largest logit, c = log2(e) / temp.  The bin is taken in fp32, which is monotone too.
 struct Weight {
     float m, cf;
-    double c;
+    double cs;                                           // STEPS log2(e) / temp
     int F;
     const double* table;
     WZY_DEV int bin(float l) const {
         const float x = l == m ? 0.0f : (m - l) * cf * BIN_OCT;
         return (int) fminf(x, (float) (BINS - 1));
     }
-    WZY_DEV double x(float l) const { return l == m ? 0.0 : ((double) m - (double) l) * c; }
-    // 2^-x: x = n + j / 64 + r / 64, |r| <= 1/2; the series of 2^(-r / 64) to the fifth power leaves 2e-18
-    WZY_DEV double w(float l) const {
-        const double v = x(l);
-        if (!(v < 1000.0)) return 0.0;
-        const double t = v * 64.0, k = rint(t), r = (t - k) * (-0.6931471805599453094 / 64.0);
-        const int i = (int) k;
-        double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-        p = fma(p, r, 1.0 / 6.0);
-        p = fma(p, r, 0.5);
-        p = fma(p, r, 1.0);
-        p = fma(p, r, 1.0);
-        return ldexp(p * table[i & 63], -(i >> 6));
+    // 2^-x as an integer of 2^-F: 256 x = k + r, |r| <= 1/2; 2^(-r / 256) by its series, whose fourth term is 2e-13 at most; 2^-(k / 256)
+    // from the table and the exponent field.  Adding 1.5 2^52 rounds to an integer and leaves it in the low bits.
+    WZY_DEV uint64_t fixed(float l) const {
+        return __builtin_bit_cast(uint64_t, scaled(l, F) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
     }
-    WZY_DEV uint64_t fixed(float l) const { return (uint64_t) rint(ldexp(w(l), F)); }
+    WZY_DEV double w(float l) const { return scaled(l, 0); }
+    WZY_DEV double scaled(float l, int f) const {
+        constexpr double MAGIC = 6755399441055744.0, A = -0.6931471805599453094 / STEPS;
+        const double t = (l == m ? 0.0 : (double) m - (double) l) * cs;
+        const double n = t + MAGIC, r = t - (n - MAGIC);
+        const int i = (int) (uint32_t) __builtin_bit_cast(uint64_t, n);
+        double p = __builtin_fma(r, A * A * A / 6.0, A * A / 2.0);
+        p = __builtin_fma(p, r, A);
+        const uint64_t b = __builtin_bit_cast(uint64_t, table[i & (STEPS - 1)]) + ((uint64_t) (uint32_t) ((f - (i >> LSTEPS)) << 20) << 32);
+        const double base = __builtin_bit_cast(double, b);                   // 2^-1000 at least: no denormal
+        const double v = __builtin_fma(base * r, p, base);
+        return t < 1000.0 * STEPS ? v : 0.0;
+    }
 };
 WZY_DEV float temp_of(const SampleArgs& a, int row) { return a.temp ? a.temp[row] : 1.0f; }
-WZY_DEV bool greedy(float t) { return !(t > GREEDY); }
 
-// f(value, id) over elements from .. from + n * threads - 1 (limited to end) of a row: 16 bytes a thread where the row allows
-template <int T, bool VEC, int N, class F>
-WZY_DEV void each(const void* row, int from, int end, F&& f) {
-    constexpr int E = T == WZY_F32 ? 4 : 8;
+// N elements a thread of the row's from .. (16 bytes at a time where the row allows), -infinity past end; which they are
+template <int T, bool VEC>
+WZY_DEV int element(int from, int j) {
+    constexpr int E = !VEC ? 1 : T == WZY_F32 ? 4 : 8;
+    return from + ((j / E) * (int) blockDim.x + (int) threadIdx.x) * E + j % E;
+}
+template <int T>
+WZY_DEV float load_logit(const void* row, int i) {
+    if constexpr (T == WZY_F32) return ((const float*) row)[i];
+    else if constexpr (T == WZY_BF16) return bf16_to_f(((const uint16_t*) row)[i]);
+    else return h16_to_f(((const uint16_t*) row)[i]);
+}
+template <int T, bool VEC, int N>
+WZY_DEV void load_elements(const void* row, int from, int end, float (&x)[N]) {
     if constexpr (VEC) {
-        // loads first, then their use
+        constexpr int E = T == WZY_F32 ? 4 : 8;
         uint4 v[N / E];
 #pragma unroll
         for (int i = 0; i < N / E; ++i) {
-            const int e = from + (i * (int) blockDim.x + (int) threadIdx.x) * E;
-            v[i] = e + E <= end ? *(const uint4*) ((const char*) row + (size_t) e * (16 / E)) : make_uint4(0, 0, 0, 0);
+            const int e = element<T, true>(from, i * E);
+            if (e + E <= end) v[i] = *(const uint4*) ((const char*) row + (size_t) e * (16 / E));
+            else v[i] = make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < N / E; ++i) {
-            const int e = from + (i * (int) blockDim.x + (int) threadIdx.x) * E;
             const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-            if (e + E <= end) {
 #pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    float x;
-                    if constexpr (T == WZY_F32) x = __builtin_bit_cast(float, w[j]);
-                    else if constexpr (T == WZY_BF16) x = j & 1 ? bf16_hi(w[j / 2]) : bf16_lo(w[j / 2]);
-                    else x = h16_to_f((uint16_t) (w[j / 2] >> (16 * (j & 1))));
-                    f(x, e + j);
-                }
-            } else {
-                for (int j = e; j < end; ++j) {
-                    float x;
-                    if constexpr (T == WZY_F32) x = ((const float*) row)[j];
-                    else if constexpr (T == WZY_BF16) x = bf16_to_f(((const uint16_t*) row)[j]);
-                    else x = h16_to_f(((const uint16_t*) row)[j]);
-                    f(x, j);
-                }
+            for (int j = 0; j < E; ++j) {
+                if constexpr (T == WZY_F32) x[i * E + j] = __builtin_bit_cast(float, w[j]);
+                else if constexpr (T == WZY_BF16) x[i * E + j] = j & 1 ? bf16_hi(w[j / 2]) : bf16_lo(w[j / 2]);
+                else x[i * E + j] = h16_to_f((uint16_t) (w[j / 2] >> (16 * (j & 1))));
+            }
+        }
+        if (from + N * (int) blockDim.x > end) {                // the row's end
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int e = element<T, true>(from, j);
+                if (e - j % E + E > end) x[j] = e < end ? load_logit<T>(row, e) : -INFINITY;
             }
         }
     } else {
-        float v[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = min(from + i * (int) blockDim.x + (int) threadIdx.x, end - 1);
-            if constexpr (T == WZY_F32) v[i] = ((const float*) row)[e];
-            else if constexpr (T == WZY_BF16) v[i] = bf16_to_f(((const uint16_t*) row)[e]);
-            else v[i] = h16_to_f(((const uint16_t*) row)[e]);
-        }
+        for (int j = 0; j < N; ++j) x[j] = load_logit<T>(row, min(element<T, false>(from, j), end - 1));
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = from + i * (int) blockDim.x + (int) threadIdx.x;
-            if (e < end) f(v[i], e);
-        }
+        for (int j = 0; j < N; ++j) x[j] = element<T, false>(from, j) < end ? x[j] : -INFINITY;
     }
 }
 template <int T>
 WZY_DEV const void* row_of(const SampleArgs& a, int row) {
     return (const char*) a.logits + (size_t) row * a.ld * (T == WZY_F32 ? 4 : 2);
+}
+
+// f(values, first) over the slice's elements, PER a thread at a time
+template <int T, bool VEC, class F>
+WZY_DEV void each_unit(const SampleArgs& a, int row, int slice, F&& f) {
+    const void* const r = row_of<T>(a, row);
+    for (int u = 0; u < a.units; ++u) {
+        const int from = (slice * a.units + u) * SLICE;
+        if (from >= a.vocab) break;
+        float x[PER];
+        load_elements<T, VEC>(r, from, min(from + SLICE, a.vocab), x);
+        f(x, from);
+    }
 }
 
 template <int T, bool VEC>
@@ -147,9 +181,12 @@ __global__ void __launch_bounds__(ST) sample_max_kernel(SampleArgs a) {
         a.mass[(size_t) row * BINS + i] = 0;
         a.count[(size_t) row * BINS + i] = 0;
     }
+    if (slice == 0 && tid == 0) a.listed[row] = 0;
     uint64_t b = 0;
-    const int from = slice * SLICE;
-    each<T, VEC, PER>(row_of<T>(a, row), from, min(from + SLICE, a.vocab), [&](float v, int i) { b = max_u64(b, order_u64(v, i)); });
+    each_unit<T, VEC>(a, row, slice, [&](const float (&x)[PER], int from) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) b = max_u64(b, order_u64(x[j], element<T, VEC>(from, j)));
+    });
     b = wave_max_u64(b);
     if ((tid & 63) == 0) s_best[tid >> 6] = b;
     __syncthreads();
@@ -176,68 +213,30 @@ WZY_DEV uint64_t row_best(const SampleArgs& a, int row, uint64_t* s) {
 WZY_DEV Weight weight_of(const SampleArgs& a, uint64_t best, float t, const double* table) {
     Weight w;
     w.m = key_value((uint32_t) (best >> 32));
-    w.c = 1.44269504088896340736 / (double) t;
-    w.cf = (float) w.c;
+    const double c = 1.44269504088896340736 / (double) t;
+    w.cs = c * STEPS;
+    w.cf = (float) c;
     w.F = a.F;
     w.table = table;
     return w;
 }
 
-template <int T, bool VEC>
-__global__ void __launch_bounds__(ST) sample_hist_kernel(SampleArgs a) {
-    __shared__ unsigned long long s_mass[BINS];
-    __shared__ uint32_t s_count[BINS];
-    __shared__ double s_table[64];
-    __shared__ uint64_t s_best[ST / 64];
-    const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
-    const float t = temp_of(a, row);
-    if (greedy(t)) return;
-    fill_table(s_table);
-    for (int i = tid; i < BINS; i += ST) {
-        s_mass[i] = 0;
-        s_count[i] = 0;
-    }
-    const uint64_t best = row_best<ST>(a, row, s_best);          // its barriers cover what was stored before
-    if ((uint32_t) (best >> 32) == KEY_NONE) return;
-    const Weight w = weight_of(a, best, t, s_table);
-    uint32_t far = 0;
-    uint64_t far_mass = 0;
-    const int from = slice * SLICE;
-    each<T, VEC, PER>(row_of<T>(a, row), from, min(from + SLICE, a.vocab), [&](float l, int) {
-        if (!(l > -INFINITY)) return;
-        const int b = w.bin(l);
-        const uint64_t f = w.fixed(l);
-        if (b == BINS - 1) {                                    // many of a row may be here: one add a thread
-            ++far;
-            far_mass += f;
-        } else {
-            atomicAdd(&s_mass[b], (unsigned long long) f);
-            atomicAdd(&s_count[b], 1u);
-        }
-    });
-    if (far) {
-        atomicAdd(&s_mass[BINS - 1], (unsigned long long) far_mass);
-        atomicAdd(&s_count[BINS - 1], far);
-    }
-    __syncthreads();
-    for (int i = tid; i < BINS; i += ST)
-        if (s_count[i]) {
-            atomicAdd((unsigned long long*) a.mass + (size_t) row * BINS + i, s_mass[i]);
-            atomicAdd(a.count + (size_t) row * BINS + i, s_count[i]);
-        }
-}
-
-// ---- sample_pick ----------------------------------------------------------------------------------------
 // inclusive sums of (mass, count) over the workgroup's threads
 struct Sum { uint64_t mass; uint32_t count; };
+template <int CTRL, int ROWMASK>
+WZY_DEV void add_lanes(Sum& v) {
+    const uint32_t lo = dpp_u32<CTRL, ROWMASK>((uint32_t) v.mass), hi = dpp_u32<CTRL, ROWMASK>((uint32_t) (v.mass >> 32));
+    v.mass += (uint64_t) hi << 32 | lo;
+    v.count += dpp_u32<CTRL, ROWMASK>(v.count);
+}
 WZY_DEV Sum block_sums(Sum v, Sum* s_part) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t m = (uint64_t) __shfl_up((unsigned long long) v.mass, d);
-        const uint32_t c = __shfl_up(v.count, d);
-        if (lane >= d) { v.mass += m; v.count += c; }
-    }
+    add_lanes<0x111, 0xF>(v);                            // row_shr 1, 2, 4, 8, then the rows' last lanes on to the next rows
+    add_lanes<0x112, 0xF>(v);
+    add_lanes<0x114, 0xF>(v);
+    add_lanes<0x118, 0xF>(v);
+    add_lanes<DPP_ROW_BCAST15, 0xA>(v);
+    add_lanes<DPP_ROW_BCAST31, 0xC>(v);
     if (lane == 63) s_part[wv] = v;
     __syncthreads();
     for (int i = 0; i < wv; ++i) {
@@ -247,17 +246,314 @@ WZY_DEV Sum block_sums(Sum v, Sum* s_part) {
     __syncthreads();
     return v;
 }
+// the first integer at or above f * sum, 1 .. sum
+WZY_DEV uint64_t share(double f, uint64_t sum) {
+    const double x = ceil(f * (double) sum);
+    const uint64_t v = x >= (double) sum ? sum : (uint64_t) x;
+    return v < 1 ? (uint64_t) 1 : v;
+}
+// a row's parameters, made harmless
+struct Params {
+    float temp, top_p, min_p;
+    double u;
+    int k;
+    bool first;                                          // the best token, whatever u
+    WZY_DEV Params(const SampleArgs& a, int row) {
+        temp = a.temp ? a.temp[row] : 1.0f;
+        k = a.top_k ? a.top_k[row] : 0;
+        top_p = a.top_p ? a.top_p[row] : 1.0f;
+        min_p = a.min_p ? a.min_p[row] : 0.0f;
+        const float v = a.u[row];
+        u = v > 0.0f ? fmin((double) v, 1.0) : 0.0;
+        first = !(temp > GREEDY) || min_p > 1.0f || k == 1;
+    }
+    WZY_DEV bool cut_p() const { return top_p > 0.0f && top_p < 1.0f; }
+    WZY_DEV bool cut_m() const { return min_p > 0.0f; }
+    WZY_DEV bool counts_only() const { return k >= 1 && k <= SMALL_K; }
+    WZY_DEV bool counts() const { return k >= 1; }
+};
 
+// The bins that the places may lie in.  A place that hangs on one inside a bin is bracketed by the bin's ends.  One wave; lane 0
+// has the lower ends' targets, the others the upper ones'.  mass, count: inclusive sums (count where top-k wants it).
+WZY_DEV void plan_row(const Params& q, const uint64_t* mass, const uint32_t* count, RowPlan& out) {
+    const bool upper = (threadIdx.x & 63) != 0;
+    auto at_mass = [&](uint64_t t) {                     // the first bin whose sum reaches t
+        int lo = -1, hi = BINS - 1;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (mass[mid] >= t) hi = mid;
+            else lo = mid;
+        }
+        return hi;
+    };
+    auto before = [&](int b) { return b > 0 ? mass[b - 1] : 0; };
+    auto first_lane = [](int v) { return __builtin_amdgcn_readlane(v, 0); };
+    auto other_lane = [](int v) { return __builtin_amdgcn_readlane(v, 1); };
+    // intervals of top-k, top-p, min-p, the draw
+    int lo[4] = {BINS, BINS, BINS, BINS}, hi[4] = {-1, -1, -1, -1};
+    const uint32_t all = count[BINS - 1];
+    const bool cut_k = q.k >= 1 && (uint32_t) q.k < all;
+    int kb = BINS - 1, m0 = -1, m1 = -1;
+    if (q.counts()) {
+        const uint32_t t = cut_k ? (uint32_t) q.k : all;
+        int a = -1;
+        while (kb - a > 1) {
+            const int mid = (a + kb) >> 1;
+            if (count[mid] >= t) kb = mid;
+            else a = mid;
+        }
+    }
+    if (q.counts_only()) {
+        lo[0] = 0;
+        hi[0] = kb;
+    } else {
+        // what is left lies between the sums at these two
+        uint64_t end = mass[BINS - 1];
+        int last = BINS - 1;
+        if (cut_k) {
+            end = upper ? mass[kb] : before(kb);
+            lo[0] = hi[0] = last = kb;
+        }
+        if (q.cut_p()) {
+            const int b = at_mass(share((double) q.top_p, end));
+            lo[1] = first_lane(b);
+            hi[1] = other_lane(b);
+            last = min(last, hi[1]);
+            const uint64_t to = upper ? mass[b] : before(b);
+            end = to < end ? to : end;
+        }
+        if (q.cut_m()) {
+            // the bins are taken in fp32, to 1e-3 of a bin
+            const float x = -log2f(q.min_p) * BIN_OCT;
+            const int b = (int) fmaxf(upper ? x + 0.02f : x - 0.02f, 0.0f), b0 = first_lane(b), b1 = other_lane(b);
+            if (b1 < BINS - 1 && b0 <= last) {
+                lo[2] = m0 = b0;
+                hi[2] = m1 = b1;
+                const uint64_t to = upper ? mass[b1] : before(b0);
+                end = to < end ? to : end;
+            }
+        }
+        const int b = at_mass(share(q.u, end));
+        lo[3] = first_lane(b);
+        hi[3] = other_lane(b);
+    }
+    auto order = [&](int i, int j) {
+        const bool sw = lo[j] < lo[i];
+        const int x = sw ? lo[j] : lo[i], y = sw ? hi[j] : hi[i];
+        lo[j] = sw ? lo[i] : lo[j];
+        hi[j] = sw ? hi[i] : hi[j];
+        lo[i] = x;
+        hi[i] = y;
+    };
+    order(0, 1); order(2, 3); order(0, 2); order(1, 3); order(1, 2);
+    // one where they touch
+    if (threadIdx.x & 63) return;
+    int n = 0;
+    uint32_t tokens = 0;
+    uint64_t sum = 0;
+    int from = lo[0], to = hi[0];
+    auto close = [&] {
+        out.lo[n] = from;
+        out.hi[n] = to;
+        out.before_count[n] = from > 0 ? count[from - 1] : 0;
+        out.before_mass[n] = before(from);
+        out.list_mass[n] = sum;
+        tokens += count[to] - out.before_count[n];
+        sum += mass[to] - before(from);
+        ++n;
+    };
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+        if (lo[i] == BINS) continue;
+        if (lo[i] <= to + 1) to = max(to, hi[i]);
+        else {
+            close();
+            from = lo[i];
+            to = hi[i];
+        }
+    }
+    close();
+    out.n = n;
+    out.mode = tokens > CAP ? ROW_ALONE : ROW_LIST;      // not counted: the list will tell
+    out.mass = mass[BINS - 1];
+    out.count = all;
+    out.m0 = m0;
+    out.m1 = m1;
+    out.m_mass = m0 > 0 ? before(m0) : 0;
+}
+
+template <int T, bool VEC>
+__global__ void __launch_bounds__(ST) sample_hist_kernel(SampleArgs a) {
+    __shared__ unsigned long long s_mass[BINS + 64];
+    __shared__ uint32_t s_count[BINS + 64];
+    __shared__ double s_table[STEPS];
+    __shared__ uint64_t s_best[ST / 64];
+    const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
+    const Params q(a, row);
+    const bool masses = !q.counts_only(), counts = q.counts();      // top-k wants counts, the others sums
+    if (masses) fill_table(s_table);
+    for (int i = tid; i < BINS; i += ST) {
+        s_mass[i] = 0;
+        s_count[i] = 0;
+    }
+    const uint64_t best = row_best<ST>(a, row, s_best);          // its barriers cover what was stored before
+    if (q.first || (uint32_t) (best >> 32) == KEY_NONE) return;
+    const Weight w = weight_of(a, best, q.temp, s_table);
+    // Tokens of the last bin (w 0, and many of a row may be there) and what is not a number go to slots that are not looked at, a lane
+    // one: no branch an element.
+    const int lane = tid & 63;
+    uint32_t far = 0;
+    if (masses)
+        each_unit<T, VEC>(a, row, slice, [&](const float (&x)[PER], int) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int b = w.bin(x[j]);
+                atomicAdd(&s_mass[b == BINS - 1 ? BINS + lane : b], (unsigned long long) w.fixed(x[j]));
+            }
+        });
+    if (counts)
+        each_unit<T, VEC>(a, row, slice, [&](const float (&x)[PER], int) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int b = w.bin(x[j]);
+                atomicAdd(&s_count[b == BINS - 1 ? BINS + lane : b], 1u);
+                far += b == BINS - 1 && x[j] > -INFINITY ? 1 : 0;
+            }
+        });
+    if (far) atomicAdd(&s_count[BINS - 1], far);
+    __syncthreads();
+    for (int i = tid; i < BINS; i += ST) {
+        if (s_mass[i]) atomicAdd((unsigned long long*) a.mass + (size_t) row * BINS + i, s_mass[i]);
+        if (s_count[i]) atomicAdd(a.count + (size_t) row * BINS + i, s_count[i]);
+    }
+}
+
+__global__ void __launch_bounds__(ST) sample_plan_kernel(SampleArgs a) {
+    __shared__ uint64_t s_mass[BINS], s_best[ST / 64];
+    __shared__ uint32_t s_count[BINS];
+    __shared__ Sum s_part[ST / 64];
+    __shared__ RowPlan s_plan;
+    const int row = blockIdx.x, tid = threadIdx.x;
+    const Params q(a, row);
+    constexpr int Q = BINS / ST;
+    Sum v[Q], all{0, 0};
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+        v[i] = Sum{a.mass[(size_t) row * BINS + Q * tid + i], a.count[(size_t) row * BINS + Q * tid + i]};
+        all.mass += v[i].mass;
+        all.count += v[i].count;
+    }
+    const uint64_t best = row_best<ST>(a, row, s_best);
+    if (q.first || (uint32_t) (best >> 32) == KEY_NONE) {
+        if (tid == 0) a.plan[row].mode = ROW_FIRST;
+        return;
+    }
+    Sum at = block_sums(all, s_part);
+    at.mass -= all.mass;
+    at.count -= all.count;
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+        at.mass += v[i].mass;
+        at.count += v[i].count;
+        s_mass[Q * tid + i] = at.mass;
+        s_count[Q * tid + i] = at.count;
+    }
+    __syncthreads();
+    if (tid >= 64) return;
+    plan_row(q, s_mass, s_count, s_plan);
+    wave_lds_sync();
+    // the intervals' ends as logits, a lane an end: the bin falls as the key rises
+    if (tid < 2 * s_plan.n) {
+        const Weight w = weight_of(a, best, q.temp, nullptr);
+        const int j = tid >> 1;
+        uint32_t lo = KEY_NONE, hi = (uint32_t) (best >> 32) + 1;
+        if (tid & 1) {                                          // the largest whose bin is lo or more
+            const int b = s_plan.lo[j];
+            while (hi - lo > 1) {
+                const uint32_t mid = lo + (hi - lo) / 2;
+                if (w.bin(key_value(mid)) >= b) lo = mid;
+                else hi = mid;
+            }
+            s_plan.most[j] = key_value(lo);
+        } else {                                                // the least whose bin is hi or less
+            const int b = s_plan.hi[j];
+            --hi;                                               // the best one's is 0
+            while (hi - lo > 1) {
+                const uint32_t mid = lo + (hi - lo) / 2;
+                if (w.bin(key_value(mid)) <= b) hi = mid;
+                else lo = mid;
+            }
+            s_plan.least[j] = key_value(hi);
+        }
+    }
+    wave_lds_sync();
+    const uint32_t* const from = (const uint32_t*) &s_plan;
+    uint32_t* const to = (uint32_t*) (a.plan + row);
+    for (int i = tid; i < (int) (sizeof(RowPlan) / 4); i += 64) to[i] = from[i];
+}
+
+template <int T, bool VEC>
+__global__ void __launch_bounds__(ST) sample_gather_kernel(SampleArgs a) {
+    constexpr int BUF = 1024;
+    __shared__ uint64_t s_token[BUF];
+    __shared__ uint32_t s_n, s_at;
+    const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
+    const RowPlan& p = a.plan[row];
+    const int mode = p.mode, n = p.n;
+    if (mode != ROW_LIST) return;
+    float most[4], least[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        most[i] = i < n ? p.most[i] : -INFINITY;
+        least[i] = i < n ? p.least[i] : INFINITY;
+    }
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    auto put = [&](uint32_t at, uint64_t token) {
+        if (at < CAP) a.list[(size_t) row * CAP + at] = token;
+    };
+    // a bit an element, then the few that are set: no branch an element
+    const void* const r = row_of<T>(a, row);
+    static_assert(PER == 32, "a bit an element");
+    each_unit<T, VEC>(a, row, slice, [&](const float (&x)[PER], int from) {
+        uint32_t hits = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) hits |= (x[j] >= least[0] && x[j] <= most[0]) || (x[j] >= least[1] && x[j] <= most[1]) ? 1u << j : 0u;
+        if (n > 2)
+#pragma unroll
+            for (int j = 0; j < PER; ++j) hits |= (x[j] >= least[2] && x[j] <= most[2]) || (x[j] >= least[3] && x[j] <= most[3]) ? 1u << j : 0u;
+        while (hits) {
+            const int i = element<T, VEC>(from, __builtin_ctz(hits));
+            hits &= hits - 1;
+            const uint64_t token = order_u64(load_logit<T>(r, i), i);
+            const uint32_t at = atomicAdd(&s_n, 1u);
+            if (at < BUF) s_token[at] = token;
+            else put(atomicAdd(a.listed + row, 1u), token);
+        }
+    });
+    __syncthreads();
+    const uint32_t here = min(s_n, (uint32_t) BUF);
+    if (here == 0) return;
+    if (tid == 0) s_at = atomicAdd(a.listed + row, here);
+    __syncthreads();
+    for (uint32_t i = tid; i < here; i += ST) put(s_at + i, s_token[i]);
+}
+
+// ---- sample_pick ----------------------------------------------------------------------------------------
 enum Mode { BY_COUNT, BY_MASS, BY_KEY };
 // a place in the order: sums up to it, itself included, and the token there
 struct Place { uint64_t mass; uint32_t count; uint64_t token; };
 
 struct PickShared {
     uint64_t token[CAP];                                 // gathered, sorted: largest first
-    uint64_t token_mass[CAP];                            // sums up to each
+    union {
+        uint64_t token_mass[CAP];                        // sums up to each
+        uint64_t unsorted[CAP];
+    };
+    uint32_t bucket[CAP];
     uint64_t bin_mass[BINS];                             // sums up to each bin, itself included
     uint32_t bin_count[BINS];
-    double table[64];
+    double table[STEPS];
     Sum part[PT / 64];
     uint64_t best[PT / 64];
     unsigned n;
@@ -277,10 +573,35 @@ struct Picker {
     static constexpr int STEP = 16;
     template <class F>
     WZY_DEV void scan(F&& f) const {
-        for (int from = 0; from < a.vocab; from += PT * STEP) each<T, VEC, STEP>(row, from, min(from + PT * STEP, a.vocab), f);
+        for (int from = 0; from < a.vocab; from += PT * STEP) {
+            float x[STEP];
+            load_elements<T, VEC>(row, from, min(from + PT * STEP, a.vocab), x);
+#pragma unroll
+            for (int j = 0; j < STEP; ++j) f(x[j], element<T, VEC>(from, j));
+        }
     }
     WZY_DEV Sum before_bin(int b) const { return b > 0 ? Sum{s.bin_mass[b - 1], s.bin_count[b - 1]} : Sum{0, 0}; }
 
+    // s.token[0 .. n - 1], largest first
+    WZY_DEV void sort(int n) {
+        const int tid = threadIdx.x;
+        int n2 = 64;
+        while (n2 < n) n2 <<= 1;
+        for (int i = n + tid; i < n2; i += PT) s.token[i] = 0;
+        for (int k = 2; k <= n2; k <<= 1)                        // bitonic
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                __syncthreads();
+                for (int i = tid; i < n2 / 2; i += PT) {
+                    const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+                    const uint64_t x = s.token[lo], y = s.token[hi];
+                    if ((x < y) == ((lo & k) == 0)) {
+                        s.token[lo] = y;
+                        s.token[hi] = x;
+                    }
+                }
+            }
+        __syncthreads();
+    }
     // the tokens for which take(logit) holds, at most CAP of them, sorted, with their sums from `sum_before` on
     template <class F>
     WZY_DEV void gather(F&& take, Sum sum_before) {
@@ -296,23 +617,7 @@ struct Picker {
         });
         __syncthreads();
         const int n = min((int) s.n, CAP);
-        int n2 = 64;
-        while (n2 < n) n2 <<= 1;
-        for (int i = n + tid; i < n2; i += PT) s.token[i] = 0;
-        // bitonic, largest first
-        for (int k = 2; k <= n2; k <<= 1)
-            for (int j = k >> 1; j > 0; j >>= 1) {
-                __syncthreads();
-                for (int i = tid; i < n2 / 2; i += PT) {
-                    const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
-                    const uint64_t x = s.token[lo], y = s.token[hi];
-                    if ((x < y) == ((lo & k) == 0)) {
-                        s.token[lo] = y;
-                        s.token[hi] = x;
-                    }
-                }
-            }
-        __syncthreads();
+        sort(n);
         // CAP / PT neighbours a thread
         constexpr int Q = CAP / PT;
         uint64_t m[Q], sum = 0;
@@ -461,62 +766,209 @@ struct Picker {
     }
 };
 
+// a row by itself: its histogram, then the places, with a pass over the row for each range that is gathered
+template <int T, bool VEC>
+WZY_DEV void pick_alone(const SampleArgs& a, int row, const Params& q, uint64_t best, PickShared& s, Picker<T, VEC>& p) {
+    const int tid = threadIdx.x;
+    unsigned long long* const h = (unsigned long long*) s.bin_mass;
+    h[tid] = 0;
+    s.bin_count[tid] = 0;
+    __syncthreads();
+    p.scan([&](float l, int) {
+        if (!(l > -INFINITY)) return;
+        const int b = p.w.bin(l);
+        if (b < BINS - 1) atomicAdd(&h[b], (unsigned long long) p.w.fixed(l));
+        atomicAdd(&s.bin_count[b], 1u);
+    });
+    __syncthreads();
+    const Sum own{s.bin_mass[tid], s.bin_count[tid]}, sum = block_sums(own, s.part);
+    s.bin_mass[tid] = sum.mass;
+    s.bin_count[tid] = sum.count;
+    __syncthreads();
+    Place end{s.bin_mass[BINS - 1], s.bin_count[BINS - 1], 0};
+    if (q.k >= 1 && (uint32_t) q.k < end.count) end = p.locate(BY_COUNT, (uint64_t) q.k);
+    if (q.cut_p()) {
+        const Place x = p.locate(BY_MASS, share((double) q.top_p, end.mass));
+        if (x.count < end.count) end = x;
+    }
+    if (q.cut_m()) {
+        // the lowest key whose weight is min_p or more: halving, every thread the same
+        uint32_t hi = (uint32_t) (best >> 32), lo = KEY_NONE;             // hi passes, lo does not
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (p.w.w(key_value(mid)) >= (double) q.min_p) hi = mid;
+            else lo = mid;
+        }
+        // where the last token kept so far passes, nothing is cut
+        if (end.token == 0 || (uint32_t) (end.token >> 32) < hi) {
+            const Place x = p.locate(BY_KEY, hi);
+            if (x.count < end.count) end = x;
+        }
+    }
+    const Place x = p.locate(BY_MASS, share(q.u, end.mass));
+    if (tid == 0) {
+        a.ids[row] = (int) ~(uint32_t) x.token;
+        if (a.probs) a.probs[row] = (float) (p.w.scaled(key_value((uint32_t) (x.token >> 32)), a.F) / (double) end.mass);
+    }
+}
+
 template <int T, bool VEC>
 __global__ void __launch_bounds__(PT) sample_pick_kernel(SampleArgs a) {
     __shared__ PickShared s;
     const int row = blockIdx.x, tid = threadIdx.x;
-    const float t = temp_of(a, row);
+    const Params q(a, row);
+    const RowPlan& plan = a.plan[row];
+    const int mode = plan.mode;
     fill_table(s.table);
     const uint64_t best = row_best<PT>(a, row, s.best);
-    const bool none = (uint32_t) (best >> 32) == KEY_NONE;
-    if (none || greedy(t)) {
+    if (mode == ROW_FIRST) {
+        const bool none = (uint32_t) (best >> 32) == KEY_NONE;
         if (tid == 0) {
             a.ids[row] = none ? -1 : (int) ~(uint32_t) best;
             if (a.probs) a.probs[row] = none ? 0.0f : 1.0f;
         }
         return;
     }
-    const Sum h = block_sums(Sum{a.mass[(size_t) row * BINS + tid], a.count[(size_t) row * BINS + tid]}, s.part);
-    s.bin_mass[tid] = h.mass;
-    s.bin_count[tid] = h.count;
-    __syncthreads();
-    Picker<T, VEC> p{a, s, row_of<T>(a, row), weight_of(a, best, t, s.table)};
-    Place end{s.bin_mass[BINS - 1], s.bin_count[BINS - 1], 0};
-    const int k = a.top_k ? a.top_k[row] : 0;
-    if (k >= 1 && (uint32_t) k < end.count) end = p.locate(BY_COUNT, (uint64_t) k);
-    const uint64_t of_k = end.mass;
-    const float top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f;
-    // targets: the first integer at or above share * sum; the sum itself at most
-    auto share = [](double f, uint64_t sum) {
-        const double x = ceil(f * (double) sum);
-        const uint64_t v = x >= (double) sum ? sum : (uint64_t) x;
-        return v < 1 ? (uint64_t) 1 : v;
+    Picker<T, VEC> p{a, s, row_of<T>(a, row), weight_of(a, best, q.temp, s.table)};
+    const uint32_t listed = mode == ROW_LIST ? a.listed[row] : 0;
+    if (mode == ROW_ALONE || listed > CAP) {
+        pick_alone<T, VEC>(a, row, q, best, s, p);
+        return;
+    }
+    // The list: whole bins, so a token's place is its place in the list and what lies before its interval and is not in the list.
+    // Sorted by CAP buckets, as many for each bin: in its bucket a token counts those before it.
+    const int n = (int) listed;
+    int lo[4], skip[4], bins = 0;                        // skip: bins of the intervals before
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const bool is = k < plan.n;
+        lo[k] = is ? plan.lo[k] : BINS;
+        skip[k] = bins;
+        bins += is ? plan.hi[k] - plan.lo[k] + 1 : 0;
+    }
+    const int per = CAP / bins;
+    const float scale = p.w.cf * BIN_OCT;
+    auto bucket_of = [&](uint64_t token) {
+        const float l = key_value((uint32_t) (token >> 32));
+        const int b = p.w.bin(l);
+        int v = 0;
+#pragma unroll
+        for (int k = 1; k < 4; ++k) v = b >= lo[k] ? k : v;
+        const float in = l == p.w.m ? 0.0f : fminf((p.w.m - l) * scale, (float) (BINS - 1)) - (float) b;
+        const int at = b - (v == 0 ? lo[0] : v == 1 ? lo[1] : v == 2 ? lo[2] : lo[3]) + (v == 0 ? skip[0] : v == 1 ? skip[1] : v == 2 ? skip[2] : skip[3]);
+        return min(at * per + min((int) (fmaxf(in, 0.0f) * (float) per), per - 1), CAP - 1);
     };
-    if (top_p > 0.0f && top_p < 1.0f) {
-        const Place q = p.locate(BY_MASS, share((double) top_p, of_k));
-        if (q.count < end.count) end = q;
+    constexpr int E = CAP / PT;
+    for (int i = tid; i < CAP; i += PT) s.bucket[i] = 0;
+    __syncthreads();
+    uint64_t mine[E];
+    int to[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+        const int i = tid + j * PT;
+        mine[j] = i < n ? a.list[(size_t) row * CAP + i] : 0;
+        to[j] = i < n ? bucket_of(mine[j]) : 0;
+        if (i < n) atomicAdd(&s.bucket[to[j]], 1u);
     }
-    if (min_p > 1.0f) end = Place{p.w.fixed(p.w.m), 1, best};            // the first alone
-    else if (min_p > 0.0f) {
-        // the lowest key whose weight is min_p or more (the largest logit's, if none is): halving, every thread the same
-        uint32_t hi = (uint32_t) (best >> 32), lo = KEY_NONE;             // hi passes or is the largest, lo does not
-        while (hi - lo > 1) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (p.w.w(key_value(mid)) >= (double) min_p) hi = mid;
-            else lo = mid;
-        }
-        // where the last token kept so far passes, nothing is cut
-        const bool binds = end.token == 0 || (uint32_t) (end.token >> 32) < hi;
-        if (binds) {
-            const Place q = p.locate(BY_KEY, hi);
-            if (q.count < end.count) end = q;
-        }
+    __syncthreads();
+    uint32_t size[E], own = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+        size[j] = s.bucket[E * tid + j];
+        own += size[j];
     }
-    const float u = a.u[row];
-    const Place q = p.locate(BY_MASS, share(u > 0.0f ? fmin((double) u, 1.0) : 0.0, end.mass));
+    uint32_t start = block_sums(Sum{0, own}, s.part).count - own;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+        s.bucket[E * tid + j] = start;                   // of the bucket; then, as tokens come, its end
+        start += size[j];
+    }
+    __syncthreads();
+    int in_list[4];                                      // tokens of the list before each interval
+#pragma unroll
+    for (int k = 0; k < 4; ++k) in_list[k] = lo[k] < BINS ? (int) s.bucket[skip[k] * per] : CAP;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+        if (tid + j * PT < n) s.unsorted[atomicAdd(&s.bucket[to[j]], 1u)] = mine[j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+        if (tid + j * PT < n) {
+            const int first = to[j] > 0 ? (int) s.bucket[to[j] - 1] : 0, last = (int) s.bucket[to[j]];
+            int place = first;
+            for (int i = first; i < last; ++i) place += s.unsorted[i] > mine[j] ? 1 : 0;
+            s.token[place] = mine[j];
+        }
+    __syncthreads();
+    constexpr int Q = CAP / PT;
+    uint64_t m[Q], sum = 0;
+#pragma unroll
+    for (int j = 0; j < Q; ++j) {
+        const int i = Q * tid + j;
+        m[j] = i < n ? p.w.fixed(key_value((uint32_t) (s.token[i] >> 32))) : 0;
+        sum += m[j];
+    }
+    uint64_t at = block_sums(Sum{sum, 0}, s.part).mass - sum;
+    uint32_t count[Q];
+#pragma unroll
+    for (int j = 0; j < Q; ++j) {
+        const int i = Q * tid + j;
+        at += m[j];
+        int v = 0;                                       // the token's interval: the last that starts at or before it
+#pragma unroll
+        for (int k = 1; k < 4; ++k) v = (uint32_t) i >= in_list[k] ? k : v;
+        count[j] = (uint32_t) (i + 1 - (v == 0 ? in_list[0] : v == 1 ? in_list[1] : v == 2 ? in_list[2] : in_list[3])) + plan.before_count[v];
+        m[j] = at - plan.list_mass[v] + plan.before_mass[v];
+        if (i < n) s.token_mass[i] = m[j];
+    }
+    // the first of the list for which here(sum, count, i) holds; the last, if none
+    auto first = [&](auto&& here) {
+        if (tid == 0) s.found = n - 1;
+        __syncthreads();
+        int f = n;
+#pragma unroll
+        for (int j = Q - 1; j >= 0; --j)
+            if (Q * tid + j < n && here(m[j], count[j], Q * tid + j)) f = Q * tid + j;
+        if (f < n) atomicMin(&s.found, f);
+        __syncthreads();
+        const int i = s.found;
+        __syncthreads();
+        return i;
+    };
+    // What is left, as a sum: of two places the one with the smaller sum comes first.  Counted only: the list begins with the row's
+    // first token and has all that top-k leaves.
+    __syncthreads();
+    uint64_t end = q.counts_only() ? s.token_mass[n - 1] : plan.mass;
+    if (q.k >= 1 && (uint32_t) q.k < plan.count) end = s.token_mass[first([&](uint64_t, uint32_t c, int) { return c >= (uint32_t) q.k; })];
+    const uint64_t of_k = end;
+    if (q.cut_p()) {
+        const uint64_t t = share((double) q.top_p, of_k), x = s.token_mass[first([&](uint64_t y, uint32_t, int) { return y >= t; })];
+        end = x < end ? x : end;
+    }
+    if (q.cut_m() && (q.counts_only() || plan.m0 >= 0)) {
+        // of the bins in which min-p ends, those that pass; the bins before pass, the bins behind do not
+        const int m0 = q.counts_only() ? 0 : plan.m0, m1 = q.counts_only() ? BINS - 1 : plan.m1;
+        Sum pass{0, 0};
+#pragma unroll
+        for (int j = 0; j < Q; ++j) {
+            if (Q * tid + j >= n) continue;
+            const float l = key_value((uint32_t) (s.token[Q * tid + j] >> 32));
+            const int b = p.w.bin(l);
+            if (b >= m0 && b <= m1 && p.w.w(l) >= (double) q.min_p) pass.mass += p.w.fixed(l);
+        }
+        pass = block_sums(pass, s.part);
+        if (tid == PT - 1) s.part[0] = pass;
+        __syncthreads();
+        const uint64_t x = s.part[0].mass + (q.counts_only() ? 0 : plan.m_mass);
+        __syncthreads();
+        end = x < end ? x : end;
+    }
+    const uint64_t t = share(q.u, end);
+    const int i = first([&](uint64_t x, uint32_t, int) { return x >= t; });
     if (tid == 0) {
-        a.ids[row] = (int) ~(uint32_t) q.token;
-        if (a.probs) a.probs[row] = (float) (ldexp(p.w.w(key_value((uint32_t) (q.token >> 32))), a.F) / (double) end.mass);
+        a.ids[row] = (int) ~(uint32_t) s.token[i];
+        if (a.probs) a.probs[row] = (float) (p.w.scaled(key_value((uint32_t) (s.token[i] >> 32)), a.F) / (double) end);
     }
 }
 
@@ -527,18 +979,31 @@ int launch(const SampleArgs& a, void* stream) {
     WZY_LAUNCH_CHECK();
     sample_hist_kernel<T, VEC><<<grid, ST, 0, as_stream(stream)>>>(a);
     WZY_LAUNCH_CHECK();
+    sample_plan_kernel<<<a.rows, ST, 0, as_stream(stream)>>>(a);
+    WZY_LAUNCH_CHECK();
+    sample_gather_kernel<T, VEC><<<grid, ST, 0, as_stream(stream)>>>(a);
+    WZY_LAUNCH_CHECK();
     sample_pick_kernel<T, VEC><<<a.rows, PT, 0, as_stream(stream)>>>(a);
     WZY_LAUNCH_CHECK();
     return WZY_OK;
 }
 constexpr int MAX_VOCAB = 1 << 22, MAX_ROWS = 65535;
+// slices: enough of them for all CUs, and where there are many rows larger ones, with fewer histograms to add
 size_t space(int rows, int vocab, SampleArgs* a, void* base, size_t cap) {
-    const int slices = pg_div_up(vocab, SLICE);
+    const int units = pg_div_up(vocab, SLICE), most = std::max(1, 2048 / rows), per = pg_div_up(units, std::min(units, most));
+    const int slices = pg_div_up(units, per);
     Arena w(base, cap);
     uint64_t* const best = w.take<uint64_t>((size_t) rows * slices);
     uint64_t* const mass = w.take<uint64_t>((size_t) rows * BINS);
     uint32_t* const count = w.take<uint32_t>((size_t) rows * BINS);
-    if (a) { a->best = best; a->mass = mass; a->count = count; a->slices = slices; }
+    RowPlan* const plan = w.take<RowPlan>((size_t) rows);
+    uint32_t* const listed = w.take<uint32_t>((size_t) rows);
+    uint64_t* const list = w.take<uint64_t>((size_t) rows * CAP);
+    if (a) {
+        a->best = best; a->mass = mass; a->count = count; a->plan = plan; a->listed = listed; a->list = list;
+        a->slices = slices;
+        a->units = per;
+    }
     return w.off;
 }
 }  // namespace
@@ -566,7 +1031,7 @@ extern "C" int wzy_sample(const void* logits, int type, int64_t ld, int rows, in
                 workspace_bytes, workspace, want);
     a.logits = logits; a.ld = ld; a.rows = rows; a.vocab = vocab;
     a.temp = temp; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p; a.u = u; a.ids = ids; a.probs = probs;
-    a.F = 62;
+    a.F = 51;
     while (a.F > 40 && (int64_t) vocab > (1ll << (62 - a.F))) --a.F;
     const bool vec = (uintptr_t) logits % 16 == 0 && ld * n % 16 == 0;
     return mx_with_type(type, [&](auto t) { return vec ? launch<t(), true>(a, stream) : launch<t(), false>(a, stream); });
