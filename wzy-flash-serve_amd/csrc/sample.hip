@@ -7,7 +7,9 @@
 //   sample_max     a slice of a row a workgroup: its best token
 //   sample_hist    the same slices: x against the row's best, histogram in LDS, added to the row's
 //   sample_plan    a workgroup a row: which bins are wanted.  (The row's last workgroup of sample_hist, told by a counter, could do it:
-//                  the fences between their atomics and its loads took 200 us at 256 rows.)
+//                  the fences between their atomics and its loads took 200 us at 256 rows.)  Rows with a small top-k need no
+//                  histogram: sample_max left the largest token of every 32, whose k-th largest bounds the row's, and the few
+//                  groups above it are all that has to be read again; they get their token here
 //   sample_gather  the slices again: tokens of those bins to the row's list
 //   sample_pick    a workgroup a row: the list sorted, sums, places
 // Rows whose bins hold more than CAP tokens (thousands of equal logits) are done by sample_pick alone, from the row.
@@ -23,6 +25,7 @@ using namespace wzy;
 namespace {
 constexpr int ST = 256, PER = 32, SLICE = ST * PER;      // sample_max, sample_hist
 constexpr int PT = 1024, CAP = 4096;                     // sample_pick; tokens gathered at most
+constexpr int GROUP_K = CAP / PER;                       // top-k up to which the groups' largest tokens say what to gather
 constexpr int SMALL_K = 2048;                            // top-k up to which all that it leaves is gathered
 constexpr int BINS = 1024;                               // 64 octaves of w
 constexpr float BIN_OCT = 16.0f;
@@ -30,9 +33,9 @@ constexpr float GREEDY = 1e-5f;
 constexpr uint32_t KEY_NONE = 0x007FFFFFu;               // order key of -infinity
 
 // What sample_plan leaves to the next kernels.
-enum { ROW_FIRST, ROW_LIST, ROW_ALONE };
+enum { ROW_DONE, ROW_LIST, ROW_ALONE };
 struct RowPlan {
-    int mode;                                            // the best token (or none at all); a list; neither
+    int mode;                                            // the row has its token; a list; neither
     int n, lo[4], hi[4];                                 // intervals of bins that are gathered, in order
     float most[4], least[4];                             // the logits at their ends
     uint64_t before_mass[4], list_mass[4];               // sums before each, of the row and of the list
@@ -59,6 +62,8 @@ struct SampleArgs {
     RowPlan* plan;                                       // [rows]
     uint32_t* listed;                                    // [rows] tokens in the list
     uint64_t* list;                                      // [rows x CAP]
+    uint32_t* group;                                     // [rows x groups] each thread's largest key of a unit (null: no row wants them)
+    int groups;
 };
 
 // a logit's bits in numeric order (both zeros alike); a NaN as -infinity
@@ -184,8 +189,11 @@ __global__ void __launch_bounds__(ST) sample_max_kernel(SampleArgs a) {
     if (slice == 0 && tid == 0) a.listed[row] = 0;
     uint64_t b = 0;
     each_unit<T, VEC>(a, row, slice, [&](const float (&x)[PER], int from) {
+        uint64_t g = 0;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) b = max_u64(b, order_u64(x[j], element<T, VEC>(from, j)));
+        for (int j = 0; j < PER; ++j) g = max_u64(g, order_u64(x[j], element<T, VEC>(from, j)));
+        if (a.group) a.group[(size_t) row * a.groups + from / PER + tid] = (uint32_t) (g >> 32);
+        b = max_u64(b, g);
     });
     b = wave_max_u64(b);
     if ((tid & 63) == 0) s_best[tid >> 6] = b;
@@ -271,6 +279,7 @@ struct Params {
     WZY_DEV bool cut_m() const { return min_p > 0.0f; }
     WZY_DEV bool counts_only() const { return k >= 1 && k <= SMALL_K; }
     WZY_DEV bool counts() const { return k >= 1; }
+    WZY_DEV bool from_groups() const { return k >= 1 && k <= GROUP_K; }
 };
 
 // The bins that the places may lie in.  A place that hangs on one inside a bin is bracketed by the bin's ends.  One wave; lane 0
@@ -397,7 +406,7 @@ __global__ void __launch_bounds__(ST) sample_hist_kernel(SampleArgs a) {
         s_count[i] = 0;
     }
     const uint64_t best = row_best<ST>(a, row, s_best);          // its barriers cover what was stored before
-    if (q.first || (uint32_t) (best >> 32) == KEY_NONE) return;
+    if (q.first || q.from_groups() || (uint32_t) (best >> 32) == KEY_NONE) return;
     const Weight w = weight_of(a, best, q.temp, s_table);
     // Tokens of the last bin (w 0, and many of a row may be there) and what is not a number go to slots that are not looked at, a lane
     // one: no branch an element.
@@ -426,70 +435,6 @@ __global__ void __launch_bounds__(ST) sample_hist_kernel(SampleArgs a) {
         if (s_mass[i]) atomicAdd((unsigned long long*) a.mass + (size_t) row * BINS + i, s_mass[i]);
         if (s_count[i]) atomicAdd(a.count + (size_t) row * BINS + i, s_count[i]);
     }
-}
-
-__global__ void __launch_bounds__(ST) sample_plan_kernel(SampleArgs a) {
-    __shared__ uint64_t s_mass[BINS], s_best[ST / 64];
-    __shared__ uint32_t s_count[BINS];
-    __shared__ Sum s_part[ST / 64];
-    __shared__ RowPlan s_plan;
-    const int row = blockIdx.x, tid = threadIdx.x;
-    const Params q(a, row);
-    constexpr int Q = BINS / ST;
-    Sum v[Q], all{0, 0};
-#pragma unroll
-    for (int i = 0; i < Q; ++i) {
-        v[i] = Sum{a.mass[(size_t) row * BINS + Q * tid + i], a.count[(size_t) row * BINS + Q * tid + i]};
-        all.mass += v[i].mass;
-        all.count += v[i].count;
-    }
-    const uint64_t best = row_best<ST>(a, row, s_best);
-    if (q.first || (uint32_t) (best >> 32) == KEY_NONE) {
-        if (tid == 0) a.plan[row].mode = ROW_FIRST;
-        return;
-    }
-    Sum at = block_sums(all, s_part);
-    at.mass -= all.mass;
-    at.count -= all.count;
-#pragma unroll
-    for (int i = 0; i < Q; ++i) {
-        at.mass += v[i].mass;
-        at.count += v[i].count;
-        s_mass[Q * tid + i] = at.mass;
-        s_count[Q * tid + i] = at.count;
-    }
-    __syncthreads();
-    if (tid >= 64) return;
-    plan_row(q, s_mass, s_count, s_plan);
-    wave_lds_sync();
-    // the intervals' ends as logits, a lane an end: the bin falls as the key rises
-    if (tid < 2 * s_plan.n) {
-        const Weight w = weight_of(a, best, q.temp, nullptr);
-        const int j = tid >> 1;
-        uint32_t lo = KEY_NONE, hi = (uint32_t) (best >> 32) + 1;
-        if (tid & 1) {                                          // the largest whose bin is lo or more
-            const int b = s_plan.lo[j];
-            while (hi - lo > 1) {
-                const uint32_t mid = lo + (hi - lo) / 2;
-                if (w.bin(key_value(mid)) >= b) lo = mid;
-                else hi = mid;
-            }
-            s_plan.most[j] = key_value(lo);
-        } else {                                                // the least whose bin is hi or less
-            const int b = s_plan.hi[j];
-            --hi;                                               // the best one's is 0
-            while (hi - lo > 1) {
-                const uint32_t mid = lo + (hi - lo) / 2;
-                if (w.bin(key_value(mid)) <= b) hi = mid;
-                else lo = mid;
-            }
-            s_plan.least[j] = key_value(hi);
-        }
-    }
-    wave_lds_sync();
-    const uint32_t* const from = (const uint32_t*) &s_plan;
-    uint32_t* const to = (uint32_t*) (a.plan + row);
-    for (int i = tid; i < (int) (sizeof(RowPlan) / 4); i += 64) to[i] = from[i];
 }
 
 template <int T, bool VEC>
@@ -764,6 +709,85 @@ struct Picker {
         }
         return among(mode, target);
     }
+    // The places in s.token[0 .. n - 1], sorted, and the answer.  plan: whole bins, where the sums before an interval are the row's;
+    // null: the row's first tokens, all that top-k leaves among them.
+    WZY_DEV void finish(const Params& q, int r, int n, const RowPlan* plan, const int (&in_list)[4]) {
+        const int tid = threadIdx.x;
+        const bool all = !plan || q.counts_only();
+        constexpr int Q = CAP / PT;
+        uint64_t m[Q], sum = 0;
+#pragma unroll
+        for (int j = 0; j < Q; ++j) {
+            const int i = Q * tid + j;
+            m[j] = i < n ? w.fixed(key_value((uint32_t) (s.token[i] >> 32))) : 0;
+            sum += m[j];
+        }
+        uint64_t at = block_sums(Sum{sum, 0}, s.part).mass - sum;
+        uint32_t count[Q];
+#pragma unroll
+        for (int j = 0; j < Q; ++j) {
+            const int i = Q * tid + j;
+            at += m[j];
+            count[j] = (uint32_t) i + 1;
+            m[j] = at;
+            if (plan) {
+                int v = 0;                               // the token's interval: the last that starts at or before it
+#pragma unroll
+                for (int k = 1; k < 4; ++k) v = i >= in_list[k] ? k : v;
+                count[j] = (uint32_t) (i + 1 - (v == 0 ? in_list[0] : v == 1 ? in_list[1] : v == 2 ? in_list[2] : in_list[3])) + plan->before_count[v];
+                m[j] = at - plan->list_mass[v] + plan->before_mass[v];
+            }
+            if (i < n) s.token_mass[i] = m[j];
+        }
+        // the first of the list for which here(sum, count) holds; the last, if none
+        auto first = [&](auto&& here) {
+            if (tid == 0) s.found = n - 1;
+            __syncthreads();
+            int f = n;
+#pragma unroll
+            for (int j = Q - 1; j >= 0; --j)
+                if (Q * tid + j < n && here(m[j], count[j])) f = Q * tid + j;
+            if (f < n) atomicMin(&s.found, f);
+            __syncthreads();
+            const int i = s.found;
+            __syncthreads();
+            return i;
+        };
+        // What is left, as a sum: of two places the one with the smaller sum comes first.
+        __syncthreads();
+        uint64_t end = all ? s.token_mass[n - 1] : plan->mass;
+        if (!plan) end = s.token_mass[min(q.k, n) - 1];
+        else if (q.k >= 1 && (uint32_t) q.k < plan->count) end = s.token_mass[first([&](uint64_t, uint32_t c) { return c >= (uint32_t) q.k; })];
+        const uint64_t of_k = end;
+        if (q.cut_p()) {
+            const uint64_t t = share((double) q.top_p, of_k), x = s.token_mass[first([&](uint64_t y, uint32_t) { return y >= t; })];
+            end = x < end ? x : end;
+        }
+        if (q.cut_m() && (all || plan->m0 >= 0)) {
+            // of the bins in which min-p ends, those that pass; the bins before pass, the bins behind do not
+            const int m0 = all ? 0 : plan->m0, m1 = all ? BINS - 1 : plan->m1;
+            Sum pass{0, 0};
+#pragma unroll
+            for (int j = 0; j < Q; ++j) {
+                if (Q * tid + j >= n) continue;
+                const float l = key_value((uint32_t) (s.token[Q * tid + j] >> 32));
+                const int b = w.bin(l);
+                if (b >= m0 && b <= m1 && w.w(l) >= (double) q.min_p) pass.mass += w.fixed(l);
+            }
+            pass = block_sums(pass, s.part);
+            if (tid == PT - 1) s.part[0] = pass;
+            __syncthreads();
+            const uint64_t x = s.part[0].mass + (all ? 0 : plan->m_mass);
+            __syncthreads();
+            end = x < end ? x : end;
+        }
+        const uint64_t t = share(q.u, end);
+        const int i = first([&](uint64_t x, uint32_t) { return x >= t; });
+        if (tid == 0) {
+            a.ids[r] = (int) ~(uint32_t) s.token[i];
+            if (a.probs) a.probs[r] = (float) (w.scaled(key_value((uint32_t) (s.token[i] >> 32)), a.F) / (double) end);
+        }
+    }
 };
 
 // a row by itself: its histogram, then the places, with a pass over the row for each range that is gathered
@@ -812,6 +836,148 @@ WZY_DEV void pick_alone(const SampleArgs& a, int row, const Params& q, uint64_t 
     }
 }
 
+// Rows with a small top-k, from the groups' largest keys: the k-th largest of those is at most the row's k-th largest, so the tokens
+// at or above it are k or more, and they lie in the groups whose largest is: k groups of PER, and ties.  False: too many of those.
+template <int T, bool VEC>
+WZY_DEV bool pick_from_groups(const SampleArgs& a, int row, const Params& q, PickShared& s, Picker<T, VEC>& p) {
+    const int tid = threadIdx.x;
+    const uint32_t* const g = a.group + (size_t) row * a.groups;
+    // the k-th largest key (0 where there are fewer), 10 or 11 bits at a time
+    uint32_t prefix = 0, k = (uint32_t) q.k;
+    int shift = 32;
+    for (int bits : {11, 11, 10}) {
+        shift -= bits;
+        for (int i = tid; i < 2048; i += PT) s.bucket[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < a.groups; i += PT) {
+            const uint32_t x = g[i];
+            if (shift + bits == 32 || x >> (shift + bits) == prefix) atomicAdd(&s.bucket[2047 - (x >> shift & ((1u << bits) - 1))], 1u);
+        }
+        __syncthreads();
+        const uint32_t c0 = s.bucket[2 * tid], c1 = s.bucket[2 * tid + 1];
+        const uint32_t up = block_sums(Sum{0, c0 + c1}, s.part).count, b = up - c0 - c1;
+        if (tid == 0) s.found = -1;
+        __syncthreads();
+        if (b < k && up >= k) {
+            s.found = b + c0 >= k ? 2 * tid : 2 * tid + 1;
+            s.n = b + c0 >= k ? b : b + c0;
+        }
+        __syncthreads();
+        if (s.found < 0) {                               // fewer groups than k: all of them
+            prefix = 0;
+            shift = 0;
+            __syncthreads();
+            break;
+        }
+        prefix = prefix << bits | (uint32_t) (2047 - s.found);
+        k -= s.n;
+        __syncthreads();
+    }
+    const uint32_t least = max(prefix, KEY_NONE + 1);
+    // the groups, then their tokens, a thread a token at a time
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    for (int i = tid; i < a.groups; i += PT)
+        if (g[i] >= least) {
+            const unsigned at = atomicAdd(&s.n, 1u);
+            if (at < GROUP_K) s.bucket[at] = (uint32_t) i;
+        }
+    __syncthreads();
+    const int groups = (int) s.n;
+    __syncthreads();
+    if (groups > GROUP_K) return false;
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    constexpr int E = !VEC ? 1 : T == WZY_F32 ? 4 : 8;
+    for (int i = tid; i < groups * PER; i += PT) {
+        const int group = (int) s.bucket[i / PER], j = i % PER, e = group / ST * SLICE + ((j / E) * ST + group % ST) * E + j % E;
+        if (e < a.vocab) {
+            const float l = load_logit<T>(p.row, e);
+            if (order_key(l) >= least) s.token[atomicAdd(&s.n, 1u)] = order_u64(l, e);
+        }
+    }
+    __syncthreads();
+    const int n = (int) s.n;                             // GROUP_K * PER = CAP at most
+    if (n <= PT / 4) {
+        // four threads count a token's predecessors
+        const int i = tid >> 2;
+        const uint64_t mine = i < n ? s.token[i] : 0;
+        int before = 0;
+        for (int j = tid & 3; j < n; j += 4) before += s.token[j] > mine ? 1 : 0;
+        before += dpp_i<DPP_XOR1>(before);
+        before += dpp_i<DPP_XOR2>(before);
+        __syncthreads();
+        if (i < n && (tid & 3) == 0) s.token[before] = mine;
+        __syncthreads();
+    } else p.sort(n);
+    const int none[4] = {0, 0, 0, 0};
+    p.finish(q, row, n, nullptr, none);
+    return true;
+}
+
+// Rows that need no list get their token here; for the others, which bins are wanted
+template <int T, bool VEC>
+__global__ void __launch_bounds__(PT) sample_plan_kernel(SampleArgs a) {
+    __shared__ PickShared s;
+    __shared__ RowPlan s_plan;
+    static_assert(BINS == PT, "a thread a bin");
+    const int row = blockIdx.x, tid = threadIdx.x;
+    const Params q(a, row);
+    const Sum own{a.mass[(size_t) row * BINS + tid], a.count[(size_t) row * BINS + tid]};
+    fill_table(s.table);
+    const uint64_t best = row_best<PT>(a, row, s.best);
+    if (q.first || (uint32_t) (best >> 32) == KEY_NONE) {
+        const bool none = (uint32_t) (best >> 32) == KEY_NONE;
+        if (tid == 0) {
+            a.plan[row].mode = ROW_DONE;
+            a.ids[row] = none ? -1 : (int) ~(uint32_t) best;
+            if (a.probs) a.probs[row] = none ? 0.0f : 1.0f;
+        }
+        return;
+    }
+    if (q.from_groups()) {
+        Picker<T, VEC> p{a, s, row_of<T>(a, row), weight_of(a, best, q.temp, s.table)};
+        const bool done = pick_from_groups<T, VEC>(a, row, q, s, p);
+        if (tid == 0) a.plan[row].mode = done ? ROW_DONE : ROW_ALONE;
+        return;
+    }
+    const Sum at = block_sums(own, s.part);
+    s.bin_mass[tid] = at.mass;
+    s.bin_count[tid] = at.count;
+    __syncthreads();
+    if (tid >= 64) return;
+    plan_row(q, s.bin_mass, s.bin_count, s_plan);
+    wave_lds_sync();
+    // the intervals' ends as logits, a lane an end: the bin falls as the key rises
+    if (tid < 2 * s_plan.n) {
+        const Weight w = weight_of(a, best, q.temp, nullptr);
+        const int j = tid >> 1;
+        uint32_t lo = KEY_NONE, hi = (uint32_t) (best >> 32) + 1;
+        if (tid & 1) {                                   // the largest whose bin is lo or more
+            const int b = s_plan.lo[j];
+            while (hi - lo > 1) {
+                const uint32_t mid = lo + (hi - lo) / 2;
+                if (w.bin(key_value(mid)) >= b) lo = mid;
+                else hi = mid;
+            }
+            s_plan.most[j] = key_value(lo);
+        } else {                                         // the least whose bin is hi or less
+            const int b = s_plan.hi[j];
+            --hi;                                        // the best one's is 0
+            while (hi - lo > 1) {
+                const uint32_t mid = lo + (hi - lo) / 2;
+                if (w.bin(key_value(mid)) <= b) hi = mid;
+                else lo = mid;
+            }
+            s_plan.least[j] = key_value(hi);
+        }
+    }
+    wave_lds_sync();
+    const uint32_t* const from = (const uint32_t*) &s_plan;
+    uint32_t* const to = (uint32_t*) (a.plan + row);
+    for (int i = tid; i < (int) (sizeof(RowPlan) / 4); i += 64) to[i] = from[i];
+}
+
 template <int T, bool VEC>
 __global__ void __launch_bounds__(PT) sample_pick_kernel(SampleArgs a) {
     __shared__ PickShared s;
@@ -819,16 +985,9 @@ __global__ void __launch_bounds__(PT) sample_pick_kernel(SampleArgs a) {
     const Params q(a, row);
     const RowPlan& plan = a.plan[row];
     const int mode = plan.mode;
+    if (mode == ROW_DONE) return;
     fill_table(s.table);
     const uint64_t best = row_best<PT>(a, row, s.best);
-    if (mode == ROW_FIRST) {
-        const bool none = (uint32_t) (best >> 32) == KEY_NONE;
-        if (tid == 0) {
-            a.ids[row] = none ? -1 : (int) ~(uint32_t) best;
-            if (a.probs) a.probs[row] = none ? 0.0f : 1.0f;
-        }
-        return;
-    }
     Picker<T, VEC> p{a, s, row_of<T>(a, row), weight_of(a, best, q.temp, s.table)};
     const uint32_t listed = mode == ROW_LIST ? a.listed[row] : 0;
     if (mode == ROW_ALONE || listed > CAP) {
@@ -901,75 +1060,7 @@ __global__ void __launch_bounds__(PT) sample_pick_kernel(SampleArgs a) {
             s.token[place] = mine[j];
         }
     __syncthreads();
-    constexpr int Q = CAP / PT;
-    uint64_t m[Q], sum = 0;
-#pragma unroll
-    for (int j = 0; j < Q; ++j) {
-        const int i = Q * tid + j;
-        m[j] = i < n ? p.w.fixed(key_value((uint32_t) (s.token[i] >> 32))) : 0;
-        sum += m[j];
-    }
-    uint64_t at = block_sums(Sum{sum, 0}, s.part).mass - sum;
-    uint32_t count[Q];
-#pragma unroll
-    for (int j = 0; j < Q; ++j) {
-        const int i = Q * tid + j;
-        at += m[j];
-        int v = 0;                                       // the token's interval: the last that starts at or before it
-#pragma unroll
-        for (int k = 1; k < 4; ++k) v = (uint32_t) i >= in_list[k] ? k : v;
-        count[j] = (uint32_t) (i + 1 - (v == 0 ? in_list[0] : v == 1 ? in_list[1] : v == 2 ? in_list[2] : in_list[3])) + plan.before_count[v];
-        m[j] = at - plan.list_mass[v] + plan.before_mass[v];
-        if (i < n) s.token_mass[i] = m[j];
-    }
-    // the first of the list for which here(sum, count, i) holds; the last, if none
-    auto first = [&](auto&& here) {
-        if (tid == 0) s.found = n - 1;
-        __syncthreads();
-        int f = n;
-#pragma unroll
-        for (int j = Q - 1; j >= 0; --j)
-            if (Q * tid + j < n && here(m[j], count[j], Q * tid + j)) f = Q * tid + j;
-        if (f < n) atomicMin(&s.found, f);
-        __syncthreads();
-        const int i = s.found;
-        __syncthreads();
-        return i;
-    };
-    // What is left, as a sum: of two places the one with the smaller sum comes first.  Counted only: the list begins with the row's
-    // first token and has all that top-k leaves.
-    __syncthreads();
-    uint64_t end = q.counts_only() ? s.token_mass[n - 1] : plan.mass;
-    if (q.k >= 1 && (uint32_t) q.k < plan.count) end = s.token_mass[first([&](uint64_t, uint32_t c, int) { return c >= (uint32_t) q.k; })];
-    const uint64_t of_k = end;
-    if (q.cut_p()) {
-        const uint64_t t = share((double) q.top_p, of_k), x = s.token_mass[first([&](uint64_t y, uint32_t, int) { return y >= t; })];
-        end = x < end ? x : end;
-    }
-    if (q.cut_m() && (q.counts_only() || plan.m0 >= 0)) {
-        // of the bins in which min-p ends, those that pass; the bins before pass, the bins behind do not
-        const int m0 = q.counts_only() ? 0 : plan.m0, m1 = q.counts_only() ? BINS - 1 : plan.m1;
-        Sum pass{0, 0};
-#pragma unroll
-        for (int j = 0; j < Q; ++j) {
-            if (Q * tid + j >= n) continue;
-            const float l = key_value((uint32_t) (s.token[Q * tid + j] >> 32));
-            const int b = p.w.bin(l);
-            if (b >= m0 && b <= m1 && p.w.w(l) >= (double) q.min_p) pass.mass += p.w.fixed(l);
-        }
-        pass = block_sums(pass, s.part);
-        if (tid == PT - 1) s.part[0] = pass;
-        __syncthreads();
-        const uint64_t x = s.part[0].mass + (q.counts_only() ? 0 : plan.m_mass);
-        __syncthreads();
-        end = x < end ? x : end;
-    }
-    const uint64_t t = share(q.u, end);
-    const int i = first([&](uint64_t x, uint32_t, int) { return x >= t; });
-    if (tid == 0) {
-        a.ids[row] = (int) ~(uint32_t) s.token[i];
-        if (a.probs) a.probs[row] = (float) (p.w.scaled(key_value((uint32_t) (s.token[i] >> 32)), a.F) / (double) end);
-    }
+    p.finish(q, row, n, &plan, in_list);
 }
 
 template <int T, bool VEC>
@@ -979,7 +1070,7 @@ int launch(const SampleArgs& a, void* stream) {
     WZY_LAUNCH_CHECK();
     sample_hist_kernel<T, VEC><<<grid, ST, 0, as_stream(stream)>>>(a);
     WZY_LAUNCH_CHECK();
-    sample_plan_kernel<<<a.rows, ST, 0, as_stream(stream)>>>(a);
+    sample_plan_kernel<T, VEC><<<a.rows, PT, 0, as_stream(stream)>>>(a);
     WZY_LAUNCH_CHECK();
     sample_gather_kernel<T, VEC><<<grid, ST, 0, as_stream(stream)>>>(a);
     WZY_LAUNCH_CHECK();
@@ -999,8 +1090,11 @@ size_t space(int rows, int vocab, SampleArgs* a, void* base, size_t cap) {
     RowPlan* const plan = w.take<RowPlan>((size_t) rows);
     uint32_t* const listed = w.take<uint32_t>((size_t) rows);
     uint64_t* const list = w.take<uint64_t>((size_t) rows * CAP);
+    uint32_t* const group = w.take<uint32_t>((size_t) rows * units * ST);
     if (a) {
         a->best = best; a->mass = mass; a->count = count; a->plan = plan; a->listed = listed; a->list = list;
+        a->group = group;
+        a->groups = units * ST;
         a->slices = slices;
         a->units = per;
     }
@@ -1031,6 +1125,7 @@ extern "C" int wzy_sample(const void* logits, int type, int64_t ld, int rows, in
                 workspace_bytes, workspace, want);
     a.logits = logits; a.ld = ld; a.rows = rows; a.vocab = vocab;
     a.temp = temp; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p; a.u = u; a.ids = ids; a.probs = probs;
+    if (!top_k) a.group = nullptr;
     a.F = 51;
     while (a.F > 40 && (int64_t) vocab > (1ll << (62 - a.F))) --a.F;
     const bool vec = (uintptr_t) logits % 16 == 0 && ld * n % 16 == 0;
