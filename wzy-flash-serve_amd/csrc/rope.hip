@@ -7,6 +7,8 @@
 // one thread an angle, and kept in LDS for all heads of the row: at far positions fp32 angles would be off by whole turns.
 // The rows are read and written once, 8 elements (and their partners) a thread where alignment allows 16-byte accesses, a pair
 // a thread elsewhere.  Bound by memory at large sizes, by the launch at one row.
+#include <algorithm>
+
 #include "wzy_paged.h"
 
 using namespace wzy;
@@ -60,98 +62,108 @@ WZY_DEV void store1(void* p, size_t i, float v) {
     else ((uint16_t*) p)[i] = f_to_h16(v);
 }
 
-// One workgroup does rows_block rows: their angles, then all pieces of all heads.  WIDE pieces: 8 elements and, in rotated
-// halves, the 8 they pair with; others: one pair or one element.
+// A piece of a row: WIDE, 8 elements and, in rotated halves, the 8 they pair with; else a pair or one element.
 template <int TI, int TO, bool PAIRS, bool WIDE>
-__global__ void __launch_bounds__(RT) rope_kernel(RopeArgs a) {
-    __shared__ float2 s_cs[ROPE_MAX];
-    const int tid = threadIdx.x, row0 = blockIdx.x * a.rows_block, rows = min(a.rows - row0, a.rows_block);
-    const int half = a.n_rot >> 1;
-    if (a.freqs) {
-        for (int i = tid; i < rows * half; i += RT) {
-            const int r = i / half, j = i - r * half;
-            s_cs[i] = turn((double) a.positions[row0 + r] * a.freqs[j], a.freqs[half]);
-        }
-        __syncthreads();
-    }
-    for (int i = tid; i < rows * a.per_row; i += RT) {
-        const int r = (int) fast_div((uint32_t) i, a.div_row), x = i - r * a.per_row;
-        int h = (int) fast_div((uint32_t) x, a.div_head);
+struct Piece {
+    static constexpr int N = WIDE ? 8 : 1;
+    float u[N], v[N];
+    int row, set, e0, e1, turned;              // first element; its partner's (-1: none); its pair (-1: not turned)
+    int h;
+    WZY_DEV void locate(const RopeArgs& a, int row0, int i) {
+        const int half = a.n_rot >> 1, r = (int) fast_div((uint32_t) i, a.div_row), x = i - r * a.per_row;
+        h = (int) fast_div((uint32_t) x, a.div_head);
         const int piece = x - h * a.per_head;
-        int set = 0;
+        row = row0 + r;
+        set = 0;
         if (a.n_sets > 1) {
             if (h >= a.heads[0]) { h -= a.heads[0]; set = 1; }
             if (set == 1 && h >= a.heads[1]) { h -= a.heads[1]; set = 2; }
         }
-        const int row = row0 + r;
-        const void* const src = set == 0 ? a.in[0].p : set == 1 ? a.in[1].p : a.in[2].p;
+        const bool turn = set < 2 && a.freqs;                  // values are not turned
+        e1 = -1;
+        if constexpr (WIDE && PAIRS) {
+            e0 = 8 * piece;
+            turned = turn && e0 < a.n_rot ? 4 * piece : -1;
+        } else if (piece * N < half) {
+            e0 = WIDE ? 8 * piece : PAIRS ? 2 * piece : piece;
+            e1 = PAIRS ? e0 + 1 : e0 + half;
+            turned = turn ? N * piece : -1;
+        } else {                                               // behind the pairs
+            e0 = a.n_rot + N * piece - half;
+            turned = -1;
+        }
+    }
+    WZY_DEV void load(const RopeArgs& a) {
+        const View& in = set == 0 ? a.in[0] : set == 1 ? a.in[1] : a.in[2];
+        const size_t at = (size_t) row * in.ld + (size_t) h * in.ldh;
+        if constexpr (WIDE) {
+            load8<TI>(in.p, at + e0, u);
+            if (!PAIRS && e1 >= 0) load8<TI>(in.p, at + e1, v);
+        } else {
+            u[0] = load1<TI>(in.p, at + e0);
+            if (e1 >= 0) v[0] = load1<TI>(in.p, at + e1);
+        }
+    }
+    static WZY_DEV void turn(float& x, float& y, float2 t) {
+        const float p = x * t.x - y * t.y;
+        y = y * t.x + x * t.y;
+        x = p;
+    }
+    WZY_DEV void store(const RopeArgs& a, const float2* cs) {
+        if (turned >= 0) {
+            if constexpr (WIDE && PAIRS) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) turn(u[2 * j], u[2 * j + 1], cs[turned + j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) turn(u[j], v[j], cs[turned + j]);
+            }
+        }
         void* const dst = (void*) (set == 0 ? a.out[0].p : set == 1 ? a.out[1].p : a.out[2].p);
-        const size_t at = (size_t) row * (set == 0 ? a.in[0].ld : set == 1 ? a.in[1].ld : a.in[2].ld) +
-                          (size_t) h * (set == 0 ? a.in[0].ldh : set == 1 ? a.in[1].ldh : a.in[2].ldh);
         size_t to;
         if (set == 0) to = (size_t) row * a.out[0].ld + (size_t) h * a.out[0].ldh;
         else {
             const int slot = a.slots[row];
-            if (slot < 0 || slot >= a.n_cells) continue;
+            if (slot < 0 || slot >= a.n_cells) return;
             to = (size_t) (slot >> a.lp) * a.ld_page + (size_t) (slot & ((1 << a.lp) - 1)) * a.out[1].ld + (size_t) h * a.out[1].ldh;
         }
-        const float2* const cs = s_cs + r * half;
-        const int n_rot = set < 2 && a.freqs ? a.n_rot : 0;        // values are not turned
         if constexpr (WIDE) {
-            // pieces: of a turned half layout first the pairs of eights, then what is left, then (values) what the pairs covered
-            float u[8], v[8];
-            if constexpr (!PAIRS) {
-                if (piece < half >> 3) {
-                    const int e = 8 * piece;
-                    load8<TI>(src, at + e, u);
-                    load8<TI>(src, at + half + e, v);
-                    if (n_rot) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float2 t = cs[e + j];
-                            const float p = u[j] * t.x - v[j] * t.y, q = v[j] * t.x + u[j] * t.y;
-                            u[j] = p;
-                            v[j] = q;
-                        }
-                    }
-                    store8<TO>(dst, to + e, u);
-                    store8<TO>(dst, to + half + e, v);
-                } else {
-                    const int e = a.n_rot + 8 * (piece - (half >> 3));
-                    load8<TI>(src, at + e, u);
-                    store8<TO>(dst, to + e, u);
-                }
-            } else {
-                const int e = 8 * piece;
-                load8<TI>(src, at + e, u);
-                if (e < n_rot) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 t = cs[(e >> 1) + j];
-                        const float p = u[2 * j] * t.x - u[2 * j + 1] * t.y, q = u[2 * j + 1] * t.x + u[2 * j] * t.y;
-                        u[2 * j] = p;
-                        u[2 * j + 1] = q;
-                    }
-                }
-                store8<TO>(dst, to + e, u);
-            }
+            store8<TO>(dst, to + e0, u);
+            if (!PAIRS && e1 >= 0) store8<TO>(dst, to + e1, v);
         } else {
-            if (piece < half) {
-                const int e0 = PAIRS ? 2 * piece : piece, e1 = PAIRS ? e0 + 1 : piece + half;
-                float u = load1<TI>(src, at + e0), v = load1<TI>(src, at + e1);
-                if (n_rot) {
-                    const float2 t = cs[piece];
-                    const float p = u * t.x - v * t.y;
-                    v = v * t.x + u * t.y;
-                    u = p;
-                }
-                store1<TO>(dst, to + e0, u);
-                store1<TO>(dst, to + e1, v);
-            } else {
-                const int e = a.n_rot + piece - half;
-                store1<TO>(dst, to + e, load1<TI>(src, at + e));
-            }
+            store1<TO>(dst, to + e0, u[0]);
+            if (e1 >= 0) store1<TO>(dst, to + e1, v[0]);
         }
+    }
+};
+
+// One workgroup does rows_block rows, or blockIdx.y's share of one: a thread's first piece is on its way while the angles are made.
+template <int TI, int TO, bool PAIRS, bool WIDE>
+__global__ void __launch_bounds__(RT) rope_kernel(RopeArgs a) {
+    __shared__ float2 s_cs[ROPE_MAX];
+    const int tid = threadIdx.x, row0 = blockIdx.x * a.rows_block, rows = min(a.rows - row0, a.rows_block);
+    const int half = a.n_rot >> 1, pieces = rows * a.per_row, step = RT * (int) gridDim.y;
+    Piece<TI, TO, PAIRS, WIDE> p;
+    int i = (int) blockIdx.y * RT + tid;
+    const bool any = i < pieces;
+    if (any) {
+        p.locate(a, row0, i);
+        p.load(a);
+    }
+    if (a.freqs) {
+        for (int k = tid; k < rows * half; k += RT) {
+            const int r = k / half, j = k - r * half;
+            s_cs[k] = turn((double) a.positions[row0 + r] * a.freqs[j], a.freqs[half]);
+        }
+        __syncthreads();
+    }
+    if (!any) return;
+    while (true) {
+        p.store(a, s_cs + (p.row - row0) * half);
+        i += step;
+        if (i >= pieces) return;
+        p.locate(a, row0, i);
+        p.load(a);
     }
 }
 
@@ -198,7 +210,9 @@ int launch(RopeArgs a, bool pairs, bool wide, void* stream) {
     int rb = 1;
     while (rb * a.per_row < 4 * RT && 2 * rb * half <= ROPE_MAX && a.rows / (2 * rb) >= 512) rb *= 2;
     a.rows_block = rb;
-    const int grid = (a.rows + rb - 1) / rb;
+    // few rows: a row's pieces to several workgroups, each with angles of its own
+    const int blocks = (a.rows + rb - 1) / rb, share = blocks >= 512 ? 1 : std::min((a.per_row * rb + RT - 1) / RT, 512 / blocks);
+    const dim3 grid((unsigned) blocks, (unsigned) share);
     const auto st = as_stream(stream);
     if (pairs && wide) rope_kernel<TI, TO, true, true><<<grid, RT, 0, st>>>(a);
     else if (pairs) rope_kernel<TI, TO, true, false><<<grid, RT, 0, st>>>(a);
