@@ -12,6 +12,8 @@
 // Rows are (token, head of the group) pairs of one key head, so a group's heads share every byte of K and V.
 //   narrow  up to 32 rows: the waves of a workgroup take every fourth block of 32 keys each, through buffers of their own,
 //           with no barrier until their results are joined
+//   middle  up to 64 rows, where no request of the step has more (verify windows): two waves share a block, the two pairs take
+//           every other one
 //   wide    128 rows, 32 a wave: the workgroup's waves share each block
 // The maximum follows the scores only when one has come 2^8 above it, so most blocks leave the accumulators alone; weights
 // then reach 2^8, and in fp16, whose numbers end at 2^-24, all are taken 2^6 larger.
@@ -80,6 +82,10 @@ WZY_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memor
 WZY_DEV void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 // this wave's loads have landed and its LDS reads are done; then all waves meet
 WZY_DEV void wait_all_and_meet() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// this wave's loads but the last N have landed; then all waves meet
+template <int N>
+WZY_DEV void wait_loads_and_meet() { asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory"); }
+WZY_DEV void wait_lds_and_meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 WZY_DEV const char* uniform(const char* p) {
     const uint64_t b = (uint64_t) (uintptr_t) p;
     return (const char*) (uintptr_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (b >> 32)) << 32 |
@@ -316,6 +322,38 @@ WZY_DEV char* out_row(const AttnArgs& a, const TileCtx& t, int row) {
     return a.out + (int64_t) (t.it.q0 + token) * a.ldo + (int64_t) (t.head * a.g + row - token * a.g) * a.ldo_head;
 }
 
+// A request that is not served: all its rows become 0.
+template <int HD>
+WZY_DEV void zero_rows(const AttnArgs& a, const TileCtx& t) {
+    for (int i = threadIdx.x; i < t.it.n_new * a.g * (HD / 8); i += 256) {
+        const int row = i / (HD / 8);
+        *(v4w_t*) (out_row(a, t, row) + 16 * (i % (HD / 8))) = v4w_t{0, 0, 0, 0};
+    }
+}
+// A lane's results: its row's columns in 16-byte (a part: fp32) or 8-byte pieces
+template <int HD, int T>
+WZY_DEV void put_row(const AttnArgs& a, const TileCtx& t, const Wave<HD, T>& w, float l, int lane, int tile_rows) {
+    if (w.row >= w.rows) return;
+    if (t.it.part < 0) {
+        const float n = l != 0.0f ? 1.0f / l : 0.0f;
+        char* const p = out_row(a, t, w.row) + 8 * (lane >> 5);
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *(uint2*) (p + 64 * d + 16 * i) = make_uint2(pack2<T>(w.o[d][4 * i] * n, w.o[d][4 * i + 1] * n),
+                                                             pack2<T>(w.o[d][4 * i + 2] * n, w.o[d][4 * i + 3] * n));
+    } else {
+        const size_t at = ((size_t) t.it.part * a.kvh + t.head) * tile_rows + (w.row - t.it.row0);
+        float4* const p = (float4*) (a.part_o + at * HD) + (lane >> 5);
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[8 * d + 2 * i] = make_float4(w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]);
+        if (lane < 32) a.part_ml[at] = make_float2(w.m, l);
+    }
+}
+
 template <int HD, int T>
 __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
     using BK = Block<HD, false>;
@@ -327,11 +365,8 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     TileCtx t;
     if (!tile_ctx(a, 0, t)) return;
-    if (t.it.lo >= t.it.hi) {                                           // not served: all its rows become 0
-        for (int i = tid; i < t.it.n_new * a.g * (HD / 8); i += 256) {
-            const int row = i / (HD / 8);
-            *(v4w_t*) (out_row(a, t, row) + 16 * (i % (HD / 8))) = v4w_t{0, 0, 0, 0};
-        }
+    if (t.it.lo >= t.it.hi) {
+        zero_rows<HD>(a, t);
         return;
     }
     Wave<HD, T> w;
@@ -402,11 +437,94 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
             const float n = l != 0.0f ? 1.0f / l : 0.0f;
             *(uint2*) (out_row(a, t, row) + 8 * col) = make_uint2(pack2<T>(o.x * n, o.y * n), pack2<T>(o.z * n, o.w * n));
         } else {
-            const size_t at = ((size_t) t.it.part * a.kvh + t.head) * PG_NARROW + row;
+            const size_t at = ((size_t) t.it.part * a.kvh + t.head) * 32 + row;
             ((float4*) (a.part_o + at * HD))[col] = o;
             if (col == 0) a.part_ml[at] = make_float2(m, l);
         }
     }
+}
+
+// Two barriers a block: the first says that V is there and K has been read (the next K's loads start), the second that the next K is
+// there and V has been read.
+template <int HD, int T>
+__global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
+    using BK = Block<HD, false>;
+    using BV = Block<HD, true>;
+    constexpr int BOTH = BK::BYTES + BV::BYTES, MINE = BK::LOADS / 2;
+    __shared__ __align__(1024) char s_buf[2][BOTH];                     // a pair's K and V; then the second pair's results in fp32
+    __shared__ float s_m[64], s_l[64];
+    static_assert(2 * BOTH >= 64 * HD * 4, "a pair's results take the buffers");
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave & 1, pair = wave >> 1;
+    TileCtx t;
+    if (!tile_ctx(a, 0, t)) return;
+    if (t.it.lo >= t.it.hi) {
+        zero_rows<HD>(a, t);
+        return;
+    }
+    Wave<HD, T> w;
+    Loader<HD> ld(a, t, lane);
+    const char* const kb = s_buf[pair];
+    const char* const vb = kb + BK::BYTES;
+    const uint32_t lk = lds_offset(kb), lv = lk + BK::BYTES;
+    const int first = t.it.lo >> 5, end = (t.it.hi + 31) >> 5;
+    int b = first + pair;
+    if (b < end) {
+        ld.at(b);
+        ld.template issue<false, MINE>(lk, half * MINE);
+        ld.template issue<true, MINE>(lv, half * MINE);
+    }
+    w.start(a, t, 32 * half, lane);
+    wait_loads<0>();
+    // both pairs go round as often as the first has blocks; where the second has one fewer, it meets the first's last time
+    const int rounds = (end - first + 1) / 2, mine = (end - first + 1 - pair) / 2;
+    for (int n = rounds - mine; n < rounds; ++n, b += 2) {
+        const bool more = b + 2 < end;
+        wait_loads_and_meet<MINE>();                                    // K is there; V, whose loads are younger, may be on its way
+        const v16f_t s = w.scores(kb);
+        wait_all_and_meet();
+        if (more) {
+            ld.at(b + 2);
+            ld.template issue<false, MINE>(lk, half * MINE);
+        }
+        v4w_t p[2];
+        w.weights(a, b, lane, s, p);
+        w.add(vb, p);
+        if (n + 1 < rounds || mine < rounds) wait_lds_and_meet();
+        if (more) ld.template issue<true, MINE>(lv, half * MINE);
+    }
+    if (mine < rounds) {
+        wait_all_and_meet();
+        wait_all_and_meet();
+    }
+    w.l = half_sum(w.l);
+    wait_all_and_meet();                                                // the buffers have been read
+    float4* const r = (float4*) (&s_buf[0][0] + half * 32 * HD * 4);
+    if (pair == 1) {
+        if (lane < 32) {
+            s_m[32 * half + lane] = w.m;
+            s_l[32 * half + lane] = w.l;
+        }
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[(4 * d + i) * 64 + lane] = make_float4(w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]);
+    }
+    __syncthreads();
+    if (pair == 1) return;
+    const float m1 = s_m[32 * half + (lane & 31)], l1 = s_l[32 * half + (lane & 31)], m = fmaxf(w.m, m1);
+    const float f0 = w.l != 0.0f ? __builtin_amdgcn_exp2f(w.m - m) : 0.0f, f1 = l1 != 0.0f ? __builtin_amdgcn_exp2f(m1 - m) : 0.0f;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 x = r[(4 * d + i) * 64 + lane];
+            w.o[d][4 * i] = w.o[d][4 * i] * f0 + x.x * f1;
+            w.o[d][4 * i + 1] = w.o[d][4 * i + 1] * f0 + x.y * f1;
+            w.o[d][4 * i + 2] = w.o[d][4 * i + 2] * f0 + x.z * f1;
+            w.o[d][4 * i + 3] = w.o[d][4 * i + 3] * f0 + x.w * f1;
+        }
+    w.m = m;
+    put_row<HD, T>(a, t, w, w.l * f0 + l1 * f1, lane, 64);
 }
 
 template <int HD, int T>
@@ -449,32 +567,14 @@ __global__ void __launch_bounds__(256, 2) paged_wide_kernel(AttnArgs a) {
         w.add(s_buf[buf] + BK::BYTES, p);
     }
     for (; b < end; ++b, buf ^= 1) next();
-    const float l = half_sum(w.l);
-    if (w.row >= w.rows) return;
-    if (t.it.part < 0) {
-        const float n = l != 0.0f ? 1.0f / l : 0.0f;
-        char* const p = out_row(a, t, w.row) + 8 * (lane >> 5);
-#pragma unroll
-        for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *(uint2*) (p + 64 * d + 16 * i) = make_uint2(pack2<T>(w.o[d][4 * i] * n, w.o[d][4 * i + 1] * n),
-                                                             pack2<T>(w.o[d][4 * i + 2] * n, w.o[d][4 * i + 3] * n));
-    } else {
-        const size_t at = ((size_t) t.it.part * a.kvh + t.head) * PG_WIDE + (w.row - t.it.row0);
-        float4* const p = (float4*) (a.part_o + at * HD) + (lane >> 5);
-#pragma unroll
-        for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[8 * d + 2 * i] = make_float4(w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]);
-        if (lane < 32) a.part_ml[at] = make_float2(w.m, l);
-    }
+    put_row<HD, T>(a, t, w, half_sum(w.l), lane, PG_WIDE);
 }
 
 // Parts of a tile joined.  HD / 4 lanes hold a row; of a workgroup's groups of lanes, several take one row's parts in turn where
 // there are many, so that all of a row's loads are under way at once.
 struct MergeArgs {
     unsigned blocks;                         // of narrow tiles
+    int narrow;                              // rows of a narrow tile
     int rows_y[2], at[2], parts[2];          // workgroups a tile, first entry, parts: narrow, wide
     const float* wide_o;
     const float2* wide_ml;
@@ -485,7 +585,7 @@ __global__ void __launch_bounds__(512) paged_merge_kernel(AttnArgs a, MergeArgs 
     __shared__ float4 s_o[512];
     __shared__ float2 s_ml[GROUPS];
     // narrow tiles' workgroups first, by rows_y of them a tile; then wide ones'
-    const int kind = blockIdx.x >= g.blocks ? 1 : 0, rows_y = g.rows_y[kind], ROWS = kind ? PG_WIDE : PG_NARROW;
+    const int kind = blockIdx.x >= g.blocks ? 1 : 0, rows_y = g.rows_y[kind], ROWS = kind ? PG_WIDE : g.narrow;
     const unsigned in = blockIdx.x - (kind ? g.blocks : 0), tile = in / (unsigned) rows_y, y = in - tile * (unsigned) rows_y;
     const int at = (int) (tile / (unsigned) a.kvh), head = (int) (tile - (unsigned) at * (unsigned) a.kvh);
     const PgHead h = *a.head;
@@ -501,40 +601,49 @@ __global__ void __launch_bounds__(512) paged_merge_kernel(AttnArgs a, MergeArgs 
         const int r = min(r0 + group / per, e.rows - 1);
         float m = -INFINITY, l = 0.0f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = sub; i < e.n; i += 4 * per) {
-            float2 ml[4];
-            float4 x[4];
+        for (int i = sub; i < e.n; i += 8 * per) {
+            float2 ml[8];
+            float4 x[8];
+            float to = m;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 8; ++j) {
                 const int k = i + j * per;
                 const size_t p = ((size_t) (e.part + min(k, e.n - 1)) * a.kvh + head) * ROWS + r;
                 ml[j] = part_ml[p];
                 x[j] = ((const float4*) (part_o + p * HD))[col];
-                if (k >= e.n) ml[j] = make_float2(-INFINITY, 0.0f);
+                if (k >= e.n) ml[j].y = 0.0f;
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (ml[j].y != 0.0f) {
-                    const float to = fmaxf(m, ml[j].x), f = l != 0.0f ? __builtin_amdgcn_exp2f(m - to) : 0.0f, g = __builtin_amdgcn_exp2f(ml[j].x - to);
-                    m = to;
-                    l = l * f + ml[j].y * g;
-                    o.x = o.x * f + x[j].x * g; o.y = o.y * f + x[j].y * g; o.z = o.z * f + x[j].z * g; o.w = o.w * f + x[j].w * g;
-                }
+            for (int j = 0; j < 8; ++j) to = ml[j].y != 0.0f ? fmaxf(to, ml[j].x) : to;
+            const float f = l != 0.0f ? __builtin_amdgcn_exp2f(m - to) : 0.0f;
+            m = to;
+            l *= f;
+            o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float g8 = ml[j].y != 0.0f ? __builtin_amdgcn_exp2f(ml[j].x - m) : 0.0f;
+                l += ml[j].y * g8;
+                o.x += x[j].x * g8; o.y += x[j].y * g8; o.z += x[j].z * g8; o.w += x[j].w * g8;
+            }
         }
         if (per > 1) {
             s_o[threadIdx.x] = o;
             if (col == 0) s_ml[group] = make_float2(m, l);
             __syncthreads();
             if (sub == 0) {
+                float to = m;
+                for (int j = 1; j < per; ++j) to = s_ml[group + j].y != 0.0f ? fmaxf(to, s_ml[group + j].x) : to;
+                float f = l != 0.0f ? __builtin_amdgcn_exp2f(m - to) : 0.0f;
+                m = to;
+                l *= f;
+                o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+#pragma unroll 4
                 for (int j = 1; j < per; ++j) {
                     const float2 ml = s_ml[group + j];
                     const float4 x = s_o[threadIdx.x + j * L];
-                    if (ml.y != 0.0f) {
-                        const float to = fmaxf(m, ml.x), f = l != 0.0f ? __builtin_amdgcn_exp2f(m - to) : 0.0f, g = __builtin_amdgcn_exp2f(ml.x - to);
-                        m = to;
-                        l = l * f + ml.y * g;
-                        o.x = o.x * f + x.x * g; o.y = o.y * f + x.y * g; o.z = o.z * f + x.z * g; o.w = o.w * f + x.w * g;
-                    }
+                    f = ml.y != 0.0f ? __builtin_amdgcn_exp2f(ml.x - m) : 0.0f;
+                    l += ml.y * f;
+                    o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
                 }
             }
             __syncthreads();
@@ -555,7 +664,7 @@ Space space_of(const PgLayout& l, const wzy_paged_work* w) {
     Space s;
     s.total = 0;
     for (int k = 0; k < 2; ++k) {
-        const size_t rows = (size_t) l.parts[k] * (k ? PG_WIDE : PG_NARROW) * w->kvh;
+        const size_t rows = (size_t) l.parts[k] * (k ? PG_WIDE : l.narrow) * w->kvh;
         s.o[k] = s.total;
         s.ml[k] = s.o[k] + align_up(rows * w->hd * 4, 256);
         s.total = s.ml[k] + align_up(rows * sizeof(float2), 256);
@@ -567,6 +676,7 @@ template <int HD, int T>
 int launch(AttnArgs a, const PgLayout& l, const Space& s, char* space, int max_rows, void* stream) {
     const auto st = as_stream(stream);
     MergeArgs g{};
+    g.narrow = l.narrow;
     unsigned blocks[2] = {0, 0};
     for (int kind = 0; kind < 2; ++kind) {
         if (l.items[kind] == 0) continue;
@@ -574,10 +684,11 @@ int launch(AttnArgs a, const PgLayout& l, const Space& s, char* space, int max_r
         a.part_o = (float*) (space + s.o[kind]);
         a.part_ml = (float2*) (space + s.ml[kind]);
         const unsigned grid = (unsigned) l.items[kind] * (unsigned) a.kvh;
-        if (kind == 0) paged_narrow_kernel<HD, T><<<grid, 256, 0, st>>>(a);
+        if (kind == 0 && l.narrow == 32) paged_narrow_kernel<HD, T><<<grid, 256, 0, st>>>(a);
+        else if (kind == 0) paged_middle_kernel<HD, T><<<grid, 256, 0, st>>>(a);
         else paged_wide_kernel<HD, T><<<grid, 256, 0, st>>>(a);
         WZY_LAUNCH_CHECK();
-        g.rows_y[kind] = kind ? 16 : std::min(PG_NARROW, max_rows);
+        g.rows_y[kind] = kind ? 16 : std::min(l.narrow, max_rows);
         g.at[kind] = l.merge_at[kind];
         g.parts[kind] = l.parts[kind];
         blocks[kind] = (unsigned) l.merges[kind] * (unsigned) a.kvh * (unsigned) g.rows_y[kind];

@@ -91,11 +91,11 @@ struct Cut { int kind, tiles, parts, blocks; };
 WZY_DEV Cut cut_of(const PlanWork& w, int c, int n, bool served, const int (&part)[2]) {
     Cut x;
     const int rows = n * w.g;
-    x.kind = rows <= PG_NARROW || !served ? 0 : 1;
+    x.kind = rows <= w.l.narrow || !served ? 0 : 1;
     x.tiles = rows == 0 ? 0 : x.kind ? (rows + PG_WIDE - 1) / PG_WIDE : 1;
     // blocks of 32 cells that a tile sees, at most: the last one's end, or as many as its tokens' windows span
     x.blocks = served ? (c + n + 31) >> 5 : 0;
-    if (w.window > 0) x.blocks = min(x.blocks, ((w.window + (int) ((uint32_t) (x.kind ? PG_WIDE : PG_NARROW) / (uint32_t) w.g)) >> 5) + 2);
+    if (w.window > 0) x.blocks = min(x.blocks, ((w.window + (int) ((uint32_t) (x.kind ? PG_WIDE : w.l.narrow) / (uint32_t) w.g)) >> 5) + 2);
     const int p = part[x.kind];
     x.parts = p > 0 && x.blocks > p ? (x.blocks + p - 1) / p : 1;
     return x;
@@ -105,7 +105,7 @@ WZY_DEV void put_item(const PlanWork& w, int kind, int i, int r, const PgBefore&
     const Cut x = cut_of(w, c, n, served, part);
     const int j = i - before.items[kind], tile = (int) ((uint32_t) j / (uint32_t) x.parts), k = j - tile * x.parts, rows = n * w.g;
     // a request's last tile sees the most cells and comes first
-    const int row0 = kind ? PG_WIDE * (x.tiles - 1 - tile) : 0, row1 = min(row0 + (kind ? PG_WIDE : PG_NARROW), rows);
+    const int row0 = kind ? PG_WIDE * (x.tiles - 1 - tile) : 0, row1 = min(row0 + (kind ? PG_WIDE : w.l.narrow), rows);
     const int hi = served ? c + (int) ((uint32_t) (row1 - 1) / (uint32_t) w.g) + 1 : 0;
     const int lo = served && w.window > 0 ? max(c + (int) ((uint32_t) row0 / (uint32_t) w.g) + 1 - w.window, 0) : 0;
     // parts of one length, but for the blocks of 32 cells
@@ -392,7 +392,7 @@ extern "C" int wzy_paged_plan(const wzy_paged_pool* pool, const wzy_paged_batch*
                     who, i, w->bytes, w->items, want);
         for (int j = 0; j < i; ++j) WZY_REQUIRE(works[j].items != w->items, "%s: work lists %d and %d are one", who, j, i);
         pw.w[i] = PlanWork{(PgHead*) w->items, l, w->qh / w->kvh, w->window, pg_geometry(w),
-                           {pg_div_up(pg_parts(0, w->hd), w->kvh), pg_div_up(pg_parts(1, w->hd), w->kvh)}, PG_MORE / w->kvh};
+                           {pg_div_up(pg_parts(0, l.narrow, w->hd), w->kvh), pg_div_up(pg_parts(1, l.narrow, w->hd), w->kvh)}, PG_MORE / w->kvh};
     }
     PlanArgs a{pool->free_pages, pool->n_free, pool->n_free_out, b->n_cached, b->n_new, b->table, b->q_start, b->kv_len, b->served,
                b->positions, b->slots, pool->n_pages, pg_log2(pool->page), b->n_req, b->max_tokens, b->max_pages, pg_max_new(b), n_works,

@@ -158,13 +158,14 @@ __global__ void __launch_bounds__(RT) rope_kernel(RopeArgs a) {
         __syncthreads();
     }
     if (!any) return;
-    while (true) {
+    for (i += step; i < pieces; i += step) {                   // the next piece loads before this one is stored
+        Piece<TI, TO, PAIRS, WIDE> next;
+        next.locate(a, row0, i);
+        next.load(a);
         p.store(a, s_cs + (p.row - row0) * half);
-        i += step;
-        if (i >= pieces) return;
-        p.locate(a, row0, i);
-        p.load(a);
+        p = next;
     }
+    p.store(a, s_cs + (p.row - row0) * half);
 }
 
 __global__ void rope_freqs_kernel(wzy_rope_cfg c, double* __restrict__ f) {

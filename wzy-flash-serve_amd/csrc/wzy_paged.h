@@ -9,15 +9,18 @@ namespace wzy {
 
 // ---- work lists ---------------------------------------------------------------------------------------
 // The rows of one request and key head are its (token, head of the group) pairs, token-major: row m is token m / g, head
-// m % g, g = qh / kvh.  They are cut into tiles: requests of up to PG_NARROW rows are one narrow tile, others have wide tiles
-// of PG_WIDE rows.  A tile's cells (from the first that its first token sees to its last token's own) are cut into parts of
-// equal length where the tiles alone do not fill the chip, all tiles of a request into as many as its longest needs; parts leave
-// partial results in the workspace, and a merge entry says which belong together.  The same list serves every key head.
-constexpr int PG_NARROW = 32, PG_WIDE = 128;
+// m % g, g = qh / kvh.  They are cut into tiles: requests of up to 32 rows are one narrow tile (of up to 64, in steps where
+// no request has more), others have wide tiles of PG_WIDE rows.  A tile's cells (from the first that its first token sees to
+// its last token's own) are cut into parts of equal length where the tiles alone do not fill the chip, all tiles of a request
+// into as many as its longest needs; parts leave partial results in the workspace, and a merge entry says which belong
+// together.  The same list serves every key head.
+constexpr int PG_WIDE = 128;
 constexpr int PG_MAX_REQ = 4096, PG_MAX_TOKENS = 1 << 20, PG_MAX_CELLS = 1 << 24;
 // Parts that a step is cut into, over all key heads: as many workgroups as the chip holds at once (by the LDS they take), and of
 // narrow tiles one more a tile, as far as PG_MORE, so that requests of different lengths come out even.
-constexpr int pg_parts(int kind, int hd) { return kind || hd == 128 ? 512 : hd == 64 ? 1024 : 256; }
+constexpr int pg_parts(int kind, int narrow, int hd) {
+    return kind ? 512 : narrow == 64 ? (hd == 256 ? 512 : 768) : hd == 64 ? 1024 : hd == 128 ? 512 : 256;
+}
 constexpr int PG_MORE = 512;
 constexpr int PG_MAGIC = 0x70616765;
 
@@ -42,6 +45,7 @@ static_assert(sizeof(PgItem) == 32 && sizeof(PgMerge) == 32 && sizeof(PgHead) ==
 
 // What one list holds at most, and where (in entries of 32 bytes behind the head; the requests' sums come last).
 struct PgLayout {
+    int narrow;                                 // rows of a narrow tile: 32 or 64
     int items[2], parts[2], merges[2];          // capacities: narrow, wide
     int min_len[2];                             // shortest part, cells
     int item_at[2], merge_at[2], before_at, total;
@@ -55,7 +59,9 @@ inline int pg_max_new(const wzy_paged_batch* b) { return b->max_new > 0 && b->ma
 inline PgLayout pg_layout(int n_req, int max_tokens, int max_new, int max_cells, const wzy_paged_work* w) {
     PgLayout l{};
     const int g = w->qh / w->kvh;
-    const bool any_wide = (int64_t) max_new * g > PG_NARROW;
+    const int64_t rows = (int64_t) max_new * g;
+    l.narrow = rows > 32 && rows <= 64 ? 64 : 32;
+    const bool any_wide = rows > l.narrow;
     const int64_t tiles[2] = {n_req, any_wide ? (int64_t) max_tokens * g / PG_WIDE + n_req : 0};
     l.min_len[0] = 64;
     l.min_len[1] = 512;
@@ -63,7 +69,7 @@ inline PgLayout pg_layout(int n_req, int max_tokens, int max_new, int max_cells,
     for (int k = 0; k < 2; ++k) {
         // n = ceil(span / len) with the sum of span / len at most per_head: all tiles' parts, and those of tiles that have several
         const int64_t more = k ? 0 : n_req < PG_MORE / w->kvh ? n_req : PG_MORE / w->kvh;
-        const int64_t per_head = pg_div_up(pg_parts(k, w->hd), w->kvh) + more;
+        const int64_t per_head = pg_div_up(pg_parts(k, l.narrow, w->hd), w->kvh) + more;
         const int64_t most = tiles[k] * pg_div_up(max_cells, l.min_len[k]);
         l.items[k] = (int) (most < tiles[k] + per_head ? most : tiles[k] + per_head);
         l.parts[k] = (int) (most < 2 * per_head ? most : 2 * per_head);
