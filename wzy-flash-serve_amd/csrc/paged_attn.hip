@@ -63,6 +63,7 @@ template <> struct Half<WZY_F16> {
     }
 };
 constexpr float RISE = 8.0f;
+constexpr int MERGE_THREADS = 256, MERGE_LOADS = 8;       // of a part's row, under way at once
 
 WZY_DEV uint32_t lds_offset(const void* p) { return (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) char*) p; }
 // 64 lanes x 16 bytes to LDS lds .. lds + 1023 in lane order, from a wave-uniform base + off, or from an address a lane
@@ -580,9 +581,9 @@ struct MergeArgs {
     const float2* wide_ml;
 };
 template <int HD, int T>
-__global__ void __launch_bounds__(512) paged_merge_kernel(AttnArgs a, MergeArgs g) {
-    constexpr int L = HD / 4, GROUPS = 512 / L;
-    __shared__ float4 s_o[512];
+__global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(AttnArgs a, MergeArgs g) {
+    constexpr int L = HD / 4, GROUPS = MERGE_THREADS / L;
+    __shared__ float4 s_o[MERGE_THREADS];
     __shared__ float2 s_ml[GROUPS];
     // narrow tiles' workgroups first, by rows_y of them a tile; then wide ones'
     const int kind = blockIdx.x >= g.blocks ? 1 : 0, rows_y = g.rows_y[kind], ROWS = kind ? PG_WIDE : g.narrow;
@@ -595,18 +596,18 @@ __global__ void __launch_bounds__(512) paged_merge_kernel(AttnArgs a, MergeArgs 
     const float* const part_o = kind ? g.wide_o : a.part_o;
     const float2* const part_ml = kind ? g.wide_ml : a.part_ml;
     int per = 1;                                                        // groups a row
-    while (per < GROUPS && per * 4 < e.n) per *= 2;
+    while (per < GROUPS && per * MERGE_LOADS < e.n) per *= 2;
     const int rows_here = GROUPS / per, group = threadIdx.x / L, col = threadIdx.x % L, sub = group & (per - 1);
     for (int r0 = (int) y * rows_here; r0 < e.rows; r0 += rows_y * rows_here) {
         const int r = min(r0 + group / per, e.rows - 1);
         float m = -INFINITY, l = 0.0f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = sub; i < e.n; i += 8 * per) {
-            float2 ml[8];
-            float4 x[8];
+        for (int i = sub; i < e.n; i += MERGE_LOADS * per) {
+            float2 ml[MERGE_LOADS];
+            float4 x[MERGE_LOADS];
             float to = m;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < MERGE_LOADS; ++j) {
                 const int k = i + j * per;
                 const size_t p = ((size_t) (e.part + min(k, e.n - 1)) * a.kvh + head) * ROWS + r;
                 ml[j] = part_ml[p];
@@ -614,16 +615,16 @@ __global__ void __launch_bounds__(512) paged_merge_kernel(AttnArgs a, MergeArgs 
                 if (k >= e.n) ml[j].y = 0.0f;
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) to = ml[j].y != 0.0f ? fmaxf(to, ml[j].x) : to;
+            for (int j = 0; j < MERGE_LOADS; ++j) to = ml[j].y != 0.0f ? fmaxf(to, ml[j].x) : to;
             const float f = l != 0.0f ? __builtin_amdgcn_exp2f(m - to) : 0.0f;
             m = to;
             l *= f;
             o.x *= f; o.y *= f; o.z *= f; o.w *= f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float g8 = ml[j].y != 0.0f ? __builtin_amdgcn_exp2f(ml[j].x - m) : 0.0f;
-                l += ml[j].y * g8;
-                o.x += x[j].x * g8; o.y += x[j].y * g8; o.z += x[j].z * g8; o.w += x[j].w * g8;
+            for (int j = 0; j < MERGE_LOADS; ++j) {
+                const float h8 = ml[j].y != 0.0f ? __builtin_amdgcn_exp2f(ml[j].x - m) : 0.0f;
+                l += ml[j].y * h8;
+                o.x += x[j].x * h8; o.y += x[j].y * h8; o.z += x[j].z * h8; o.w += x[j].w * h8;
             }
         }
         if (per > 1) {
@@ -699,7 +700,7 @@ int launch(AttnArgs a, const PgLayout& l, const Space& s, char* space, int max_r
     g.blocks = blocks[0];
     g.wide_o = (const float*) (space + s.o[1]);
     g.wide_ml = (const float2*) (space + s.ml[1]);
-    paged_merge_kernel<HD, T><<<blocks[0] + blocks[1], 512, 0, st>>>(a, g);
+    paged_merge_kernel<HD, T><<<blocks[0] + blocks[1], MERGE_THREADS, 0, st>>>(a, g);
     WZY_LAUNCH_CHECK();
     return WZY_OK;
 }
