@@ -551,6 +551,18 @@ struct Picker {
             }
         __syncthreads();
     }
+    // s.token[0 .. n - 1] of at most PT / 4, by counting: four threads a token
+    WZY_DEV void sort_few(int n) {
+        const int i = threadIdx.x >> 2;
+        const uint64_t mine = i < n ? s.token[i] : 0;
+        int before = 0;
+        for (int j = threadIdx.x & 3; j < n; j += 4) before += s.token[j] > mine ? 1 : 0;
+        before += dpp_i<DPP_XOR1>(before);
+        before += dpp_i<DPP_XOR2>(before);
+        __syncthreads();
+        if (i < n && (threadIdx.x & 3) == 0) s.token[before] = mine;
+        __syncthreads();
+    }
     // the tokens for which take(logit) holds, at most CAP of them, sorted, with their sums from `sum_before` on
     template <class F>
     WZY_DEV void gather(F&& take, Sum sum_before) {
@@ -716,9 +728,13 @@ struct Picker {
     // The places in s.token[0 .. n - 1], sorted, and the answer.  plan: whole bins, where the sums before an interval are the row's;
     // null: the row's first tokens, all that top-k leaves among them.
     WZY_DEV void finish(const Params& q, int r, int n, const RowPlan* plan, const int (&in_list)[4]) {
+        if (n <= PT) finish_with<1>(q, r, n, plan, in_list);
+        else finish_with<CAP / PT>(q, r, n, plan, in_list);
+    }
+    template <int Q>
+    WZY_DEV void finish_with(const Params& q, int r, int n, const RowPlan* plan, const int (&in_list)[4]) {
         const int tid = threadIdx.x;
         const bool all = !plan || q.counts_only();
-        constexpr int Q = CAP / PT;
         uint64_t m[Q], sum = 0;
 #pragma unroll
         for (int j = 0; j < Q; ++j) {
@@ -841,55 +857,54 @@ WZY_DEV void pick_alone(const SampleArgs& a, int row, const Params& q, uint64_t 
 }
 
 // Rows with a small top-k, from the groups' largest keys: the k-th largest of those is at most the row's k-th largest, so the tokens
-// at or above it are k or more, and they lie in the groups whose largest is: k groups of PER, and ties.  False: too many of those.
+// at or above it are k or more, and they lie in the groups whose largest is.  Which groups: a histogram of the keys' distance from
+// the best one, 64 bins an octave (keys themselves would all fall into a few), up to the bin that holds the k-th.  False: too
+// many (ties).
+WZY_DEV uint32_t distance_bin(uint32_t best, uint32_t key) {
+    const uint32_t d = best - key;
+    const int top = 31 - __builtin_clz(d | 1);
+    return d < 64 ? d : (uint32_t) (top - 5) * 64 + (d >> (top - 6) & 63);   // up to 27 * 64 - 1
+}
 template <int T, bool VEC>
-WZY_DEV bool pick_from_groups(const SampleArgs& a, int row, const Params& q, PickShared& s, Picker<T, VEC>& p) {
+WZY_DEV bool pick_from_groups(const SampleArgs& a, int row, const Params& q, uint64_t best, PickShared& s, Picker<T, VEC>& p) {
     const int tid = threadIdx.x;
     const uint32_t* const g = a.group + (size_t) row * a.groups;
-    // the k-th largest key (0 where there are fewer), 10 or 11 bits at a time
-    uint32_t prefix = 0, k = (uint32_t) q.k;
-    int shift = 32;
-    for (int bits : {11, 11, 10}) {
-        shift -= bits;
-        for (int i = tid; i < 2048; i += PT) s.bucket[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < a.groups; i += PT) {
-            const uint32_t x = g[i];
-            if (shift + bits == 32 || x >> (shift + bits) == prefix) atomicAdd(&s.bucket[2047 - (x >> shift & ((1u << bits) - 1))], 1u);
-        }
-        __syncthreads();
-        const uint32_t c0 = s.bucket[2 * tid], c1 = s.bucket[2 * tid + 1];
-        const uint32_t up = block_sums(Sum{0, c0 + c1}, s.part).count, b = up - c0 - c1;
-        if (tid == 0) s.found = -1;
-        __syncthreads();
-        if (b < k && up >= k) {
-            s.found = b + c0 >= k ? 2 * tid : 2 * tid + 1;
-            s.n = b + c0 >= k ? b : b + c0;
-        }
-        __syncthreads();
-        if (s.found < 0) {                               // fewer groups than k: all of them
-            prefix = 0;
-            shift = 0;
-            __syncthreads();
-            break;
-        }
-        prefix = prefix << bits | (uint32_t) (2047 - s.found);
-        k -= s.n;
-        __syncthreads();
+    const uint32_t top = (uint32_t) (best >> 32);
+    constexpr int HOLD = 8;                              // keys a thread keeps; more are read twice
+    uint32_t mine[HOLD];
+#pragma unroll
+    for (int j = 0; j < HOLD; ++j) mine[j] = tid + j * PT < a.groups ? g[tid + j * PT] : 0;
+    for (int i = tid; i < 2 * PT; i += PT) s.bucket[i] = 0;
+    if (tid == 0) {
+        s.found = 2 * PT - 1;
+        s.n = 0;
     }
-    const uint32_t least = max(prefix, KEY_NONE + 1);
-    // the groups, then their tokens, a thread a token at a time
-    if (tid == 0) s.n = 0;
     __syncthreads();
-    for (int i = tid; i < a.groups; i += PT)
-        if (g[i] >= least) {
+    auto each_group = [&](auto&& f) {                    // groups with a token
+#pragma unroll
+        for (int j = 0; j < HOLD; ++j)
+            if (mine[j] > KEY_NONE) f(mine[j], tid + j * PT);
+        for (int i = tid + HOLD * PT; i < a.groups; i += PT)
+            if (g[i] > KEY_NONE) f(g[i], i);
+    };
+    each_group([&](uint32_t key, int) { atomicAdd(&s.bucket[distance_bin(top, key)], 1u); });
+    __syncthreads();
+    const uint32_t c0 = s.bucket[2 * tid], c1 = s.bucket[2 * tid + 1], k = (uint32_t) q.k;
+    const uint32_t up = block_sums(Sum{0, c0 + c1}, s.part).count, b = up - c0 - c1;
+    if (b < k && up >= k) s.found = b + c0 >= k ? 2 * tid : 2 * tid + 1;       // fewer groups than k: all of them
+    __syncthreads();
+    const uint32_t last = (uint32_t) s.found;
+    // the groups, then their tokens, a thread a token at a time
+    each_group([&](uint32_t key, int i) {
+        if (distance_bin(top, key) <= last) {
             const unsigned at = atomicAdd(&s.n, 1u);
-            if (at < GROUP_K) s.bucket[at] = (uint32_t) i;
+            if (at < CAP) s.bucket[at] = (uint32_t) i;
         }
+    });
     __syncthreads();
     const int groups = (int) s.n;
     __syncthreads();
-    if (groups > GROUP_K) return false;
+    if (groups > CAP) return false;
     if (tid == 0) s.n = 0;
     __syncthreads();
     constexpr int E = !VEC ? 1 : T == WZY_F32 ? 4 : 8;
@@ -897,23 +912,18 @@ WZY_DEV bool pick_from_groups(const SampleArgs& a, int row, const Params& q, Pic
         const int group = (int) s.bucket[i / PER], j = i % PER, e = group / ST * SLICE + ((j / E) * ST + group % ST) * E + j % E;
         if (e < a.vocab) {
             const float l = load_logit<T>(p.row, e);
-            if (order_key(l) >= least) s.token[atomicAdd(&s.n, 1u)] = order_u64(l, e);
+            if (l > -INFINITY && distance_bin(top, order_key(l)) <= last) {
+                const unsigned at = atomicAdd(&s.n, 1u);
+                if (at < CAP) s.token[at] = order_u64(l, e);
+            }
         }
     }
     __syncthreads();
-    const int n = (int) s.n;                             // GROUP_K * PER = CAP at most
-    if (n <= PT / 4) {
-        // four threads count a token's predecessors
-        const int i = tid >> 2;
-        const uint64_t mine = i < n ? s.token[i] : 0;
-        int before = 0;
-        for (int j = tid & 3; j < n; j += 4) before += s.token[j] > mine ? 1 : 0;
-        before += dpp_i<DPP_XOR1>(before);
-        before += dpp_i<DPP_XOR2>(before);
-        __syncthreads();
-        if (i < n && (tid & 3) == 0) s.token[before] = mine;
-        __syncthreads();
-    } else p.sort(n);
+    const int n = (int) s.n;
+    __syncthreads();
+    if (n > CAP) return false;
+    if (n <= PT / 4) p.sort_few(n);
+    else p.sort(n);
     const int none[4] = {0, 0, 0, 0};
     p.finish(q, row, n, nullptr, none);
     return true;
@@ -941,7 +951,7 @@ __global__ void __launch_bounds__(PT) sample_plan_kernel(SampleArgs a) {
     }
     if (q.from_groups()) {
         Picker<T, VEC> p{a, s, row_of<T>(a, row), weight_of(a, best, q.temp, s.table)};
-        const bool done = pick_from_groups<T, VEC>(a, row, q, s, p);
+        const bool done = pick_from_groups<T, VEC>(a, row, q, best, s, p);
         if (tid == 0) {
             a.plan[row].best = best;
             a.plan[row].q = q;
@@ -1015,6 +1025,21 @@ __global__ void __launch_bounds__(PT) sample_pick_kernel(SampleArgs a) {
         skip[k] = bins;
         bins += is ? plan.hi[k] - plan.lo[k] + 1 : 0;
     }
+    int in_list[4];                                      // tokens of the list before each interval
+    if (n <= PT / 4) {
+        if (tid < 4) s.h_count[tid] = 0;
+        if (tid < n) s.token[tid] = a.list[(size_t) row * CAP + tid];
+        __syncthreads();
+        if (tid < n) {
+            const int b = p.w.bin(key_value((uint32_t) (s.token[tid] >> 32)));
+#pragma unroll
+            for (int k = 1; k < 4; ++k)
+                if (lo[k] < BINS && b < lo[k]) atomicAdd(&s.h_count[k], 1u);
+        }
+        p.sort_few(n);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) in_list[k] = lo[k] < BINS ? (int) s.h_count[k] : CAP;
+    } else {
     const int per = CAP / bins;
     const float scale = p.w.cf * BIN_OCT;
     auto bucket_of = [&](uint64_t token) {
@@ -1053,7 +1078,6 @@ __global__ void __launch_bounds__(PT) sample_pick_kernel(SampleArgs a) {
         start += size[j];
     }
     __syncthreads();
-    int in_list[4];                                      // tokens of the list before each interval
 #pragma unroll
     for (int k = 0; k < 4; ++k) in_list[k] = lo[k] < BINS ? (int) s.bucket[skip[k] * per] : CAP;
     __syncthreads();
@@ -1070,6 +1094,7 @@ __global__ void __launch_bounds__(PT) sample_pick_kernel(SampleArgs a) {
             s.token[place] = mine[j];
         }
     __syncthreads();
+    }
     p.finish(q, row, n, &plan, in_list);
 }
 
