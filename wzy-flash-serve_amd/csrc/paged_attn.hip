@@ -52,12 +52,16 @@ struct AttnArgs {
 template <int T> struct Half;                // of the cache's type
 template <> struct Half<WZY_BF16> {
     static constexpr float SHIFT = 0.0f;
+    static constexpr uint32_t EXP = 0x7F80;             // of what is not finite
+    static WZY_DEV float value(uint32_t b) { return bf16_lo(b); }
     static WZY_DEV v16f_t mfma(v4w_t a, v4w_t b, v16f_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b_t, a), __builtin_bit_cast(v8b_t, b), c, 0, 0, 0);
     }
 };
 template <> struct Half<WZY_F16> {
     static constexpr float SHIFT = 6.0f;
+    static constexpr uint32_t EXP = 0x7C00;
+    static WZY_DEV float value(uint32_t b) { return h16_to_f((uint16_t) b); }
     static WZY_DEV v16f_t mfma(v4w_t a, v4w_t b, v16f_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h_t, a), __builtin_bit_cast(v8h_t, b), c, 0, 0, 0);
     }
@@ -290,6 +294,19 @@ struct Wave {
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i / 4][i % 4] = pack2<T>(s[2 * i], s[2 * i + 1]);
     }
+    // Is there something in V of a block which only some rows see that is not finite?  A weight of 0 does not silence it: the rows are
+    // then done again by plain_row.  (Leaving it out of the product here costs registers that there are not: 1.7 times the time.)
+    WZY_DEV bool unsafe(const AttnArgs& a, int b, int lane, const char* vb) const {
+        if (pos_min == pos_max || !masked(a, b)) return false;
+        bool found = false;
+#pragma unroll 4
+        for (int i = 0; i < BV::LOADS; ++i) {
+            const v4w_t x = *(const v4w_t*) (vb + i * BV::STEP + 16 * lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) found |= (x[j] & Half<T>::EXP) == Half<T>::EXP || (x[j] >> 16 & Half<T>::EXP) == Half<T>::EXP;
+        }
+        return __any(found);
+    }
     WZY_DEV void add(const char* vb, const v4w_t (&p)[2]) {
         v4w_t v[AHEAD];
 #pragma unroll
@@ -323,6 +340,50 @@ WZY_DEV char* out_row(const AttnArgs& a, const TileCtx& t, int row) {
     return a.out + (int64_t) (t.it.q0 + token) * a.ldo + (int64_t) (t.head * a.g + row - token * a.g) * a.ldo_head;
 }
 
+// A row of a part by itself, on a wave: only the cells that it sees are looked at.
+template <int HD, int T>
+WZY_DEV void plain_row(const AttnArgs& a, const TileCtx& t, int row, int lane, int tile_rows) {
+    constexpr int E = HD / 64;                                          // columns a lane
+    const int token = (int) fast_div((uint32_t) row, a.div_g), pos = t.it.n_cached + token;
+    const int lo = a.window ? max(t.it.lo, pos - a.window + 1) : t.it.lo, hi = min(t.it.hi, pos + 1);
+    const uint16_t* const q = (const uint16_t*) (a.q + (int64_t) (t.it.q0 + token) * a.ldq + (int64_t) (t.head * a.g + row - token * a.g) * a.ldq_head) + E * lane;
+    float x[E], o[E], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        x[e] = Half<T>::value(q[e]);
+        o[e] = 0.0f;
+    }
+    for (int c = lo; c < hi; ++c) {
+        int id = t.pages[c >> a.lp];
+        id = (unsigned) id < (unsigned) a.n_pages ? id : 0;
+        const int64_t at = (int64_t) id * a.ld_page + (int64_t) (c & ((1 << a.lp) - 1)) * a.ld_cell + (int64_t) t.head * a.ld_head;
+        const uint16_t *const k = (const uint16_t*) (a.k + at) + E * lane, *const v = (const uint16_t*) (a.v + at) + E * lane;
+        float s = 0.0f, y[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            s = fmaf(x[e], Half<T>::value(k[e]), s);
+            y[e] = Half<T>::value(v[e]);
+        }
+        s = wave_sum(s) * a.c;
+        const float to = fmaxf(m, s), f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 0.0f;
+        const float p = to > -INFINITY || s != s ? __builtin_amdgcn_exp2f(s - to) : 0.0f;
+        m = to;
+        l = l * f + p;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = o[e] * f + p * y[e];
+    }
+    if (t.it.part < 0) {
+        const float n = l != 0.0f ? 1.0f / l : 0.0f;
+        uint16_t* const r = (uint16_t*) out_row(a, t, row) + E * lane;
+#pragma unroll
+        for (int e = 0; e < E; ++e) r[e] = (uint16_t) pack2<T>(o[e] * n, o[e] * n);
+    } else {
+        const size_t at = ((size_t) t.it.part * a.kvh + t.head) * tile_rows + (row - t.it.row0);
+#pragma unroll
+        for (int e = 0; e < E; ++e) a.part_o[at * HD + E * lane + e] = o[e];
+        if (lane == 0) a.part_ml[at] = make_float2(m, l);
+    }
+}
 // A request that is not served: all its rows become 0.
 template <int HD>
 WZY_DEV void zero_rows(const AttnArgs& a, const TileCtx& t) {
@@ -362,6 +423,7 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
     constexpr int MINE = BK::BYTES + BV::BYTES;
     __shared__ __align__(1024) char s_buf[4][MINE];                     // a wave's K and V; then its results in fp32
     __shared__ float s_m[4][32], s_l[4][32];
+    __shared__ int s_unsafe;
     static_assert(MINE >= 32 * HD * 4 && MINE % 16 == 0, "a wave's results take its buffers");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     TileCtx t;
@@ -377,6 +439,8 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
     const uint32_t lk = lds_offset(kb), lv = lds_offset(vb);
     const int end = (t.it.hi + 31) >> 5;
     int b = (t.it.lo >> 5) + wave;
+    if (tid == 0) s_unsafe = 0;
+    bool unsafe = false;
     // the first block's loads before those of q, which the compiler counts as the only ones: it waits for all of them
     if (b < end) {
         ld.at(b);
@@ -399,6 +463,7 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
             w.weights(a, b, lane, s, p);
             if (more) wait_loads<BK::LOADS>();
             else wait_loads<0>();
+            unsafe |= w.unsafe(a, b, lane, vb);
             w.add(vb, p);
             if (!more) break;
             wait_lds();
@@ -406,6 +471,8 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
         }
     }
     w.l = half_sum(w.l);
+    __syncthreads();
+    if (unsafe) s_unsafe = 1;
     if (lane < 32) {
         s_m[wave][lane] = w.m;
         s_l[wave][lane] = w.l;
@@ -421,6 +488,10 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
                 make_float4(w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]);
     __syncthreads();
     const int rows = w.rows;
+    if (s_unsafe) {
+        for (int r = wave; r < rows; r += 4) plain_row<HD, T>(a, t, r, lane, 32);
+        return;
+    }
     for (int i = tid; i < rows * (HD / 4); i += 256) {
         const int row = i / (HD / 4), col = i % (HD / 4);
         float m = s_m[0][row], l = 0.0f;
@@ -454,6 +525,7 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
     constexpr int BOTH = BK::BYTES + BV::BYTES, MINE = BK::LOADS / 2;
     __shared__ __align__(1024) char s_buf[2][BOTH];                     // a pair's K and V; then the second pair's results in fp32
     __shared__ float s_m[64], s_l[64];
+    __shared__ int s_unsafe;
     static_assert(2 * BOTH >= 64 * HD * 4, "a pair's results take the buffers");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave & 1, pair = wave >> 1;
     TileCtx t;
@@ -475,6 +547,8 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
         ld.template issue<true, MINE>(lv, half * MINE);
     }
     w.start(a, t, 32 * half, lane);
+    if (tid == 0) s_unsafe = 0;
+    bool unsafe = false;
     wait_loads<0>();
     // both pairs go round as often as the first has blocks; where the second has one fewer, it meets the first's last time
     const int rounds = (end - first + 1) / 2, mine = (end - first + 1 - pair) / 2;
@@ -489,6 +563,7 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
         }
         v4w_t p[2];
         w.weights(a, b, lane, s, p);
+        unsafe |= w.unsafe(a, b, lane, vb);
         w.add(vb, p);
         if (n + 1 < rounds || mine < rounds) wait_lds_and_meet();
         if (more) ld.template issue<true, MINE>(lv, half * MINE);
@@ -500,6 +575,7 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
     w.l = half_sum(w.l);
     wait_all_and_meet();                                                // the buffers have been read
     float4* const r = (float4*) (&s_buf[0][0] + half * 32 * HD * 4);
+    if (unsafe) s_unsafe = 1;
     if (pair == 1) {
         if (lane < 32) {
             s_m[32 * half + lane] = w.m;
@@ -511,6 +587,10 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
             for (int i = 0; i < 4; ++i) r[(4 * d + i) * 64 + lane] = make_float4(w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]);
     }
     __syncthreads();
+    if (s_unsafe) {
+        for (int r = wave; r < min(w.rows, 64); r += 4) plain_row<HD, T>(a, t, r, lane, 64);
+        return;
+    }
     if (pair == 1) return;
     const float m1 = s_m[32 * half + (lane & 31)], l1 = s_l[32 * half + (lane & 31)], m = fmaxf(w.m, m1);
     const float f0 = w.l != 0.0f ? __builtin_amdgcn_exp2f(w.m - m) : 0.0f, f1 = l1 != 0.0f ? __builtin_amdgcn_exp2f(m1 - m) : 0.0f;
@@ -560,14 +640,20 @@ __global__ void __launch_bounds__(256, 2) paged_wide_kernel(AttnArgs a) {
         if (b + 1 < end) load(b + 1, buf ^ 1);
     };
     for (; b < from && b < end; ++b, buf ^= 1) next();
+    bool unsafe = false;
     for (; b < to; ++b, buf ^= 1) {
         next();
         const v16f_t s = w.scores(s_buf[buf]);
         v4w_t p[2];
         w.weights(a, b, lane, s, p);
+        unsafe |= w.unsafe(a, b, lane, s_buf[buf] + BK::BYTES);
         w.add(s_buf[buf] + BK::BYTES, p);
     }
     for (; b < end; ++b, buf ^= 1) next();
+    if (unsafe) {
+        for (int r = 0; r < 32 && t.it.row0 + 32 * wave + r < w.rows; ++r) plain_row<HD, T>(a, t, t.it.row0 + 32 * wave + r, lane, PG_WIDE);
+        return;
+    }
     put_row<HD, T>(a, t, w, half_sum(w.l), lane, PG_WIDE);
 }
 
