@@ -381,7 +381,7 @@ WZY_DEV void plain_row(const AttnArgs& a, const TileCtx& t, int row, int lane, i
         const size_t at = ((size_t) t.it.part * a.kvh + t.head) * tile_rows + (row - t.it.row0);
 #pragma unroll
         for (int e = 0; e < E; ++e) a.part_o[at * HD + E * lane + e] = o[e];
-        if (lane == 0) a.part_ml[at] = make_float2(m, l);
+        if (lane == 0) a.part_ml[at] = make_float2(m + Half<T>::SHIFT, l);        // as other parts, whose weights are 2^SHIFT larger
     }
 }
 // A request that is not served: all its rows become 0.
@@ -698,7 +698,10 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(AttnArgs a, 
                 const size_t p = ((size_t) (e.part + min(k, e.n - 1)) * a.kvh + head) * ROWS + r;
                 ml[j] = part_ml[p];
                 x[j] = ((const float4*) (part_o + p * HD))[col];
-                if (k >= e.n) ml[j].y = 0.0f;
+                if (k >= e.n) {                          // not a part: a weight of 0 would not silence an infinity
+                    ml[j].y = 0.0f;
+                    x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
             }
 #pragma unroll
             for (int j = 0; j < MERGE_LOADS; ++j) to = ml[j].y != 0.0f ? fmaxf(to, ml[j].x) : to;
