@@ -55,7 +55,8 @@ typedef struct wzy_paged_batch {
     int* served;                 /* [n_req] out: 1, or 0 */
     int* positions;              /* [max_tokens] out: n_cached + place in the request */
     int* slots;                  /* [max_tokens] out: table[position / page] * page + position % page.  Rows behind the last, and
-                                    rows of a request that is not served: position 0, slot -1 */
+                                    rows of a request that is not served: position 0, slot -1.  A page id
+                                    outside 0 .. n_pages - 1: slot -1 */
     int max_new;                 /* the largest n_new; 0: max_tokens */
 } wzy_paged_batch;
 
@@ -153,7 +154,8 @@ int wzy_paged_append(const wzy_paged_cache* cache, const wzy_rope_tab* rope, con
 /* out[t, h] = sum_j p_j v_j,  p = softmax over j of scale * q[t, h] . k_j, for each new token t of each request: j runs over the
  * request's cells up to t's own position, the last `window` of them, key head h / (qh / kvh).  q, out [max_tokens x qh x hd]
  * of the cache's type, 16-byte aligned, strides multiples of 8; rows of a request that is not served become 0, rows behind the last
- * request's keep what they hold.  The batch is as wzy_paged_plan left it, `work` one of its lists.
+ * request's keep what they hold.  The batch is as wzy_paged_plan left it, `work` one of its lists (a list
+ * that was built for other numbers has no work: nothing is written).
  * Sums are fp32; the softmax weights are rounded to the cache's type for the second product (half a step of a weight, so of
  * an output at most as much; fp16 weights are kept 2^6 above their smallest so that small ones are not lost).
  * Page ids outside 0 .. n_pages - 1 count as page 0.  scale is finite and above 0. */

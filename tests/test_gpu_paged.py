@@ -119,6 +119,23 @@ def test_plan_refuses_requests(wz, gpu, max_tokens):
     assert b.check()[3].tolist() == [1, 0, 0, 0, 1]
 
 
+@pytest.mark.parametrize("rows", [3, 4200])
+def test_plan_gives_no_slot_in_bad_pages(wz, gpu, rows):
+    # a held page that is none of the cache's, and bad ids in the pool: slots -1, nothing else
+    b = Batch(16, [5, 20, 3], [1, rows - 2, 1], 300, 400, None)
+    b.table[0, 0] = -1
+    b.free[b.n_free - 1] = 400
+    b.d["table"], b.d["free"] = ints(b.table), ints(b.free)
+    b.c.table, b.pool.free_pages = b.d["table"].ptr, b.d["free"].ptr
+    wz.wzy_paged_plan(ref(b.pool), ref(b.c), None, 0, None)
+    want = R.plan(16, 400, b.n_free, b.free, b.n_cached, b.n_new, b.table, b.max_tokens, b.max_tokens)
+    table, slots = want[0], want[5]
+    np.testing.assert_array_equal(b.d["table"].numpy().reshape(3, -1), table)
+    slots = np.where((slots < 0) | (slots >= 6400), -1, slots)
+    assert slots[0] == -1 and (rows == 3 or (slots == -1).sum() == 17)
+    np.testing.assert_array_equal(b.read("slots", rows), slots)
+
+
 def test_plan_in_place_then_release(wz, gpu):
     b = Batch(16, [20, 0, 33, 1], [13, 1, 15, 0], 4, 20, None)
     b.pool.n_free_out = b.pool.n_free

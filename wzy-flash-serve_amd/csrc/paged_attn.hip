@@ -678,7 +678,9 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(AttnArgs a, 
     const PgHead h = *a.head;
     const PgMerge e = ((const PgMerge*) (a.head + 1))[g.at[kind] + at];
     if (h.magic != PG_MAGIC || h.geometry != a.geometry || at >= h.n_merges[kind]) return;
-    if (e.part < 0 || e.n < 1 || e.part > g.parts[kind] - e.n || e.rows < 1 || e.rows > ROWS || e.row0 < 0 || e.q0 < 0) return;
+    if (e.part < 0 || e.n < 1 || e.part > g.parts[kind] - e.n || e.rows < 1 || e.rows > ROWS || e.row0 < 0 || e.row0 >= a.max_tokens * a.g || e.q0 < 0 ||
+        e.q0 >= a.max_tokens)
+        return;
     const float* const part_o = kind ? g.wide_o : a.part_o;
     const float2* const part_ml = kind ? g.wide_ml : a.part_ml;
     int per = 1;                                                        // groups a row
@@ -828,7 +830,7 @@ extern "C" int wzy_paged_attend(const wzy_paged_cache* c, const wzy_paged_batch*
     a.q = (const char*) q->p; a.ldq = 2 * q->ld; a.ldq_head = 2 * q->ld_head;
     a.out = (char*) out->p; a.ldo = 2 * out->ld; a.ldo_head = 2 * out->ld_head;
     a.head = (const PgHead*) w->items;
-    a.g = w->qh / w->kvh; a.kvh = w->kvh; a.window = w->window; a.geometry = pg_geometry(w);
+    a.g = w->qh / w->kvh; a.kvh = w->kvh; a.window = pg_window(w); a.geometry = pg_geometry(w, l);
     a.div_g = FastDiv((uint32_t) a.g);
     a.c = scale * 1.44269504088896340736f;
     a.n_pages = c->n_pages; a.lp = pg_log2(c->page); a.max_pages = b->max_pages; a.n_req = b->n_req; a.max_tokens = b->max_tokens;

@@ -129,7 +129,8 @@ WZY_DEV void put_row(const PlanArgs& a, int t, const int* s_start, const int* s_
         const int r = find_last(s_start, a.n_req, t), c = s_cached[r];
         if (c >= 0) {                                          // served
             pos = c + t - s_start[r];
-            slot = (page_of(r, pos >> a.lp) << a.lp) | (pos & ((1 << a.lp) - 1));
+            const int page = page_of(r, pos >> a.lp);
+            if ((unsigned) page < (unsigned) a.n_pages) slot = (page << a.lp) | (pos & ((1 << a.lp) - 1));
         }
     }
     a.positions[t] = pos;
@@ -192,8 +193,8 @@ __global__ void __launch_bounds__(NT) paged_plan_kernel(PlanArgs a, PlanWorks wo
     }
     block_scan<NT>(taken, s_scan, n_taken);                    // those served are the first that need any
     if (tid == 0) *a.n_free_out = n_free - n_taken[0];
-    // pages into the table.  Page ids are limited, so that a slot is always one of the cache's.
-    auto pool = [&](int i) { return min(max(a.free_pages[n_free - 1 - i], 0), a.n_pages - 1); };
+    // pages into the table
+    auto pool = [&](int i) { return a.free_pages[n_free - 1 - i]; };
     for (int i = tid; i < n_taken[0]; i += NT) {
         const int r = find_last(s_pages, a.n_req, i);
         a.table[(size_t) r * a.max_pages + div_up_log2(s_cached[r], a.lp) + i - s_pages[r]] = pool(i);
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(NT) paged_plan_kernel(PlanArgs a, PlanWorks wo
         for (int t = tid; t < a.max_tokens; t += NT)
             put_row(a, t, s_start, s_cached, rows_total, [&](int r, int p) {
                 const int held = div_up_log2(s_cached[r], a.lp);
-                return p < held ? min(max(a.table[(size_t) r * a.max_pages + p], 0), a.n_pages - 1) : pool(s_pages[r] + p - held);
+                return p < held ? a.table[(size_t) r * a.max_pages + p] : pool(s_pages[r] + p - held);
             });
 
     for (int i = 0; i < a.n_works; ++i) {
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(PlanArgs a, PlanWorks w
         const int t = block * 256 + threadIdx.x;
         if (t < a.max_tokens)
             put_row(a, t, s_start, s_cached, s_start[a.n_req],
-                    [&](int r, int p) { return min(max(a.table[(size_t) r * a.max_pages + p], 0), a.n_pages - 1); });
+                    [&](int r, int p) { return a.table[(size_t) r * a.max_pages + p]; });
         return;
     }
     const PlanWork& w = works.w[list];
@@ -391,7 +392,7 @@ extern "C" int wzy_paged_plan(const wzy_paged_pool* pool, const wzy_paged_batch*
         WZY_REQUIRE(w->items && (uintptr_t) w->items % 16 == 0 && w->bytes >= want, "%s: work list %d: %zu bytes at %p (%zu, 16-byte aligned)",
                     who, i, w->bytes, w->items, want);
         for (int j = 0; j < i; ++j) WZY_REQUIRE(works[j].items != w->items, "%s: work lists %d and %d are one", who, j, i);
-        pw.w[i] = PlanWork{(PgHead*) w->items, l, w->qh / w->kvh, w->window, pg_geometry(w),
+        pw.w[i] = PlanWork{(PgHead*) w->items, l, w->qh / w->kvh, pg_window(w), pg_geometry(w, l),
                            {pg_div_up(pg_parts(0, l.narrow, w->hd), w->kvh), pg_div_up(pg_parts(1, l.narrow, w->hd), w->kvh)}, PG_MORE / w->kvh};
     }
     PlanArgs a{pool->free_pages, pool->n_free, pool->n_free_out, b->n_cached, b->n_new, b->table, b->q_start, b->kv_len, b->served,

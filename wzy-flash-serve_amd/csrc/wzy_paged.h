@@ -86,7 +86,15 @@ inline PgLayout pg_layout(int n_req, int max_tokens, int max_new, int max_cells,
     return l;
 }
 PgLayout pg_layout_of(const wzy_paged_batch* b, const wzy_paged_work* w);
-inline int pg_geometry(const wzy_paged_work* w) { return w->hd ^ (w->qh << 10) ^ (w->kvh << 20) ^ (w->window << 3); }
+// what a list was built for: a call whose numbers give another layout finds no work in it
+inline int pg_geometry(const wzy_paged_work* w, const PgLayout& l) {
+    uint32_t h = 2166136261u;
+    for (int v : {w->hd, w->qh, w->kvh, w->window, l.narrow, l.items[0], l.items[1], l.parts[0], l.parts[1], l.merges[0], l.merges[1], l.total})
+        h = (h ^ (uint32_t) v) * 16777619u;
+    return (int) h;
+}
+// no request has more cells than that
+inline int pg_window(const wzy_paged_work* w) { return w->window < PG_MAX_CELLS ? w->window : 0; }
 
 // ---- host checks ----------------------------------------------------------------------------------------
 inline bool pg_page_ok(int n_pages, int page) {
