@@ -12,7 +12,7 @@
 //                  groups above it are all that has to be read again; they get their token here
 //   sample_gather  the slices again: tokens of those bins to the row's list
 //   sample_pick    a workgroup a row: the list sorted, sums, places
-// Rows whose bins hold more than CAP tokens (thousands of equal logits) are done by sample_pick alone, from the row.
+// Rows of at most SHORT logits are sorted whole, by one launch.  Rows whose bins hold more than CAP tokens (thousands of equal logits) are done by sample_pick alone, from the row.
 // w is taken in 64 bits (fp32's 1e-7 would move one draw in a thousand of a flat row) and summed as integers of 2^-F, F = 62 -
 // log2(vocab), at most 51: sums do not depend on their order, so LDS and memory atomics may add them as they come.  Where top-k is
 // small, everything it leaves is gathered, and the histogram counts only.
@@ -25,6 +25,7 @@ using namespace wzy;
 namespace {
 constexpr int ST = 256, PER = 32, SLICE = ST * PER;      // sample_max, sample_hist
 constexpr int PT = 1024, CAP = 4096;                     // sample_pick; tokens gathered at most
+constexpr int SHORT = 2048;                               // rows of up to so many logits are sorted whole
 constexpr int GROUP_K = CAP / PER;                       // top-k up to which the groups' largest tokens say what to gather
 constexpr int SMALL_K = 2048;                            // top-k up to which all that it leaves is gathered
 constexpr int BINS = 1024;                               // 64 octaves of w
@@ -563,6 +564,51 @@ struct Picker {
         if (i < n && (threadIdx.x & 3) == 0) s.token[before] = mine;
         __syncthreads();
     }
+    // s.token = the threads' tokens (0: none), largest first: counted, summed and put by bucket (smaller buckets first), in its bucket a
+    // token counts those before it.  starts() is called while s.bucket holds the buckets' first places.
+    template <class F, class G>
+    WZY_DEV void sort_buckets(const uint64_t (&mine)[CAP / PT], F&& bucket_of, G&& starts) {
+        constexpr int E = CAP / PT;
+        const int tid = threadIdx.x;
+        for (int i = tid; i < CAP; i += PT) s.bucket[i] = 0;
+        __syncthreads();
+        int to[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            to[j] = mine[j] ? bucket_of(mine[j]) : 0;
+            if (mine[j]) atomicAdd(&s.bucket[to[j]], 1u);
+        }
+        __syncthreads();
+        uint32_t size[E], own = 0;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            size[j] = s.bucket[E * tid + j];
+            own += size[j];
+        }
+        uint32_t start = block_sums(Sum{0, own}, s.part).count - own;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            s.bucket[E * tid + j] = start;               // of the bucket; then, as tokens come, its end
+            start += size[j];
+        }
+        __syncthreads();
+        starts();
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (mine[j]) s.unsorted[atomicAdd(&s.bucket[to[j]], 1u)] = mine[j];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (mine[j]) {
+                const int first = to[j] > 0 ? (int) s.bucket[to[j] - 1] : 0, last = (int) s.bucket[to[j]];
+                int place = first;
+#pragma unroll 4
+                for (int i = first; i < last; ++i) place += s.unsorted[i] > mine[j] ? 1 : 0;
+                s.token[place] = mine[j];
+            }
+        __syncthreads();
+    }
     // the tokens for which take(logit) holds, at most CAP of them, sorted, with their sums from `sum_before` on
     template <class F>
     WZY_DEV void gather(F&& take, Sum sum_before) {
@@ -601,6 +647,12 @@ struct Picker {
     int gathered = 0;
     Place before{0, 0, 0};                               // the sums before the gathered tokens
 
+    // s.found = the least i of those that have one, i rising with the lanes: one atomic a wave (from all lanes they queue up at one
+    // address: 6,000 cycles)
+    WZY_DEV void lowest(bool have, int i) {
+        const uint64_t b = __ballot(have);
+        if (b && (int) (threadIdx.x & 63) == __ffsll((unsigned long long) b) - 1) atomicMin(&s.found, i);
+    }
     // the first gathered token at which the target is reached (the last with key >= target, BY_KEY); the last one, if none
     WZY_DEV Place among(Mode mode, uint64_t target) {
         if (threadIdx.x == 0) s.found = gathered - 1;
@@ -612,7 +664,7 @@ struct Picker {
             if (mode == BY_COUNT) here = before.count + i + 1 >= target;
             else if (mode == BY_MASS) here = s.token_mass[i] >= target;
             else here = i + 1 < gathered && (s.token[i + 1] >> 32) < target;
-            if (here) atomicMin(&s.found, i);
+            lowest(here, i);
         }
         __syncthreads();
         const int i = s.found;
@@ -767,7 +819,7 @@ struct Picker {
 #pragma unroll
             for (int j = Q - 1; j >= 0; --j)
                 if (Q * tid + j < n && here(m[j], count[j])) f = Q * tid + j;
-            if (f < n) atomicMin(&s.found, f);
+            lowest(f < n, f);
             __syncthreads();
             const int i = s.found;
             __syncthreads();
@@ -776,7 +828,7 @@ struct Picker {
         // What is left, as a sum: of two places the one with the smaller sum comes first.
         __syncthreads();
         uint64_t end = all ? s.token_mass[n - 1] : plan->mass;
-        if (!plan) end = s.token_mass[min(q.k, n) - 1];
+        if (!plan) end = s.token_mass[(q.k >= 1 ? min(q.k, n) : n) - 1];
         else if (q.k >= 1 && (uint32_t) q.k < plan->count) end = s.token_mass[first([&](uint64_t, uint32_t c) { return c >= (uint32_t) q.k; })];
         const uint64_t of_k = end;
         if (q.cut_p()) {
@@ -1040,62 +1092,74 @@ __global__ void __launch_bounds__(PT) sample_pick_kernel(SampleArgs a) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) in_list[k] = lo[k] < BINS ? (int) s.h_count[k] : CAP;
     } else {
-    const int per = CAP / bins;
-    const float scale = p.w.cf * BIN_OCT;
-    auto bucket_of = [&](uint64_t token) {
-        const float l = key_value((uint32_t) (token >> 32));
-        const int b = p.w.bin(l);
-        int v = 0;
+        const int per = CAP / bins;
+        const float scale = p.w.cf * BIN_OCT;
+        auto bucket_of = [&](uint64_t token) {
+            const float l = key_value((uint32_t) (token >> 32));
+            const int b = p.w.bin(l);
+            int v = 0;
 #pragma unroll
-        for (int k = 1; k < 4; ++k) v = b >= lo[k] ? k : v;
-        const float in = l == p.w.m ? 0.0f : fminf((p.w.m - l) * scale, (float) (BINS - 1)) - (float) b;
-        const int at = b - (v == 0 ? lo[0] : v == 1 ? lo[1] : v == 2 ? lo[2] : lo[3]) + (v == 0 ? skip[0] : v == 1 ? skip[1] : v == 2 ? skip[2] : skip[3]);
-        return min(at * per + min((int) (fmaxf(in, 0.0f) * (float) per), per - 1), CAP - 1);
-    };
-    constexpr int E = CAP / PT;
-    for (int i = tid; i < CAP; i += PT) s.bucket[i] = 0;
-    __syncthreads();
-    uint64_t mine[E];
-    int to[E];
+            for (int k = 1; k < 4; ++k) v = b >= lo[k] ? k : v;
+            const float in = l == p.w.m ? 0.0f : fminf((p.w.m - l) * scale, (float) (BINS - 1)) - (float) b;
+            const int at = b - (v == 0 ? lo[0] : v == 1 ? lo[1] : v == 2 ? lo[2] : lo[3]) + (v == 0 ? skip[0] : v == 1 ? skip[1] : v == 2 ? skip[2] : skip[3]);
+            return min(at * per + min((int) (fmaxf(in, 0.0f) * (float) per), per - 1), CAP - 1);
+        };
+        uint64_t mine[CAP / PT];
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-        const int i = tid + j * PT;
-        mine[j] = i < n ? a.list[(size_t) row * CAP + i] : 0;
-        to[j] = i < n ? bucket_of(mine[j]) : 0;
-        if (i < n) atomicAdd(&s.bucket[to[j]], 1u);
-    }
-    __syncthreads();
-    uint32_t size[E], own = 0;
+        for (int j = 0; j < CAP / PT; ++j) mine[j] = tid + j * PT < n ? a.list[(size_t) row * CAP + tid + j * PT] : 0;
+        p.sort_buckets(mine, bucket_of, [&] {
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-        size[j] = s.bucket[E * tid + j];
-        own += size[j];
-    }
-    uint32_t start = block_sums(Sum{0, own}, s.part).count - own;
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-        s.bucket[E * tid + j] = start;                   // of the bucket; then, as tokens come, its end
-        start += size[j];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 4; ++k) in_list[k] = lo[k] < BINS ? (int) s.bucket[skip[k] * per] : CAP;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < E; ++j)
-        if (tid + j * PT < n) s.unsorted[atomicAdd(&s.bucket[to[j]], 1u)] = mine[j];
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < E; ++j)
-        if (tid + j * PT < n) {
-            const int first = to[j] > 0 ? (int) s.bucket[to[j] - 1] : 0, last = (int) s.bucket[to[j]];
-            int place = first;
-            for (int i = first; i < last; ++i) place += s.unsorted[i] > mine[j] ? 1 : 0;
-            s.token[place] = mine[j];
-        }
-    __syncthreads();
+            for (int k = 0; k < 4; ++k) in_list[k] = lo[k] < BINS ? (int) s.bucket[skip[k] * per] : CAP;
+        });
     }
     p.finish(q, row, n, &plan, in_list);
+}
+
+// Rows of at most SHORT logits: all of them sorted, one launch (14 rows of 2,042: 16 us against 25 in five; 64 rows of 4,096 took 31
+// against 26)
+template <int T>
+__global__ void __launch_bounds__(PT) sample_short_kernel(SampleArgs a) {
+    __shared__ PickShared s;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const void* const from = row_of<T>(a, row);
+    uint64_t mine[CAP / PT], best = 0;
+#pragma unroll
+    for (int j = 0; j < CAP / PT; ++j) {                 // places past SHORT stay empty
+        const int i = tid + j * PT;
+        const float l = i < a.vocab ? load_logit<T>(from, i) : -INFINITY;
+        mine[j] = l > -INFINITY ? order_u64(l, i) : 0;
+        best = max_u64(best, mine[j]);
+    }
+    const Params q = params_of(a, row);
+    if (tid == 0) s.n = 0;
+    fill_table(s.table);
+    best = wave_max_u64(best);
+    if (lane == 0) s.best[tid >> 6] = best;
+    __syncthreads();
+    best = wave_max_u64(lane < PT / 64 ? s.best[lane] : 0);
+    if (q.first || best == 0) {
+        if (tid == 0) {
+            a.ids[row] = best == 0 ? -1 : (int) ~(uint32_t) best;
+            if (a.probs) a.probs[row] = best == 0 ? 0.0f : 1.0f;
+        }
+        return;
+    }
+    unsigned own = 0;                                    // the wave's
+#pragma unroll
+    for (int j = 0; j < CAP / PT; ++j) own += (unsigned) __popcll(__ballot(mine[j] != 0));
+    if (lane == 0 && own) atomicAdd(&s.n, own);
+    Picker<T, false> p{a, s, from, weight_of(a, best, q.temp, s.table)};
+    const float m = p.w.m;
+    if (a.vocab <= PT / 4) {
+        if (tid < PT / 4) s.token[tid] = mine[0];        // none at all is smaller than any
+        __syncthreads();
+        p.sort_few(a.vocab);
+    } else p.sort_buckets(mine, [&](uint64_t token) {                   // by the distance from the best logit, 128 buckets an octave from 2^-8 on
+        const float l = key_value((uint32_t) (token >> 32)), d = l == m ? 0.0f : m - l;
+        return min(max((__builtin_bit_cast(int, d) >> 16) - ((127 - 8) << 7), 0), CAP - 1);
+    }, [] {});
+    const int none[4] = {0, 0, 0, 0};
+    p.finish(q, row, (int) s.n, nullptr, none);
 }
 
 template <int T, bool VEC>
@@ -1163,6 +1227,12 @@ extern "C" int wzy_sample(const void* logits, int type, int64_t ld, int rows, in
     if (!top_k) a.group = nullptr;
     a.F = 51;
     while (a.F > 40 && (int64_t) vocab > (1ll << (62 - a.F))) --a.F;
+    if (vocab <= SHORT)
+        return mx_with_type(type, [&](auto t) {
+            sample_short_kernel<t()><<<rows, PT, 0, as_stream(stream)>>>(a);
+            WZY_LAUNCH_CHECK();
+            return WZY_OK;
+        });
     const bool vec = (uintptr_t) logits % 16 == 0 && ld * n % 16 == 0;
     return mx_with_type(type, [&](auto t) { return vec ? launch<t(), true>(a, stream) : launch<t(), false>(a, stream); });
 }
