@@ -157,7 +157,8 @@ int wzy_paged_append(const wzy_paged_cache* cache, const wzy_rope_tab* rope, con
  * request's keep what they hold.  The batch is as wzy_paged_plan left it, `work` one of its lists (a list
  * that was built for other numbers has no work: nothing is written).
  * Sums are fp32; the softmax weights are rounded to the cache's type for the second product (half a step of a weight, so of
- * an output at most as much; fp16 weights are kept 2^6 above their smallest so that small ones are not lost).
+ * an output at most as much; fp16 weights are taken 2^6 larger, so that small ones are not lost).  A value that is not finite
+ * reaches only the rows that see its cell; a row whose scores are all -infinity becomes 0.
  * Page ids outside 0 .. n_pages - 1 count as page 0.  scale is finite and above 0. */
 size_t wzy_paged_attend_workspace_bytes(const wzy_paged_batch* batch, const wzy_paged_work* work);
 int wzy_paged_attend(const wzy_paged_cache* cache, const wzy_paged_batch* batch, const wzy_paged_work* work, const wzy_heads* q,

@@ -298,7 +298,7 @@ def test_append(wz, gpu, ct, t, rows, qh, kvh, hd, n_rot, pairs, by_head):
 
 # ---- attention -------------------------------------------------------------------------------------------
 def attend_case(wz, t, cached, new, qh, kvh, hd, page, window=0, by_head=False, seed=0, spread=1.0, max_tokens=None, free=None,
-                scale=None, max_new=None, special=None):
+                scale=None, max_new=None, special=None, space=FILL):
     """plan, append through numpy, attend; returns (got, want, bound) a request"""
     rng = np.random.default_rng(seed)
     n_pages = sum(-(-(c + n) // page) for c, n in zip(cached, new)) + 3
@@ -329,7 +329,9 @@ def attend_case(wz, t, cached, new, qh, kvh, hd, page, window=0, by_head=False, 
     out = DA.from_numpy(filled((b.max_tokens + 1, qh, hd + 8), np.uint16))
     scale = hd ** -0.5 if scale is None else scale
     nb = wz.wzy_paged_attend_workspace_bytes(ref(b.c), ref(w))
-    ws = DA.from_numpy(filled(nb + 64, np.uint8))
+    ws = filled(nb + 64, np.uint8)
+    ws[:nb] = space
+    ws = DA.from_numpy(ws)
     qs, os_ = wzy_amd.Heads(qd.ptr, qh * hd, hd), wzy_amd.Heads(out.ptr, qh * (hd + 8), hd + 8)
     wz.wzy_paged_attend(ref(cache.c), ref(b.c), ref(w), ref(qs), ref(os_), scale, ws.ptr, nb, None)
     got = out.numpy()
@@ -383,6 +385,37 @@ def test_attend_chunks(wz, gpu, t, hd, page):
 @pytest.mark.parametrize("hd", [64, 256])
 def test_attend_window(wz, gpu, window, hd):
     attend_case(wz, BF16, [0, 200, 1030, 3], [150, 1, 40, 1], 4, 2, hd, 16, window=window, seed=window)
+
+
+@pytest.mark.parametrize("window", [1, 2, 16, 31, 33, 64, 65])
+@pytest.mark.parametrize("qh,kvh,max_new", [(1, 1, 1), (3, 3, 40), (2, 1, 20)])
+def test_attend_short_window(wz, gpu, window, qh, kvh, max_new):
+    # windows of a block or two, of requests long enough for parts; what parts do not write would be a NaN in the workspace
+    cached = [0, 31, 32, 63, 95, 96, 100, 127, 128, 500, 1000]
+    attend_case(wz, BF16, cached, [1] * len(cached), qh, kvh, 64, 16, window=window, seed=window, max_new=max_new, space=255)
+    attend_case(wz, F16, cached, [2, 1, 3] * 3 + [1, 2], qh, kvh, 256, 32, window=window, seed=window, max_new=max_new + 2, space=255)
+
+
+def test_attend_parts_write_all_that_is_joined(wz, gpu):
+    # first tiles of a prompt have fewer blocks than its tiles have parts
+    attend_case(wz, BF16, [0, 3], [1500, 200], 1, 1, 64, 16, seed=1, space=255)
+    attend_case(wz, F16, [0, 3], [1500, 1], 2, 1, 128, 64, window=700, seed=2, space=255)
+
+
+def test_attend_refused_request_of_most_rows(wz, gpu):
+    # 2^31 pieces of 16 bytes to clear; all tokens' rows in one place, so that they fit
+    b = Batch(16, [3], [1 << 20], 1, 4, None)
+    w = b.work(wz, 256, 1, 64)
+    wz.wzy_paged_plan(ref(b.pool), ref(b.c), ref(w), 1, None)
+    assert b.read("served", 1)[0] == 0
+    cache = Cache(BF16, 4, 16, 1, 64).upload()
+    qd, out = DA(256 * 64, np.uint16, zero=True), DA.from_numpy(filled(257 * 64, np.uint16))
+    nb = wz.wzy_paged_attend_workspace_bytes(ref(b.c), ref(w))
+    ws = DA(nb, np.uint8)
+    qs, os_ = wzy_amd.Heads(qd.ptr, 0, 64), wzy_amd.Heads(out.ptr, 0, 64)
+    wz.wzy_paged_attend(ref(cache.c), ref(b.c), ref(w), ref(qs), ref(os_), 0.125, ws.ptr, nb, None)
+    got = out.numpy()
+    assert (got[:256 * 64] == 0).all() and (got[256 * 64:].view(np.uint8) == FILL).all()
 
 
 def test_attend_long_chunk_in_parts(wz, gpu):

@@ -387,10 +387,9 @@ WZY_DEV void plain_row(const AttnArgs& a, const TileCtx& t, int row, int lane, i
 // A request that is not served: all its rows become 0.
 template <int HD>
 WZY_DEV void zero_rows(const AttnArgs& a, const TileCtx& t) {
-    for (int i = threadIdx.x; i < t.it.n_new * a.g * (HD / 8); i += 256) {
-        const int row = i / (HD / 8);
-        *(v4w_t*) (out_row(a, t, row) + 16 * (i % (HD / 8))) = v4w_t{0, 0, 0, 0};
-    }
+    constexpr int L = HD / 8;                                           // threads a row
+    for (int row = threadIdx.x / L; row < t.it.n_new * a.g; row += 256 / L)
+        *(v4w_t*) (out_row(a, t, row) + 16 * (threadIdx.x % L)) = v4w_t{0, 0, 0, 0};
 }
 // A lane's results: its row's columns in 16-byte (a part: fp32) or 8-byte pieces
 template <int HD, int T>
@@ -428,7 +427,7 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     TileCtx t;
     if (!tile_ctx(a, 0, t)) return;
-    if (t.it.lo >= t.it.hi) {
+    if (t.it.part < 0 && t.it.lo >= t.it.hi) {
         zero_rows<HD>(a, t);
         return;
     }
@@ -530,7 +529,7 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave & 1, pair = wave >> 1;
     TileCtx t;
     if (!tile_ctx(a, 0, t)) return;
-    if (t.it.lo >= t.it.hi) {
+    if (t.it.part < 0 && t.it.lo >= t.it.hi) {
         zero_rows<HD>(a, t);
         return;
     }

@@ -93,9 +93,11 @@ WZY_DEV Cut cut_of(const PlanWork& w, int c, int n, bool served, const int (&par
     const int rows = n * w.g;
     x.kind = rows <= w.l.narrow || !served ? 0 : 1;
     x.tiles = rows == 0 ? 0 : x.kind ? (rows + PG_WIDE - 1) / PG_WIDE : 1;
-    // blocks of 32 cells that a tile sees, at most: the last one's end, or as many as its tokens' windows span
+    // blocks of 32 cells that a tile sees: of a narrow one, which is its request's only one, just so many; of a wide one at most, the
+    // last one's end or as many as its tokens' windows span
     x.blocks = served ? (c + n + 31) >> 5 : 0;
-    if (w.window > 0) x.blocks = min(x.blocks, ((w.window + (int) ((uint32_t) (x.kind ? PG_WIDE : w.l.narrow) / (uint32_t) w.g)) >> 5) + 2);
+    if (w.window > 0 && served)
+        x.blocks = x.kind ? min(x.blocks, ((w.window + (int) ((uint32_t) PG_WIDE / (uint32_t) w.g)) >> 5) + 2) : x.blocks - (max(c + 1 - w.window, 0) >> 5);
     const int p = part[x.kind];
     x.parts = p > 0 && x.blocks > p ? (x.blocks + p - 1) / p : 1;
     return x;

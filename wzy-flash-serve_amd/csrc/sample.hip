@@ -12,7 +12,8 @@
 //                  groups above it are all that has to be read again; they get their token here
 //   sample_gather  the slices again: tokens of those bins to the row's list
 //   sample_pick    a workgroup a row: the list sorted, sums, places
-// Rows of at most SHORT logits are sorted whole, by one launch.  Rows whose bins hold more than CAP tokens (thousands of equal logits) are done by sample_pick alone, from the row.
+// Rows of at most SHORT logits are sorted whole, by one launch.  Rows whose bins hold more than CAP tokens (thousands of equal
+// logits) are done by sample_pick alone, from the row.
 // w is taken in 64 bits (fp32's 1e-7 would move one draw in a thousand of a flat row) and summed as integers of 2^-F, F = 62 -
 // log2(vocab), at most 51: sums do not depend on their order, so LDS and memory atomics may add them as they come.  Where top-k is
 // small, everything it leaves is gathered, and the histogram counts only.
@@ -25,7 +26,7 @@ using namespace wzy;
 namespace {
 constexpr int ST = 256, PER = 32, SLICE = ST * PER;      // sample_max, sample_hist
 constexpr int PT = 1024, CAP = 4096;                     // sample_pick; tokens gathered at most
-constexpr int SHORT = 2048;                               // rows of up to so many logits are sorted whole
+constexpr int SHORT = 2048;                              // rows of up to so many logits are sorted whole
 constexpr int GROUP_K = CAP / PER;                       // top-k up to which the groups' largest tokens say what to gather
 constexpr int SMALL_K = 2048;                            // top-k up to which all that it leaves is gathered
 constexpr int BINS = 1024;                               // 64 octaves of w
@@ -1115,8 +1116,8 @@ __global__ void __launch_bounds__(PT) sample_pick_kernel(SampleArgs a) {
     p.finish(q, row, n, &plan, in_list);
 }
 
-// Rows of at most SHORT logits: all of them sorted, one launch (14 rows of 2,042: 16 us against 25 in five; 64 rows of 4,096 took 31
-// against 26)
+// Rows of at most SHORT logits: all of them sorted, one launch (14 rows of 2,042: 11 to 13 us against 25 in five launches, 100
+// logits 6 to 7; 64 rows of 4,096 take 26 to 28 either way)
 template <int T>
 __global__ void __launch_bounds__(PT) sample_short_kernel(SampleArgs a) {
     __shared__ PickShared s;
