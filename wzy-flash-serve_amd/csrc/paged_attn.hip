@@ -175,7 +175,8 @@ struct Loader {
         piece_v = (piece ^ (BV::swap(r0) << BV::SHIFT)) * 16;
     }
     WZY_DEV const char* cell(int c) const {
-        int id = t.pages[c >> a.lp];
+        // through the scalar cache: a vector load would be waited for together with the keys and values on their way
+        int id = ((const __attribute__((address_space(4))) int*) t.pages)[__builtin_amdgcn_readfirstlane(c >> a.lp)];
         id = (unsigned) id < (unsigned) a.n_pages ? id : 0;
         return a.k + (int64_t) id * a.ld_page + (int64_t) (c & ((1 << a.lp) - 1)) * a.ld_cell + (int64_t) t.head * a.ld_head;
     }
@@ -238,6 +239,9 @@ struct Wave {
         const char* const p = a.q + (int64_t) (t.it.q0 + token) * a.ldq + (int64_t) (t.head * a.g + h) * a.ldq_head + (lane >> 5) * 16;
 #pragma unroll
         for (int s = 0; s < KS; ++s) q[s] = row < rows ? *(const v4w_t*) (p + 32 * s) : v4w_t{0, 0, 0, 0};
+        // taken here: else the compiler waits for them in the loop, each time, and for the keys on their way with them
+#pragma unroll
+        for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[s]));
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = v16f_t{};
         m = -INFINITY;
