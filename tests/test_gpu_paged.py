@@ -227,6 +227,29 @@ def test_rope(wz, gpu, pairs, t, rows, heads, hd, n_rot, gap):
     np.testing.assert_array_equal(xd.numpy(), got)
 
 
+@pytest.mark.parametrize("pairs", [0, 1])
+@pytest.mark.parametrize("t,rows", [(F32, 2100), (BF16, 4201), (F16, 4201)])
+def test_rope_large_call_equals_small_ones(wz, gpu, t, rows, pairs):
+    # more than 32 MB of output: the same bits as calls of 1,000 rows, in place too
+    rng = np.random.default_rng(rows)
+    heads, hd, n_rot = 32, 128, 96
+    bits = typed(rng.standard_normal((rows, heads, hd)), t)[0]
+    size, pd = bits.itemsize, ints(rng.integers(0, 2 ** 20, rows))
+    f = freqs(wz, n_rot)
+    tab = wzy_amd.RopeTab(f.ptr, n_rot, pairs)
+    xd, one, many = DA.from_numpy(bits), DA.from_numpy(filled(bits.shape, bits.dtype)), DA.from_numpy(filled(bits.shape, bits.dtype))
+
+    def rows_of(d, r):
+        return wzy_amd.Heads(d.ptr + r * heads * hd * size, heads * hd, hd)
+    assert rows * heads * hd * size > 32 << 20
+    for r in range(0, rows, 1000):
+        wz.wzy_rope(ref(tab), ref(rows_of(xd, r)), t, min(1000, rows - r), heads, hd, pd.ptr + 4 * r, ref(rows_of(many, r)), None)
+    wz.wzy_rope(ref(tab), ref(rows_of(xd, 0)), t, rows, heads, hd, pd.ptr, ref(rows_of(one, 0)), None)
+    wz.wzy_rope(ref(tab), ref(rows_of(xd, 0)), t, rows, heads, hd, pd.ptr, ref(rows_of(xd, 0)), None)
+    np.testing.assert_array_equal(one.numpy(), many.numpy())
+    np.testing.assert_array_equal(xd.numpy(), many.numpy())
+
+
 class Cache:
     """K and V of [page][cell][head] or [page][head][cell], gaps between, all NaN to begin with"""
 
@@ -294,6 +317,29 @@ def test_append(wz, gpu, ct, t, rows, qh, kvh, hd, n_rot, pairs, by_head):
     for g in (gk, gv):                                                    # nothing else is touched
         c.rows(g)[at // page, at % page] = NAN[ct]
         assert (g == NAN[ct]).all()
+
+
+@pytest.mark.parametrize("t,ct", [(F32, BF16), (BF16, BF16), (F16, F16)])
+def test_append_large_call_equals_small_ones(wz, gpu, t, ct):
+    rng = np.random.default_rng(t)
+    rows, qh, kvh, hd, n_rot, page = 3001, 24, 2, 256, 64, 64
+    n_pages, ld = 50, (qh + 2 * kvh) * hd
+    bits = typed(rng.standard_normal((rows, qh + 2 * kvh, hd)), t)[0]
+    size, xd, pd = bits.itemsize, DA.from_numpy(bits), ints(rng.integers(0, 300000, rows))
+    sd = ints(rng.permutation(n_pages * page)[:rows])
+    f = freqs(wz, n_rot, 0, 1e6)
+    tab = wzy_amd.RopeTab(f.ptr, n_rot, 0)
+    assert rows * ld * 2 > 32 << 20
+    got = []
+    for step in (rows, 500):
+        c, qo = Cache(ct, n_pages, page, kvh, hd).upload(), DA.from_numpy(filled((rows, qh, hd), np.uint16))
+        for r in range(0, rows, step):
+            q, k, v = (wzy_amd.Heads(xd.ptr + (r * ld + at * hd) * size, ld, hd) for at in (0, qh, qh + kvh))
+            qs = wzy_amd.Heads(qo.ptr + 2 * r * qh * hd, qh * hd, hd)
+            wz.wzy_paged_append(ref(c.c), ref(tab), ref(q), qh, ref(qs), ref(k), ref(v), t, min(step, rows - r), pd.ptr + 4 * r, sd.ptr + 4 * r, None)
+        got.append((qo.numpy(), c.dk.numpy(), c.dv.numpy()))
+    for x, y in zip(*got):
+        np.testing.assert_array_equal(x, y)
 
 
 # ---- attention -------------------------------------------------------------------------------------------

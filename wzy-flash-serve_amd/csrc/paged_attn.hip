@@ -11,10 +11,17 @@
 //
 // Rows are (token, head of the group) pairs of one key head, so a group's heads share every byte of K and V.
 //   narrow  up to 32 rows: the waves of a workgroup take every fourth block of 32 keys each, through buffers of their own,
-//           with no barrier until their results are joined
+//           with no barrier until their results are joined.  Bound by memory: 64 single tokens of requests of up to 6,000 cells,
+//           8 key heads of 128, 280 us (5.5 TB/s).  One of 32,768 cells, 2 heads of 256, 18 us and 7 for the merge of its 256 parts:
+//           67 MB in one wave of workgroups, whose first loads and joins are half of it
 //   middle  up to 64 rows, where no request of the step has more (verify windows): two waves share a block, the two pairs take
-//           every other one
-//   wide    128 rows, 32 a wave: the workgroup's waves share each block
+//           every other one.  16 windows of 4 tokens x 12 heads of 256 over 4,096 cells: 32 us and 7 for the merge (with the wide form,
+//           whose tiles would hold 80 empty rows, 47 for both before it was there and 40 after).  Bound by memory and the start of
+//           each part
+//   wide    128 rows, 32 a wave: the workgroup's waves share each block.  2,047 tokens x 12 heads of 256 behind 30,001 cells:
+//           1,440 us, 1,085 TFLOP/s (a library's 8,192^3 product: 1,184); prompts, heads of 128: 950 us, 930 TFLOP/s.  Bound by the
+//           matrix cores and the vector units' exponentials in turn: neither fewer operations a block nor fewer LDS reads (64 rows
+//           a wave, in twice the registers: 1,255 us for the prompts) make it faster.  256 rows on 8 waves: 1,185
 // The maximum follows the scores only when one has come 2^8 above it, so most blocks leave the accumulators alone; weights
 // then reach 2^8, and in fp16, whose numbers end at 2^-24, all are taken 2^6 larger.
 #include <algorithm>

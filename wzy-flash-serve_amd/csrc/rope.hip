@@ -6,12 +6,17 @@
 // way, goes into the Taylor polynomials of sine and cosine in 64 bits (to x^13 and x^14: 2e-14).  They are made once a row, by
 // one thread an angle, and kept in LDS for all heads of the row: at far positions fp32 angles would be off by whole turns.
 // The rows are read and written once, 8 elements (and their partners) a thread where alignment allows 16-byte accesses, a pair
-// a thread elsewhere.  Bound by memory at large sizes, by the launch at one row.
+// a thread elsewhere.  Bound by memory at large sizes, by the launch at one row: a row of 24 + 2 + 2 heads of 256 from fp32 2.7 us,
+// 8,192 of them in bf16 40 us where part of them is still in a cache and 62 where none is (235 MB; a copy of as much: 45), 4,097 rows of 32 heads of
+// 128 in fp16 12.5 us (67 MB, 5.4 TB/s).
 #include <algorithm>
 
 #include "wzy_paged.h"
 
 using namespace wzy;
+
+typedef float v4f_t __attribute__((ext_vector_type(4)));
+typedef uint32_t v4w_t __attribute__((ext_vector_type(4)));
 
 namespace {
 constexpr int RT = 256, ROPE_MAX = 512;
@@ -29,6 +34,7 @@ struct RopeArgs {
     FastDiv div_row, div_head;
     int64_t ld_page, n_cells;
     int lp, rows_block;
+    bool stream;                          // stores past the caches
 };
 
 // cos and sin of 2 pi x, amplitude in
@@ -60,6 +66,23 @@ WZY_DEV void store1(void* p, size_t i, float v) {
     if constexpr (T == WZY_F32) ((float*) p)[i] = v;
     else if constexpr (T == WZY_BF16) ((uint16_t*) p)[i] = (uint16_t) pack2<WZY_BF16>(v, v);
     else ((uint16_t*) p)[i] = f_to_h16(v);
+}
+
+// 8 elements; stream: past the caches, which hold less than the call writes (8,192 rows of 24 + 2 + 2 heads of 256 in bf16, buffers
+// changing from call to call: 68 -> 62 us, 4,097 of 32 of 128 17.4 -> 12.6; the loads likewise: no faster, and 20 us slower where the
+// rows are still in a cache)
+template <int T>
+WZY_DEV void store_wide(void* p, size_t i, const float (&v)[8], bool stream) {
+    if (!stream) {
+        store8<T>(p, i, v);
+        return;
+    }
+    if constexpr (T == WZY_F32) {
+        __builtin_nontemporal_store(v4f_t{v[0], v[1], v[2], v[3]}, (v4f_t*) ((float*) p + i));
+        __builtin_nontemporal_store(v4f_t{v[4], v[5], v[6], v[7]}, (v4f_t*) ((float*) p + i) + 1);
+    } else
+        __builtin_nontemporal_store(v4w_t{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])},
+                                    (v4w_t*) ((uint16_t*) p + i));
 }
 
 // A piece of a row: WIDE, 8 elements and, in rotated halves, the 8 they pair with; else a pair or one element.
@@ -128,8 +151,8 @@ struct Piece {
             to = (size_t) (slot >> a.lp) * a.ld_page + (size_t) (slot & ((1 << a.lp) - 1)) * a.out[1].ld + (size_t) h * a.out[1].ldh;
         }
         if constexpr (WIDE) {
-            store8<TO>(dst, to + e0, u);
-            if (!PAIRS && e1 >= 0) store8<TO>(dst, to + e1, v);
+            store_wide<TO>(dst, to + e0, u, a.stream);
+            if (!PAIRS && e1 >= 0) store_wide<TO>(dst, to + e1, v, a.stream);
         } else {
             store1<TO>(dst, to + e0, u[0]);
             if (e1 >= 0) store1<TO>(dst, to + e1, v[0]);
@@ -209,8 +232,9 @@ int launch(RopeArgs a, bool pairs, bool wide, void* stream) {
     a.div_row = FastDiv((uint32_t) a.per_row);
     a.div_head = FastDiv((uint32_t) a.per_head);
     int rb = 1;
-    while (rb * a.per_row < 4 * RT && 2 * rb * half <= ROPE_MAX && a.rows / (2 * rb) >= 512) rb *= 2;
+    while (rb * a.per_row < 2 * RT && 2 * rb * half <= ROPE_MAX && a.rows / (2 * rb) >= 512) rb *= 2;
     a.rows_block = rb;
+    a.stream = (int64_t) a.rows * heads * a.hd * mx_type_bytes(TO) > 32 << 20;
     // few rows: a row's pieces to several workgroups, each with angles of its own
     const int blocks = (a.rows + rb - 1) / rb, share = blocks >= 512 ? 1 : std::min((a.per_row * rb + RT - 1) / RT, 512 / blocks);
     const dim3 grid((unsigned) blocks, (unsigned) share);
