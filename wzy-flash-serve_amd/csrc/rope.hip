@@ -7,8 +7,8 @@
 // one thread an angle, and kept in LDS for all heads of the row: at far positions fp32 angles would be off by whole turns.
 // The rows are read and written once, 8 elements (and their partners) a thread where alignment allows 16-byte accesses, a pair
 // a thread elsewhere.  Bound by memory at large sizes, by the launch at one row: a row of 24 + 2 + 2 heads of 256 from fp32 2.7 us,
-// 8,192 of them in bf16 40 us where part of them is still in a cache and 62 where none is (235 MB; a copy of as much: 45), 4,097 rows of 32 heads of
-// 128 in fp16 12.5 us (67 MB, 5.4 TB/s).
+// 8,192 of them in bf16 42 us where part of them is still in a cache and 65 where none is (235 MB; a copy of as much: 45), 4,097 rows
+// of 32 heads of 128 in fp16 12.5 us (67 MB, 5.4 TB/s).
 #include <algorithm>
 
 #include "wzy_paged.h"
@@ -69,7 +69,7 @@ WZY_DEV void store1(void* p, size_t i, float v) {
 }
 
 // 8 elements; stream: past the caches, which hold less than the call writes (8,192 rows of 24 + 2 + 2 heads of 256 in bf16, buffers
-// changing from call to call: 68 -> 62 us, 4,097 of 32 of 128 17.4 -> 12.6; the loads likewise: no faster, and 20 us slower where the
+// changing from call to call: 68 -> 65 us, 4,097 of 32 of 128 17.4 -> 12.8; the loads likewise: no faster, and 20 us slower where the
 // rows are still in a cache)
 template <int T>
 WZY_DEV void store_wide(void* p, size_t i, const float (&v)[8], bool stream) {

@@ -1,10 +1,9 @@
 """ctypes bindings of libwzy_amd.so, the MI355X decode-path library.
 
 The C ABI (include/wzy_kernels.h, include/wzy_mx.h, include/wzy_paged.h, include/wzy_synth.h,
-include/wzy_stage.h) takes plain pointers and
-sizes; these bindings pass integers (device pointers from any allocator, numpy buffer addresses)
-and raise WzyError on a negative status.  Loading fails loudly when the shared library has not been
-built: there is no CPU fallback behind this module.
+include/wzy_stage.h) takes plain pointers and sizes; these bindings pass integers (device pointers
+from any allocator, numpy buffer addresses) and raise WzyError on a negative status.  Loading fails
+loudly when the shared library has not been built: there is no CPU fallback behind this module.
 """
 import ctypes as C
 import os
