@@ -14,10 +14,13 @@
 //   sample_pick    a workgroup a row: the list sorted, sums, places
 // Rows of at most SHORT logits are sorted whole, by one launch.  Rows whose bins hold more than CAP tokens (thousands of equal
 // logits) are done by sample_pick alone, from the row.
+// 256 rows of 151,936 fp32 logits with top-p: 25 + 42 + 8 + 28 + 10 us; the first and fourth are bound by memory (6 TB/s), the second
+// by its 64-bit operations and LDS atomics.  4 rows with top-k: 4 + 2 + 10 + 1 + 1, bound by latencies.
 // w is taken in 64 bits (fp32's 1e-7 would move one draw in a thousand of a flat row) and summed as integers of 2^-F, F = 62 -
 // log2(vocab), at most 51: sums do not depend on their order, so LDS and memory atomics may add them as they come.  Where top-k is
 // small, everything it leaves is gathered, and the histogram counts only.
 #include <algorithm>
+#include <type_traits>
 
 #include "wzy_paged.h"
 
@@ -30,7 +33,8 @@ constexpr int SHORT = 2048;                              // rows of up to so man
 constexpr int GROUP_K = CAP / PER;                       // top-k up to which the groups' largest tokens say what to gather
 constexpr int SMALL_K = 2048;                            // top-k up to which all that it leaves is gathered
 constexpr int BINS = 1024;                               // 64 octaves of w
-constexpr float BIN_OCT = 16.0f;
+constexpr float BIN_OCT = 16.0f;                         // bins an octave; a bin's tokens are within 1/32 of a bin of its ends
+constexpr float BIN_SLACK = 1.0f / 32;
 constexpr float GREEDY = 1e-5f;
 constexpr uint32_t KEY_NONE = 0x007FFFFFu;               // order key of -infinity
 
@@ -94,37 +98,43 @@ WZY_DEV float key_value(uint32_t k) {
 WZY_DEV uint64_t order_u64(float v, int i) { return (uint64_t) order_key(v) << 32 | (uint32_t) ~i; }
 
 // 2^(-j / STEPS)
-constexpr int LSTEPS = 8, STEPS = 1 << LSTEPS;
+constexpr int LSTEPS = 8, STEPS = 1 << LSTEPS, BIN_STEPS_LOG2 = LSTEPS - 4;
 WZY_DEV void fill_table(double* s) {
     for (int i = threadIdx.x; i < STEPS; i += blockDim.x) s[i] = exp2(-(double) i / STEPS);
 }
-// A row's weights: m its largest logit, c = log2(e) / temp.  The bin is taken in fp32, which is monotone too.
+// A row's weights: m its largest logit, c = log2(e) / temp.  A token's 256 x, rounded, gives its bin and its weight.
 struct Weight {
+    static constexpr double MAGIC = 6755399441055744.0;  // 1.5 2^52: adding it rounds to an integer and leaves it in the low bits
     float m, cf;
     double cs;                                           // STEPS log2(e) / temp
     int F;
     const double* table;
-    WZY_DEV int bin(float l) const {
-        const float x = l == m ? 0.0f : (m - l) * cf * BIN_OCT;
-        return (int) fminf(x, (float) (BINS - 1));
+    // 256 x, at most 1,000 octaves, and that for what is not a number.  ANY: m may be infinite
+    template <bool ANY = true>
+    WZY_DEV double steps(float l) const {
+        const double t = ((double) m - (double) l) * cs;
+        return fmin(ANY && l == m ? 0.0 : t, 1000.0 * STEPS);
     }
+    static WZY_DEV int rounded(double n) { return (int) (uint32_t) __builtin_bit_cast(uint64_t, n); }
+    static WZY_DEV int bin_at(double t) { return min(rounded(t + MAGIC) >> BIN_STEPS_LOG2, BINS - 1); }
+    WZY_DEV int bin(float l) const { return bin_at(steps(l)); }
     // 2^-x as an integer of 2^-F: 256 x = k + r, |r| <= 1/2; 2^(-r / 256) by its series, whose fourth term is 2e-13 at most; 2^-(k / 256)
-    // from the table and the exponent field.  Adding 1.5 2^52 rounds to an integer and leaves it in the low bits.
-    WZY_DEV uint64_t fixed(float l) const {
-        return __builtin_bit_cast(uint64_t, scaled(l, F) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+    // from the table and the exponent field.
+    WZY_DEV uint64_t fixed_at(double t) const {
+        return __builtin_bit_cast(uint64_t, scaled_at(t, F) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
     }
+    WZY_DEV uint64_t fixed(float l) const { return fixed_at(steps(l)); }
     WZY_DEV double w(float l) const { return scaled(l, 0); }
-    WZY_DEV double scaled(float l, int f) const {
-        constexpr double MAGIC = 6755399441055744.0, A = -0.6931471805599453094 / STEPS;
-        const double t = (l == m ? 0.0 : (double) m - (double) l) * cs;
+    WZY_DEV double scaled(float l, int f) const { return scaled_at(steps(l), f); }
+    WZY_DEV double scaled_at(double t, int f) const {
+        constexpr double A = -0.6931471805599453094 / STEPS;
         const double n = t + MAGIC, r = t - (n - MAGIC);
-        const int i = (int) (uint32_t) __builtin_bit_cast(uint64_t, n);
+        const int i = rounded(n);
         double p = __builtin_fma(r, A * A * A / 6.0, A * A / 2.0);
         p = __builtin_fma(p, r, A);
         const uint64_t b = __builtin_bit_cast(uint64_t, table[i & (STEPS - 1)]) + ((uint64_t) (uint32_t) ((f - (i >> LSTEPS)) << 20) << 32);
         const double base = __builtin_bit_cast(double, b);                   // 2^-1000 at least: no denormal
-        const double v = __builtin_fma(base * r, p, base);
-        return t < 1000.0 * STEPS ? v : 0.0;
+        return __builtin_fma(base * r, p, base);
     }
 };
 WZY_DEV Params params_of(const SampleArgs& a, int row) {
@@ -340,9 +350,9 @@ WZY_DEV void plan_row(const Params& q, const uint64_t* mass, const uint32_t* cou
             within(lo[1], hi[1]);
         }
         if (q.cut_m()) {
-            // the bins are taken in fp32, to 1e-3 of a bin
+            // log2f in fp32: to 1e-3 of a bin
             const float x = -log2f(q.min_p) * BIN_OCT;
-            const int b0 = (int) fmaxf(x - 0.02f, 0.0f), b1 = (int) (x + 0.02f);
+            const int b0 = (int) fmaxf(x - BIN_SLACK - 0.01f, 0.0f), b1 = (int) (x + BIN_SLACK + 0.01f);
             if (b1 < BINS - 1 && b0 <= last) {
                 lo[2] = m0 = b0;
                 hi[2] = m1 = b1;
@@ -418,14 +428,18 @@ __global__ void __launch_bounds__(ST) sample_hist_kernel(SampleArgs a) {
     // one: no branch an element.
     const int lane = tid & 63;
     uint32_t far = 0;
-    if (masses)
+    auto add_masses = [&](auto any) {
         each_unit<T, VEC>(a, row, slice, [&](const float (&x)[PER], int) {
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                const int b = w.bin(x[j]);
-                atomicAdd(&s_mass[b == BINS - 1 ? BINS + lane : b], (unsigned long long) w.fixed(x[j]));
+                const double t = w.template steps<any()>(x[j]);
+                const int b = Weight::bin_at(t);
+                atomicAdd(&s_mass[b == BINS - 1 ? BINS + lane : b], (unsigned long long) w.fixed_at(t));
             }
         });
+    };
+    if (masses && w.m < INFINITY) add_masses(std::false_type{});
+    else if (masses) add_masses(std::true_type{});
     if (counts)
         each_unit<T, VEC>(a, row, slice, [&](const float (&x)[PER], int) {
 #pragma unroll
@@ -1026,8 +1040,9 @@ __global__ void __launch_bounds__(PT) sample_plan_kernel(SampleArgs a) {
         const int j = tid >> 1, b = tid & 1 ? s_plan.lo[j] - 1 : s_plan.hi[j];
         auto at_most = [&](uint32_t k) { return w.bin(key_value(k)) <= b; };
         uint32_t lo = KEY_NONE, hi = (uint32_t) (best >> 32) + 1;             // lo is not, hi is (or past the best one)
-        const uint32_t at = order_key(w.m - (float) (b + 1) / (w.cf * BIN_OCT));
-        const uint32_t from = at > lo + 128 ? at - 128 : lo, to = at + 128 < hi && at + 128 > at ? at + 128 : hi;
+        constexpr uint32_t NEAR = 4;
+        const uint32_t at = order_key((float) ((double) w.m - ((double) ((b + 1) << BIN_STEPS_LOG2) - 0.5) / w.cs));
+        const uint32_t from = at > lo + NEAR ? at - NEAR : lo, to = at + NEAR < hi && at + NEAR > at ? at + NEAR : hi;
         if (from > lo && from < hi && !at_most(from)) lo = from;
         if (to > lo && to < hi && at_most(to)) hi = to;
         while (hi - lo > 1) {
@@ -1101,7 +1116,7 @@ __global__ void __launch_bounds__(PT) sample_pick_kernel(SampleArgs a) {
             int v = 0;
 #pragma unroll
             for (int k = 1; k < 4; ++k) v = b >= lo[k] ? k : v;
-            const float in = l == p.w.m ? 0.0f : fminf((p.w.m - l) * scale, (float) (BINS - 1)) - (float) b;
+            const float in = l == p.w.m ? 0.0f : fminf((p.w.m - l) * scale, (float) (BINS - 1)) + BIN_SLACK - (float) b;
             const int at = b - (v == 0 ? lo[0] : v == 1 ? lo[1] : v == 2 ? lo[2] : lo[3]) + (v == 0 ? skip[0] : v == 1 ? skip[1] : v == 2 ? skip[2] : skip[3]);
             return min(at * per + min((int) (fmaxf(in, 0.0f) * (float) per), per - 1), CAP - 1);
         };
