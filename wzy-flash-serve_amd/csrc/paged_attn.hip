@@ -75,6 +75,7 @@ template <> struct Half<WZY_F16> {
 };
 constexpr float RISE = 8.0f;
 constexpr int MERGE_THREADS = 256, MERGE_LOADS = 8;       // of a part's row, under way at once
+constexpr unsigned MERGE_SHARED = 1024;                   // workgroups of a merge, up to which they share rows
 
 WZY_DEV uint32_t lds_offset(const void* p) { return (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) char*) p; }
 // 64 lanes x 16 bytes to LDS lds .. lds + 1023 in lane order, from a wave-uniform base + off, or from an address a lane
@@ -667,8 +668,10 @@ __global__ void __launch_bounds__(256, 2) paged_wide_kernel(AttnArgs a) {
     put_row<HD, T>(a, t, w, half_sum(w.l), lane, PG_WIDE);
 }
 
-// Parts of a tile joined.  HD / 4 lanes hold a row; of a workgroup's groups of lanes, several take one row's parts in turn where
-// there are many, so that all of a row's loads are under way at once.
+// Parts of a tile joined.  COLS / 4 lanes hold COLS columns of a row; of a workgroup's groups of lanes, several take one row's parts in
+// turn where there are many, so that all of a row's loads are under way at once.  Where all workgroups run at once, a row is shared by
+// HD / 64 of them (one token's 12 rows of 128 parts in each of 2 heads: 7 -> 5.5 us; 16 verify windows, which would have 6,144
+// workgroups: 7 -> 9), else it is one's.  Bound by latency: the list's entry, then a round of loads.
 struct MergeArgs {
     unsigned blocks;                         // of narrow tiles
     int narrow;                              // rows of a narrow tile
@@ -676,14 +679,14 @@ struct MergeArgs {
     const float* wide_o;
     const float2* wide_ml;
 };
-template <int HD, int T>
+template <int HD, int T, int COLS>
 __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(AttnArgs a, MergeArgs g) {
-    constexpr int L = HD / 4, GROUPS = MERGE_THREADS / L;
+    constexpr int L = COLS / 4, GROUPS = MERGE_THREADS / L, SLICES = HD / COLS;
     __shared__ float4 s_o[MERGE_THREADS];
     __shared__ float2 s_ml[GROUPS];
     // narrow tiles' workgroups first, by rows_y of them a tile; then wide ones'
     const int kind = blockIdx.x >= g.blocks ? 1 : 0, rows_y = g.rows_y[kind], ROWS = kind ? PG_WIDE : g.narrow;
-    const unsigned in = blockIdx.x - (kind ? g.blocks : 0), tile = in / (unsigned) rows_y, y = in - tile * (unsigned) rows_y;
+    const unsigned in = (blockIdx.x - (kind ? g.blocks : 0)) / SLICES, tile = in / (unsigned) rows_y, y = in - tile * (unsigned) rows_y;
     const int at = (int) (tile / (unsigned) a.kvh), head = (int) (tile - (unsigned) at * (unsigned) a.kvh);
     const PgHead h = *a.head;
     const PgMerge e = ((const PgMerge*) (a.head + 1))[g.at[kind] + at];
@@ -695,7 +698,8 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(AttnArgs a, 
     const float2* const part_ml = kind ? g.wide_ml : a.part_ml;
     int per = 1;                                                        // groups a row
     while (per < GROUPS && per * MERGE_LOADS < e.n) per *= 2;
-    const int rows_here = GROUPS / per, group = threadIdx.x / L, col = threadIdx.x % L, sub = group & (per - 1);
+    const int rows_here = GROUPS / per, group = threadIdx.x / L, sub = group & (per - 1);
+    const int col = (int) (blockIdx.x % SLICES) * L + (int) (threadIdx.x % L);
     for (int r0 = (int) y * rows_here; r0 < e.rows; r0 += rows_y * rows_here) {
         const int r = min(r0 + group / per, e.rows - 1);
         float m = -INFINITY, l = 0.0f;
@@ -730,7 +734,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(AttnArgs a, 
         }
         if (per > 1) {
             s_o[threadIdx.x] = o;
-            if (col == 0) s_ml[group] = make_float2(m, l);
+            if (threadIdx.x % L == 0) s_ml[group] = make_float2(m, l);
             __syncthreads();
             if (sub == 0) {
                 float to = m;
@@ -798,10 +802,16 @@ int launch(AttnArgs a, const PgLayout& l, const Space& s, char* space, int max_r
     if (blocks[0] + blocks[1] == 0) return WZY_OK;
     a.part_o = (float*) (space + s.o[0]);
     a.part_ml = (float2*) (space + s.ml[0]);
-    g.blocks = blocks[0];
     g.wide_o = (const float*) (space + s.o[1]);
     g.wide_ml = (const float2*) (space + s.ml[1]);
-    paged_merge_kernel<HD, T><<<blocks[0] + blocks[1], MERGE_THREADS, 0, st>>>(a, g);
+    const unsigned all = blocks[0] + blocks[1];
+    if (HD > 64 && all * (HD / 64) <= MERGE_SHARED) {
+        g.blocks = blocks[0] * (HD / 64);
+        paged_merge_kernel<HD, T, 64><<<all * (HD / 64), MERGE_THREADS, 0, st>>>(a, g);
+    } else {
+        g.blocks = blocks[0];
+        paged_merge_kernel<HD, T, HD><<<all, MERGE_THREADS, 0, st>>>(a, g);
+    }
     WZY_LAUNCH_CHECK();
     return WZY_OK;
 }
