@@ -12,7 +12,7 @@
 // Rows are (token, head of the group) pairs of one key head, so a group's heads share every byte of K and V.
 //   narrow  up to 32 rows: the waves of a workgroup take every fourth block of 32 keys each, through buffers of their own,
 //           with no barrier until their results are joined.  Bound by memory: 64 single tokens of requests of up to 6,000 cells,
-//           8 key heads of 128, 280 us (5.5 TB/s).  One of 32,768 cells, 2 heads of 256, 18 us and 7 for the merge of its 256 parts:
+//           8 key heads of 128, 280 us (5.5 TB/s).  One of 32,768 cells, 2 heads of 256, 18 us and 6 for the merge of its 256 parts:
 //           67 MB in one wave of workgroups, whose first loads and joins are half of it
 //   middle  up to 64 rows, where no request of the step has more (verify windows): two waves share a block, the two pairs take
 //           every other one.  16 windows of 4 tokens x 12 heads of 256 over 4,096 cells: 32 us and 7 for the merge (with the wide form,

@@ -7,7 +7,7 @@
 // one thread an angle, and kept in LDS for all heads of the row: at far positions fp32 angles would be off by whole turns.
 // The rows are read and written once, 8 elements (and their partners) a thread where alignment allows 16-byte accesses, a pair
 // a thread elsewhere.  Bound by memory at large sizes, by the launch at one row: a row of 24 + 2 + 2 heads of 256 from fp32 2.7 us,
-// 8,192 of them in bf16 42 us where part of them is still in a cache and 65 where none is (235 MB; a copy of as much: 45), 4,097 rows
+// 8,192 of them in bf16 42 us where part of them is still in a cache and 64 where none is (235 MB; a copy of as much: 45), 4,097 rows
 // of 32 heads of 128 in fp16 12.5 us (67 MB, 5.4 TB/s).
 #include <algorithm>
 
