@@ -306,18 +306,29 @@ struct Wave {
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i / 4][i % 4] = pack2<T>(s[2 * i], s[2 * i + 1]);
     }
-    // Is there something in V of a block which only some rows see that is not finite?  A weight of 0 does not silence it: the rows are
-    // then done again by plain_row.  (Leaving it out of the product here costs registers that there are not: 1.7 times the time.)
-    WZY_DEV bool unsafe(const AttnArgs& a, int b, int lane, const char* vb) const {
-        if (pos_min == pos_max || !masked(a, b)) return false;
-        bool found = false;
-#pragma unroll 4
-        for (int i = 0; i < BV::LOADS; ++i) {
-            const v4w_t x = *(const v4w_t*) (vb + i * BV::STEP + 16 * lane);
+    // Is there something in V of a block that is not finite, where some row has a weight of 0 for what lies there: a cell that it does not
+    // see (another wave's token may, also where this wave's rows are all of one), or the repeat of one at the part's ends?  A weight of 0
+    // does not silence it: the rows are then done again by plain_row.  (Leaving it out of the product here costs registers that there are
+    // not: 1.7 times the time.)  FEW: single tokens are common (one over 2,000 cells, 12.6 us: looking over the whole block takes 0.5 us
+    // more, over its ends 0.2).
+    template <bool FEW>
+    WZY_DEV bool unsafe(const AttnArgs& a, const PgItem& it, int b, int lane, const char* vb) const {
+        if (!masked(a, b)) return false;
+        constexpr uint32_t EXP2 = Half<T>::EXP * 0x10001u, ONE2 = (0x8000u - Half<T>::EXP) * 0x10001u;
+        uint32_t found = 0;                                             // an exponent of all ones and one more: the half's top bit
+        auto look = [&](const char* p) {
+            const v4w_t x = *(const v4w_t*) p;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) found |= (x[j] & Half<T>::EXP) == Half<T>::EXP || (x[j] >> 16 & Half<T>::EXP) == Half<T>::EXP;
+            for (int j = 0; j < 4; ++j) found |= (x[j] & EXP2) + ONE2;
+        };
+        if (FEW && it.n_new == 1) {                                     // nothing but repeats of the first and the last cell
+            const int edge = lane < 32 ? max(it.lo - 32 * b, 0) : min(it.hi - 32 * b, 32) - 1;
+            look(vb + BV::row_at(edge) + 16 * (lane % BV::PIECES));
+        } else {
+#pragma unroll 4
+            for (int i = 0; i < BV::LOADS; ++i) look(vb + i * BV::STEP + 16 * lane);
         }
-        return __any(found);
+        return __any((found & 0x80008000u) != 0);
     }
     WZY_DEV void add(const char* vb, const v4w_t (&p)[2]) {
         v4w_t v[AHEAD];
@@ -474,7 +485,7 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
             w.weights(a, b, lane, s, p);
             if (more) wait_loads<BK::LOADS>();
             else wait_loads<0>();
-            unsafe |= w.unsafe(a, b, lane, vb);
+            unsafe |= w.template unsafe<true>(a, t.it, b, lane, vb);
             w.add(vb, p);
             if (!more) break;
             wait_lds();
@@ -574,7 +585,7 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
         }
         v4w_t p[2];
         w.weights(a, b, lane, s, p);
-        unsafe |= w.unsafe(a, b, lane, vb);
+        unsafe |= w.template unsafe<false>(a, t.it, b, lane, vb);
         w.add(vb, p);
         if (n + 1 < rounds || mine < rounds) wait_lds_and_meet();
         if (more) ld.template issue<true, MINE>(lv, half * MINE);
@@ -657,7 +668,7 @@ __global__ void __launch_bounds__(256, 2) paged_wide_kernel(AttnArgs a) {
         const v16f_t s = w.scores(s_buf[buf]);
         v4w_t p[2];
         w.weights(a, b, lane, s, p);
-        unsafe |= w.unsafe(a, b, lane, s_buf[buf] + BK::BYTES);
+        unsafe |= w.template unsafe<false>(a, t.it, b, lane, s_buf[buf] + BK::BYTES);
         w.add(s_buf[buf] + BK::BYTES, p);
     }
     for (; b < end; ++b, buf ^= 1) next();
