@@ -2,7 +2,7 @@
 //
 //   (a, b) -> A (a cos t - b sin t, b cos t + a sin t),   t = 2 pi * frac(position * f_i / 2 pi)
 //
-// Angles: position * (f / 2 pi) in 64 bits, less its nearest eighth of a turn's multiple; what is left, at most pi / 4 either
+// Angles: position * (f / 2 pi) in 64 bits, less the nearest multiple of a quarter turn; what is left, at most pi / 4 either
 // way, goes into the Taylor polynomials of sine and cosine in 64 bits (to x^13 and x^14: 2e-14).  They are made once a row, by
 // one thread an angle, and kept in LDS for all heads of the row: at far positions fp32 angles would be off by whole turns.
 // The rows are read and written once, 8 elements (and their partners) a thread where alignment allows 16-byte accesses, a pair
@@ -40,8 +40,8 @@ struct RopeArgs {
 // cos and sin of 2 pi x, amplitude in
 WZY_DEV float2 turn(double x, double amplitude) {
     x -= floor(x);                                             // 0 .. 1
-    const int oct = (int) (x * 8.0 + 0.5) & ~1;                 // nearest quarter turn, in eighths
-    const double y = (x - (double) oct * 0.125) * 6.283185307179586476925, z = y * y;
+    const int near = (int) (x * 4.0 + 0.5);                    // quarter turns, the nearest
+    const double y = (x - (double) near * 0.25) * 6.283185307179586476925, z = y * y;
     double c = -1.0 / 87178291200.0, s = 1.0 / 6227020800.0;
     c = fma(c, z, 1.0 / 479001600.0); s = fma(s, z, -1.0 / 39916800.0);
     c = fma(c, z, -1.0 / 3628800.0);  s = fma(s, z, 1.0 / 362880.0);
@@ -50,7 +50,7 @@ WZY_DEV float2 turn(double x, double amplitude) {
     c = fma(c, z, 1.0 / 24.0);        s = fma(s, z, -1.0 / 6.0);
     c = fma(c, z, -0.5);              s = fma(s, z, 1.0) * y;
     c = fma(c, z, 1.0);
-    const int q = (oct >> 1) & 3;                               // quarter turns
+    const int q = near & 3;
     const double cc = q & 1 ? s : c, ss = q & 1 ? c : s;
     return make_float2((float) (amplitude * (q == 1 || q == 2 ? -cc : cc)), (float) (amplitude * (q >= 2 ? -ss : ss)));
 }
