@@ -28,3 +28,25 @@ def test_rope_turns_are_rounded_as_the_sine_is(wz, gpu, degrees):
     c, s = d.numpy()[0].reshape(2, 4, 64)
     for got in (s[0], -c[1], -s[2], c[3]):
         np.testing.assert_array_equal(got, lower)
+
+
+def test_rope_of_more_rows_than_one_launch_takes(wz, gpu):
+    # 2^25 rows and a few, two a workgroup: rows at the ends and around the borders of launches equal small calls' rows
+    rows, hd = (1 << 25) + 5, 512
+    rng = np.random.default_rng(1)
+    xd = DA.from_numpy(rng.integers(0x3F00, 0x4100, hd).astype(np.uint16))            # every row the same, in bf16
+    pd = DA.from_numpy(np.arange(rows, dtype=np.int32))
+    f = DA(hd // 2 + 1, np.float64)
+    wz.wzy_rope_freqs(ref(wzy_amd.RopeCfg(1e4, 1.0, 1.0, 32.0, 1.0, 4096, hd, 0)), f.ptr, None)
+    tab, x = wzy_amd.RopeTab(f.ptr, hd, 0), wzy_amd.Heads(xd.ptr, 0, hd)
+    out = DA((rows + 1) * hd * 2, np.uint8)                                           # 34 GB
+    wz.wzy_memset(out.ptr + rows * hd * 2, 0xA5, hd * 2, None)
+    wz.wzy_rope(ref(tab), ref(x), wzy_amd.TYPE_BF16, rows, 1, hd, pd.ptr, ref(wzy_amd.Heads(out.ptr, hd, hd)), None)
+    small = DA(3 * hd, np.uint16)
+    got = np.zeros(3 * hd, np.uint16)
+    for at in (0, (1 << 23) - 1, (1 << 24) - 1, (1 << 25) - 1, rows - 3):
+        wz.wzy_rope(ref(tab), ref(x), wzy_amd.TYPE_BF16, 3, 1, hd, pd.ptr + 4 * at, ref(wzy_amd.Heads(small.ptr, hd, hd)), None)
+        wz.wzy_memcpy_d2h(got.ctypes.data, out.ptr + at * hd * 2, got.nbytes, None)
+        np.testing.assert_array_equal(got, small.numpy())
+    wz.wzy_memcpy_d2h(got.ctypes.data, out.ptr + rows * hd * 2, hd * 2, None)
+    assert (got[:hd].view(np.uint8) == 0xA5).all()

@@ -19,7 +19,7 @@ typedef float v4f_t __attribute__((ext_vector_type(4)));
 typedef uint32_t v4w_t __attribute__((ext_vector_type(4)));
 
 namespace {
-constexpr int RT = 256, ROPE_MAX = 512;
+constexpr int RT = 256, ROPE_MAX = 512, MOST_BLOCKS = 1 << 23;
 
 struct View { const void* p; int64_t ld, ldh; };
 struct RopeArgs {
@@ -33,7 +33,7 @@ struct RopeArgs {
     int per_row, per_head;                // pieces of work: of all heads of a row, of a head
     FastDiv div_row, div_head;
     int64_t ld_page, n_cells;
-    int lp, rows_block;
+    int lp, rows_block, first;            // first: row of the launch's first workgroup
     bool stream;                          // stores past the caches
 };
 
@@ -164,7 +164,7 @@ struct Piece {
 template <int TI, int TO, bool PAIRS, bool WIDE>
 __global__ void __launch_bounds__(RT) rope_kernel(RopeArgs a) {
     __shared__ float2 s_cs[ROPE_MAX];
-    const int tid = threadIdx.x, row0 = blockIdx.x * a.rows_block, rows = min(a.rows - row0, a.rows_block);
+    const int tid = threadIdx.x, row0 = a.first + (int) blockIdx.x * a.rows_block, rows = min(a.rows - row0, a.rows_block);
     const int half = a.n_rot >> 1, pieces = rows * a.per_row, step = RT * (int) gridDim.y;
     Piece<TI, TO, PAIRS, WIDE> p;
     int i = (int) blockIdx.y * RT + tid;
@@ -236,14 +236,17 @@ int launch(RopeArgs a, bool pairs, bool wide, void* stream) {
     a.rows_block = rb;
     a.stream = (int64_t) a.rows * heads * a.hd * mx_type_bytes(TO) > 32 << 20;
     // few rows: a row's pieces to several workgroups, each with angles of its own
-    const int blocks = (a.rows + rb - 1) / rb, share = blocks >= 512 ? 1 : std::min((a.per_row * rb + RT - 1) / RT, 512 / blocks);
-    const dim3 grid((unsigned) blocks, (unsigned) share);
+    const int blocks = pg_div_up(a.rows, rb), share = blocks >= 512 ? 1 : std::min((a.per_row * rb + RT - 1) / RT, 512 / blocks);
     const auto st = as_stream(stream);
-    if (pairs && wide) rope_kernel<TI, TO, true, true><<<grid, RT, 0, st>>>(a);
-    else if (pairs) rope_kernel<TI, TO, true, false><<<grid, RT, 0, st>>>(a);
-    else if (wide) rope_kernel<TI, TO, false, true><<<grid, RT, 0, st>>>(a);
-    else rope_kernel<TI, TO, false, false><<<grid, RT, 0, st>>>(a);
-    WZY_LAUNCH_CHECK();
+    for (int64_t at = 0; at < blocks; at += MOST_BLOCKS) {     // a launch has fewer than 2^32 threads
+        const dim3 grid((unsigned) std::min<int64_t>(blocks - at, MOST_BLOCKS), (unsigned) share);
+        a.first = (int) (at * rb);
+        if (pairs && wide) rope_kernel<TI, TO, true, true><<<grid, RT, 0, st>>>(a);
+        else if (pairs) rope_kernel<TI, TO, true, false><<<grid, RT, 0, st>>>(a);
+        else if (wide) rope_kernel<TI, TO, false, true><<<grid, RT, 0, st>>>(a);
+        else rope_kernel<TI, TO, false, false><<<grid, RT, 0, st>>>(a);
+        WZY_LAUNCH_CHECK();
+    }
     return WZY_OK;
 }
 }  // namespace
