@@ -64,7 +64,7 @@ typedef struct wzy_paged_batch {
  * wzy_paged_attend of that step; layers that differ in these numbers need lists of their own. */
 typedef struct wzy_paged_work {
     int qh, kvh, hd;             /* query heads (a multiple of kvh, at most 256 of them a key head), key heads (1 .. 64),
-                                    head size: 64, 128 or 256 */
+                                    head size: 64, 128 or 256; max_tokens * qh + 128 * n_req * kvh at most 2^31 - 2^17 */
     int window;                  /* a token sees itself and the window - 1 cells before it; 0: all */
     void* items;                 /* device memory of wzy_paged_work_bytes() bytes, 16-byte aligned */
     size_t bytes;

@@ -829,8 +829,10 @@ int launch(AttnArgs a, const PgLayout& l, const Space& s, char* space, int max_r
 }  // namespace
 
 extern "C" size_t wzy_paged_attend_workspace_bytes(const wzy_paged_batch* b, const wzy_paged_work* w) {
-    if (pg_check_batch("wzy_paged_attend_workspace_bytes", b, 1) != WZY_OK || pg_check_work("wzy_paged_attend_workspace_bytes", w) != WZY_OK) return 0;
-    return space_of(pg_layout_of(b, w), w).total;
+    const char* const who = "wzy_paged_attend_workspace_bytes";
+    if (pg_check_batch(who, b, 1) != WZY_OK || pg_check_work(who, w) != WZY_OK) return 0;
+    const PgLayout l = pg_layout_of(b, w);
+    return pg_check_launch(who, b, w, l) == WZY_OK ? space_of(l, w).total : 0;
 }
 
 extern "C" int wzy_paged_attend(const wzy_paged_cache* c, const wzy_paged_batch* b, const wzy_paged_work* w, const wzy_heads* q,
@@ -842,6 +844,7 @@ extern "C" int wzy_paged_attend(const wzy_paged_cache* c, const wzy_paged_batch*
     WZY_REQUIRE(w->kvh == c->kvh && w->hd == c->hd, "%s: work list of %d heads of %d, cache of %d of %d", who, w->kvh, w->hd, c->kvh, c->hd);
     WZY_REQUIRE(b->table, "%s: table is null", who);
     const PgLayout l = pg_layout_of(b, w);
+    WZY_TRY(pg_check_launch(who, b, w, l));
     WZY_REQUIRE(w->items && (uintptr_t) w->items % 16 == 0 && w->bytes >= sizeof(PgHead) + sizeof(PgItem) * (size_t) l.total,
                 "%s: work list of %zu bytes at %p", who, w->bytes, w->items);
     WZY_TRY(pg_check_heads(who, "q", q, c->type, w->qh, c->hd));

@@ -374,8 +374,10 @@ PgLayout pg_layout_of(const wzy_paged_batch* b, const wzy_paged_work* w) { retur
 }
 
 extern "C" size_t wzy_paged_work_bytes(const wzy_paged_batch* b, const wzy_paged_work* w) {
-    if (pg_check_batch("wzy_paged_work_bytes", b, 1) != WZY_OK || pg_check_work("wzy_paged_work_bytes", w) != WZY_OK) return 0;
-    return sizeof(PgHead) + sizeof(PgItem) * (size_t) layout_of(b, w).total;
+    const char* const who = "wzy_paged_work_bytes";
+    if (pg_check_batch(who, b, 1) != WZY_OK || pg_check_work(who, w) != WZY_OK) return 0;
+    const PgLayout l = layout_of(b, w);
+    return pg_check_launch(who, b, w, l) == WZY_OK ? sizeof(PgHead) + sizeof(PgItem) * (size_t) l.total : 0;
 }
 
 extern "C" int wzy_paged_plan(const wzy_paged_pool* pool, const wzy_paged_batch* b, const wzy_paged_work* works, int n_works,
@@ -391,6 +393,7 @@ extern "C" int wzy_paged_plan(const wzy_paged_pool* pool, const wzy_paged_batch*
         const wzy_paged_work* const w = works + i;
         WZY_TRY(pg_check_work(who, w));
         const PgLayout l = layout_of(b, w);
+        WZY_TRY(pg_check_launch(who, b, w, l));
         const size_t want = sizeof(PgHead) + sizeof(PgItem) * (size_t) l.total;
         WZY_REQUIRE(w->items && (uintptr_t) w->items % 16 == 0 && w->bytes >= want, "%s: work list %d: %zu bytes at %p (%zu, 16-byte aligned)",
                     who, i, w->bytes, w->items, want);

@@ -117,6 +117,12 @@ inline int pg_check_work(const char* who, const wzy_paged_work* w) {
     WZY_REQUIRE(w->window >= 0, "%s: window %d", who, w->window);
     return WZY_OK;
 }
+// a list's workgroups fit one launch, which has fewer than 2^32 threads
+inline int pg_check_launch(const char* who, const wzy_paged_batch* b, const wzy_paged_work* w, const PgLayout& l) {
+    for (int items : l.items)
+        WZY_REQUIRE((int64_t) items * w->kvh < 1 << 24, "%s: %d rows of %d query heads (their product below 2^31)", who, b->max_tokens, w->qh);
+    return WZY_OK;
+}
 // rows of heads at any alignment of an element
 inline int pg_check_heads(const char* who, const char* what, const wzy_heads* h, int type, int heads, int hd) {
     WZY_REQUIRE(h && h->p, "%s: %s is null", who, what);
