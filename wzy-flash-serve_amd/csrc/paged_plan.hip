@@ -233,7 +233,8 @@ __global__ void __launch_bounds__(NT) paged_plan_kernel(PlanArgs a, PlanWorks wo
             const int64_t all = ((int64_t) sums[2 + 2 * kind] << 16) + sums[3 + 2 * kind];
             const int slots = w.per_head[kind], nt = sums[kind];
             const int per_head = 4 * nt <= slots ? slots - nt : slots + (kind ? 0 : min(nt, w.more));
-            part[kind] = max((int) ceil((double) all / (double) per_head), w.l.min_len[kind] / 32);
+            // (at most all blocks of the longest request: the quotient may pass 31 bits)
+            part[kind] = max((int) fmin(ceil((double) all / (double) per_head), PG_MAX_CELLS / 32), w.l.min_len[kind] / 32);
         }
         // items, parts and merges before each request
         Cut x[PER];
