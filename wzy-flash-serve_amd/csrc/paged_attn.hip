@@ -306,30 +306,6 @@ struct Wave {
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i / 4][i % 4] = pack2<T>(s[2 * i], s[2 * i + 1]);
     }
-    // Is there something in V of a block that is not finite, where some row has a weight of 0 for what lies there: a cell that it does not
-    // see (another wave's token may, also where this wave's rows are all of one), or the repeat of one at the part's ends?  A weight of 0
-    // does not silence it: the rows are then done again by plain_row.  (Leaving it out of the product here costs registers that there are
-    // not: 1.7 times the time.)  FEW: single tokens are common (one over 2,000 cells, 12.6 us: looking over the whole block takes 0.5 us
-    // more, over its ends 0.2).
-    template <bool FEW>
-    WZY_DEV bool unsafe(const AttnArgs& a, const PgItem& it, int b, int lane, const char* vb) const {
-        if (!masked(a, b)) return false;
-        constexpr uint32_t EXP2 = Half<T>::EXP * 0x10001u, ONE2 = (0x8000u - Half<T>::EXP) * 0x10001u;
-        uint32_t found = 0;                                             // an exponent of all ones and one more: the half's top bit
-        auto look = [&](const char* p) {
-            const v4w_t x = *(const v4w_t*) p;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) found |= (x[j] & EXP2) + ONE2;
-        };
-        if (FEW && it.n_new == 1) {                                     // nothing but repeats of the first and the last cell
-            const int edge = lane < 32 ? max(it.lo - 32 * b, 0) : min(it.hi - 32 * b, 32) - 1;
-            look(vb + BV::row_at(edge) + 16 * (lane % BV::PIECES));
-        } else {
-#pragma unroll 4
-            for (int i = 0; i < BV::LOADS; ++i) look(vb + i * BV::STEP + 16 * lane);
-        }
-        return __any((found & 0x80008000u) != 0);
-    }
     WZY_DEV void add(const char* vb, const v4w_t (&p)[2]) {
         v4w_t v[AHEAD];
 #pragma unroll
@@ -344,6 +320,40 @@ struct Wave {
     }
 };
 
+// The blocks from .. to - 1 that every token at pos_min .. pos_max sees whole.
+struct Seen {
+    int from, to;
+    WZY_DEV Seen(const AttnArgs& a, int pos_min, int pos_max)
+        : from(a.window != 0 && pos_max >= a.window ? ((pos_max - a.window) >> 5) + 1 : 0), to((pos_min + 1) >> 5) {}
+    WZY_DEV bool all(int b) const { return b >= from && b < to; }
+};
+// A weight of 0 does not silence a value that is not finite.  So where some row of a tile does not see all of a block (or the block
+// repeats a cell at the part's ends), such values of V become 0 in LDS before the products, and add_hidden brings them to the rows that
+// see their cells afterwards.  (Leaving them out of the operands costs registers that there are not: 1.7 times the time.  Doing the
+// rows again one by one over the whole part: a chunk of 2,047 tokens behind 30,001 cells 240 ms.)  Loads start .. start + N - 1 of V's,
+// which have landed; was there one?
+template <int HD, int T, int N>
+WZY_DEV bool hide(char* vb, int start, int lane) {
+    constexpr uint32_t EXP2 = Half<T>::EXP * 0x10001u, ONE2 = (0x8000u - Half<T>::EXP) * 0x10001u;
+    using BV = Block<HD, true>;
+    bool found = false;
+#pragma unroll 4
+    for (int i = 0; i < N; ++i) {
+        v4w_t* const p = (v4w_t*) (vb + (start + i) * BV::STEP + 16 * lane);
+        v4w_t x = *p;
+        uint32_t hot[4], any = 0;                                       // an exponent of all ones and one more: the half's top bit
+#pragma unroll
+        for (int j = 0; j < 4; ++j) any |= hot[j] = ((x[j] & EXP2) + ONE2) & 0x80008000u;
+        if (any) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] &= ~((hot[j] >> 15) * 0xFFFFu);
+            *p = x;
+            found = true;
+        }
+    }
+    wave_lds_sync();
+    return __any(found);
+}
 // the workgroup's item and key head; false where there is none, or the list is not one of this step
 WZY_DEV bool tile_ctx(const AttnArgs& a, int kind, TileCtx& t) {
     const int at = (int) (blockIdx.x / (unsigned) a.kvh);
@@ -363,48 +373,63 @@ WZY_DEV char* out_row(const AttnArgs& a, const TileCtx& t, int row) {
     return a.out + (int64_t) (t.it.q0 + token) * a.ldo + (int64_t) (t.head * a.g + row - token * a.g) * a.ldo_head;
 }
 
-// A row of a part by itself, on a wave: only the cells that it sees are looked at.
+// is there such a value in the first or the last row of lo .. hi - 1 that a block holds?
 template <int HD, int T>
-WZY_DEV void plain_row(const AttnArgs& a, const TileCtx& t, int row, int lane, int tile_rows) {
-    constexpr int E = HD / 64;                                          // columns a lane
-    const int token = (int) fast_div((uint32_t) row, a.div_g), pos = t.it.n_cached + token;
-    const int lo = a.window ? max(t.it.lo, pos - a.window + 1) : t.it.lo, hi = min(t.it.hi, pos + 1);
-    const uint16_t* const q = (const uint16_t*) (a.q + (int64_t) (t.it.q0 + token) * a.ldq + (int64_t) (t.head * a.g + row - token * a.g) * a.ldq_head) + E * lane;
-    float x[E], o[E], m = -INFINITY, l = 0.0f;
+WZY_DEV bool hot_ends(const char* vb, int lo, int hi, int lane) {
+    using BV = Block<HD, true>;
+    const int row = lane < 32 ? max(lo, 0) : min(hi, 32) - 1;
+    const v4w_t x = *(const v4w_t*) (vb + BV::row_at(row) + 16 * (lane % BV::PIECES));
+    bool hot = false;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        x[e] = Half<T>::value(q[e]);
-        o[e] = 0.0f;
-    }
-    for (int c = lo; c < hi; ++c) {
-        int id = t.pages[c >> a.lp];
-        id = (unsigned) id < (unsigned) a.n_pages ? id : 0;
-        const int64_t at = (int64_t) id * a.ld_page + (int64_t) (c & ((1 << a.lp) - 1)) * a.ld_cell + (int64_t) t.head * a.ld_head;
-        const uint16_t *const k = (const uint16_t*) (a.k + at) + E * lane, *const v = (const uint16_t*) (a.v + at) + E * lane;
-        float s = 0.0f, y[E];
+    for (int j = 0; j < 4; ++j) hot |= (x[j] & Half<T>::EXP) == Half<T>::EXP || (x[j] >> 16 & Half<T>::EXP) == Half<T>::EXP;
+    return __any(hot);
+}
+// Results of rows from .. to - 1, which are out, get what hide() took from V: whatever its weight, a value that is not finite makes the
+// sum infinite, or with another not a number.  A wave reads the cells of all blocks outside `seen`, E columns a lane, CELLS at once.
+// (What was there already may come again: the sum is the same.)
+template <int HD, int T>
+WZY_DEV void add_hidden(const AttnArgs& a, const TileCtx& t, const Seen& seen, int from, int to, int lane, int tile_rows) {
+    constexpr int E = HD / 64, CELLS = 8;
+    const int split = max(seen.from, seen.to) == seen.to ? 32 * seen.from : t.it.hi;         // no block is seen whole: all cells
+    auto add = [&](int cell, const float (&v)[E]) {
+        for (int row = from; row < to; ++row) {
+            const int pos = t.it.n_cached + (int) fast_div((uint32_t) row, a.div_g);
+            if (cell > pos || (a.window != 0 && cell <= pos - a.window)) continue;
+            uint16_t* const out = (uint16_t*) out_row(a, t, row) + E * lane;
+            float* const part = a.part_o + (((size_t) t.it.part * a.kvh + t.head) * tile_rows + (row - t.it.row0)) * HD + E * lane;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            s = fmaf(x[e], Half<T>::value(k[e]), s);
-            y[e] = Half<T>::value(v[e]);
+            for (int e = 0; e < E; ++e) {
+                if (fabsf(v[e]) < INFINITY) continue;
+                if (t.it.part < 0) {
+                    const float y = Half<T>::value(out[e]) + v[e];
+                    out[e] = (uint16_t) pack2<T>(y, y);
+                } else part[e] += v[e];
+            }
         }
-        s = wave_sum(s) * a.c;
-        const float to = fmaxf(m, s), f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 0.0f;
-        const float p = to > -INFINITY || s != s ? __builtin_amdgcn_exp2f(s - to) : 0.0f;
-        m = to;
-        l = l * f + p;
+    };
+    for (int k = 0; k < 2; ++k) {                                       // before the blocks that are seen whole, behind them
+        const int c0 = k ? max(t.it.lo, max(split, 32 * seen.to)) : t.it.lo, c1 = k ? t.it.hi : min(t.it.hi, split);
+        for (int c = c0; c < c1; c += CELLS) {
+            float v[CELLS][E];
+            bool hot[CELLS];
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * f + p * y[e];
-    }
-    if (t.it.part < 0) {
-        const float n = l != 0.0f ? 1.0f / l : 0.0f;
-        uint16_t* const r = (uint16_t*) out_row(a, t, row) + E * lane;
+            for (int j = 0; j < CELLS; ++j) {
+                const int cell = min(c + j, c1 - 1);
+                int id = t.pages[cell >> a.lp];
+                id = (unsigned) id < (unsigned) a.n_pages ? id : 0;
+                const uint16_t* const p = (const uint16_t*) (a.v + (int64_t) id * a.ld_page + (int64_t) (cell & ((1 << a.lp) - 1)) * a.ld_cell +
+                                                             (int64_t) t.head * a.ld_head) + E * lane;
+                hot[j] = false;
 #pragma unroll
-        for (int e = 0; e < E; ++e) r[e] = (uint16_t) pack2<T>(o[e] * n, o[e] * n);
-    } else {
-        const size_t at = ((size_t) t.it.part * a.kvh + t.head) * tile_rows + (row - t.it.row0);
+                for (int e = 0; e < E; ++e) {
+                    v[j][e] = Half<T>::value(p[e]);
+                    hot[j] |= !(fabsf(v[j][e]) < INFINITY);
+                }
+            }
 #pragma unroll
-        for (int e = 0; e < E; ++e) a.part_o[at * HD + E * lane + e] = o[e];
-        if (lane == 0) a.part_ml[at] = make_float2(m + Half<T>::SHIFT, l);        // as other parts, whose weights are 2^SHIFT larger
+            for (int j = 0; j < CELLS; ++j)
+                if (c + j < c1 && __any(hot[j])) add(c + j, v[j]);
+        }
     }
 }
 // A request that is not served: all its rows become 0.
@@ -445,7 +470,7 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
     constexpr int MINE = BK::BYTES + BV::BYTES;
     __shared__ __align__(1024) char s_buf[4][MINE];                     // a wave's K and V; then its results in fp32
     __shared__ float s_m[4][32], s_l[4][32];
-    __shared__ int s_unsafe;
+    __shared__ int s_hidden[4];
     static_assert(MINE >= 32 * HD * 4 && MINE % 16 == 0, "a wave's results take its buffers");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     TileCtx t;
@@ -461,8 +486,7 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
     const uint32_t lk = lds_offset(kb), lv = lds_offset(vb);
     const int end = (t.it.hi + 31) >> 5;
     int b = (t.it.lo >> 5) + wave;
-    if (tid == 0) s_unsafe = 0;
-    bool unsafe = false;
+    if (lane == 0) s_hidden[wave] = 0;
     // the first block's loads before those of q, which the compiler counts as the only ones: it waits for all of them
     if (b < end) {
         ld.at(b);
@@ -470,6 +494,7 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
         ld.template issue<true, BV::LOADS>(lv, 0);
     }
     w.start(a, t, 0, lane);
+    const Seen seen(a, w.pos_min, w.pos_max);
     if (b < end) {
         wait_loads<0>();
         for (;; b += 4) {
@@ -485,7 +510,12 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
             w.weights(a, b, lane, s, p);
             if (more) wait_loads<BK::LOADS>();
             else wait_loads<0>();
-            unsafe |= w.template unsafe<true>(a, t.it, b, lane, vb);
+            if (!seen.all(b)) {
+                // of a single token, which is common, only the ends, which are repeated (over 2,000 cells, 12.6 us: all of V 0.5 us more)
+                bool look = t.it.n_new > 1;
+                if (!look) look = hot_ends<HD, T>(vb, t.it.lo - 32 * b, t.it.hi - 32 * b, lane);
+                if (look && hide<HD, T, BV::LOADS>(vb, 0, lane) && lane == 0) s_hidden[wave] = 1;
+            }
             w.add(vb, p);
             if (!more) break;
             wait_lds();
@@ -493,8 +523,6 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
         }
     }
     w.l = half_sum(w.l);
-    __syncthreads();
-    if (unsafe) s_unsafe = 1;
     if (lane < 32) {
         s_m[wave][lane] = w.m;
         s_l[wave][lane] = w.l;
@@ -510,10 +538,6 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
                 make_float4(w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]);
     __syncthreads();
     const int rows = w.rows;
-    if (s_unsafe) {
-        for (int r = wave; r < rows; r += 4) plain_row<HD, T>(a, t, r, lane, 32);
-        return;
-    }
     for (int i = tid; i < rows * (HD / 4); i += 256) {
         const int row = i / (HD / 4), col = i % (HD / 4);
         float m = s_m[0][row], l = 0.0f;
@@ -536,10 +560,15 @@ __global__ void __launch_bounds__(256) paged_narrow_kernel(AttnArgs a) {
             if (col == 0) a.part_ml[at] = make_float2(m, l);
         }
     }
+    if (s_hidden[0] | s_hidden[1] | s_hidden[2] | s_hidden[3]) {
+        __syncthreads();
+        add_hidden<HD, T>(a, t, seen, 8 * wave, min(8 * wave + 8, rows), lane, 32);
+    }
 }
 
-// Two barriers a block: the first says that V is there and K has been read (the next K's loads start), the second that the next K is
-// there and V has been read.
+// Three times a block all waves meet: when K is there; when it has been read and V is there (the next K's loads start); when V has been
+// read (its next loads start), but after the last block.  Both pairs meet as often, so a pair without a block in the first's last round
+// meets twice more.
 template <int HD, int T>
 __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
     using BK = Block<HD, false>;
@@ -547,7 +576,7 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
     constexpr int BOTH = BK::BYTES + BV::BYTES, MINE = BK::LOADS / 2;
     __shared__ __align__(1024) char s_buf[2][BOTH];                     // a pair's K and V; then the second pair's results in fp32
     __shared__ float s_m[64], s_l[64];
-    __shared__ int s_unsafe;
+    __shared__ int s_hidden[4];
     static_assert(2 * BOTH >= 64 * HD * 4, "a pair's results take the buffers");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave & 1, pair = wave >> 1;
     TileCtx t;
@@ -559,7 +588,7 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
     Wave<HD, T> w;
     Loader<HD> ld(a, t, lane);
     const char* const kb = s_buf[pair];
-    const char* const vb = kb + BK::BYTES;
+    char* const vb = s_buf[pair] + BK::BYTES;
     const uint32_t lk = lds_offset(kb), lv = lk + BK::BYTES;
     const int first = t.it.lo >> 5, end = (t.it.hi + 31) >> 5;
     int b = first + pair;
@@ -569,8 +598,8 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
         ld.template issue<true, MINE>(lv, half * MINE);
     }
     w.start(a, t, 32 * half, lane);
-    if (tid == 0) s_unsafe = 0;
-    bool unsafe = false;
+    if (lane == 0) s_hidden[wave] = 0;
+    const Seen seen(a, t.it.n_cached, t.it.n_cached + t.it.n_new - 1);  // of all of the tile's rows, which are the request's
     wait_loads<0>();
     // both pairs go round as often as the first has blocks; where the second has one fewer, it meets the first's last time
     const int rounds = (end - first + 1) / 2, mine = (end - first + 1 - pair) / 2;
@@ -578,6 +607,10 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
         const bool more = b + 2 < end;
         wait_loads_and_meet<MINE>();                                    // K is there; V, whose loads are younger, may be on its way
         const v16f_t s = w.scores(kb);
+        if (!seen.all(b)) {                                             // what this wave loaded
+            wait_loads<0>();
+            if (hide<HD, T, MINE>(vb, half * MINE, lane) && lane == 0) s_hidden[wave] = 1;
+        }
         wait_all_and_meet();
         if (more) {
             ld.at(b + 2);
@@ -585,7 +618,6 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
         }
         v4w_t p[2];
         w.weights(a, b, lane, s, p);
-        unsafe |= w.template unsafe<false>(a, t.it, b, lane, vb);
         w.add(vb, p);
         if (n + 1 < rounds || mine < rounds) wait_lds_and_meet();
         if (more) ld.template issue<true, MINE>(lv, half * MINE);
@@ -597,7 +629,6 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
     w.l = half_sum(w.l);
     wait_all_and_meet();                                                // the buffers have been read
     float4* const r = (float4*) (&s_buf[0][0] + half * 32 * HD * 4);
-    if (unsafe) s_unsafe = 1;
     if (pair == 1) {
         if (lane < 32) {
             s_m[32 * half + lane] = w.m;
@@ -609,10 +640,6 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
             for (int i = 0; i < 4; ++i) r[(4 * d + i) * 64 + lane] = make_float4(w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]);
     }
     __syncthreads();
-    if (s_unsafe) {
-        for (int r = wave; r < min(w.rows, 64); r += 4) plain_row<HD, T>(a, t, r, lane, 64);
-        return;
-    }
     if (pair == 1) return;
     const float m1 = s_m[32 * half + (lane & 31)], l1 = s_l[32 * half + (lane & 31)], m = fmaxf(w.m, m1);
     const float f0 = w.l != 0.0f ? __builtin_amdgcn_exp2f(w.m - m) : 0.0f, f1 = l1 != 0.0f ? __builtin_amdgcn_exp2f(m1 - m) : 0.0f;
@@ -628,6 +655,10 @@ __global__ void __launch_bounds__(256, 2) paged_middle_kernel(AttnArgs a) {
         }
     w.m = m;
     put_row<HD, T>(a, t, w, w.l * f0 + l1 * f1, lane, 64);
+    if (s_hidden[0] | s_hidden[1] | s_hidden[2] | s_hidden[3]) {
+        __threadfence_block();
+        add_hidden<HD, T>(a, t, seen, 32 * half, min(32 * half + 32, w.rows), lane, 64);
+    }
 }
 
 template <int HD, int T>
@@ -636,6 +667,7 @@ __global__ void __launch_bounds__(256, 2) paged_wide_kernel(AttnArgs a) {
     using BV = Block<HD, true>;
     constexpr int BOTH = BK::BYTES + BV::BYTES;
     __shared__ __align__(1024) char s_buf[2][BOTH];                     // two blocks' K and V
+    __shared__ int s_hidden[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     TileCtx t;
     if (!tile_ctx(a, 1, t)) return;
@@ -644,8 +676,9 @@ __global__ void __launch_bounds__(256, 2) paged_wide_kernel(AttnArgs a) {
     const uint32_t lk = lds_offset(s_buf);
     const int end = (t.it.hi + 31) >> 5;
     int b = t.it.lo >> 5, buf = 0;
+    const bool any = b < end;
+    constexpr int MINE = BK::LOADS / 4;                                 // of each matrix, a wave
     auto load = [&](int block, int into) {
-        constexpr int MINE = BK::LOADS / 4;                             // of each matrix, a wave
         const uint32_t at = lk + (uint32_t) (into * BOTH);
         ld.at(block);
         ld.template issue<false, MINE>(at, wave * MINE);
@@ -657,26 +690,33 @@ __global__ void __launch_bounds__(256, 2) paged_wide_kernel(AttnArgs a) {
     // the blocks that the wave's rows see: others' it helps to load and waits for.  (A loop each: a branch around the work in one loop
     // costs a second set of accumulators.)
     const int from = a.window ? max(b, (max(w.pos_min - a.window + 1, 0)) >> 5) : b, to = min(end, (w.pos_max >> 5) + 1);
+    // of all of the tile's rows
+    const Seen seen(a, t.it.n_cached + (int) fast_div((uint32_t) t.it.row0, a.div_g),
+                    t.it.n_cached + (int) fast_div((uint32_t) min(t.it.row0 + PG_WIDE, w.rows) - 1u, a.div_g));
+    if (lane == 0) s_hidden[wave] = 0;
     auto next = [&] {
+        if (!seen.all(b)) {                                             // what this wave loaded
+            wait_loads<0>();
+            if (hide<HD, T, MINE>(s_buf[buf] + BK::BYTES, wave * MINE, lane) && lane == 0) s_hidden[wave] = 1;
+        }
         wait_all_and_meet();                                            // the block is there; the other buffer has been read
         if (b + 1 < end) load(b + 1, buf ^ 1);
     };
     for (; b < from && b < end; ++b, buf ^= 1) next();
-    bool unsafe = false;
     for (; b < to; ++b, buf ^= 1) {
         next();
         const v16f_t s = w.scores(s_buf[buf]);
         v4w_t p[2];
         w.weights(a, b, lane, s, p);
-        unsafe |= w.template unsafe<false>(a, t.it, b, lane, s_buf[buf] + BK::BYTES);
         w.add(s_buf[buf] + BK::BYTES, p);
     }
     for (; b < end; ++b, buf ^= 1) next();
-    if (unsafe) {
-        for (int r = 0; r < 32 && t.it.row0 + 32 * wave + r < w.rows; ++r) plain_row<HD, T>(a, t, t.it.row0 + 32 * wave + r, lane, PG_WIDE);
-        return;
-    }
     put_row<HD, T>(a, t, w, half_sum(w.l), lane, PG_WIDE);
+    if (any && (s_hidden[0] | s_hidden[1] | s_hidden[2] | s_hidden[3])) {
+        __threadfence_block();
+        const int row0 = t.it.row0 + 32 * wave;
+        add_hidden<HD, T>(a, t, seen, row0, min(row0 + 32, w.rows), lane, PG_WIDE);
+    }
 }
 
 // Parts of a tile joined.  COLS / 4 lanes hold COLS columns of a row; of a workgroup's groups of lanes, several take one row's parts in
