@@ -158,7 +158,9 @@ int wzy_paged_append(const wzy_paged_cache* cache, const wzy_rope_tab* rope, con
  * that was built for other numbers has no work: nothing is written).
  * Sums are fp32; the softmax weights are rounded to the cache's type for the second product (half a step of a weight, so of
  * an output at most as much; fp16 weights are taken 2^6 larger, so that small ones are not lost).  A value that is not finite
- * reaches only the rows that see its cell; a row whose scores are all -infinity becomes 0.
+ * reaches only the rows that see its cell: of V, its column of those rows becomes infinite or not a number (not a number also where
+ * the weight is too small for its type, or rounds to 0 beside the largest).  A row whose scores are all -infinity becomes 0, but for
+ * such columns.
  * Page ids outside 0 .. n_pages - 1 count as page 0.  scale is finite and above 0. */
 size_t wzy_paged_attend_workspace_bytes(const wzy_paged_batch* batch, const wzy_paged_work* work);
 int wzy_paged_attend(const wzy_paged_cache* cache, const wzy_paged_batch* batch, const wzy_paged_work* work, const wzy_heads* q,
@@ -175,11 +177,11 @@ int wzy_paged_attend(const wzy_paged_cache* cache, const wzy_paged_batch* batch,
  *   min_p        of those, w_i >= min_p * w_0
  *   top_p        of those, the first until their sum reaches top_p * Z, that one included (top_p <= 0 or >= 1: all)
  *   id           the first whose running sum reaches u * (the sum of what is left); prob = its share of that sum
- * as the host sampler of wzy_engine.h does, over any number of logits.  temp at or below 1e-5: the first of the order,
+ * as the host sampler of wzy_engine.h does, but for its repetition penalty, over any number of logits.  temp at or below 1e-5: the first of the order,
  * prob 1.  A row without a logit above -infinity gives id -1, prob 0; +infinity takes all there is, shared by those that
  * have it.  Sums are integers of 2^-40 to 2^-51 of w_0, so results do not depend on the order of additions.
  * temp, top_k, top_p, min_p [rows] may each be NULL: 1, all, all, all; u [rows] in 0 .. 1 (below 0 counts as 0, above 1 as 1,
- * NaN as 0).  probs may be NULL.  1 <= vocab <= 2^22; any alignment of an element. */
+ * NaN as 0).  probs may be NULL.  1 <= vocab <= 2^22, rows at most 65,535; any alignment of an element. */
 size_t wzy_sample_workspace_bytes(int rows, int vocab);
 int wzy_sample(const void* logits, int type, int64_t ld, int rows, int vocab, const float* temp, const int* top_k,
                const float* top_p, const float* min_p, const float* u, int* ids, float* probs, void* workspace,

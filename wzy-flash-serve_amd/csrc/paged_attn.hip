@@ -12,15 +12,15 @@
 // Rows are (token, head of the group) pairs of one key head, so a group's heads share every byte of K and V.
 //   narrow  up to 32 rows: the waves of a workgroup take every fourth block of 32 keys each, through buffers of their own,
 //           with no barrier until their results are joined.  Bound by memory: 64 single tokens of requests of up to 6,000 cells,
-//           8 key heads of 128, 280 us (5.5 TB/s).  One of 32,768 cells, 2 heads of 256, 18 us and 6 for the merge of its 256 parts:
+//           8 key heads of 128, 280 us (5.5 TB/s).  One of 32,768 cells, 2 heads of 256, 17 us and 6 for the merge of its 256 parts:
 //           67 MB in one wave of workgroups, whose first loads and joins are half of it
 //   middle  up to 64 rows, where no request of the step has more (verify windows): two waves share a block, the two pairs take
-//           every other one.  16 windows of 4 tokens x 12 heads of 256 over 4,096 cells: 32 us and 7 for the merge (with the wide form,
+//           every other one.  16 windows of 4 tokens x 12 heads of 256 over 4,096 cells: 30 us and 7 for the merge (with the wide form,
 //           whose tiles would hold 80 empty rows, 47 for both before it was there and 40 after).  Bound by memory and the start of
 //           each part
 //   wide    128 rows, 32 a wave: the workgroup's waves share each block.  2,047 tokens x 12 heads of 256 behind 30,001 cells:
-//           1,440 us, 1,085 TFLOP/s (a library's 8,192^3 product: 1,184); prompts, heads of 128: 950 us, 930 TFLOP/s.  Bound by the
-//           matrix cores and the vector units' exponentials in turn: neither fewer operations a block nor fewer LDS reads (64 rows
+//           1,420 us with 36 for the merge, 1,100 TFLOP/s (a library's 8,192^3 product: 1,184); prompts, heads of 128: 940 us, 945
+//           TFLOP/s (boxes differ by 5 % in both).  Bound by the matrix cores and the vector units' exponentials in turn: neither fewer operations a block nor fewer LDS reads (64 rows
 //           a wave, in twice the registers: 1,255 us for the prompts) make it faster.  256 rows on 8 waves: 1,185
 // The maximum follows the scores only when one has come 2^8 above it, so most blocks leave the accumulators alone; weights
 // then reach 2^8, and in fp16, whose numbers end at 2^-24, all are taken 2^6 larger.
@@ -276,7 +276,10 @@ struct Wave {
         __builtin_amdgcn_sched_barrier(0);
         return s;
     }
-    // scores to weights, rounded and packed
+    // Scores to weights, rounded to the cache's type and packed, as the product takes them: the sum has them unrounded, so an output is off
+    // by half a step of its weights' at most.  (A second product of what the rounding left off would take that away, for half as many
+    // matrix instructions again in the wide form; but an infinity that a row sees would meet remainders that are 0 or negative, and
+    // the sum would not be a number.)
     WZY_DEV void weights(const AttnArgs& a, int b, int lane, v16f_t s, v4w_t (&p)[2]) {
         if (masked(a, b)) {
             const int low = a.window ? pos - a.window : -1;
@@ -395,15 +398,15 @@ WZY_DEV void add_hidden(const AttnArgs& a, const TileCtx& t, const Seen& seen, i
         for (int row = from; row < to; ++row) {
             const int pos = t.it.n_cached + (int) fast_div((uint32_t) row, a.div_g);
             if (cell > pos || (a.window != 0 && cell <= pos - a.window)) continue;
-            uint16_t* const out = (uint16_t*) out_row(a, t, row) + E * lane;
-            float* const part = a.part_o + (((size_t) t.it.part * a.kvh + t.head) * tile_rows + (row - t.it.row0)) * HD + E * lane;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 if (fabsf(v[e]) < INFINITY) continue;
+                const int column = E * lane + e;
                 if (t.it.part < 0) {
-                    const float y = Half<T>::value(out[e]) + v[e];
-                    out[e] = (uint16_t) pack2<T>(y, y);
-                } else part[e] += v[e];
+                    uint16_t* const out = (uint16_t*) out_row(a, t, row) + column;
+                    const float y = Half<T>::value(*out) + v[e];
+                    *out = (uint16_t) pack2<T>(y, y);
+                } else a.part_o[(((size_t) t.it.part * a.kvh + t.head) * tile_rows + (row - t.it.row0)) * HD + column] += v[e];
             }
         }
     };

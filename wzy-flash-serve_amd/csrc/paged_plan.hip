@@ -4,11 +4,12 @@
 //   slot of row t of request r = table[r][(c_r + i) / P] * P + (c_r + i) % P,   i = t - q_start[r]
 //
 // A few integers a request and a row: what bounds it is the chain from the lengths to the last slot, not bytes.  One workgroup
-// of 16 waves does requests, tables and work lists: the prefix sums over requests (4 a thread: wave shifts, then the 16 waves'
+// of 16 waves (4 for up to 256 requests and rows) does requests, tables and work lists: the prefix sums over requests (4 a thread: wave shifts, then the 16 waves'
 // sums) stay in LDS, and everything that is counted in pages, parts or rows is numbered through and dealt to the threads, each
 // finding its request by a search in those sums, so that one long prompt does not make one thread's loop long.  Up to PLAN_ROWS
 // rows the same launch fills positions, slots and work lists; more rows take a second one with a workgroup per 256 of them.
-// 8 requests' next tokens, one list: 6.6 us.  1,000 requests with 24,000 rows of prompts: 7.2 us and 5.6 us.
+// 8 requests' next tokens, one list: 6.6 us.  1,000 requests with 24,000 rows of prompts: 6.8 us and 6.1 us.  Release is one workgroup
+// too, its pages numbered through: 8 requests of 512 pages each 4 us, 125 of 300 pages (of 1,000 requests) 51, all 1,000 of them 390.
 #include "wzy_paged.h"
 
 using namespace wzy;

@@ -8,7 +8,8 @@
 // The rows are read and written once, 8 elements (and their partners) a thread where alignment allows 16-byte accesses, a pair
 // a thread elsewhere.  Bound by memory at large sizes, by the launch at one row: a row of 24 + 2 + 2 heads of 256 from fp32 2.7 us,
 // 8,192 of them in bf16 42 us where part of them is still in a cache and 64 where none is (235 MB; a copy of as much: 45), 4,097 rows
-// of 32 heads of 128 in fp16 12.5 us (67 MB, 5.4 TB/s).
+// of 32 heads of 128 in fp16 12.3 us (67 MB, 5.5 TB/s).  A pair a thread: the same rows in bf16 with 120 of their elements turned 36 to
+// 38 us (1.8 TB/s), with 22 of them 50 to 53; 8,192 rows of 28 heads of 256, 60 turned, 140.
 #include <algorithm>
 
 #include "wzy_paged.h"

@@ -12,8 +12,11 @@
 //                  groups above it are all that has to be read again; they get their token here
 //   sample_gather  the slices again: tokens of those bins to the row's list
 //   sample_pick    a workgroup a row: the list sorted, sums, places
-// Rows of at most SHORT logits are sorted whole, by one launch.  Rows whose bins hold more than CAP tokens (thousands of equal
-// logits) are done by sample_pick alone, from the row.
+// Rows of at most SHORT logits are sorted whole, by one launch.  Rows whose bins hold more than CAP tokens are done by sample_pick alone,
+// from the row: thousands of equal logits, and flat rows too (a bin of 1/16 octave has about 1,000 x temp tokens of 151,936 normal
+// logits of deviation 2.5).  With top-p 0.95, 4 of those rows take 30 us at temp 1 and 183 at temp 2, 256 of them 110 and 267; of
+// deviation 0.5 at temp 1, 290 and 418.
+// Few rows: 1 of 151,936 with top-k 40 19 us, top-k 500 29, top-p 27, no filter 25; 8 of them 21, 33, 32, 30 (bf16 within 3 us).
 // 256 rows of 151,936 fp32 logits with top-p: 25 + 42 + 8 + 28 + 10 us; the first and fourth are bound by memory (6 TB/s), the second
 // by its 64-bit operations and LDS atomics.  4 rows with top-k: 4 + 2 + 10 + 1 + 1, bound by latencies.
 // w is taken in 64 bits (fp32's 1e-7 would move one draw in a thousand of a flat row) and summed as integers of 2^-F, F = 62 -

@@ -16,8 +16,12 @@ namespace wzy {
 // together.  The same list serves every key head.
 constexpr int PG_WIDE = 128;
 constexpr int PG_MAX_REQ = 4096, PG_MAX_TOKENS = 1 << 20, PG_MAX_CELLS = 1 << 24;
-// Parts that a step is cut into, over all key heads: as many workgroups as the chip holds at once (by the LDS they take), and of
-// narrow tiles one more a tile, as far as PG_MORE, so that requests of different lengths come out even.
+// Parts that a step is cut into, over all key heads, and of narrow tiles one more a tile, as far as PG_MORE, so that requests of
+// different lengths come out even.  Narrow: as many workgroups as the chip holds at once by their LDS, 4, 2 or 1 a CU.  Middle: 3 a CU, of
+// heads of 256 the 2 that their registers allow (4 x 12 tokens over 20,000 cells, 32 heads on 8: heads of 64 36 us, with 1,024 parts 37;
+// of 128 74, with 512 70; of 256 135, with 768 142).  Wide: 2 a CU, all that heads of 256 have registers for (a chunk of 2,047: 1,425 us,
+// with 1,024 parts 1,510).  Smaller heads have them for more, and few tiles over many cells would gain by it: 512 tokens behind 30,000
+// cells, 32 heads on 8, of 64 275 us (with 1,024 parts 196), of 128 355 (with 768 301).
 constexpr int pg_parts(int kind, int narrow, int hd) {
     return kind ? 512 : narrow == 64 ? (hd == 256 ? 512 : 768) : hd == 64 ? 1024 : hd == 128 ? 512 : 256;
 }
