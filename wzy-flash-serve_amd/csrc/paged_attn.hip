@@ -20,7 +20,7 @@
 //           each part
 //   wide    128 rows, 32 a wave: the workgroup's waves share each block.  2,047 tokens x 12 heads of 256 behind 30,001 cells:
 //           1,420 us with 36 for the merge, 1,100 TFLOP/s (a library's 8,192^3 product: 1,184); prompts, heads of 128: 940 us, 945
-//           TFLOP/s (boxes differ by 5 % in both).  Bound by the matrix cores and the vector units' exponentials in turn: neither fewer operations a block nor fewer LDS reads (64 rows
+//           TFLOP/s (cards differ by 5 % in both).  Bound by the matrix cores and the vector units' exponentials in turn: neither fewer operations a block nor fewer LDS reads (64 rows
 //           a wave, in twice the registers: 1,255 us for the prompts) make it faster.  256 rows on 8 waves: 1,185
 // The maximum follows the scores only when one has come 2^8 above it, so most blocks leave the accumulators alone; weights
 // then reach 2^8, and in fp16, whose numbers end at 2^-24, all are taken 2^6 larger.
