@@ -20,8 +20,9 @@
 //           each part
 //   wide    128 rows, 32 a wave: the workgroup's waves share each block.  2,047 tokens x 12 heads of 256 behind 30,001 cells:
 //           1,420 us with 36 for the merge, 1,100 TFLOP/s (a library's 8,192^3 product: 1,184); prompts, heads of 128: 940 us, 945
-//           TFLOP/s (cards differ by 5 % in both).  Bound by the matrix cores and the vector units' exponentials in turn: neither fewer operations a block nor fewer LDS reads (64 rows
-//           a wave, in twice the registers: 1,255 us for the prompts) make it faster.  256 rows on 8 waves: 1,185
+//           TFLOP/s (cards differ by 5 % in both).  Bound by the matrix cores and the vector units' exponentials in turn: neither
+//           fewer operations a block nor fewer LDS reads (64 rows a wave, in twice the registers: 1,255 us for the prompts) make it
+//           faster.  256 rows on 8 waves: 1,185
 // The maximum follows the scores only when one has come 2^8 above it, so most blocks leave the accumulators alone; weights
 // then reach 2^8, and in fp16, whose numbers end at 2^-24, all are taken 2^6 larger.
 #include <algorithm>
@@ -394,27 +395,11 @@ template <int HD, int T>
 WZY_DEV void add_hidden(const AttnArgs& a, const TileCtx& t, const Seen& seen, int from, int to, int lane, int tile_rows) {
     constexpr int E = HD / 64, CELLS = 8;
     const int split = max(seen.from, seen.to) == seen.to ? 32 * seen.from : t.it.hi;         // no block is seen whole: all cells
-    auto add = [&](int cell, const float (&v)[E]) {
-        for (int row = from; row < to; ++row) {
-            const int pos = t.it.n_cached + (int) fast_div((uint32_t) row, a.div_g);
-            if (cell > pos || (a.window != 0 && cell <= pos - a.window)) continue;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                if (fabsf(v[e]) < INFINITY) continue;
-                const int column = E * lane + e;
-                if (t.it.part < 0) {
-                    uint16_t* const out = (uint16_t*) out_row(a, t, row) + column;
-                    const float y = Half<T>::value(*out) + v[e];
-                    *out = (uint16_t) pack2<T>(y, y);
-                } else a.part_o[(((size_t) t.it.part * a.kvh + t.head) * tile_rows + (row - t.it.row0)) * HD + column] += v[e];
-            }
-        }
-    };
     for (int k = 0; k < 2; ++k) {                                       // before the blocks that are seen whole, behind them
         const int c0 = k ? max(t.it.lo, max(split, 32 * seen.to)) : t.it.lo, c1 = k ? t.it.hi : min(t.it.hi, split);
         for (int c = c0; c < c1; c += CELLS) {
-            float v[CELLS][E];
-            bool hot[CELLS];
+            float v[CELLS][E];                                          // what is not finite
+            bool hot = false;
 #pragma unroll
             for (int j = 0; j < CELLS; ++j) {
                 const int cell = min(c + j, c1 - 1);
@@ -422,16 +407,34 @@ WZY_DEV void add_hidden(const AttnArgs& a, const TileCtx& t, const Seen& seen, i
                 id = (unsigned) id < (unsigned) a.n_pages ? id : 0;
                 const uint16_t* const p = (const uint16_t*) (a.v + (int64_t) id * a.ld_page + (int64_t) (cell & ((1 << a.lp) - 1)) * a.ld_cell +
                                                              (int64_t) t.head * a.ld_head) + E * lane;
-                hot[j] = false;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    v[j][e] = Half<T>::value(p[e]);
-                    hot[j] |= !(fabsf(v[j][e]) < INFINITY);
+                    const float x = Half<T>::value(p[e]);
+                    v[j][e] = fabsf(x) < INFINITY ? 0.0f : x;
+                    hot |= !(fabsf(x) < INFINITY);
                 }
             }
+            if (!__any(hot)) continue;
+            for (int row = from; row < to; ++row) {
+                const int pos = t.it.n_cached + (int) fast_div((uint32_t) row, a.div_g);
+                const int lo = a.window != 0 ? pos - a.window + 1 : 0, hi = min(pos + 1, c1);
+                float x[E] = {};
 #pragma unroll
-            for (int j = 0; j < CELLS; ++j)
-                if (c + j < c1 && __any(hot[j])) add(c + j, v[j]);
+                for (int j = 0; j < CELLS; ++j)
+                    if (c + j >= lo && c + j < hi)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) x[e] += v[j][e];
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if (x[e] == 0.0f) continue;
+                    const int column = E * lane + e;
+                    if (t.it.part < 0) {
+                        uint16_t* const out = (uint16_t*) out_row(a, t, row) + column;
+                        const float y = Half<T>::value(*out) + x[e];
+                        *out = (uint16_t) pack2<T>(y, y);
+                    } else a.part_o[(((size_t) t.it.part * a.kvh + t.head) * tile_rows + (row - t.it.row0)) * HD + column] += x[e];
+                }
+            }
         }
     }
 }
